@@ -73,6 +73,10 @@ enum oasr_op {
     OASR_OP_FLASH_ATTN_EXT = 2,
     OASR_OP_SET_ROWS = 3,
     OASR_OP_ARGMAX_FIRST = 4,
+    OASR_OP_QK_NORM_ROPE = 5,    /* src0 = qkv, src1 = k_pages */
+    OASR_OP_FLASH_ATTN_TREE = 6, /* src0 = q, src1 = k_pages */
+    OASR_OP_TREE_COMMIT = 7,     /* src0 = tokens, src1 = k_pages */
+    OASR_OP_KV_PAGES_COPY = 8,   /* src0 = k_pages */
 };
 
 /* GGML_BACKEND_GRAPH_CANCEL_* mechanisms and observation granularities -- ffi.rs:118-124 */
@@ -265,6 +269,70 @@ int oasr_b200_set_rows(oasr_backend *be, oasr_tensor *dst, const oasr_tensor *sr
  * each row of f32 logits [n, rows] the lowest index whose finite value is
  * maximal; out I32 [rows]. */
 int oasr_b200_argmax_first(oasr_backend *be, const oasr_tensor *logits, oasr_tensor *out);
+
+/* ---- paged K/V cache and drafted trees ---------------------------------------------
+ * No reference counterpart: the reference decodes one token per sequence and step over a
+ * dense cache.  These four operators verify a tree of drafted tokens per sequence in one
+ * pass over a cache kept in pages, so that sequences share, fork and free memory by the
+ * page.  Shapes (ne order, ne[0] fastest; n = nodes per sequence in the tensors):
+ *   k_pages, v_pages  F16 [D, page, H_kv, n_pages], D 64 or 128, page a multiple of 8;
+ *                     rows contiguous, other strides free (multiples of 16 bytes)
+ *   page_table        I32 [max_pages, n_seq]: the page that holds positions
+ *                     [j * page, (j + 1) * page) of a sequence
+ *   n_past            I32 [n_seq]: committed positions; node i of sequence s sits at
+ *                     position n_past[s] + i
+ *   n_nodes           I32 [n_seq] or NULL (= n): live nodes; the rest of the n rows is
+ *                     padding, whose outputs are zeros
+ * All of them live in device memory and are read when the kernel runs, so a captured step
+ * can be replayed while the sequences grow.  Page ids and lengths are checked by the
+ * kernels: one out of range makes oasr_b200_synchronize return
+ * OASR_STATUS_EXECUTION_FAILED, nothing outside the pages is touched, and the call's
+ * outputs for that sequence are undefined.  Pages that a call writes must belong to one
+ * sequence.  Work over all layers takes the pages of the layers one after the other along
+ * ne[3] (n_layers * n_pages), page ids counting within a layer.
+ *
+ * oasr_b200_qk_norm_rope: the heads of a fused projection, qkv F32 [D, H + 2 H_kv, n,
+ * n_seq] (query heads, key heads, value heads).  Query and key heads: RMSNorm over the
+ * head with gains q_norm / k_norm F32 [D] (NULL: none), then the NeoX rotation of the
+ * pairs (i, i + D/2) by rope F32 [2, D/2, n_pos] = (cos, sin) per position (NULL: none)
+ * at pos I32 [n, n_seq] (NULL: n_past + i; a tree passes n_past + depth).  Queries go to q
+ * F32 or F16 [D, H, n, n_seq], keys and values to their rows of the pages. */
+int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_tensor *q_norm,
+                           const oasr_tensor *k_norm, float eps, const oasr_tensor *rope, const oasr_tensor *pos,
+                           const oasr_tensor *page_table, const oasr_tensor *n_past, const oasr_tensor *n_nodes,
+                           oasr_tensor *q, oasr_tensor *k_pages, oasr_tensor *v_pages);
+/* Attention of the nodes over the pages: node i of sequence s sees the committed positions
+ * and those nodes j whose bit is set in its words of tree I32 [ceil(n / 32), n, n_seq]
+ * (n <= 1024; oasr_b200_tree_mask makes them from parents).  tree NULL: a chain, node i
+ * sees the nodes 0..i; with n = 1 that is a decode step over the pages.  q F32 or F16 [D,
+ * n, H, n_seq], dst F32 or F16 [D, H, n, n_seq] as in oasr_b200_flash_attn_ext, H % H_kv
+ * == 0.  A row that sees nothing is zeros.  What a row does not see does not reach it: K
+ * and V rows of hidden nodes and of positions past the last node may hold anything. */
+int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages,
+                              const oasr_tensor *v_pages, const oasr_tensor *page_table, const oasr_tensor *n_past,
+                              const oasr_tensor *n_nodes, const oasr_tensor *tree, float scale, oasr_tensor *dst);
+/* Greedy acceptance and compaction.  tokens, parents, target I32 [n, n_seq] (n <= 1024):
+ * the drafted tokens, each node's parent (node 0 is the root, whose token the model chose
+ * before; -1 elsewhere: not part of the tree), and the model's own choice after each node
+ * (oasr_b200_argmax_first of its logits).  Node 0 is accepted; after node c the lowest node
+ * j > c with parents[j] == c and tokens[j] == target[c].  path I32 [n, n_seq] gets the
+ * accepted nodes, then -1; n_accept their number; next_token the choice after the last (-1
+ * for a sequence without nodes); n_past_out = n_past + n_accept (not the n_past tensor).
+ * The K and V rows of the accepted nodes move to positions n_past, n_past + 1, ... in each
+ * of the n_layers layers; the rows after them are undefined. */
+int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oasr_tensor *parents,
+                          const oasr_tensor *target, const oasr_tensor *n_nodes, const oasr_tensor *n_past,
+                          const oasr_tensor *page_table, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
+                          oasr_tensor *path, oasr_tensor *n_accept, oasr_tensor *next_token, oasr_tensor *n_past_out);
+/* Copy pages in each of the n_layers layers, K and V: pairs I32 [2, n] = (source,
+ * destination) page.  Destinations are distinct and no source is a destination; a pair
+ * with a negative page is left out. */
+int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
+                            const oasr_tensor *pairs);
+/* Host helper: the tree words of one sequence from parents[n] (-1 for the root, otherwise
+ * an earlier node): words [n][ceil(n / 32)], each node seeing itself and its ancestors.
+ * OASR_STATUS_FAILED for a parent that does not come first, or n > 1024. */
+int oasr_b200_tree_mask(const int32_t *parents, int32_t n, int32_t *words);
 
 /* ---- memory API v1 (the optional table the plugin loader resolves through
  * ggml_backend_reg_get_proc_address("ggml_backend_memory_get_api_v1"); layouts and

@@ -22,6 +22,7 @@ LIB_PATH = os.path.join(HERE, "liboasr_b200.so")
 F32, F16, Q4_0, Q8_0, Q4_K, I32, I64 = 0, 1, 2, 8, 12, 26, 27
 PREC_DEFAULT, PREC_F32 = 0, 10
 OP_MUL_MAT, OP_FLASH_ATTN_EXT, OP_SET_ROWS, OP_ARGMAX_FIRST = 1, 2, 3, 4
+OP_QK_NORM_ROPE, OP_FLASH_ATTN_TREE, OP_TREE_COMMIT, OP_KV_PAGES_COPY = 5, 6, 7, 8
 
 STATUS_ALLOC_FAILED, STATUS_FAILED, STATUS_SUCCESS = -2, -1, 0
 STATUS_ABORTED, STATUS_EXECUTION_FAILED, STATUS_DEVICE_LOST, STATUS_BACKEND_POISONED = 1, 2, 3, 4
@@ -282,6 +283,11 @@ SIGNATURES = {
     "oasr_b200_flash_attn_causal": ([_P, _TP, _TP, _TP, _F, _I32, _TP], ctypes.c_int),
     "oasr_b200_set_rows": ([_P, _TP, _TP, _TP], ctypes.c_int),
     "oasr_b200_argmax_first": ([_P, _TP, _TP], ctypes.c_int),
+    "oasr_b200_qk_norm_rope": ([_P, _TP, _TP, _TP, _F, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP], ctypes.c_int),
+    "oasr_b200_flash_attn_tree": ([_P, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _F, _TP], ctypes.c_int),
+    "oasr_b200_tree_commit": ([_P, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _I32, _TP, _TP, _TP, _TP], ctypes.c_int),
+    "oasr_b200_kv_pages_copy": ([_P, _TP, _TP, _I32, _TP], ctypes.c_int),
+    "oasr_b200_tree_mask": ([_P, _I32, _P], ctypes.c_int),
     "oasr_b200_whisper_load": ([_P, ctypes.POINTER(OasrWhisperConfig), ctypes.POINTER(OasrNamedTensor), _I32,
                                 ctypes.POINTER(_P)], ctypes.c_int),
     "oasr_b200_whisper_free": ([_P], ctypes.c_int),
@@ -382,6 +388,11 @@ def describe(t, ggml_type: int | None = None) -> OasrTensor:
     d.ne[:] = shape[:4]
     d.nb[:] = strides[:4]
     return d
+
+
+def _opt(t):
+    """descriptor of an optional tensor"""
+    return None if t is None else describe(t)
 
 
 class Weight:
@@ -612,6 +623,49 @@ class Backend:
 
     def argmax_first(self, logits, out) -> None:
         self._check(lib().oasr_b200_argmax_first(self.handle, ctypes.byref(describe(logits)), ctypes.byref(describe(out))))
+
+
+    # -- paged K/V cache and drafted trees (shapes below are torch's: slowest dimension first) --
+    def qk_norm_rope(self, qkv, q_norm, k_norm, eps: float, rope, pos, page_table, n_past, n_nodes, q, k_pages,
+                     v_pages) -> None:
+        """Norms, rotation and the cache write of new nodes: qkv f32 [S, n, H + 2 H_kv, D] ->
+        q f32|f16 [S, n, H, D] and the K/V rows at positions n_past + i of the pages
+        f16 [P, H_kv, page, D].  q_norm / k_norm f32 [D], rope f32 [n_pos, D / 2, 2], pos and
+        n_nodes may be None (see the C header)."""
+        self._check(lib().oasr_b200_qk_norm_rope(
+            self.handle, describe(qkv), _opt(q_norm), _opt(k_norm), eps, _opt(rope), _opt(pos), describe(page_table),
+            describe(n_past), _opt(n_nodes), describe(q), describe(k_pages), describe(v_pages)))
+
+    def flash_attn_tree(self, q, k_pages, v_pages, page_table, n_past, n_nodes, tree, scale: float, out) -> None:
+        """Attention of the nodes q f32|f16 [S, H, n, D] over the pages -> out f32|f16 [S, n, H, D];
+        tree i32 [S, n, ceil(n / 32)] of visible nodes, or None for a chain."""
+        self._check(lib().oasr_b200_flash_attn_tree(
+            self.handle, describe(q), describe(k_pages), describe(v_pages), describe(page_table), describe(n_past),
+            _opt(n_nodes), _opt(tree), scale, describe(out)))
+
+    def tree_commit(self, tokens, parents, target, n_nodes, n_past, page_table, k_pages, v_pages, n_layers: int, path,
+                    n_accept, next_token, n_past_out) -> None:
+        """Accept the drafted path that agrees with target (all i32 [S, n]) and compact its K/V rows
+        in pages f16 [n_layers * P, H_kv, page, D]; path [S, n], the others [S]."""
+        self._check(lib().oasr_b200_tree_commit(
+            self.handle, describe(tokens), describe(parents), describe(target), _opt(n_nodes), describe(n_past),
+            describe(page_table), describe(k_pages), describe(v_pages), n_layers, describe(path), describe(n_accept),
+            describe(next_token), describe(n_past_out)))
+
+    def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
+        """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
+        self._check(lib().oasr_b200_kv_pages_copy(self.handle, describe(k_pages), describe(v_pages), n_layers,
+                                                  describe(pairs)))
+
+
+def tree_mask(parents) -> np.ndarray:
+    """int32 words [n, ceil(n / 32)] of a drafted tree: each node sees itself and its ancestors."""
+    par = np.ascontiguousarray(parents, np.int32)
+    words = np.zeros((len(par), (len(par) + 31) // 32), np.int32)
+    rc = lib().oasr_b200_tree_mask(par.ctypes.data, len(par), words.ctypes.data)
+    if rc != 0:
+        raise UnsupportedInputs(rc, "tree_mask: a parent comes before its children, at most 1024 nodes")
+    return words
 
 
 def device_count() -> int:

@@ -567,6 +567,24 @@ int oasr_b200_supports_op(oasr_backend *be, int32_t op, const oasr_tensor *src0,
         return src0->type == OASR_TYPE_F16 || src0->type == OASR_TYPE_F32;
     case OASR_OP_ARGMAX_FIRST:
         return src0->type == OASR_TYPE_F32;
+    case OASR_OP_QK_NORM_ROPE:
+    case OASR_OP_FLASH_ATTN_TREE:
+    case OASR_OP_TREE_COMMIT:
+    case OASR_OP_KV_PAGES_COPY: {
+        // F16 pages [D, page, H_kv, n_pages] in src1 (the page copy has them in src0)
+        const oasr_tensor *k = op == OASR_OP_KV_PAGES_COPY ? src0 : src1;
+        if (!k || k->type != OASR_TYPE_F16 || (k->ne[0] != 64 && k->ne[0] != 128) || k->ne[1] < 8 || k->ne[1] % 8 ||
+            k->ne[2] < 1)
+            return 0;
+        if (op == OASR_OP_TREE_COMMIT) return src0->type == OASR_TYPE_I32;
+        if (op == OASR_OP_QK_NORM_ROPE)
+            return src0->type == OASR_TYPE_F32 && src0->ne[0] == k->ne[0] && src0->ne[1] > 2 * k->ne[2] &&
+                   src0->ne[1] % k->ne[2] == 0;
+        if (op == OASR_OP_FLASH_ATTN_TREE)
+            return (src0->type == OASR_TYPE_F32 || src0->type == OASR_TYPE_F16) && src0->ne[0] == k->ne[0] &&
+                   src0->ne[2] >= 1 && src0->ne[2] % k->ne[2] == 0;
+        return 1;
+    }
     default:
         return 0;
     }

@@ -1,0 +1,481 @@
+// kv_pages.cu -- the paged K/V cache around the tree attention: per-head norms, rotation
+// and the cache write of new nodes (qk_norm_rope), acceptance of a drafted tree with the
+// compaction of its rows (tree_commit), and page copies (kv_pages_copy).
+//
+// The cache of one layer is a pool of pages [D, page, n_kv_heads, n_pages] f16; a sequence
+// owns positions through its row of the page table.  Node i of sequence s sits at position
+// n_past[s] + i; lengths live in device memory, so a step can be captured once and replayed.
+#include <string.h>
+
+#include <algorithm>
+
+#include "pages.cuh"
+
+using namespace oasr;
+
+namespace oasr {
+
+static bool is_vec_i32(const oasr_tensor *t, int64_t n) {
+    return t && t->type == OASR_TYPE_I32 && t->data && t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 && t->ne[3] == 1 &&
+           (t->nb[0] == 4 || n <= 1);
+}
+
+static int fail_op(oasr_backend *be, const char *op, const char *what) {
+    return oasr_internal_fail(be, OASR_STATUS_FAILED, std::string(op) + ": " + what);
+}
+
+int pages_check(oasr_backend *be, const char *op, const oasr_tensor *k, const oasr_tensor *v, int layers, KvPages *out) {
+    if (!k || !v) return fail_op(be, op, "null argument");
+    if (k->type != OASR_TYPE_F16 || v->type != OASR_TYPE_F16) return fail_op(be, op, "k/v pages must be F16");
+    for (int i = 0; i < 4; ++i)
+        if (k->ne[i] != v->ne[i]) return fail_op(be, op, "k/v pages must have one shape");
+    if (k->ne[0] != 64 && k->ne[0] != 128) return fail_op(be, op, "head_dim must be 64 or 128");
+    if (k->ne[1] < 8 || k->ne[1] % 8 || k->ne[1] > (1 << 24))
+        return fail_op(be, op, "positions per page must be a multiple of 8");
+    if (k->ne[2] < 1 || k->ne[2] > 65535 || k->ne[3] < 1 || k->ne[3] > (1 << 30)) return fail_op(be, op, "bad page pool shape");
+    if (layers < 1 || k->ne[3] % layers) return fail_op(be, op, "n_layers must divide the pages");
+    if (!k->data || !v->data) return fail_op(be, op, "null argument");
+    for (const oasr_tensor *t : {k, v}) {
+        if (t->nb[0] != 2) return fail_op(be, op, "rows of the pages must be contiguous");
+        if (((uintptr_t)t->data & 15) || t->nb[1] % 16 || t->nb[2] % 16 || t->nb[3] % 16 || t->nb[1] < 0 || t->nb[2] < 0 ||
+            t->nb[3] < 0)
+            return fail_op(be, op, "rows of the pages must be 16-byte aligned");
+    }
+    *out = KvPages{(char *)k->data, (char *)v->data, k->nb[1], k->nb[2], k->nb[3], v->nb[1], v->nb[2], v->nb[3],
+                   (int)(k->ne[3] / layers), (int)k->ne[1]};
+    return OASR_STATUS_SUCCESS;
+}
+
+int seqs_check(oasr_backend *be, const char *op, const oasr_tensor *table, const oasr_tensor *n_past,
+               const oasr_tensor *n_nodes, int64_t S, int64_t N, KvSeqs *out) {
+    if (!table || !n_past) return fail_op(be, op, "null argument");
+    if (S > (1 << 20) || N > (1 << 24) || S * N > INT32_MAX) return fail_op(be, op, "too many sequences or nodes");
+    if (table->type != OASR_TYPE_I32 || !table->data || table->ne[1] != S || table->ne[2] != 1 || table->ne[3] != 1 ||
+        table->ne[0] < 1 || table->ne[0] > (1 << 24) || (table->nb[0] != 4 && table->ne[0] > 1) || table->nb[1] % 4)
+        return fail_op(be, op, "page_table must be I32 [max_pages, n_seq]");
+    if (!is_vec_i32(n_past, S)) return fail_op(be, op, "n_past must be I32 [n_seq]");
+    if (n_nodes && !is_vec_i32(n_nodes, S)) return fail_op(be, op, "n_nodes must be I32 [n_seq]");
+    *out = KvSeqs{(const int *)table->data, table->nb[1] / 4, (int)table->ne[0], (const int *)n_past->data,
+                  n_nodes ? (const int *)n_nodes->data : nullptr, (int)N};
+    return OASR_STATUS_SUCCESS;
+}
+
+}  // namespace oasr
+
+namespace {
+
+// ---- norms, rotation and the cache write -------------------------------------------------
+struct NormRope {
+    const char *x;
+    int64_t x_nb1, x_nb2, x_nb3;  // head, node, sequence
+    char *q;
+    int64_t q_nb1, q_nb2, q_nb3;
+    const float *q_norm, *k_norm;  // [D], or null: no norm
+    const float *rope;             // [n_pos][D / 2][2], or null: no rotation
+    int n_pos;
+    const int *pos;  // [S][N], or null: n_past[s] + i
+    int64_t pos_ld;
+    int S, H, HKV;
+    float eps;
+};
+
+// y = x / sqrt(mean(x^2) + eps) * w, then pair (i, i + D/2) turned by the angle of the node's
+// position: (a cos - b sin, b cos + a sin).  One warp per (node, head): D / 32 values per lane,
+// the pair's other half 16 lanes away.  The squares are summed in 64 bits and every product
+// rounded as the Qwen driver's own kernel does, so both give the same bits.
+template <int D, bool QF16>
+__global__ void __launch_bounds__(128) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, int *err) {
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int HH = a.H + 2 * a.HKV;
+    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (unit >= (int64_t)a.S * sq.N * HH) return;
+    const int h = (int)(unit % HH);
+    const int i = (int)(unit / HH % sq.N), s = (int)(unit / HH / sq.N);
+    int past, n;
+    if (!seq_lengths(sq, s, p.page, past, n) && lane == 0) atomicOr(err, ERR_BAD_INDEX);
+    float v[V];
+    {
+        const float *x = reinterpret_cast<const float *>(a.x + h * a.x_nb1 + i * a.x_nb2 + s * a.x_nb3) + V * lane;
+        if (V == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(x);
+        else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(x);
+    }
+    const bool live = i < n;
+    if (!live) {
+        if (h >= a.H) return;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = 0.0f;  // padding nodes leave zeros in q, nothing in the cache
+    }
+    const float *w = h < a.H ? a.q_norm : h < a.H + a.HKV ? a.k_norm : nullptr;
+    if (live && w) {
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss += (double)__fmul_rn(v[j], v[j]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(ss / (double)D), a.eps)));
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], scale), w[V * lane + j]);
+    }
+    if (live && a.rope && h < a.H + a.HKV) {
+        int t = a.pos ? a.pos[s * a.pos_ld + i] : past + i;
+        if (t < 0 || t >= a.n_pos) {
+            if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
+            t = 0;
+        }
+        const float2 *cs = reinterpret_cast<const float2 *>(a.rope) + (int64_t)t * (D / 2) + V * (lane & 15);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
+            const float2 c = cs[j];
+            v[j] = lane < 16 ? __fsub_rn(__fmul_rn(v[j], c.x), __fmul_rn(other, c.y))
+                             : __fadd_rn(__fmul_rn(other, c.y), __fmul_rn(v[j], c.x));
+        }
+    }
+    if (h < a.H && !QF16) {
+        float *q = reinterpret_cast<float *>(a.q + h * a.q_nb1 + i * a.q_nb2 + s * a.q_nb3) + V * lane;
+        if (V == 4) *reinterpret_cast<float4 *>(q) = *reinterpret_cast<const float4 *>(v);
+        else *reinterpret_cast<float2 *>(q) = *reinterpret_cast<const float2 *>(v);
+        return;
+    }
+    char *dst;
+    if (h < a.H) {
+        dst = a.q + h * a.q_nb1 + i * a.q_nb2 + s * a.q_nb3;
+    } else {
+        const int at = past + i;
+        const int pg = sq.table[s * sq.table_ld + at / p.page];
+        if (pg < 0 || pg >= p.n_pages) {
+            if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
+            return;
+        }
+        const bool is_k = h < a.H + a.HKV;
+        const int64_t off = at % p.page;
+        dst = is_k ? p.k + pg * p.k_nb3 + (h - a.H) * p.k_nb2 + off * p.k_nb1
+                   : p.v + pg * p.v_nb3 + (h - a.H - a.HKV) * p.v_nb2 + off * p.v_nb1;
+    }
+    __half2 o[V / 2];
+#pragma unroll
+    for (int j = 0; j < V; j += 2) o[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
+    if (V == 4) *reinterpret_cast<uint2 *>(dst + 8 * lane) = *reinterpret_cast<const uint2 *>(o);
+    else *reinterpret_cast<uint32_t *>(dst + 4 * lane) = *reinterpret_cast<const uint32_t *>(o);
+}
+
+// ---- acceptance and compaction -------------------------------------------------------------
+struct Commit {
+    const int *tokens, *parents, *target;  // [S][N]
+    int64_t tok_ld, par_ld, tgt_ld;
+    int *path;  // [S][N]
+    int64_t path_ld;
+    int *n_accept, *next, *n_past_out;  // [S]
+    int S, L, HKV, D;
+    int groups;  // CTAs per sequence
+};
+
+// The walk: node 0 is accepted; after node c, the first node j > c with parents[j] = c and
+// tokens[j] = target[c].  Every node votes for itself at its parent (atomicMin keeps the first),
+// then one thread follows the links.  The accepted path is strictly increasing and path[i] >= i,
+// so a thread that moves its 16 bytes of every row in path order, a few rows loaded before they
+// are stored, never overwrites a row that it has still to read.  Each CTA repeats the walk and
+// moves 256 columns of 16 bytes of (layer, K or V, head).
+__global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, KvSeqs sq, int *err) {
+    __shared__ int s_next[TREE_MAX_NODES], s_path[TREE_MAX_NODES], s_tgt[TREE_MAX_NODES];
+    __shared__ int s_len, s_bad;
+    const int s = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
+    int past, n;
+    const bool ok = seq_lengths(sq, s, p.page, past, n);
+    if (!ok && threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
+    if (threadIdx.x == 0) s_bad = 0;
+    for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        s_next[c] = n;
+        s_tgt[c] = a.target[s * a.tgt_ld + c];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        const int up = a.parents[s * a.par_ld + c];
+        if (up >= 0 && up < c && a.tokens[s * a.tok_ld + c] == s_tgt[up]) atomicMin(&s_next[up], c);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int len = 0;
+        for (int c = 0; c < n; c = s_next[c]) s_path[len++] = c;  // links only go forward
+        s_len = len;
+    }
+    __syncthreads();
+    const int len = s_len;
+    if (g == 0) {
+        for (int c = threadIdx.x; c < sq.N; c += blockDim.x) a.path[s * a.path_ld + c] = c < len ? s_path[c] : -1;
+        if (threadIdx.x == 0) {
+            a.n_accept[s] = len;
+            a.next[s] = len ? s_tgt[s_path[len - 1]] : -1;
+            a.n_past_out[s] = sq.n_past[s] + len;
+        }
+        __syncthreads();
+    }
+    // (page << 32 | offset) of the rows: source replaces the path entry, destination the link
+    __shared__ int s_spg[TREE_MAX_NODES];
+    for (int c = threadIdx.x; c < len; c += blockDim.x) {
+        const int from = past + s_path[c], to = past + c;
+        const int fp = sq.table[s * sq.table_ld + from / p.page], tp = sq.table[s * sq.table_ld + to / p.page];
+        if (fp < 0 || fp >= p.n_pages || tp < 0 || tp >= p.n_pages) s_bad = 1;
+        s_spg[c] = fp;
+        s_next[c] = tp;
+    }
+    __syncthreads();
+    if (s_bad) {
+        if (threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
+        return;
+    }
+    const int cpr = a.D / 8;  // 16-byte columns per row
+    const int col = g * 256 + threadIdx.x;
+    if (col >= a.L * 2 * a.HKV * cpr) return;
+    const int c16 = col % cpr, h = col / cpr % a.HKV, kv = col / cpr / a.HKV % 2, l = col / cpr / a.HKV / 2;
+    const int64_t nb1 = kv ? p.v_nb1 : p.k_nb1, nb3 = kv ? p.v_nb3 : p.k_nb3;
+    char *base = (kv ? p.v : p.k) + (int64_t)l * p.n_pages * nb3 + h * (kv ? p.v_nb2 : p.k_nb2) + 16 * c16;
+    constexpr int U = 4;
+    for (int b = 1; b < len; b += U) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b + u < len && s_path[b + u] != b + u)
+                r[u] = *reinterpret_cast<const uint4 *>(base + s_spg[b + u] * nb3 + (past + s_path[b + u]) % p.page * nb1);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b + u < len && s_path[b + u] != b + u)
+                *reinterpret_cast<uint4 *>(base + s_next[b + u] * nb3 + (past + b + u) % p.page * nb1) = r[u];
+    }
+}
+
+// ---- page copies -------------------------------------------------------------------------
+// pair j: page src[j] -> page dst[j] of every layer, K and V; a negative source or destination
+// leaves the pair out.  16 bytes per thread and step; FLAT: a page is one run of bytes.
+template <bool FLAT>
+__global__ void __launch_bounds__(256) kv_pages_copy_kernel(const int *pairs, int64_t pair_ld, KvPages p, int L, int HKV,
+                                                            int cpr, int chunks, int *err) {
+    constexpr int U = 4;
+    const int64_t b = blockIdx.x;
+    const int ch = (int)(b % chunks), kv = (int)(b / chunks % 2), l = (int)(b / chunks / 2 % L);
+    const int64_t j = b / chunks / 2 / L;
+    const int src = pairs[j * pair_ld], dst = pairs[j * pair_ld + 1];
+    if (src < 0 || dst < 0) return;
+    if (src >= p.n_pages || dst >= p.n_pages) {
+        if (threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
+        return;
+    }
+    const int64_t nb1 = kv ? p.v_nb1 : p.k_nb1, nb2 = kv ? p.v_nb2 : p.k_nb2, nb3 = kv ? p.v_nb3 : p.k_nb3;
+    char *layer = (kv ? p.v : p.k) + (int64_t)l * p.n_pages * nb3;
+    const int total = HKV * p.page * cpr;
+    const int e0 = ch * (256 * U) + threadIdx.x;
+    uint4 r[U];
+    int64_t off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int e = e0 + 256 * u;
+        off[u] = FLAT ? (int64_t)e * 16 : (e / cpr / p.page) * nb2 + (e / cpr % p.page) * nb1 + (e % cpr) * 16;
+        if (e < total) r[u] = *reinterpret_cast<const uint4 *>(layer + src * nb3 + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (e0 + 256 * u < total) *reinterpret_cast<uint4 *>(layer + dst * nb3 + off[u]) = r[u];
+}
+
+int launched(oasr_backend *be, cudaError_t e, const char *what) {
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, what, __LINE__);
+    return oasr_internal_launch_check(be, what);
+}
+
+bool rows16(const oasr_tensor *t) {
+    return ((uintptr_t)t->data & 15) == 0 && t->nb[1] % 16 == 0 && t->nb[2] % 16 == 0 && t->nb[3] % 16 == 0;
+}
+
+// I32 [N, S] with contiguous rows
+bool is_rows_i32(const oasr_tensor *t, int64_t N, int64_t S) {
+    return t && t->type == OASR_TYPE_I32 && t->data && t->ne[0] == N && t->ne[1] == S && t->ne[2] == 1 && t->ne[3] == 1 &&
+           (t->nb[0] == 4 || N <= 1) && t->nb[1] % 4 == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_tensor *q_norm, const oasr_tensor *k_norm,
+                           float eps, const oasr_tensor *rope, const oasr_tensor *pos, const oasr_tensor *page_table,
+                           const oasr_tensor *n_past, const oasr_tensor *n_nodes, oasr_tensor *q, oasr_tensor *k_pages,
+                           oasr_tensor *v_pages) {
+    int st = oasr_internal_precheck(be);
+    if (st) return st;
+    const char *op = "qk_norm_rope";
+    if (!qkv || !q) return fail_op(be, op, "null argument");
+    NormRope a = {};
+    KvPages p;
+    KvSeqs sq;
+    st = pages_check(be, op, k_pages, v_pages, 1, &p);
+    if (st) return st;
+    const int64_t D = k_pages->ne[0], HKV = k_pages->ne[2], N = qkv->ne[2], S = qkv->ne[3], H = qkv->ne[1] - 2 * HKV;
+    if (qkv->type != OASR_TYPE_F32 || qkv->ne[0] != D || H < 1 || H % HKV || H > 65535)
+        return fail_op(be, op, "qkv must be F32 [D, H + 2 * H_kv, n, n_seq] with H a multiple of H_kv");
+    if ((q->type != OASR_TYPE_F32 && q->type != OASR_TYPE_F16) || q->ne[0] != D || q->ne[1] != H || q->ne[2] != N || q->ne[3] != S)
+        return fail_op(be, op, "q must be F32 or F16 [D, H, n, n_seq]");
+    for (const oasr_tensor *w : {q_norm, k_norm})
+        if (w && (w->type != OASR_TYPE_F32 || !w->data || w->ne[0] != D || w->ne[1] != 1 || w->ne[2] != 1 || w->ne[3] != 1 ||
+                  w->nb[0] != 4))
+            return fail_op(be, op, "q_norm and k_norm must be F32 [D]");
+    if ((q_norm || k_norm) && !(eps >= 0.0f)) return fail_op(be, op, "eps must not be negative");
+    if (rope && (rope->type != OASR_TYPE_F32 || !rope->data || rope->ne[0] != 2 || rope->ne[1] != D / 2 || rope->ne[2] < 1 ||
+                 rope->ne[2] > INT32_MAX || rope->ne[3] != 1 || rope->nb[0] != 4 || rope->nb[1] != 8 ||
+                 (rope->nb[2] != 4 * D && rope->ne[2] > 1) || ((uintptr_t)rope->data & 7)))
+        return fail_op(be, op, "rope must be contiguous F32 [2, D / 2, n_pos]");
+    if (pos && !is_rows_i32(pos, N, S)) return fail_op(be, op, "pos must be I32 [n, n_seq]");
+    if (qkv->nb[0] != 4 || q->nb[0] != (q->type == OASR_TYPE_F16 ? 2 : 4)) return fail_op(be, op, "rows must be contiguous");
+    st = seqs_check(be, op, page_table, n_past, n_nodes, S, N, &sq);
+    if (st) return st;
+    const int64_t units = S * N * qkv->ne[1];
+    if (units == 0) return OASR_STATUS_SUCCESS;
+    if (!qkv->data || !q->data) return fail_op(be, op, "null argument");
+    if (!rows16(qkv) || !rows16(q)) return fail_op(be, op, "rows must be 16-byte aligned");
+    if (units > ((int64_t)1 << 32)) return fail_op(be, op, "too many rows");
+    a.x = (const char *)qkv->data;
+    a.x_nb1 = qkv->nb[1], a.x_nb2 = qkv->nb[2], a.x_nb3 = qkv->nb[3];
+    a.q = (char *)q->data;
+    a.q_nb1 = q->nb[1], a.q_nb2 = q->nb[2], a.q_nb3 = q->nb[3];
+    a.q_norm = q_norm ? (const float *)q_norm->data : nullptr;
+    a.k_norm = k_norm ? (const float *)k_norm->data : nullptr;
+    a.rope = rope ? (const float *)rope->data : nullptr;
+    a.n_pos = rope ? (int)rope->ne[2] : 0;
+    a.pos = pos ? (const int *)pos->data : nullptr;
+    a.pos_ld = pos ? pos->nb[1] / 4 : 0;
+    a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
+    a.eps = eps;
+    const dim3 grid((unsigned)((units + 3) / 4));
+    const bool f16 = q->type == OASR_TYPE_F16;
+    cudaError_t e;
+    if (D == 128) e = f16 ? launch_k(be, qk_norm_rope_kernel<128, true>, grid, dim3(128), 0, a, p, sq, be->err_word)
+                          : launch_k(be, qk_norm_rope_kernel<128, false>, grid, dim3(128), 0, a, p, sq, be->err_word);
+    else e = f16 ? launch_k(be, qk_norm_rope_kernel<64, true>, grid, dim3(128), 0, a, p, sq, be->err_word)
+                 : launch_k(be, qk_norm_rope_kernel<64, false>, grid, dim3(128), 0, a, p, sq, be->err_word);
+    return launched(be, e, op);
+}
+
+int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages, const oasr_tensor *v_pages,
+                              const oasr_tensor *page_table, const oasr_tensor *n_past, const oasr_tensor *n_nodes,
+                              const oasr_tensor *tree, float scale, oasr_tensor *dst) {
+    int st = oasr_internal_precheck(be);
+    if (st) return st;
+    const char *op = "flash_attn_tree";
+    if (!q || !dst) return fail_op(be, op, "null argument");
+    KvPages p;
+    KvSeqs sq;
+    st = pages_check(be, op, k_pages, v_pages, 1, &p);
+    if (st) return st;
+    const int64_t D = q->ne[0], N = q->ne[1], H = q->ne[2], S = q->ne[3], HKV = k_pages->ne[2];
+    if ((q->type != OASR_TYPE_F32 && q->type != OASR_TYPE_F16) || D != k_pages->ne[0] || H < 1 || H % HKV || H > 65535)
+        return fail_op(be, op, "q must be F32 or F16 [D, n, H, n_seq] with H a multiple of H_kv");
+    if ((dst->type != OASR_TYPE_F32 && dst->type != OASR_TYPE_F16) || dst->ne[0] != D || dst->ne[1] != H || dst->ne[2] != N ||
+        dst->ne[3] != S)
+        return fail_op(be, op, "dst must be F32 or F16 [D, H, n, n_seq]");
+    if (q->nb[0] != (q->type == OASR_TYPE_F16 ? 2 : 4) || dst->nb[0] != (dst->type == OASR_TYPE_F16 ? 2 : 4))
+        return fail_op(be, op, "rows must be contiguous");
+    if (!(scale == scale)) return fail_op(be, op, "scale must be a number");
+    st = seqs_check(be, op, page_table, n_past, n_nodes, S, N, &sq);
+    if (st) return st;
+    if (tree && (tree->type != OASR_TYPE_I32 || tree->ne[0] != (N + 31) / 32 || tree->ne[1] != N || tree->ne[2] != S ||
+                 tree->ne[3] != 1 || (tree->nb[0] != 4 && tree->ne[0] > 1) || tree->nb[1] % 4 || tree->nb[2] % 4))
+        return fail_op(be, op, "tree must be I32 [ceil(n / 32), n, n_seq]");
+    if (tree && N > TREE_MAX_NODES) return fail_op(be, op, "a tree has at most 1024 nodes");
+    if (N == 0 || S == 0) return OASR_STATUS_SUCCESS;
+    if (!q->data || !dst->data || (tree && !tree->data)) return fail_op(be, op, "null argument");
+    if (!rows16(q) || !rows16(dst)) return fail_op(be, op, "rows must be 16-byte aligned");
+    TreeAttn a;
+    a.q = (const char *)q->data;
+    a.q_nb1 = q->nb[1], a.q_nb2 = q->nb[2], a.q_nb3 = q->nb[3];
+    a.dst = (char *)dst->data;
+    a.d_nb1 = dst->nb[1], a.d_nb2 = dst->nb[2], a.d_nb3 = dst->nb[3];
+    a.tree = tree ? (const int *)tree->data : nullptr;
+    a.t_nb1 = tree ? tree->nb[1] / 4 : 0, a.t_nb2 = tree ? tree->nb[2] / 4 : 0;
+    a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV, a.D = (int)D, a.W = (int)((N + 31) / 32);
+    a.scale = scale;
+    a.q_f16 = q->type == OASR_TYPE_F16, a.d_f16 = dst->type == OASR_TYPE_F16;
+    return launch_flash_attn_tree(be, a, p, sq);
+}
+
+int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oasr_tensor *parents, const oasr_tensor *target,
+                          const oasr_tensor *n_nodes, const oasr_tensor *n_past, const oasr_tensor *page_table,
+                          oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers, oasr_tensor *path,
+                          oasr_tensor *n_accept, oasr_tensor *next_token, oasr_tensor *n_past_out) {
+    int st = oasr_internal_precheck(be);
+    if (st) return st;
+    const char *op = "tree_commit";
+    if (!tokens || !n_past_out || !n_past) return fail_op(be, op, "null argument");
+    KvPages p;
+    KvSeqs sq;
+    st = pages_check(be, op, k_pages, v_pages, n_layers, &p);
+    if (st) return st;
+    const int64_t N = tokens->ne[0], S = tokens->ne[1];
+    if (N > TREE_MAX_NODES) return fail_op(be, op, "a tree has at most 1024 nodes");
+    st = seqs_check(be, op, page_table, n_past, n_nodes, S, N, &sq);
+    if (st) return st;
+    if (S == 0) return OASR_STATUS_SUCCESS;
+    if (N == 0) return fail_op(be, op, "a tree has at least one node");
+    if (!is_rows_i32(tokens, N, S) || !is_rows_i32(parents, N, S) || !is_rows_i32(target, N, S) || !is_rows_i32(path, N, S))
+        return fail_op(be, op, "tokens, parents, target and path must be I32 [n, n_seq]");
+    if (!is_vec_i32(n_accept, S) || !is_vec_i32(next_token, S) || !is_vec_i32(n_past_out, S))
+        return fail_op(be, op, "n_accept, next_token and n_past_out must be I32 [n_seq]");
+    if (n_past_out->data == n_past->data)
+        return fail_op(be, op, "n_past_out must not be n_past (it is still read while n_past_out is written)");
+    Commit a;
+    a.tokens = (const int *)tokens->data, a.tok_ld = tokens->nb[1] / 4;
+    a.parents = (const int *)parents->data, a.par_ld = parents->nb[1] / 4;
+    a.target = (const int *)target->data, a.tgt_ld = target->nb[1] / 4;
+    a.path = (int *)path->data, a.path_ld = path->nb[1] / 4;
+    a.n_accept = (int *)n_accept->data;
+    a.next = (int *)next_token->data;
+    a.n_past_out = (int *)n_past_out->data;
+    a.S = (int)S, a.L = n_layers, a.HKV = (int)k_pages->ne[2], a.D = (int)k_pages->ne[0];
+    const int64_t cols = (int64_t)a.L * 2 * a.HKV * (a.D / 8);
+    if (cols > INT32_MAX / 2) return fail_op(be, op, "too many layers");
+    a.groups = (int)((cols + 255) / 256);
+    if (S * a.groups > INT32_MAX) return fail_op(be, op, "too many sequences");
+    return launched(be, launch_k(be, tree_commit_kernel, dim3((unsigned)(S * a.groups)), dim3(256), 0, a, p, sq, be->err_word), op);
+}
+
+int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
+                            const oasr_tensor *pairs) {
+    int st = oasr_internal_precheck(be);
+    if (st) return st;
+    const char *op = "kv_pages_copy";
+    KvPages p;
+    st = pages_check(be, op, k_pages, v_pages, n_layers, &p);
+    if (st) return st;
+    if (!pairs || pairs->type != OASR_TYPE_I32 || pairs->ne[0] != 2 || pairs->ne[2] != 1 || pairs->ne[3] != 1 ||
+        pairs->nb[0] != 4 || pairs->nb[1] % 4)
+        return fail_op(be, op, "pairs must be I32 [2, n]");
+    if (pairs->ne[1] == 0) return OASR_STATUS_SUCCESS;
+    if (!pairs->data) return fail_op(be, op, "null argument");
+    const int HKV = (int)k_pages->ne[2], cpr = (int)k_pages->ne[0] / 8;
+    const int64_t total = (int64_t)HKV * p.page * cpr;
+    if (total > INT32_MAX / 2) return fail_op(be, op, "pages too large");
+    const int64_t chunks = (total + 1023) / 1024, grid = pairs->ne[1] * n_layers * 2 * chunks;
+    if (grid > INT32_MAX) return fail_op(be, op, "too many pages in one call");
+    const int64_t row = k_pages->ne[0] * 2, head = row * p.page;
+    const bool flat = p.k_nb1 == row && p.v_nb1 == row && (HKV == 1 || (p.k_nb2 == head && p.v_nb2 == head));
+    cudaError_t e;
+    if (flat) e = launch_k(be, kv_pages_copy_kernel<true>, dim3((unsigned)grid), dim3(256), 0, (const int *)pairs->data,
+                           pairs->nb[1] / 4, p, n_layers, HKV, cpr, (int)chunks, be->err_word);
+    else e = launch_k(be, kv_pages_copy_kernel<false>, dim3((unsigned)grid), dim3(256), 0, (const int *)pairs->data,
+                      pairs->nb[1] / 4, p, n_layers, HKV, cpr, (int)chunks, be->err_word);
+    return launched(be, e, op);
+}
+
+int oasr_b200_tree_mask(const int32_t *parents, int32_t n, int32_t *words) {
+    if (!parents || !words || n < 0 || n > TREE_MAX_NODES) return OASR_STATUS_FAILED;
+    const int W = (n + 31) / 32;
+    for (int i = 0; i < n; ++i) {
+        if (parents[i] >= i || parents[i] < -1) return OASR_STATUS_FAILED;  // a parent comes before its children
+        int32_t *row = words + (int64_t)i * W;
+        if (parents[i] >= 0) memcpy(row, words + (int64_t)parents[i] * W, W * 4);
+        else memset(row, 0, W * 4);
+        row[i / 32] = (int32_t)((uint32_t)row[i / 32] | 1u << (i % 32));
+    }
+    return OASR_STATUS_SUCCESS;
+}
+
+}  // extern "C"

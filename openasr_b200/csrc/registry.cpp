@@ -27,16 +27,19 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_flash_attn_causal),
     OASR_ENTRY(oasr_b200_flash_attn_ext),
     OASR_ENTRY(oasr_b200_flash_attn_ext_static),
+    OASR_ENTRY(oasr_b200_flash_attn_tree),
     OASR_ENTRY(oasr_b200_free),
     OASR_ENTRY(oasr_b200_get_proc_address),
     OASR_ENTRY(oasr_b200_get_stream),
     OASR_ENTRY(oasr_b200_init),
+    OASR_ENTRY(oasr_b200_kv_pages_copy),
     OASR_ENTRY(oasr_b200_last_error),
     OASR_ENTRY(oasr_b200_mem_stats),
     OASR_ENTRY(oasr_b200_memory_get_api_v1),
     OASR_ENTRY(oasr_b200_mul_mat),
     OASR_ENTRY(oasr_b200_mul_mat_qact),
     OASR_ENTRY(oasr_b200_props),
+    OASR_ENTRY(oasr_b200_qk_norm_rope),
     OASR_ENTRY(oasr_b200_quantize_act),
     OASR_ENTRY(oasr_b200_quantize_chunk),
     OASR_ENTRY(oasr_b200_qwen_decode_step),
@@ -57,6 +60,8 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_synchronize),
     OASR_ENTRY(oasr_b200_synchronize_ex),
     OASR_ENTRY(oasr_b200_synth_normal),
+    OASR_ENTRY(oasr_b200_tree_commit),
+    OASR_ENTRY(oasr_b200_tree_mask),
     OASR_ENTRY(oasr_b200_weight_download),
     OASR_ENTRY(oasr_b200_weight_free),
     OASR_ENTRY(oasr_b200_weight_info),
