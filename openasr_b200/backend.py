@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -362,32 +363,55 @@ def synth_normal(seed: int, n: int, mean: float = 0.0, std: float = 1.0, offset:
 
 
 # ---- tensor descriptors -----------------------------------------------------------------
-_TORCH_TYPES = None
+_TORCH_TYPES = None  # torch dtype -> (ggml type, element size), filled at the first use
+_DESC_PACK = struct.Struct("=iiQ8q").pack  # the fields of OasrTensor
+_ELEMENT = {F32: 4, F16: 2, I32: 4, I64: 8}
 
 
 def _torch_type(t) -> int:
-    import torch
+    global _TORCH_TYPES
+    if _TORCH_TYPES is None:
+        import torch
 
-    m = {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int64: I64}
-    if t.dtype not in m:
+        _TORCH_TYPES = {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int64: I64}
+    ty = _TORCH_TYPES.get(t.dtype)
+    if ty is None:
         raise UnsupportedInputs(STATUS_FAILED, f"unsupported tensor dtype {t.dtype}")
-    return m[t.dtype]
+    return ty
 
 
 def describe(t, ggml_type: int | None = None) -> OasrTensor:
-    """oasr_tensor for a torch tensor: ne = reversed shape, nb = reversed byte strides."""
-    d = OasrTensor()
-    d.type = _torch_type(t) if ggml_type is None else ggml_type
-    d.flags = 0
-    d.data = t.data_ptr()
-    shape = list(t.shape)[::-1] + [1] * (4 - t.dim())
-    es = t.element_size()
-    strides = [s * es for s in list(t.stride())[::-1]]
-    while len(strides) < 4:
-        strides.append(strides[-1] * shape[len(strides) - 1] if strides else es)
-    d.ne[:] = shape[:4]
-    d.nb[:] = strides[:4]
-    return d
+    """oasr_tensor for a torch tensor: ne = reversed shape, nb = reversed byte strides.  A
+    descriptor passes through, so a loop over static buffers can describe them once."""
+    if type(t) is OasrTensor:
+        return t
+    if ggml_type is None:
+        ggml_type = _torch_type(t)
+        es = _ELEMENT[ggml_type]
+    else:
+        es = t.element_size()
+    ne, nb = t.shape, t.stride()
+    dim = len(ne)
+    if dim == 4:
+        c3, c2, c1, c0 = ne
+        b3, b2, b1, b0 = nb
+        return OasrTensor.from_buffer_copy(
+            _DESC_PACK(ggml_type, 0, t.data_ptr(), c0, c1, c2, c3, b0 * es, b1 * es, b2 * es, b3 * es))
+    if dim == 2:
+        c1, c0 = ne
+        b1, b0 = nb
+        b1 *= es
+        return OasrTensor.from_buffer_copy(
+            _DESC_PACK(ggml_type, 0, t.data_ptr(), c0, c1, 1, 1, b0 * es, b1, b1 * c1, b1 * c1))
+    if dim == 1:
+        c0, b0 = ne[0], nb[0] * es
+        return OasrTensor.from_buffer_copy(
+            _DESC_PACK(ggml_type, 0, t.data_ptr(), c0, 1, 1, 1, b0, b0 * c0, b0 * c0, b0 * c0))
+    ne = list(ne)[::-1] + [1] * (4 - dim)
+    nb = [x * es for x in nb[::-1]]
+    while len(nb) < 4:
+        nb.append(nb[-1] * ne[len(nb) - 1] if nb else es)
+    return OasrTensor.from_buffer_copy(_DESC_PACK(ggml_type, 0, t.data_ptr(), *ne[:4], *nb[:4]))
 
 
 def _opt(t):
