@@ -4,15 +4,26 @@
 //   p < n_past[s], or p = n_past[s] + j with bit j of tree[s][i] set (no tree: j <= i);
 // a node that sees nothing, or that is padding, gets zeros.
 //
-// K and V are read once per tile of rows and dominate the traffic, so the G query heads of a
-// K/V head and all nodes of a sequence share a tile.  The kernel below takes tiles of 16 or 32
-// rows with warp-level matrix instructions (m16n8k16): at 64 positions of D = 128 an SM's share
-// of the HBM rate allows about 1400 clocks, and 16 rows need 256 instructions.
+// K and V dominate the traffic, so the G query heads of a K/V head and the nodes of a sequence
+// share a tile of R = 16, 32, 64 or 128 rows and one read of K and V.  The rows are few, the
+// positions many: both products run on the tcgen05 tensor cores with the long side as M,
+//   S^T (128 positions x R) = K (128 x D) . Q^T        both operands as they lie (K-major)
+//   O^T (D x R)             = V^T (D x 128) . P^T      V as it lies (M-major), P as written
+// so no row of the matrix unit is padding, K and V are used in the layout of the pages, and the
+// work of the softmax threads -- one per position, R weights each -- shrinks with R.
 //
-// A producer warp streams units of 64 positions of K and V into a ring by TMA (one box per run
-// of positions within a page, 128-byte swizzle); of four consumer warps per 16 rows each takes
-// 16 of the 64 positions with a running maximum, sum and output of its own, and the four are
-// joined at the end of a segment.
+// f32 accuracy from 16-bit operands: an f32 query (after a power of two that brings the tile's
+// largest value to 2^8) and every weight are two f16 halves, hi + lo, 22 bits; both go through
+// the same product, added in the f32 accumulator.  A unit's O^T is added to the running output
+// in registers, because the tensor cores cut off the bits below a large accumulator.
+//
+// Softmax: a weight is 2^(s - off), off = (a maximum seen before) - 7.  As long as no score
+// exceeds off by more than 15, f16 holds the weight and nothing is rescaled; one vote of the 128
+// threads per unit decides, and only then are the true maxima found and the sums rescaled.
+//
+// CTA: per 64 rows (or all of them) a group of 4 softmax warps, one TMA warp that streams K and
+// V tiles of 128 positions (boxes that end with the pages) through a ring, one MMA warp.  S^T of
+// the next unit is computed while this one's weights are; every wait is bounded.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -21,57 +32,109 @@
 
 namespace oasr {
 
-template <int D_, int RT_>
-struct TreeMma {
-    static constexpr int D = D_, RT = RT_;
-    static constexpr int M = 16 * RT;             // rows per tile
-    static constexpr int NS = 3;                  // units in flight
-    static constexpr int HALF = TREE_BKV * 128;   // 64 positions x 64 values
-    static constexpr int KBYTES = HALF * (D / 64);
-    static constexpr int STAGE = 2 * KBYTES;      // K, then V
-    static constexpr int CW = 4 * RT;             // consumer warps
-    static constexpr int NT = 32 * (CW + 1);
-    static constexpr int OFF_ML = NS * STAGE;     // [CW][16] (max, sum)
-    static constexpr int OFF_BAR = OFF_ML + CW * 16 * 8;
-    static constexpr int OFF_MISC = OFF_BAR + 2 * NS * 8;
-    static constexpr int SMEM = OFF_MISC + 16;
-    static constexpr int PART = M * (D + 2);      // floats of an unfinished segment
-    static_assert(4 * 16 * D * 4 == STAGE, "the outputs of four warps fit the stage they were read from");
+template <int D_, int RW_, int NWG_, bool QF16_>
+struct TreeTc {
+    static constexpr int D = D_, RW = RW_, NWG = NWG_, R = RW * NWG;
+    static constexpr bool QF16 = QF16_;
+    static constexpr int HALF = TREE_BKV * 128;          // 128 positions x 64 values
+    static constexpr int TILE = HALF * (D / 64);         // one K or V tile
+    static constexpr int QHALF = R * 128;                // R rows x 64 values
+    static constexpr int QBYTES = QHALF * (D / 64);      // Q hi (lo follows for f32 queries)
+    static constexpr int PBYTES = TREE_BKV * R * 2;      // P hi, then lo
+    static constexpr int CTAS = R == 16 ? 2 : 1;
+    static constexpr int MISC = CTAS == 2 ? 1024 : 3072;
+    static constexpr int FIXED = QBYTES * (QF16 ? 1 : 2) + 2 * PBYTES + MISC;
+    static constexpr int MOST = (CTAS == 2 ? 115712 : 232448) - FIXED;
+    static constexpr int NS = MOST / TILE > 8 ? 8 : MOST / TILE;  // tiles in flight
+    static_assert(NS >= 3, "K of the next unit and K, V of this one");
+    static constexpr int OFF_Q = NS * TILE;
+    static constexpr int OFF_P = OFF_Q + QBYTES * (QF16 ? 1 : 2);
+    static constexpr int OFF_MISC = OFF_P + 2 * PBYTES;
+    // misc: off[R], see[NWG][4][RW], barriers, flags
+    static constexpr int OFF_SEE = OFF_MISC + 4 * R;
+    static constexpr int OFF_BAR = OFF_SEE + 16 * R;
+    static constexpr int NBAR = 2 * NS + 6;
+    static constexpr int OFF_FLAG = OFF_BAR + 8 * NBAR;
+    static constexpr int SMEM = OFF_MISC + MISC;
+    static_assert(OFF_FLAG + 32 <= SMEM, "misc");
+    static constexpr int SW = 4 * NWG;                   // softmax warps
+    static constexpr int NT = 32 * (SW + 2);
+    static constexpr int TMEM = 4 * R < 32 ? 32 : 4 * R; // S twice, O twice
+    static constexpr int PART = R * (D + 2);             // floats of an unfinished segment
+    static constexpr bool JOINS = R == 16;               // the last CTA joins them (else fattn_tree_join_kernel)
 };
 
-static __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
+constexpr float TREE_MOST = 15.0f;  // weights up to 2^15 stay below f16's 65504
+
+// K-major operand, 128-byte swizzle: sw128_desc.  M- or N-major operand in the same swizzle
+// (64 values of M contiguous per position): 8-position groups 1024 bytes apart, 64-value blocks
+// `block` bytes apart.
+static __device__ __forceinline__ uint64_t mn_sw128_desc(uint32_t addr, uint32_t block) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
 }
-static __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
+// N-major operand without swizzle: 8 x 8 blocks of 128 bytes (8 values of N contiguous, 8
+// positions), `kgroup` bytes to the next 8 positions, `nblock` to the next 8 values of N.
+static __device__ __forceinline__ uint64_t mn_plain_desc(uint32_t addr, uint32_t kgroup, uint32_t nblock) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(kgroup >> 4) << 16;
+    d |= (uint64_t)(nblock >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    return d;
 }
-static __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// any of the group's 128 threads
+static __device__ __forceinline__ bool group_any(int id, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"((uint32_t)x)
+        : "memory");
+    return r != 0;
 }
+static __device__ __forceinline__ void group_sync(int id, int threads) {
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+static __device__ __forceinline__ float warp_max_f32(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+// lane l gets the sum over the lanes of v[l] (N = 16: lanes l and l + 16 both)
 template <int N>
-static __device__ __forceinline__ void consumers_sync() {
-    asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
-}
-// halves that are infinite or NaN to zero; `bad` notes that there were some
-static __device__ __forceinline__ uint32_t finite2(uint32_t x, uint32_t &bad) {
-    const uint32_t m = __vcmpeq2(x & 0x7C007C00u, 0x7C007C00u);
-    bad |= m;
-    return x & ~m;
+static __device__ __forceinline__ float lane_sums(float (&v)[N]) {
+    const int lane = threadIdx.x & 31;
+    if (N == 16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+    }
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float keep = up ? v[i + o] : v[i], give = up ? v[i] : v[i + o];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+    return v[0];
 }
 
-template <int D, int RT, bool QF16>
-__global__ void __launch_bounds__(TreeMma<D, RT>::NT, RT == 1 ? 2 : 1)
-    fattn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, TreeAttn a,
-                      KvPages p, KvSeqs sq, int box, int least, float *parts, unsigned int *tickets, int *err) {
-    using C = TreeMma<D, RT>;
+template <int D, int RW, int NWG, bool QF16>
+__global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NWG, QF16>::CTAS)
+    fattn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const __grid_constant__ TreeAttn a, const __grid_constant__ KvPages p,
+                      const __grid_constant__ KvSeqs sq, int box, int least, float *parts, unsigned int *tickets, int *err) {
+    using C = TreeTc<D, RW, NWG, QF16>;
+    constexpr int R = C::R, NS = C::NS;
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
     griddep_wait();
@@ -79,319 +142,454 @@ __global__ void __launch_bounds__(TreeMma<D, RT>::NT, RT == 1 ? 2 : 1)
         if (threadIdx.x == 0) atomicOr(err, ERR_BAD_SHAPE);
         return;
     }
-    uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + C::NS;
-    volatile int *abort_flag = (volatile int *)(smem + C::OFF_MISC);
-    unsigned int *s_bad = (unsigned int *)(smem + C::OFF_MISC + 4);
-    int *s_last = (int *)(smem + C::OFF_MISC + 8);
+    float *s_off = (float *)(smem + C::OFF_MISC);
+    uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + NS;
+    uint64_t *s_full = empty + NS /* [2] */, *p_full = s_full + 2, *o_full = p_full + 1, *q_full = o_full + 1,
+             *done = q_full + 1;
+    volatile int *abort_flag = (volatile int *)(smem + C::OFF_FLAG);
+    uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_FLAG + 4);
+    unsigned int *s_bad = (unsigned int *)(smem + C::OFF_FLAG + 8);
+    int *s_last = (int *)(smem + C::OFF_FLAG + 12);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.H / a.HKV;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::NS; ++i) {
+        for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], C::CW);
+            mbar_init(&empty[i], 1);
         }
+        mbar_init(&s_full[0], 1);
+        mbar_init(&s_full[1], 1);
+        mbar_init(p_full, 128 * NWG);
+        mbar_init(o_full, 1);
+        mbar_init(q_full, 128 * NWG);
+        mbar_init(done, 1);
         *abort_flag = 0;
         *s_bad = 0;
         fence_mbar_init();
     }
-    TreeUnits w;
-    w.total = tree_count(a, sq, p.page, C::M, err);
-    w.ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, w.total / least));
-    const int64_t u0 = (int)blockIdx.x < w.ctas ? tree_start(w, blockIdx.x) : 0;
-    const int64_t u1 = (int)blockIdx.x < w.ctas ? tree_start(w, blockIdx.x + 1) : 0;
+    if (warp == C::SW + 1) tmem_alloc(tmem_slot, C::TMEM);
+    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
+    const int u0 = tree_start(w, blockIdx.x), u1 = tree_start(w, blockIdx.x + 1);
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;  // S at columns 0 and R, O at 2 R and 3 R
 
-    if (warp == C::CW) {
-        // ---- producer: lane = (box, half of D, K or V) ----
-        constexpr int PER = 2 * (D / 64);  // copies per box
-        const int boxes = TREE_BKV / box;
-        const int b = lane / PER, half = lane / 2 % (D / 64), kv = lane & 1;
-        const bool mine = b < boxes;
-        const CUtensorMap *map = kv ? &tm_v : &tm_k;
-        int64_t it = 0;
-        for (int64_t u = u0; u < u1;) {
-            const TreeSeg g = tree_locate(a, sq, p.page, C::M, u, u1);
+    if (warp == C::SW) {
+        // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
+        constexpr int HALVES = D / 64;
+        const int b = lane / HALVES, half = lane % HALVES;
+        const bool mine = b < TREE_BKV / box;
+        int q = 0;  // tiles issued
+        for (int u = u0; u < u1;) {
+            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
             const int *row = sq.table + g.s * sq.table_ld;
-            for (int k = g.k0; k < g.k1; ++k, ++it) {
-                // positions past the end read page n_pages: zeros
+            auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
                 const int t = k * TREE_BKV + b * box;
                 int pg = p.n_pages;
                 if (mine && t < g.T) {
-                    pg = __ldg(row + t / p.page);
+                    pg = __ldg(row + a.page(t));
                     if (pg < 0 || pg >= p.n_pages) {
                         atomicOr(err, ERR_BAD_INDEX);
                         pg = p.n_pages;
                     }
                 }
-                const int slot = (int)(it % C::NS);
-                if (!mbar_wait(&empty[slot], (uint32_t)(it / C::NS & 1) ^ 1u, abort_flag, err)) continue;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::STAGE);
-                __syncwarp();
-                if (mine)
-                    tma_load_4d(smem + slot * C::STAGE + kv * C::KBYTES + half * C::HALF + b * box * 128, map, &full[slot],
-                                64 * half, t % p.page, g.hk, pg);
-                __syncwarp();
-            }
-            u = g.first + g.k1;
-        }
-        // copies still in flight when the consumers gave up land before the block ends
-        if (*abort_flag)
-            for (int i = 0; i < C::NS; ++i) {
-                const long long t0 = clock64();
-                const uint32_t ph = (uint32_t)((it + C::NS - 1 - i) / C::NS & 1) ^ 1u;
-                while (!mbar_try_wait(&full[i], ph) && clock64() - t0 < (1LL << 24)) {
+                return pg;
+            };
+            auto issue = [&](const CUtensorMap *map, int k, int pg) {
+                const int slot = q % NS;
+                if (mbar_wait(&empty[slot], (uint32_t)(q / NS & 1) ^ 1u, abort_flag, err)) {
+                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::TILE);
+                    __syncwarp();
+                    if (mine)
+                        tma_load_4d(smem + slot * C::TILE + half * C::HALF + b * box * 128, map, &full[slot], 64 * half,
+                                    k * TREE_BKV + b * box - a.page(k * TREE_BKV + b * box) * p.page, g.hk, pg);
+                    ++q;
                 }
+                __syncwarp();
+            };
+            int pg = page_of(g.k0);
+            issue(&tm_k, g.k0, pg);
+            for (int k = g.k0; k < g.k1; ++k) {
+                const int next = k + 1 < g.k1 ? page_of(k + 1) : 0;
+                if (k + 1 < g.k1) issue(&tm_k, k + 1, next);
+                issue(&tm_v, k, pg);
+                pg = next;
             }
-        return;
-    }
-
-    // ---- consumers ----
-    tree_zero_padding(a, sq, p.page, (int64_t)blockIdx.x * C::CW + warp, (int64_t)gridDim.x * C::CW);
-    const int kg = warp & 3, rl = warp >> 2;  // 16 positions of the unit, 16 rows of the tile
-    const int gr = lane >> 2, c = lane & 3;   // fragment row and column pair
-    float2 *s_ml = (float2 *)(smem + C::OFF_ML);
-    int64_t it = 0;
-    for (int64_t u = u0; u < u1;) {
-        const TreeSeg g = tree_locate(a, sq, p.page, C::M, u, u1);
-        const int R = g.n * G;
-        // Q fragments: rows r0 and r0 + 8; f32 queries as two f16 halves after a power of two
-        // that brings the row's largest value to 2^8
-        const int r0 = g.rt * C::M + 16 * rl + gr;
-        uint32_t qh[D / 16][4], ql[QF16 ? 1 : D / 16][4];
-        float sc[2];
+            u = g.next;
+        }
+        // every copy lands before the block ends, also when the others gave up
+        for (int i = max(0, q - NS); i < q; ++i) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
+            }
+        }
+    } else if (warp == C::SW + 1) {
+        // ---- MMA ----
+        constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, R);
+        constexpr uint32_t id_o = idesc_f16_f32(D, R) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
+        int q = 0, it = 0, seg = 0;
+        bool ok = true;
+        for (int u = u0; u < u1; ++seg) {
+            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
+            if (lane == 0) {
+                const int n = g.k1 - g.k0;
+                auto scores = [&](int j) {
+                    const int slot = q % NS;
+                    ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t kb = smem_u32(smem + slot * C::TILE), qb = smem_u32(smem + C::OFF_Q);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int r = r0 + 8 * x;
-            const bool in = r < R;
-            const char *qr = a.q + (in ? r / G : 0) * a.q_nb1 + (g.hk * G + (in ? r % G : 0)) * a.q_nb2 + g.s * a.q_nb3;
-            sc[x] = a.scale * 1.4426950408889634f;
+                    for (int part = 0; part < (QF16 ? 1 : 2); ++part)
+#pragma unroll
+                        for (int x = 0; x < D / 16; ++x)
+                            umma_f16(tmem + (uint32_t)(j & 1) * R, sw128_desc(kb + (x >> 2) * C::HALF) + 2 * (x & 3),
+                                     sw128_desc(qb + part * C::QBYTES + (x >> 2) * C::QHALF) + 2 * (x & 3), id_s, part + x != 0);
+                    umma_commit(&s_full[j & 1]);
+                    umma_commit(&empty[slot]);
+                    ++q;
+                };
+                ok = ok && mbar_wait(q_full, (uint32_t)seg & 1u, abort_flag, err);
+                scores(it);
+                for (int j = it; j < it + n; ++j) {
+                    // S buffer (j + 1) & 1 was read before the weights of unit j - 1 were complete
+                    if (j + 1 < it + n) scores(j + 1);
+                    const int slot = q % NS;
+                    ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
+                    ok = ok && mbar_wait(p_full, (uint32_t)j & 1u, abort_flag, err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t vb = smem_u32(smem + slot * C::TILE), pb = smem_u32(smem + C::OFF_P);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int x = 0; x < TREE_BKV / 16; ++x)
+                            umma_f16(tmem + (uint32_t)(2 + (j & 1)) * R, mn_sw128_desc(vb + x * 2048, D == 128 ? C::HALF : 16),
+                                     mn_plain_desc(pb + part * C::PBYTES + x * 256, 128, TREE_BKV * 16), id_o, part + x != 0);
+                    umma_commit(o_full);
+                    umma_commit(&empty[slot]);
+                    ++q;
+                }
+                it += n;
+            }
+            __syncwarp();
+            u = g.next;
+        }
+        if (lane == 0) {
+            umma_commit(done);
+            const long long t0 = clock64();
+            while (!mbar_try_wait(done, 0) && clock64() - t0 < kMbarWaitLimit) {
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = position for the weights, = value of D for the output ----
+        tree_zero_padding(a, sq, p.page, (int64_t)blockIdx.x * C::SW + warp, (int64_t)gridDim.x * C::SW);
+        const int wg = warp / 4, tid = threadIdx.x & 127;
+        const int row0 = wg * RW;                                  // the group's first row of the tile
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + row0;
+        // D = 64 products fill 16 of a warp's 32 lanes
+        const int d = D == 128 ? tid : 16 * (warp & 3) + lane;
+        const bool has_d = D == 128 || lane < 16;
+        float *off = s_off + row0;
+        uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0 + (warp & 3) * RW;  // this warp's positions, by row
+        // the group's part of P, while it is free: maxima and sums [4][RW], then the output rows,
+        // RW / 2 in the place of the high halves and RW / 2 in that of the low ones
+        uint8_t *own_p = smem + C::OFF_P + row0 / 8 * (TREE_BKV * 16);
+        float *red = (float *)own_p, *fac = red;
+        int it = 0, q = 0;
+        for (int u = u0; u < u1;) {
+            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
+            const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
+            // -- Q: 16 bytes of f16 per thread and step --
+            float c = a.scale * 1.4426950408889634f;
+            constexpr int QC = RW * (D / 8) / 128;  // chunks of 8 values per thread
+            uint8_t *qs = smem + C::OFF_Q;
+            auto q_row = [&](int r) -> const char * {
+                const int gr = g.rt * R + row0 + r, node = a.group(gr);
+                return a.q + node * a.q_nb1 + (g.hk * G + gr - node * G) * a.q_nb2 + g.s * a.q_nb3;
+            };
             if (QF16) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    qh[k][x] = in ? *reinterpret_cast<const uint32_t *>(qr + 2 * (16 * k + 2 * c)) : 0u;
-                    qh[k][x + 2] = in ? *reinterpret_cast<const uint32_t *>(qr + 2 * (16 * k + 8 + 2 * c)) : 0u;
+                for (int x = 0; x < QC; ++x) {
+                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < live) v = *reinterpret_cast<const uint4 *>(q_row(r) + 16 * ch);
+                    *reinterpret_cast<uint4 *>(qs + (ch >> 3) * C::QHALF + sw128_off(row0 + r, ch & 7)) = v;
                 }
             } else {
-                float2 v[D / 8];
                 float m = 0.0f;
+                float4 v[2 * QC];
 #pragma unroll
-                for (int k = 0; k < D / 8; ++k) {
-                    v[k] = in ? *reinterpret_cast<const float2 *>(qr + 4 * (8 * k + 2 * c)) : make_float2(0.0f, 0.0f);
-                    m = fmaxf(m, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
+                for (int x = 0; x < QC; ++x) {
+                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+                    v[2 * x] = v[2 * x + 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (r < live) {
+                        v[2 * x] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
+                        v[2 * x + 1] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
+                    }
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[2 * x].x), fabsf(v[2 * x].y)), fmaxf(fabsf(v[2 * x].z), fabsf(v[2 * x].w))));
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[2 * x + 1].x), fabsf(v[2 * x + 1].y)),
+                                       fmaxf(fabsf(v[2 * x + 1].z), fabsf(v[2 * x + 1].w))));
                 }
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                // exponents of the factor 2^(8 - e) and of its inverse, both in the normal range
-                const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-                const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-                sc[x] *= __uint_as_float((uint32_t)(127 + e - 8) << 23);
+                m = warp_max_f32(m);
+                if (lane == 0) red[warp & 3] = m;
+                group_sync(1 + wg, 128);
+                m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+                // 2^(8 - e) and its inverse, both in the normal range
+                const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
+                const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
+                c *= __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    tree_split2(v[2 * k].x * up, v[2 * k].y * up, qh[k][x], ql[k][x]);
-                    tree_split2(v[2 * k + 1].x * up, v[2 * k + 1].y * up, qh[k][x + 2], ql[k][x + 2]);
+                for (int x = 0; x < QC; ++x) {
+                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+                    uint4 hi, lo;
+                    tree_split2(v[2 * x].x * up, v[2 * x].y * up, hi.x, lo.x);
+                    tree_split2(v[2 * x].z * up, v[2 * x].w * up, hi.y, lo.y);
+                    tree_split2(v[2 * x + 1].x * up, v[2 * x + 1].y * up, hi.z, lo.z);
+                    tree_split2(v[2 * x + 1].z * up, v[2 * x + 1].w * up, hi.w, lo.w);
+                    uint8_t *dst = qs + (ch >> 3) * C::QHALF + sw128_off(row0 + r, ch & 7);
+                    *reinterpret_cast<uint4 *>(dst) = hi;
+                    *reinterpret_cast<uint4 *>(dst + C::QBYTES) = lo;
                 }
             }
-        }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-        float o[D / 8][4];
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        uint32_t bad = 0;
-
-        for (int k = g.k0; k < g.k1; ++k, ++it) {
-            const int slot = (int)(it % C::NS);
-            const bool tail = (k + 1) * TREE_BKV > g.past;  // some of the positions are nodes, or past the end
-            uint32_t see[2] = {0xffffu, 0xffffu};
-            if (tail) {
-                see[0] = tree_sees(a, g, r0 / G, k * TREE_BKV + 16 * kg);
-                see[1] = tree_sees(a, g, (r0 + 8) / G, k * TREE_BKV + 16 * kg);
-            }
-            if (mbar_wait(&full[slot], (uint32_t)(it / C::NS & 1), abort_flag, err)) {
-                const uint32_t kb = smem_u32(smem + slot * C::STAGE), vb = kb + C::KBYTES;
-                // S = Q K^T: two 8-position tiles, the 16-bit halves of Q in accumulators of their own
-                float s[2][2][4] = {};
-                const int kr = 16 * kg + (lane & 7) + 8 * (lane >> 4);  // this lane's row of the K matrices
-#pragma unroll
-                for (int x = 0; x < D / 16; ++x) {
-                    // matrices: positions 0-7 x values 0-7, 8-15; positions 8-15 x values 0-7, 8-15
-                    uint32_t f[4];
-                    ldsm4(f, kb + (x / 4) * C::HALF + sw128_off(kr, (x & 3) * 2 + (lane >> 3 & 1)));
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        mma16816(s[t][QF16 ? x & 1 : 0], qh[x], f[2 * t], f[2 * t + 1]);
-                        if (!QF16) mma16816(s[t][1], ql[x], f[2 * t], f[2 * t + 1]);
-                    }
-                }
-                float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int x = e >> 1;
-                        float v = (s[t][0][e] + s[t][1][e]) * sc[x];
-                        if (tail && !(see[x] >> (8 * t + 2 * c + (e & 1)) & 1u)) v = -INFINITY;
-                        s[t][0][e] = v;
-                        mx[x] = fmaxf(mx[x], v);
-                    }
-                float f[2], off[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                    mx[x] = fmaxf(mx[x], m[x]);
-                    off[x] = mx[x] == -INFINITY ? 0.0f : mx[x] - TREE_WEIGHT_EXP;
-                    f[x] = mx[x] == -INFINITY ? 1.0f : tree_exp2(m[x] - mx[x]);
-                    m[x] = mx[x];
-                    l[x] *= f[x];
-                }
-                uint32_t ph[4], pl[4];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const float p0 = tree_exp2(s[t][0][2 * x] - off[x]), p1 = tree_exp2(s[t][0][2 * x + 1] - off[x]);
-                        l[x] += p0 + p1;
-                        tree_split2(p0, p1, ph[2 * t + x], pl[2 * t + x]);
-                    }
-                // O = f O + P V, the product of this unit in accumulators of its own: the tensor
-                // cores cut the bits below a large running sum off, an f32 multiply-add rounds
-                const int vr = 16 * kg + (lane & 15);
-                uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-                if (tail) {  // positions past the end hold anything
-                    const int left = g.T - (k * TREE_BKV + 16 * kg + 2 * c);
-                    keep0 = left >= 2 ? 0xffffffffu : left == 1 ? 0xffffu : 0u;
-                    keep1 = left >= 10 ? 0xffffffffu : left == 9 ? 0xffffu : 0u;
-                }
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) {
-                    // matrices: positions 0-7, 8-15 x values 0-7; the same x values 8-15
-                    uint32_t v[4];
-                    ldsm4_t(v, vb + (j / 4) * C::HALF + sw128_off(vr, (j & 3) * 2 + (lane >> 4)));
-                    if (tail) {
-                        v[0] = finite2(v[0] & keep0, bad);
-                        v[1] = finite2(v[1] & keep1, bad);
-                        v[2] = finite2(v[2] & keep0, bad);
-                        v[3] = finite2(v[3] & keep1, bad);
-                    }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        float d[4] = {};
-                        mma16816(d, ph, v[2 * t], v[2 * t + 1]);
-                        mma16816(d, pl, v[2 * t], v[2 * t + 1]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[2 * j + t][e] = fmaf(o[2 * j + t][e], f[e >> 1], d[e]);
-                    }
-                }
-            }
-            if (k + 1 < g.k1) {  // the last one is kept for the join below
-                fence_proxy_async_smem();  // these reads before the copy that refills the stage
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[slot]);
-            }
-        }
-
-        // ---- join the four warps of each 16 rows, 16 rows at a time through the last stage ----
-        uint8_t *last = smem + (int)((it - 1) % C::NS) * C::STAGE;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-            if (c == 0) s_ml[warp * 16 + gr + 8 * x] = make_float2(m[x], l[x]);
-        }
-        if (bad) atomicOr(s_bad, 1u);
-        consumers_sync<32 * C::CW>();
-        const bool anybad = *s_bad != 0;
-        const bool whole = g.k0 == 0 && g.k1 == g.kt;
-        float *part = parts + tree_slot(w, blockIdx.x, g.first) * C::PART;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {  // this warp's factor for its rows
-            const int r = gr + 8 * x;
-            float M = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[(rl * 4 + i) * 16 + r].x);
-            const float f = m[x] == -INFINITY ? 0.0f : tree_exp2(m[x] - M);
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-                o[j][2 * x] *= f;
-                o[j][2 * x + 1] *= f;
-            }
-        }
-#pragma unroll
-        for (int pass = 0; pass < RT; ++pass) {
-            if (rl == pass) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int j = 0; j < D / 8; ++j) {
-                        const int r = gr + 8 * x, ch = (2 * j + (c >> 1)) ^ gr;  // 16-byte pieces spread over the banks
-                        *reinterpret_cast<float2 *>(last + (((kg * 16 + r) * D + 4 * ch) * 4 + 8 * (c & 1))) =
-                            make_float2(o[j][2 * x], o[j][2 * x + 1]);
-                    }
-            }
-            consumers_sync<32 * C::CW>();
-            if (threadIdx.x == 0) *s_bad = 0;  // everybody has read it
-            for (int e = threadIdx.x; e < 16 * (D / 4); e += 32 * C::CW) {
-                const int r = e / (D / 4), ch = e % (D / 4);
-                const int gl = g.rt * C::M + 16 * pass + r;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float M = -INFINITY, L = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[(pass * 4 + i) * 16 + r].x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 ml = s_ml[(pass * 4 + i) * 16 + r];
-                    L += ml.x == -INFINITY ? 0.0f : ml.y * tree_exp2(ml.x - M);
-                    const float4 x = *reinterpret_cast<const float4 *>(last + ((i * 16 + r) * D + 4 * (ch ^ (r & 7))) * 4);
-                    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-                }
-                if (anybad && gl < R) v = tree_nonfinite4(a, p, sq, g, gl / G, 4 * ch, v);
-                if (whole) {
-                    if (gl < R) {
-                        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                        tree_store4(a, g.s, g.hk * G + gl % G, gl / G, 4 * ch, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                    }
-                } else {
-                    *reinterpret_cast<float4 *>(part + (16 * pass + r) * D + 4 * ch) = v;
-                    if (ch == 0) *reinterpret_cast<float2 *>(part + C::M * D + 2 * (16 * pass + r)) = make_float2(M, L);
-                }
-            }
+            if (tid < RW) off[tid] = -INFINITY;
             fence_proxy_async_smem();
-            consumers_sync<32 * C::CW>();
-        }
-        if (lane == 0) mbar_arrive(&empty[(it - 1) % C::NS]);
+            mbar_arrive(q_full);
+            group_sync(1 + wg, 128);
 
-        // ---- the last of the CTAs that share the item joins their parts in order ----
-        if (!whole) {
-            const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.kt - 1);
-            if (threadIdx.x == 0) {
-                const bool is_last = atom_add_acq_rel_gpu(tickets + c0, 1u) == (unsigned)(c1 - c0);
-                if (is_last) atomicExch(tickets + c0, 0u);
-                *s_last = is_last;
-            }
-            consumers_sync<32 * C::CW>();
-            if (*s_last) {
-                for (int e = threadIdx.x; e < C::M * (D / 4); e += 32 * C::CW) {
-                    const int r = e / (D / 4), ch = e % (D / 4), gl = g.rt * C::M + r;
-                    if (gl >= R) continue;
-                    float M = -INFINITY, L = 0.0f;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int x = c0; x <= c1; ++x)
-                        M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(parts + tree_slot(w, x, g.first) * C::PART + C::M * D) + r).x);
-                    for (int x = c0; x <= c1; ++x) {
-                        const float *pt = parts + tree_slot(w, x, g.first) * C::PART;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pt + C::M * D) + r);
-                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(pt + r * D) + ch);
-                        const float f = ml.x == -INFINITY ? 0.0f : tree_exp2(ml.x - M);
-                        L = fmaf(ml.y, f, L);
-                        v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y);
-                        v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+            float o[RW], l[RW];
+#pragma unroll
+            for (int r = 0; r < RW; ++r) o[r] = l[r] = 0.0f;
+            // O^T of unit j from TMEM to the running output
+            auto drain = [&](int j) {
+                mbar_wait(o_full, (uint32_t)j & 1u, abort_flag, err);
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < RW / 16; ++x) {
+                    uint32_t v[16];
+                    tmem_ld16(tl + (uint32_t)(2 + (j & 1)) * R + 16 * x, v);
+                    tmem_ld_wait(v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[16 * x + i] += __uint_as_float(v[i]);
+                }
+            };
+            const int n = g.k1 - g.k0, it0 = it;
+            for (int k = g.k0; k < g.k1; ++k, ++it) {
+                const int t = k * TREE_BKV + tid;             // this thread's position
+                const bool tail = (k + 1) * TREE_BKV > g.past;  // nodes among the positions, or the end
+                if (tail) {
+                    group_sync(1 + wg, 128);  // the last unit's bits have been read
+                    for (int e = tid; e < 4 * RW; e += 128) {
+                        const int r = e % RW, t0 = k * TREE_BKV + e / RW * 32;
+                        ((uint32_t *)(smem + C::OFF_SEE) + 4 * row0)[e] =
+                            r < live ? tree_sees32(a, g, a.group(g.rt * R + row0 + r), t0) : 0u;
                     }
-                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                    tree_store4(a, g.s, g.hk * G + gl % G, gl / G, 4 * ch, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                    group_sync(1 + wg, 128);
+                }
+                mbar_wait(&s_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, err);
+                tc_fence_after();
+                const uint32_t ts = tl + (uint32_t)(it & 1) * R;
+                // 16 scores minus their offsets
+                auto load16 = [&](int x, float (&z)[16]) {
+                    uint32_t v[16];
+                    tmem_ld16(ts + 16 * x, v);
+                    tmem_ld_wait(v);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(off + 16 * x + i);
+                        z[i] = fmaf(__uint_as_float(v[i]), c, -f.x);
+                        z[i + 1] = fmaf(__uint_as_float(v[i + 1]), c, -f.y);
+                        z[i + 2] = fmaf(__uint_as_float(v[i + 2]), c, -f.z);
+                        z[i + 3] = fmaf(__uint_as_float(v[i + 3]), c, -f.w);
+                    }
+                    if (tail) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (!(see[16 * x + i] >> lane & 1u)) z[i] = -INFINITY;
+                    }
+                };
+                float z[16], top = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < RW / 16; ++x) {
+                    load16(x, z);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, z[i]);
+                }
+                const bool fresh = it == it0;
+                if (group_any(1 + wg, top > TREE_MOST)) {
+                    // -- new maxima: of the unit's 128 positions, then with what was --
+                    if (!fresh) drain(it - 1);
+#pragma unroll
+                    for (int x = 0; x < RW / 16; ++x) {
+                        uint32_t v[16];
+                        tmem_ld16(ts + 16 * x, v);
+                        tmem_ld_wait(v);
+                        float keep = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float y = __uint_as_float(v[i]) * c;
+                            if (tail && !(see[16 * x + i] >> lane & 1u)) y = -INFINITY;
+                            y = warp_max_f32(y);
+                            if (lane == i) keep = y;
+                        }
+                        if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = keep;
+                    }
+                    group_sync(1 + wg, 128);
+                    if (tid < RW) {
+                        const float old = off[tid];
+                        const float m = fmaxf(fmaxf(red[tid], red[RW + tid]), fmaxf(red[2 * RW + tid], red[3 * RW + tid]));
+                        const float now = fmaxf(old, m - TREE_EXP);
+                        off[tid] = now;
+                        fac[tid] = now == -INFINITY ? 1.0f : tree_exp2(old - now);
+                    }
+                    group_sync(1 + wg, 128);
+#pragma unroll
+                    for (int r = 0; r < RW; r += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(fac + r);
+                        o[r] *= f.x; o[r + 1] *= f.y; o[r + 2] *= f.z; o[r + 3] *= f.w;
+                        l[r] *= f.x; l[r + 1] *= f.y; l[r + 2] *= f.z; l[r + 3] *= f.w;
+                    }
+                    group_sync(1 + wg, 128);  // the factors lie where the weights go
+                    if (RW == 16) load16(0, z);
+                } else if (!fresh) {
+                    drain(it - 1);  // also: P of the last unit has been read
+                }
+                // -- weights: 16 bytes per 8 rows into the N-major P tiles --
+#pragma unroll
+                for (int x = 0; x < RW / 16; ++x) {
+                    if (RW != 16) load16(x, z);
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float p0 = tree_exp2(z[i]), p1 = tree_exp2(z[i + 1]);
+                        l[16 * x + i] += p0;
+                        l[16 * x + i + 1] += p1;
+                        tree_split2(p0, p1, hi[i / 2], lo[i / 2]);
+                    }
+                    uint8_t *dst = smem + C::OFF_P + (row0 / 8 + 2 * x) * (TREE_BKV * 16) + tid * 16;
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(dst + TREE_BKV * 16) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                    *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    *reinterpret_cast<uint4 *>(dst + C::PBYTES + TREE_BKV * 16) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                }
+                if (tail && wg == 0) {
+                    // values past the end, infinite or NaN would make NaN of zero weights
+                    const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
+                    mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
+                    uint8_t *vt = smem + qi % NS * C::TILE;
+#pragma unroll
+                    for (int ch = 0; ch < D / 8; ++ch) {
+                        uint4 *at = reinterpret_cast<uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
+                        const uint4 v = *at;
+                        uint4 m;
+                        m.x = __vcmpeq2(v.x & 0x7C007C00u, 0x7C007C00u), m.y = __vcmpeq2(v.y & 0x7C007C00u, 0x7C007C00u);
+                        m.z = __vcmpeq2(v.z & 0x7C007C00u, 0x7C007C00u), m.w = __vcmpeq2(v.w & 0x7C007C00u, 0x7C007C00u);
+                        if (m.x | m.y | m.z | m.w) {
+                            *at = make_uint4(v.x & ~m.x, v.y & ~m.y, v.z & ~m.z, v.w & ~m.w);
+                            if (t < g.T) *s_bad = 1u;
+                        }
+                    }
+                }
+                tc_fence_before();
+                fence_proxy_async_smem();
+                mbar_arrive(p_full);
+            }
+            drain(it - 1);
+            tc_fence_before();
+            q += 2 * n;
+
+            // -- sums of the weights over the group's positions --
+#pragma unroll
+            for (int x = 0; x < RW / 16; ++x) {
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = l[16 * x + i];
+                const float sum = lane_sums<16>(v);
+                if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = sum;
+            }
+            group_sync(1 + wg, 128);
+            const bool whole = g.k0 == 0 && g.k1 == g.kt;
+            float *part = parts + (int64_t)tree_slot(w, blockIdx.x, g.first) * C::PART;
+            if (tid < RW) {
+                const float L = (red[tid] + red[RW + tid]) + (red[2 * RW + tid] + red[3 * RW + tid]);
+                if (!whole) reinterpret_cast<float2 *>(part + R * D)[row0 + tid] = make_float2(off[tid], L);
+                off[tid] = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
+            }
+            // V was cleaned by the first group for both
+            group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
+            const bool anybad = *(volatile unsigned int *)s_bad != 0;
+            // -- the output through shared memory: rows in a loop, 16 bytes at a time --
+            if (has_d) {
+#pragma unroll
+                for (int r = 0; r < RW; ++r)
+                    reinterpret_cast<float *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * D + d] = o[r];
+            }
+            group_sync(1 + wg, 128);
+            for (int e = tid; e < min(RW, live) * (D / 4); e += 128) {
+                const int r = e / (D / 4), ch = e % (D / 4);
+                const int gr = g.rt * R + row0 + r, node = a.group(gr);
+                float4 x = reinterpret_cast<const float4 *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * (D / 4) + ch];
+                if (anybad) x = tree_nonfinite4(a, p, sq, g, node, 4 * ch, x);
+                const float f = off[r];
+                x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+                if (whole) tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch, x);
+                else *reinterpret_cast<float4 *>(part + (row0 + r) * D + 4 * ch) = x;
+            }
+            // -- one small tile: the last of the CTAs that share the item joins the parts here --
+            if (C::JOINS && !whole) {
+                const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.kt - 1);
+                group_sync(1, 128);
+                if (threadIdx.x == 0) {
+                    const bool is_last = atom_add_acq_rel_gpu(tickets + c0, 1u) == (unsigned)(c1 - c0);
+                    if (is_last) atomicExch(tickets + c0, 0u);
+                    *s_last = is_last;
+                }
+                group_sync(1, 128);
+                if (*(volatile int *)s_last) {
+                    for (int e = threadIdx.x; e < min(R, live) * (D / 4); e += 128) {
+                        const int r = e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
+                        tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch,
+                                    tree_join4(w, parts, C::PART, R, D, g.first, c0, c1, r, ch));
+                    }
                 }
             }
+            u = g.next;
+            if (u < u1) {  // the next segment reuses the flag, the sums, P and Q
+                group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
+                if (threadIdx.x == 0) *s_bad = 0;
+                group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
+            }
         }
-        u = g.first + g.k1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == C::SW + 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM);
+    }
+}
+
+// Joins the items that several CTAs of fattn_tree_kernel shared: block (c, rows) takes 16 rows of
+// the item whose last unit of CTA c's range is not the item's last.
+template <int D, int R>
+__global__ void __launch_bounds__(128) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, KvSeqs sq, int page,
+                                                              int ctas, int least, const float *parts) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const TreeUnits w = tree_count(a, sq, page, R, least, ctas, nullptr);
+    const int c0 = blockIdx.x / (R / 16), r0 = blockIdx.x % (R / 16) * 16;
+    const int end = tree_start(w, c0 + 1);
+    if (c0 + 1 >= w.ctas || end <= tree_start(w, c0)) return;
+    const TreeSeg g = tree_locate(a, sq, page, R, end - 1, w.total);
+    const int live = g.n * a.group.d - g.rt * R - r0;
+    if (g.k1 - 1 == g.k0 || live <= 0 || tree_owner(w, g.first) != c0) return;  // ends here, or began before
+    const int c1 = tree_owner(w, g.first + g.kt - 1);
+    for (int e = threadIdx.x; e < min(16, live) * (D / 4); e += 128) {
+        const int r = r0 + e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
+        tree_store4(a, g.s, g.hk * a.group.d + gr - node * a.group.d, node, 4 * ch,
+                    tree_join4(w, parts, R * (D + 2), R, D, g.first, c0, c1, r, ch));
     }
 }
 
@@ -417,43 +615,60 @@ bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int RT, bool QF16>
-static int launch_tree_mma(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s, const CUtensorMap &mk,
-                           const CUtensorMap &mv, int box) {
-    using C = TreeMma<D, RT>;
-    static std::atomic<bool> attr_set{false};
-    if (!attr_set) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(fattn_tree_kernel<D, RT, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-        if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
-        attr_set = true;
-    }
-    const int64_t rts = ((int64_t)s.N * (a.H / a.HKV) + C::M - 1) / C::M;
-    const int64_t most = rts * a.HKV * a.S * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * (RT == 1 ? 2 : 1)));
-    int st = 0;
-    float *parts = (float *)oasr_internal_scratch(be, (size_t)grid * 2 * C::PART * 4, &st);
-    if (st) return st;
-    const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RT, QF16>, dim3(grid), dim3(C::NT), C::SMEM, mk, mv, a, p, s, box,
-                                   1, parts, be->counters, be->err_word);
-    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
-    return oasr_internal_launch_check(be, "flash_attn_tree");
-}
-
-int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s) {
+template <int D, int RW, int NWG, bool QF16>
+static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvSeqs &s) {
+    using C = TreeTc<D, RW, NWG, QF16>;
     // the longest run of positions, up to a unit, that never crosses a page
     const int box = std::min(TREE_BKV, p.page & -p.page);
     CUtensorMap mk, mv;
     if (!tree_page_map(&mk, p.k, p.k_nb1, p.k_nb2, p.k_nb3, a.D, p.page, a.HKV, p.n_pages, box) ||
         !tree_page_map(&mv, p.v, p.v_nb1, p.v_nb2, p.v_nb3, a.D, p.page, a.HKV, p.n_pages, box))
         return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: the pages' strides make no tensor map");
-    const bool two = (int64_t)s.N * (a.H / a.HKV) > 16;
-#define FT(DD, RR, Q) \
-    if (a.D == DD && two == (RR == 2) && a.q_f16 == Q) return launch_tree_mma<DD, RR, Q>(be, a, p, s, mk, mv, box)
-    FT(64, 1, false); FT(64, 1, true); FT(64, 2, false); FT(64, 2, true);
-    FT(128, 1, false); FT(128, 1, true); FT(128, 2, false); FT(128, 2, true);
+    static std::atomic<bool> attr_set{false};
+    if (!attr_set) {
+        const cudaError_t e = cudaFuncSetAttribute(fattn_tree_kernel<D, RW, NWG, QF16>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
+        attr_set = true;
+    }
+    const int least = 1;
+    a.group = FastDiv(a.H / a.HKV);
+    a.page = FastDiv(p.page);
+    a.by_item = (int64_t)s.MP * p.page <= 4 * TREE_BKV;
+    const int64_t tiles = ((int64_t)s.N * (a.H / a.HKV) + C::R - 1) / C::R;
+    const int64_t most = tiles * a.HKV * a.S * (a.by_item ? 1 : ((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
+    if (most > INT32_MAX / 2 || (int64_t)s.N * (a.H / a.HKV) > INT32_MAX / 2)
+        return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * C::CTAS));
+    int st = 0;
+    float *parts = (float *)oasr_internal_scratch(be, (size_t)grid * 2 * C::PART * 4, &st);
+    if (st) return st;
+    const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RW, NWG, QF16>, dim3(grid), dim3(C::NT), C::SMEM, mk, mv, a, p, s,
+                                   box, least, parts, be->counters, be->err_word);
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
+    if (!C::JOINS && !a.by_item && grid > 1) {
+        // started while the attention still runs; it waits for its end
+        const bool pdl = be->pdl;
+        be->pdl = true;
+        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 16)), dim3(128), 0, a, s, p.page,
+                                        grid, least, (const float *)parts);
+        be->pdl = pdl;
+        if (je != cudaSuccess) return oasr_internal_cuda_fail(be, je, "flash_attn_tree join launch", __LINE__);
+    }
+    return oasr_internal_launch_check(be, "flash_attn_tree");
+}
+
+int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s) {
+    // the smallest tile that takes all rows of a K/V head, so that K and V are read once
+    const int64_t rows = (int64_t)s.N * (a.H / a.HKV);
+#define FT(RW, NWG)                                                                                      \
+    if (rows <= RW * NWG || RW * NWG == 128) {                                                           \
+        if (a.D == 64) return a.q_f16 ? launch_tree<64, RW, NWG, true>(be, a, p, s) : launch_tree<64, RW, NWG, false>(be, a, p, s); \
+        return a.q_f16 ? launch_tree<128, RW, NWG, true>(be, a, p, s) : launch_tree<128, RW, NWG, false>(be, a, p, s);              \
+    }
+    FT(16, 1) FT(32, 1) FT(64, 1) FT(64, 2)
 #undef FT
-    return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: head_dim must be 64 or 128");
+    return OASR_STATUS_FAILED;
 }
 
 }  // namespace oasr

@@ -1,14 +1,14 @@
-// fattn_tree.cuh -- what the two tree-attention kernels share: how the work is split over the
-// CTAs, which nodes a row sees, and where unfinished sums wait to be joined.
+// fattn_tree.cuh -- around the tree attention's inner loop: how the work is split over the CTAs,
+// which nodes a row sees, and where unfinished sums wait to be joined.
 //
-// Work is counted in units: 64 positions of one (sequence, K/V head, tile of M rows), a row
-// being one query head of one node (row = node * G + head in the group).  The lengths are in
-// device memory, so every warp counts the units itself and CTA c of C takes the units
-// [c T / C, (c + 1) T / C): ragged batches balance without the host knowing them, and one long
-// sequence spreads over all SMs.  A CTA's range is a list of segments, each within one
-// (sequence, head, tile); a segment that is not the whole of it leaves (max, sum, output) in
-// the scratch, and the CTA that arrives last joins the parts in the order of the positions, so
-// the bits do not depend on the order of arrival.
+// Work is counted in units: 128 positions of one item, an item being (sequence, K/V head, tile of
+// R rows) and a row one query head of one node (row = node * G + head in the group).  The lengths
+// are in device memory, so every warp counts the units itself and each CTA takes an equal run of
+// them: ragged batches balance without the host knowing them, and one long sequence spreads over
+// all SMs.  A CTA's range is a list of segments, each within one item; a segment that is not the
+// whole of it leaves (maximum, sum, output) in the scratch, and the parts are joined in the order
+// of the positions, so the bits do not depend on which CTA came first.  Where the page table has
+// room for a few units only, the runs are of whole items instead: nothing is left to join.
 #pragma once
 
 #include "pages.cuh"
@@ -16,104 +16,122 @@
 
 namespace oasr {
 
-constexpr int TREE_BKV = 64;  // positions per unit
+constexpr int TREE_BKV = 128;  // positions per unit
 
 struct TreeSeg {
     int s, hk, rt;         // sequence, K/V head, row tile
     int past, n, T, kt;    // committed positions, live nodes, past + n, units of the item
     int k0, k1;            // units of this segment
-    int64_t first;         // the item's first unit, counted from the call's first
+    int first, next;       // the item's first unit, and where this segment ends, counted from the call's first
 };
 
+// T units shared by C CTAs: the first `more` take q + 1 units, the others q.
 struct TreeUnits {
-    int64_t total;  // T above
-    int ctas;       // C above
+    int total, ctas, q, more;
 };
 
-// units of sequence s
-static __device__ __forceinline__ int64_t tree_seq_units(const KvSeqs &q, int s, int page, int G, int HKV, int M,
-                                                         bool &ok) {
-    int past, n;
-    ok = seq_lengths(q, s, page, past, n);
+// Lane l of every warp: lengths of sequence s0 + l, its units and items (below 2^31: the launch
+// checks).  Runs of whole items count the items.
+static __device__ __forceinline__ int tree_lane_units(const TreeAttn &a, const KvSeqs &q, int page, int R, int s, int &past,
+                                                      int &n, bool &ok) {
+    ok = true;
+    past = n = 0;
+    if (s < a.S) ok = seq_lengths(q, s, page, past, n);
     if (n == 0) return 0;
-    return (int64_t)((n * G + M - 1) / M) * HKV * ((past + n + TREE_BKV - 1) / TREE_BKV);
+    return (n * a.group.d + R - 1) / R * a.HKV * (a.by_item ? 1 : (past + n + TREE_BKV - 1) / TREE_BKV);
 }
 
-// All warps: the call's units.  A sequence with lengths out of range counts none (reported).
-static __device__ __forceinline__ int64_t tree_count(const TreeAttn &a, const KvSeqs &q, int page, int M, int *err) {
-    const int lane = threadIdx.x & 31, G = a.H / a.HKV;
-    int64_t sum = 0;
-    for (int s = lane; s < a.S; s += 32) {
+// All warps: the call's units and their split; a CTA gets at least `least` units where there are
+// that many.  A sequence with lengths out of range counts none (reported).
+static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int least,
+                                                       int ctas, int *err) {
+    const int lane = threadIdx.x & 31;
+    int sum = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 32) {
+        int past, n;
         bool ok;
-        sum += tree_seq_units(q, s, page, G, a.HKV, M, ok);
-        if (!ok && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
+        sum += tree_lane_units(a, q, page, R, s0 + lane, past, n, ok);
+        if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+    TreeUnits w;
+    w.total = __reduce_add_sync(0xffffffffu, sum);
+    w.ctas = max(1, min(ctas, w.total / least));
+    w.q = w.total / w.ctas;
+    w.more = w.total - w.q * w.ctas;
+    return w;
+}
+
+static __device__ __forceinline__ int tree_start(const TreeUnits &w, int c) {
+    return c >= w.ctas ? w.total : c * w.q + min(c, w.more);
+}
+// the CTA whose range holds unit u
+static __device__ __forceinline__ int tree_owner(const TreeUnits &w, int u) {
+    const int big = w.more * (w.q + 1);
+    return u < big ? u / (w.q + 1) : w.more + (u - big) / w.q;
+}
+// A CTA leaves at most two unfinished segments: its first (slot 2c) and its last (2c + 1).
+static __device__ __forceinline__ int tree_slot(const TreeUnits &w, int c, int item_first) {
+    return 2 * c + (item_first > tree_start(w, c) ? 1 : 0);
 }
 
 // All lanes: the segment that starts at unit u (u < total) and ends before `end`.
-static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, int page, int M, int64_t u,
-                                                      int64_t end) {
-    const int lane = threadIdx.x & 31, G = a.H / a.HKV;
-    int64_t base = 0;
+static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, int page, int R, int u, int end) {
+    const int lane = threadIdx.x & 31;
+    int base = 0;
     TreeSeg g = {};
     for (int s0 = 0; s0 < a.S; s0 += 32) {
+        int past, n;
         bool ok;
-        const int64_t mine = s0 + lane < a.S ? tree_seq_units(q, s0 + lane, page, G, a.HKV, M, ok) : 0;
-        int64_t run = mine;  // inclusive prefix sum over the lanes
+        const int mine = tree_lane_units(a, q, page, R, s0 + lane, past, n, ok);
+        int run = mine;  // inclusive prefix sum over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, run, o);
+            const int up = __shfl_up_sync(0xffffffffu, run, o);
             if (lane >= o) run += up;
         }
-        const int64_t all = __shfl_sync(0xffffffffu, run, 31);
-        if (u < base + all) {
-            const int l = __ffs(__ballot_sync(0xffffffffu, u < base + run)) - 1;
+        const unsigned hit = __ballot_sync(0xffffffffu, u < base + run);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
             g.first = __shfl_sync(0xffffffffu, base + run - mine, l);
+            g.past = __shfl_sync(0xffffffffu, past, l);
+            g.n = __shfl_sync(0xffffffffu, n, l);
             g.s = s0 + l;
             break;
         }
-        base += all;
+        base += __shfl_sync(0xffffffffu, run, 31);
     }
-    seq_lengths(q, g.s, page, g.past, g.n);
     g.T = g.past + g.n;
     g.kt = (g.T + TREE_BKV - 1) / TREE_BKV;
-    const int rts = (g.n * G + M - 1) / M;
-    const int item = (int)((u - g.first) / g.kt);
+    const int rts = (g.n * a.group.d + R - 1) / R, per = a.by_item ? 1 : g.kt;
+    const int item = (u - g.first) / per;
     g.hk = item / rts;
-    g.rt = item % rts;
-    g.first += (int64_t)item * g.kt;
-    g.k0 = (int)(u - g.first);
-    g.k1 = (int)min((int64_t)g.kt, end - g.first);
+    g.rt = item - g.hk * rts;
+    g.first += item * per;
+    g.next = min(g.first + per, end);
+    g.k0 = a.by_item ? 0 : u - g.first;
+    g.k1 = a.by_item ? g.kt : g.next - g.first;
     return g;
 }
 
-static __device__ __forceinline__ int64_t tree_start(const TreeUnits &w, int64_t c) { return c * w.total / w.ctas; }
-// the CTA whose range holds unit u
-static __device__ __forceinline__ int tree_owner(const TreeUnits &w, int64_t u) {
-    return (int)(((u + 1) * w.ctas - 1) / w.total);
-}
-// A CTA leaves at most two unfinished segments: its first (slot 2c) and its last (2c + 1).
-static __device__ __forceinline__ int64_t tree_slot(const TreeUnits &w, int c, int64_t item_first) {
-    return 2 * (int64_t)c + (item_first > tree_start(w, c) ? 1 : 0);
+// Whether the row of a live node sees position t < T.
+static __device__ __forceinline__ bool tree_sees(const TreeAttn &a, const TreeSeg &g, int node, int t) {
+    const int j = t - g.past;
+    if (j < 0) return true;
+    return a.tree ? (uint32_t)__ldg(a.tree + g.s * a.t_nb2 + node * a.t_nb1 + (j >> 5)) >> (j & 31) & 1u : j <= node;
 }
 
-// Which of the positions t0 .. t0 + 31 the row of node `node` sees, as bits: all committed
-// positions, and the nodes of its words (or the nodes up to itself).
-static __device__ __forceinline__ uint32_t tree_sees(const TreeAttn &a, const TreeSeg &g, int node, int t0) {
-    const int j = t0 - g.past;  // node number of bit 0
-    if (node >= g.n || j >= g.n) return j < 0 && node < g.n ? 0xffffffffu : 0u;
+// Which of the positions t0 .. t0 + 31 it sees, as bits (positions past the end: none).
+static __device__ __forceinline__ uint32_t tree_sees32(const TreeAttn &a, const TreeSeg &g, int node, int t0) {
+    const int j = t0 - g.past, live = g.n - j;  // node number of bit 0, and where the nodes end
+    if (j <= -32) return 0xffffffffu;
+    if (live <= 0) return 0u;
     uint32_t w;
     if (!a.tree) {
         const int c = node + 1 - j;
         w = c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1u;
     } else {
         const int *row = a.tree + g.s * a.t_nb2 + node * a.t_nb1;
-        if (j <= -32) {
-            w = 0u;
-        } else if (j < 0) {
+        if (j < 0) {
             w = (uint32_t)__ldg(row) << -j;
         } else {
             const int i = j >> 5, sh = j & 31;
@@ -121,10 +139,8 @@ static __device__ __forceinline__ uint32_t tree_sees(const TreeAttn &a, const Tr
             if (sh && i + 1 < a.W) w |= (uint32_t)__ldg(row + i + 1) << (32 - sh);
         }
     }
-    const int live = g.n - j;  // nodes end here
     if (live < 32) w &= (1u << live) - 1u;
-    if (j < 0) w |= j <= -32 ? 0xffffffffu : (1u << -j) - 1u;
-    return w;
+    return j < 0 ? w | ((1u << -j) - 1u) : w;
 }
 
 // Rows of padding nodes of every sequence: zeros.  Each of the `warps` warps of the grid, this
@@ -164,29 +180,24 @@ static __device__ __forceinline__ void tree_store4(const TreeAttn &a, int s, int
 // and come back here, for the rows that see them.
 static __device__ __noinline__ float4 tree_nonfinite4(const TreeAttn &a, const KvPages &p, const KvSeqs &q, const TreeSeg &g,
                                                       int node, int c, float4 o) {
-    float *f = reinterpret_cast<float *>(&o);
     for (int t = max(g.k0, g.past / TREE_BKV) * TREE_BKV; t < min(g.k1 * TREE_BKV, g.T); ++t) {
-        if (!(tree_sees(a, g, node, t) & 1u)) continue;
+        if (!tree_sees(a, g, node, t)) continue;
         const int pg = q.table[g.s * q.table_ld + t / p.page];
         if (pg < 0 || pg >= p.n_pages) continue;
-        const __half *v =
-            reinterpret_cast<const __half *>(p.v + pg * p.v_nb3 + g.hk * p.v_nb2 + t % p.page * p.v_nb1) + c;
+        const char *v = p.v + pg * p.v_nb3 + g.hk * p.v_nb2 + t % p.page * p.v_nb1;
         for (int x = 0; x < 4; ++x) {
-            const float y = __half2float(v[x]);
-            if (!isfinite(y)) f[x] += y;
+            const float y = __half2float(reinterpret_cast<const __half *>(v)[c + x]);
+            if (!isfinite(y)) (x == 0 ? o.x : x == 1 ? o.y : x == 2 ? o.z : o.w) += y;
         }
     }
     return o;
 }
 
-// 2^x, and the power of two that the weights carry: 2^15 times the weight keeps both 16-bit
-// halves of a weight of 2^-20 exact to 2^-22 (f16 ends at 65504 and thins out below 2^-14).
 static __device__ __forceinline__ float tree_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-constexpr float TREE_WEIGHT_EXP = 15.0f;
 
 // x = hi + lo, both f16: 22 bits of an f32
 static __device__ __forceinline__ void tree_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
@@ -195,6 +206,40 @@ static __device__ __forceinline__ void tree_split2(float x, float y, uint32_t &h
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// The parts of an item in CTAs c0 .. c1, joined at row r and the four columns from 4 ch: each part
+// is R rows of D sums, then R pairs (maximum, sum of weights).
+static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const float *parts, int size, int R, int D, int first,
+                                                    int c0, int c1, int r, int ch) {
+    float M = -INFINITY, L = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int U = 6;  // parts loaded before any is used
+    for (int x = c0; x <= c1; x += U) {
+        float2 ml[U];
+        float4 y[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            ml[i] = make_float2(-INFINITY, 0.0f);
+            y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (x + i <= c1) {
+                const float *pt = parts + (int64_t)tree_slot(w, x + i, first) * size;
+                ml[i] = __ldcg(reinterpret_cast<const float2 *>(pt + R * D) + r);
+                y[i] = __ldcg(reinterpret_cast<const float4 *>(pt + r * D) + ch);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (ml[i].x == -INFINITY) continue;  // nothing seen
+            const float m = fmaxf(M, ml[i].x), f = tree_exp2(M - m), k = tree_exp2(ml[i].x - m);
+            L = fmaf(L, f, ml[i].y * k);
+            v.x = fmaf(v.x, f, y[i].x * k); v.y = fmaf(v.y, f, y[i].y * k);
+            v.z = fmaf(v.z, f, y[i].z * k); v.w = fmaf(v.w, f, y[i].w * k);
+            M = m;
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
 }
 
 // 4-D tensor map over pages [D, page, H_kv, n_pages]: boxes of 64 values x `rows` positions,

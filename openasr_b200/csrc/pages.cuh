@@ -46,6 +46,22 @@ int pages_check(oasr_backend *be, const char *op, const oasr_tensor *k, const oa
 int seqs_check(oasr_backend *be, const char *op, const oasr_tensor *table, const oasr_tensor *n_past,
                const oasr_tensor *n_nodes, int64_t S, int64_t N, KvSeqs *out);
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994): with s =
+// ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, n / d = (mulhi(n, m) + n) >> s.
+struct FastDiv {
+    uint32_t m;
+    int s, d;
+    FastDiv() = default;
+    explicit FastDiv(int div) : d(div) {
+        for (s = 0; (1ll << s) < div; ++s) {
+        }
+        m = (uint32_t)((((1ull << s) - (uint64_t)div) << 32) / (uint64_t)div + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
+    }
+};
+
 // attention of N nodes per sequence over the pages (fattn_tree.cu)
 struct TreeAttn {
     const char *q;
@@ -57,6 +73,8 @@ struct TreeAttn {
     int S, H, HKV, D, W;
     float scale;
     bool q_f16, d_f16;
+    FastDiv group, page;          // H / HKV, positions per page
+    bool by_item;                 // whole (sequence, K/V head, row tile) items per CTA
 };
 int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s);
 
