@@ -36,19 +36,25 @@ template <int D_, int RW_, int NWG_, bool QF16_>
 struct TreeTc {
     static constexpr int D = D_, RW = RW_, NWG = NWG_, R = RW * NWG;
     static constexpr bool QF16 = QF16_;
+    // up to 32 rows the halves of Q, and those of P, are 2 R columns of one product (half the
+    // instructions: at these sizes an instruction costs the same for 32 columns as for 16);
+    // beyond that they are two products into the same R columns
+    static constexpr bool WIDE = R <= 32;
+    static constexpr int SCOLS = WIDE && !QF16 ? 2 * R : R, OCOLS = WIDE ? 2 * R : R;
     static constexpr int HALF = TREE_BKV * 128;          // 128 positions x 64 values
     static constexpr int TILE = HALF * (D / 64);         // one K or V tile
-    static constexpr int QHALF = R * 128;                // R rows x 64 values
-    static constexpr int QBYTES = QHALF * (D / 64);      // Q hi (lo follows for f32 queries)
+    static constexpr int QROWS = QF16 ? R : 2 * R;       // rows of Q hi, then of Q lo
+    static constexpr int QHALF = QROWS * 128;            // they x 64 values
+    static constexpr int QBYTES = QHALF * (D / 64);
     static constexpr int PBYTES = TREE_BKV * R * 2;      // P hi, then lo
-    static constexpr int CTAS = R == 16 ? 2 : 1;
+    static constexpr int CTAS = NWG == 1 ? 2 : 1;
     static constexpr int MISC = CTAS == 2 ? 1024 : 3072;
-    static constexpr int FIXED = QBYTES * (QF16 ? 1 : 2) + 2 * PBYTES + MISC;
+    static constexpr int FIXED = QBYTES + 2 * PBYTES + MISC;
     static constexpr int MOST = (CTAS == 2 ? 115712 : 232448) - FIXED;
     static constexpr int NS = MOST / TILE > 8 ? 8 : MOST / TILE;  // tiles in flight
     static_assert(NS >= 3, "K of the next unit and K, V of this one");
     static constexpr int OFF_Q = NS * TILE;
-    static constexpr int OFF_P = OFF_Q + QBYTES * (QF16 ? 1 : 2);
+    static constexpr int OFF_P = OFF_Q + QBYTES;
     static constexpr int OFF_MISC = OFF_P + 2 * PBYTES;
     // misc: off[R], see[NWG][4][RW], barriers, flags
     static constexpr int OFF_SEE = OFF_MISC + 4 * R;
@@ -58,10 +64,14 @@ struct TreeTc {
     static constexpr int SMEM = OFF_MISC + MISC;
     static_assert(OFF_FLAG + 32 <= SMEM, "misc");
     static constexpr int SW = 4 * NWG;                   // softmax warps
-    static constexpr int NT = 32 * (SW + 2);
-    static constexpr int TMEM = 4 * R < 32 ? 32 : 4 * R; // S twice, O twice
+    // 64 rows per thread want more than the 168 registers that 10 warps leave: the other two
+    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 216 + 4 x 72)
+    static constexpr bool MOVE_REGS = RW == 64;
+    static constexpr int NT = 32 * (SW + (MOVE_REGS ? 4 : 2));
+    static constexpr int COLS = 2 * SCOLS + 2 * OCOLS;   // S twice, O twice
+    static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int PART = R * (D + 2);             // floats of an unfinished segment
-    static constexpr bool JOINS = R == 16;               // the last CTA joins them (else fattn_tree_join_kernel)
+    static constexpr bool JOINS = R <= 32;               // the last CTA joins them (else fattn_tree_join_kernel)
 };
 
 constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
@@ -88,6 +98,23 @@ static __device__ __forceinline__ uint64_t mn_plain_desc(uint32_t addr, uint32_t
     d |= (uint64_t)(nblock >> 4) << 32;
     d |= (uint64_t)1u << 46;
     return d;
+}
+static __device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// N columns of this warp's 32 lanes (16 at a time, one wait)
+template <int N>
+static __device__ __forceinline__ void tmem_load(uint32_t addr, f32x2 (&v)[N / 2]) {
+    uint32_t r[N / 16][16];
+#pragma unroll
+    for (int x = 0; x < N / 16; ++x) tmem_ld16(addr + 16 * x, r[x]);
+    // the first wait is for all; the others keep the uses of their registers behind it
+#pragma unroll
+    for (int x = 0; x < N / 16; ++x) tmem_ld_wait(r[x]);
+#pragma unroll
+    for (int x = 0; x < N / 2; ++x) v[x] = pack2(__uint_as_float(r[x / 8][2 * (x % 8)]), __uint_as_float(r[x / 8][2 * (x % 8) + 1]));
 }
 // any of the group's 128 threads
 static __device__ __forceinline__ bool group_any(int id, bool x) {
@@ -150,8 +177,9 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_FLAG + 4);
     unsigned int *s_bad = (unsigned int *)(smem + C::OFF_FLAG + 8);
     int *s_last = (int *)(smem + C::OFF_FLAG + 12);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int G = a.H / a.HKV;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int G = a.group.d;
+    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 1);
@@ -168,87 +196,98 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         fence_mbar_init();
     }
     if (warp == C::SW + 1) tmem_alloc(tmem_slot, C::TMEM);
-    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
+    if (warp == C::SW && lane < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &tm_v : &tm_k) : "memory");
     const int u0 = tree_start(w, blockIdx.x), u1 = tree_start(w, blockIdx.x + 1);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;  // S at columns 0 and R, O at 2 R and 3 R
+    const uint32_t tmem = *tmem_slot, tm_s = tmem, tm_o = tmem + 2 * C::SCOLS;
 
-    if (warp == C::SW) {
-        // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
-        constexpr int HALVES = D / 64;
-        const int b = lane / HALVES, half = lane % HALVES;
-        const bool mine = b < TREE_BKV / box;
-        int q = 0;  // tiles issued
-        for (int u = u0; u < u1;) {
-            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
-            const int *row = sq.table + g.s * sq.table_ld;
-            auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
-                const int t = k * TREE_BKV + b * box;
-                int pg = p.n_pages;
-                if (mine && t < g.T) {
-                    pg = __ldg(row + a.page(t));
-                    if (pg < 0 || pg >= p.n_pages) {
-                        atomicOr(err, ERR_BAD_INDEX);
-                        pg = p.n_pages;
+    if (warp >= C::SW) {
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == C::SW) {
+            // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
+            constexpr int HALVES = D / 64;
+            const int b = lane / HALVES, half = lane % HALVES;
+            const bool mine = b < TREE_BKV / box;
+            int q = 0;  // tiles issued
+            for (int u = u0; u < u1;) {
+                const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
+                const int *row = sq.table + g.s * sq.table_ld;
+                auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
+                    const int t = k * TREE_BKV + b * box;
+                    int pg = p.n_pages;
+                    if (mine && t < g.T) {
+                        pg = __ldg(row + a.page(t));
+                        if (pg < 0 || pg >= p.n_pages) {
+                            atomicOr(err, ERR_BAD_INDEX);
+                            pg = p.n_pages;
+                        }
                     }
-                }
-                return pg;
-            };
-            auto issue = [&](const CUtensorMap *map, int k, int pg) {
-                const int slot = q % NS;
-                if (mbar_wait(&empty[slot], (uint32_t)(q / NS & 1) ^ 1u, abort_flag, err)) {
-                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::TILE);
+                    return pg;
+                };
+                auto issue = [&](const CUtensorMap *map, int k, int pg) {
+                    const int slot = q % NS, t = k * TREE_BKV + b * box;
+                    if (mbar_wait(&empty[slot], (uint32_t)(q / NS & 1) ^ 1u, abort_flag, err)) {
+                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::TILE);
+                        __syncwarp();
+                        if (mine)
+                            tma_load_4d(smem + slot * C::TILE + half * C::HALF + b * box * 128, map, &full[slot], 64 * half,
+                                        t - a.page(t) * p.page, g.hk, pg);
+                        ++q;
+                    }
                     __syncwarp();
-                    if (mine)
-                        tma_load_4d(smem + slot * C::TILE + half * C::HALF + b * box * 128, map, &full[slot], 64 * half,
-                                    k * TREE_BKV + b * box - a.page(k * TREE_BKV + b * box) * p.page, g.hk, pg);
-                    ++q;
+                };
+                int pg = page_of(g.k0);
+                issue(&tm_k, g.k0, pg);
+                for (int k = g.k0; k < g.k1; ++k) {
+                    const int next = k + 1 < g.k1 ? page_of(k + 1) : 0;
+                    if (k + 1 < g.k1) issue(&tm_k, k + 1, next);
+                    issue(&tm_v, k, pg);
+                    pg = next;
                 }
-                __syncwarp();
-            };
-            int pg = page_of(g.k0);
-            issue(&tm_k, g.k0, pg);
-            for (int k = g.k0; k < g.k1; ++k) {
-                const int next = k + 1 < g.k1 ? page_of(k + 1) : 0;
-                if (k + 1 < g.k1) issue(&tm_k, k + 1, next);
-                issue(&tm_v, k, pg);
-                pg = next;
+                u = g.next;
             }
-            u = g.next;
-        }
-        // every copy lands before the block ends, also when the others gave up
-        for (int i = max(0, q - NS); i < q; ++i) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
+            // every copy lands before the block ends, also when the others gave up
+            for (int i = max(0, q - NS); i < q; ++i) {
+                const long long t0 = clock64();
+                while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
+                }
             }
-        }
-    } else if (warp == C::SW + 1) {
-        // ---- MMA ----
-        constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, R);
-        constexpr uint32_t id_o = idesc_f16_f32(D, R) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
-        int q = 0, it = 0, seg = 0;
-        bool ok = true;
-        for (int u = u0; u < u1; ++seg) {
-            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
-            if (lane == 0) {
+        } else if (warp == C::SW + 1) {
+            // ---- MMA: the warp stays together, one elected lane issues ----
+            constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, C::SCOLS);
+            constexpr uint32_t id_o = idesc_f16_f32(D, C::OCOLS) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
+            const uint64_t dk = sw128_desc(smem_u32(smem)), dq = sw128_desc(smem_u32(smem + C::OFF_Q));
+            const uint64_t dv = mn_sw128_desc(smem_u32(smem), D == 128 ? C::HALF : 16);
+            const uint64_t dp = mn_plain_desc(smem_u32(smem + C::OFF_P), 128, TREE_BKV * 16);
+            int q = 0, it = 0, seg = 0;
+            bool ok = true;
+            for (int u = u0; u < u1; ++seg) {
+                const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
                 const int n = g.k1 - g.k0;
                 auto scores = [&](int j) {
                     const int slot = q % NS;
                     ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    ++q;
                     if (!ok) return;
                     tc_fence_after();
-                    const uint32_t kb = smem_u32(smem + slot * C::TILE), qb = smem_u32(smem + C::OFF_Q);
+                    if (elect_one()) {
+                        const uint64_t k = dk + slot * (C::TILE >> 4);
+                        const uint32_t to = tm_s + (uint32_t)(j & 1) * C::SCOLS;
 #pragma unroll
-                    for (int part = 0; part < (QF16 ? 1 : 2); ++part)
+                        for (int part = 0; part < (QF16 || C::WIDE ? 1 : 2); ++part)
 #pragma unroll
-                        for (int x = 0; x < D / 16; ++x)
-                            umma_f16(tmem + (uint32_t)(j & 1) * R, sw128_desc(kb + (x >> 2) * C::HALF) + 2 * (x & 3),
-                                     sw128_desc(qb + part * C::QBYTES + (x >> 2) * C::QHALF) + 2 * (x & 3), id_s, part + x != 0);
-                    umma_commit(&s_full[j & 1]);
-                    umma_commit(&empty[slot]);
-                    ++q;
+                            for (int x = 0; x < D / 16; ++x)
+                                umma_f16(to, k + (x >> 2) * (C::HALF >> 4) + 2 * (x & 3),
+                                         dq + part * (R * 128 >> 4) + (x >> 2) * (C::QHALF >> 4) + 2 * (x & 3), id_s,
+                                         part + x != 0);
+                        umma_commit(&s_full[j & 1]);
+                        umma_commit(&empty[slot]);
+                    }
+                    __syncwarp();
                 };
                 ok = ok && mbar_wait(q_full, (uint32_t)seg & 1u, abort_flag, err);
                 scores(it);
@@ -258,49 +297,54 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     const int slot = q % NS;
                     ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
                     ok = ok && mbar_wait(p_full, (uint32_t)j & 1u, abort_flag, err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    ++q;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t vb = smem_u32(smem + slot * C::TILE), pb = smem_u32(smem + C::OFF_P);
+                    if (elect_one()) {
+                        const uint64_t v = dv + slot * (C::TILE >> 4);
+                        const uint32_t to = tm_o + (uint32_t)(j & 1) * C::OCOLS;
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                        for (int part = 0; part < (C::WIDE ? 1 : 2); ++part)
 #pragma unroll
-                        for (int x = 0; x < TREE_BKV / 16; ++x)
-                            umma_f16(tmem + (uint32_t)(2 + (j & 1)) * R, mn_sw128_desc(vb + x * 2048, D == 128 ? C::HALF : 16),
-                                     mn_plain_desc(pb + part * C::PBYTES + x * 256, 128, TREE_BKV * 16), id_o, part + x != 0);
-                    umma_commit(o_full);
-                    umma_commit(&empty[slot]);
-                    ++q;
+                            for (int x = 0; x < TREE_BKV / 16; ++x)
+                                umma_f16(to, v + x * (2048 >> 4), dp + part * (C::PBYTES >> 4) + x * (256 >> 4), id_o,
+                                         part + x != 0);
+                        umma_commit(o_full);
+                        umma_commit(&empty[slot]);
+                    }
+                    __syncwarp();
                 }
                 it += n;
+                u = g.next;
+            }
+            if (elect_one()) {
+                umma_commit(done);
+                const long long t0 = clock64();
+                while (!mbar_try_wait(done, 0) && clock64() - t0 < kMbarWaitLimit) {
+                }
             }
             __syncwarp();
-            u = g.next;
         }
-        if (lane == 0) {
-            umma_commit(done);
-            const long long t0 = clock64();
-            while (!mbar_try_wait(done, 0) && clock64() - t0 < kMbarWaitLimit) {
-            }
-        }
-        __syncwarp();
     } else {
         // ---- softmax: thread = position for the weights, = value of D for the output ----
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         tree_zero_padding(a, sq, p.page, (int64_t)blockIdx.x * C::SW + warp, (int64_t)gridDim.x * C::SW);
         const int wg = warp / 4, tid = threadIdx.x & 127;
         const int row0 = wg * RW;                                  // the group's first row of the tile
-        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + row0;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         // D = 64 products fill 16 of a warp's 32 lanes
         const int d = D == 128 ? tid : 16 * (warp & 3) + lane;
         const bool has_d = D == 128 || lane < 16;
-        float *off = s_off + row0;
-        uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0 + (warp & 3) * RW;  // this warp's positions, by row
+        float *noff = s_off + row0;  // minus the offsets
+        uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0;  // [4][RW]: bits of the unit's positions, by row
         // the group's part of P, while it is free: maxima and sums [4][RW], then the output rows,
         // RW / 2 in the place of the high halves and RW / 2 in that of the low ones
         uint8_t *own_p = smem + C::OFF_P + row0 / 8 * (TREE_BKV * 16);
         float *red = (float *)own_p, *fac = red;
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
-            const TreeSeg g = tree_locate(a, sq, p.page, R, u, u1);
+            const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
             const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
             // -- Q: 16 bytes of f16 per thread and step --
             float c = a.scale * 1.4426950408889634f;
@@ -329,10 +373,10 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                         v[2 * x] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
                         v[2 * x + 1] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
                     }
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[2 * x].x), fabsf(v[2 * x].y)), fmaxf(fabsf(v[2 * x].z), fabsf(v[2 * x].w))));
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[2 * x + 1].x), fabsf(v[2 * x + 1].y)),
-                                       fmaxf(fabsf(v[2 * x + 1].z), fabsf(v[2 * x + 1].w))));
                 }
+#pragma unroll
+                for (int x = 0; x < 2 * QC; ++x)
+                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[x].x), fabsf(v[x].y)), fmaxf(fabsf(v[x].z), fabsf(v[x].w))));
                 m = warp_max_f32(m);
                 if (lane == 0) red[warp & 3] = m;
                 group_sync(1 + wg, 128);
@@ -349,31 +393,35 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     tree_split2(v[2 * x].z * up, v[2 * x].w * up, hi.y, lo.y);
                     tree_split2(v[2 * x + 1].x * up, v[2 * x + 1].y * up, hi.z, lo.z);
                     tree_split2(v[2 * x + 1].z * up, v[2 * x + 1].w * up, hi.w, lo.w);
-                    uint8_t *dst = qs + (ch >> 3) * C::QHALF + sw128_off(row0 + r, ch & 7);
-                    *reinterpret_cast<uint4 *>(dst) = hi;
-                    *reinterpret_cast<uint4 *>(dst + C::QBYTES) = lo;
+                    uint8_t *half = qs + (ch >> 3) * C::QHALF;
+                    *reinterpret_cast<uint4 *>(half + sw128_off(row0 + r, ch & 7)) = hi;
+                    *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;
                 }
             }
-            if (tid < RW) off[tid] = -INFINITY;
+            if (tid < RW) noff[tid] = INFINITY;
             fence_proxy_async_smem();
             mbar_arrive(q_full);
             group_sync(1 + wg, 128);
 
-            float o[RW], l[RW];
+            const f32x2 c2 = pack2(c, c);
+            f32x2 o[RW / 2], l[RW / 2];
 #pragma unroll
-            for (int r = 0; r < RW; ++r) o[r] = l[r] = 0.0f;
+            for (int r = 0; r < RW / 2; ++r) o[r] = l[r] = 0ull;
             // O^T of unit j from TMEM to the running output
             auto drain = [&](int j) {
                 mbar_wait(o_full, (uint32_t)j & 1u, abort_flag, err);
                 tc_fence_after();
+                const uint32_t from = tm_o + lanes + (uint32_t)(j & 1) * C::OCOLS + row0;
+                constexpr int N = RW < 32 ? RW : 32;
 #pragma unroll
-                for (int x = 0; x < RW / 16; ++x) {
-                    uint32_t v[16];
-                    tmem_ld16(tl + (uint32_t)(2 + (j & 1)) * R + 16 * x, v);
-                    tmem_ld_wait(v);
+                for (int x = 0; x < C::OCOLS / R; ++x)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[16 * x + i] += __uint_as_float(v[i]);
-                }
+                    for (int y = 0; y < RW / N; ++y) {
+                        f32x2 v[N / 2];
+                        tmem_load<N>(from + x * R + y * N, v);
+#pragma unroll
+                        for (int i = 0; i < N / 2; ++i) o[y * N / 2 + i] = add2(o[y * N / 2 + i], v[i]);
+                    }
             };
             const int n = g.k1 - g.k0, it0 = it;
             for (int k = g.k0; k < g.k1; ++k, ++it) {
@@ -383,111 +431,122 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     group_sync(1 + wg, 128);  // the last unit's bits have been read
                     for (int e = tid; e < 4 * RW; e += 128) {
                         const int r = e % RW, t0 = k * TREE_BKV + e / RW * 32;
-                        ((uint32_t *)(smem + C::OFF_SEE) + 4 * row0)[e] =
-                            r < live ? tree_sees32(a, g, a.group(g.rt * R + row0 + r), t0) : 0u;
+                        see[e] = r < live ? tree_sees32(a, g, a.group(g.rt * R + row0 + r), t0) : 0u;
                     }
                     group_sync(1 + wg, 128);
                 }
+                const uint32_t *bits = see + (warp & 3) * RW;
                 mbar_wait(&s_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, err);
                 tc_fence_after();
-                const uint32_t ts = tl + (uint32_t)(it & 1) * R;
-                // 16 scores minus their offsets
-                auto load16 = [&](int x, float (&z)[16]) {
-                    uint32_t v[16];
-                    tmem_ld16(ts + 16 * x, v);
-                    tmem_ld_wait(v);
+                const uint32_t ts = tm_s + lanes + (uint32_t)(it & 1) * C::SCOLS + row0;
+                // scores plus `add` (times c)
+                auto load = [&](f32x2 (&z)[RW / 2], bool offsets) {
+                    tmem_load<RW>(ts, z);
+                    if (C::SCOLS != R) {
+                        f32x2 lo[RW / 2];
+                        tmem_load<RW>(ts + R, lo);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const float4 f = *reinterpret_cast<const float4 *>(off + 16 * x + i);
-                        z[i] = fmaf(__uint_as_float(v[i]), c, -f.x);
-                        z[i + 1] = fmaf(__uint_as_float(v[i + 1]), c, -f.y);
-                        z[i + 2] = fmaf(__uint_as_float(v[i + 2]), c, -f.z);
-                        z[i + 3] = fmaf(__uint_as_float(v[i + 3]), c, -f.w);
+                        for (int i = 0; i < RW / 2; ++i) z[i] = add2(z[i], lo[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < RW / 2; i += 2) {
+                        const ulonglong2 f = offsets ? *reinterpret_cast<const ulonglong2 *>(noff + 2 * i) : make_ulonglong2(0, 0);
+                        z[i] = fma2(z[i], c2, f.x);
+                        z[i + 1] = fma2(z[i + 1], c2, f.y);
                     }
                     if (tail) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!(see[16 * x + i] >> lane & 1u)) z[i] = -INFINITY;
+                        for (int i = 0; i < RW / 2; ++i) {
+                            float2 x = unpack2(z[i]);
+                            if (!(bits[2 * i] >> lane & 1u)) x.x = -INFINITY;
+                            if (!(bits[2 * i + 1] >> lane & 1u)) x.y = -INFINITY;
+                            z[i] = pack2(x.x, x.y);
+                        }
                     }
                 };
-                float z[16], top = -INFINITY;
-#pragma unroll
-                for (int x = 0; x < RW / 16; ++x) {
-                    load16(x, z);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) top = fmaxf(top, z[i]);
-                }
+                f32x2 z[RW / 2];
                 const bool fresh = it == it0;
+                float top = INFINITY;
+                if (!fresh) {
+                    load(z, true);
+                    top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < RW / 2; ++i) {
+                        const float2 x = unpack2(z[i]);
+                        top = fmaxf(top, fmaxf(x.x, x.y));
+                    }
+                }
                 if (group_any(1 + wg, top > TREE_MOST)) {
                     // -- new maxima: of the unit's 128 positions, then with what was --
                     if (!fresh) drain(it - 1);
+                    load(z, false);
+                    float keep[RW / 16] = {};
 #pragma unroll
-                    for (int x = 0; x < RW / 16; ++x) {
-                        uint32_t v[16];
-                        tmem_ld16(ts + 16 * x, v);
-                        tmem_ld_wait(v);
-                        float keep = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            float y = __uint_as_float(v[i]) * c;
-                            if (tail && !(see[16 * x + i] >> lane & 1u)) y = -INFINITY;
-                            y = warp_max_f32(y);
-                            if (lane == i) keep = y;
-                        }
-                        if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = keep;
+                    for (int i = 0; i < RW / 2; ++i) {
+                        const float2 x = unpack2(z[i]);
+                        const float m0 = warp_max_f32(x.x), m1 = warp_max_f32(x.y);
+                        if (lane == (2 * i) % 16) keep[i / 8] = m0;
+                        if (lane == (2 * i + 1) % 16) keep[i / 8] = m1;
                     }
+#pragma unroll
+                    for (int x = 0; x < RW / 16; ++x)
+                        if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = keep[x];
                     group_sync(1 + wg, 128);
                     if (tid < RW) {
-                        const float old = off[tid];
+                        const float old = -noff[tid];
                         const float m = fmaxf(fmaxf(red[tid], red[RW + tid]), fmaxf(red[2 * RW + tid], red[3 * RW + tid]));
                         const float now = fmaxf(old, m - TREE_EXP);
-                        off[tid] = now;
+                        noff[tid] = -now;
                         fac[tid] = now == -INFINITY ? 1.0f : tree_exp2(old - now);
                     }
                     group_sync(1 + wg, 128);
+                    if (!fresh) {
 #pragma unroll
-                    for (int r = 0; r < RW; r += 4) {
-                        const float4 f = *reinterpret_cast<const float4 *>(fac + r);
-                        o[r] *= f.x; o[r + 1] *= f.y; o[r + 2] *= f.z; o[r + 3] *= f.w;
-                        l[r] *= f.x; l[r + 1] *= f.y; l[r + 2] *= f.z; l[r + 3] *= f.w;
+                        for (int r = 0; r < RW / 2; r += 2) {
+                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
+                            o[r] = mul2(o[r], f.x), o[r + 1] = mul2(o[r + 1], f.y);
+                            l[r] = mul2(l[r], f.x), l[r + 1] = mul2(l[r + 1], f.y);
+                        }
                     }
+                    load(z, true);
                     group_sync(1 + wg, 128);  // the factors lie where the weights go
-                    if (RW == 16) load16(0, z);
-                } else if (!fresh) {
+                } else {
                     drain(it - 1);  // also: P of the last unit has been read
                 }
                 // -- weights: 16 bytes per 8 rows into the N-major P tiles --
 #pragma unroll
-                for (int x = 0; x < RW / 16; ++x) {
-                    if (RW != 16) load16(x, z);
-                    uint32_t hi[8], lo[8];
+                for (int x = 0; x < RW / 8; ++x) {
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float p0 = tree_exp2(z[i]), p1 = tree_exp2(z[i + 1]);
-                        l[16 * x + i] += p0;
-                        l[16 * x + i + 1] += p1;
-                        tree_split2(p0, p1, hi[i / 2], lo[i / 2]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 e = unpack2(z[4 * x + i]);
+                        const f32x2 wt = pack2(tree_exp2(e.x), tree_exp2(e.y));
+                        l[4 * x + i] = add2(l[4 * x + i], wt);
+                        tree_cut2(wt, hi[i], lo[i]);
                     }
-                    uint8_t *dst = smem + C::OFF_P + (row0 / 8 + 2 * x) * (TREE_BKV * 16) + tid * 16;
+                    uint8_t *dst = own_p + x * (TREE_BKV * 16) + tid * 16;
                     *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4 *>(dst + TREE_BKV * 16) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
                     *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    *reinterpret_cast<uint4 *>(dst + C::PBYTES + TREE_BKV * 16) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
                 }
                 if (tail && wg == 0) {
-                    // values past the end, infinite or NaN would make NaN of zero weights
+                    // values of nodes and past the end that are infinite or NaN would make NaN of zero
+                    // weights: zeros here, and what was visible is added at the end
                     const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
                     mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
                     uint8_t *vt = smem + qi % NS * C::TILE;
+                    if (t >= g.past) {
+                        uint32_t any = 0;
 #pragma unroll
-                    for (int ch = 0; ch < D / 8; ++ch) {
-                        uint4 *at = reinterpret_cast<uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
-                        const uint4 v = *at;
-                        uint4 m;
-                        m.x = __vcmpeq2(v.x & 0x7C007C00u, 0x7C007C00u), m.y = __vcmpeq2(v.y & 0x7C007C00u, 0x7C007C00u);
-                        m.z = __vcmpeq2(v.z & 0x7C007C00u, 0x7C007C00u), m.w = __vcmpeq2(v.w & 0x7C007C00u, 0x7C007C00u);
-                        if (m.x | m.y | m.z | m.w) {
-                            *at = make_uint4(v.x & ~m.x, v.y & ~m.y, v.z & ~m.z, v.w & ~m.w);
+                        for (int ch = 0; ch < D / 8; ++ch) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
+                            any |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
+                                   ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
+                        }
+                        if (any & 0x80008000u) {  // an exponent of all ones
+                            for (int ch = 0; ch < D / 8; ++ch) {
+                                uint32_t *v = reinterpret_cast<uint32_t *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
+                                for (int x = 0; x < 4; ++x) v[x] &= ~__vcmpeq2(v[x] & 0x7C007C00u, 0x7C007C00u);
+                            }
                             if (t < g.T) *s_bad = 1u;
                         }
                     }
@@ -505,7 +564,10 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             for (int x = 0; x < RW / 16; ++x) {
                 float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = l[16 * x + i];
+                for (int i = 0; i < 8; ++i) {
+                    const float2 y = unpack2(l[8 * x + i]);
+                    v[2 * i] = y.x, v[2 * i + 1] = y.y;
+                }
                 const float sum = lane_sums<16>(v);
                 if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = sum;
             }
@@ -514,8 +576,8 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             float *part = parts + (int64_t)tree_slot(w, blockIdx.x, g.first) * C::PART;
             if (tid < RW) {
                 const float L = (red[tid] + red[RW + tid]) + (red[2 * RW + tid] + red[3 * RW + tid]);
-                if (!whole) reinterpret_cast<float2 *>(part + R * D)[row0 + tid] = make_float2(off[tid], L);
-                off[tid] = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;
+                if (!whole) reinterpret_cast<float2 *>(part + R * D)[row0 + tid] = make_float2(-noff[tid], L);
+                noff[tid] = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;  // the rows' factors from here on
             }
             // V was cleaned by the first group for both
             group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
@@ -523,8 +585,10 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             // -- the output through shared memory: rows in a loop, 16 bytes at a time --
             if (has_d) {
 #pragma unroll
-                for (int r = 0; r < RW; ++r)
-                    reinterpret_cast<float *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * D + d] = o[r];
+                for (int r = 0; r < RW; ++r) {
+                    const float2 y = unpack2(o[r / 2]);
+                    reinterpret_cast<float *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * D + d] = r & 1 ? y.y : y.x;
+                }
             }
             group_sync(1 + wg, 128);
             for (int e = tid; e < min(RW, live) * (D / 4); e += 128) {
@@ -532,23 +596,23 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 const int gr = g.rt * R + row0 + r, node = a.group(gr);
                 float4 x = reinterpret_cast<const float4 *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * (D / 4) + ch];
                 if (anybad) x = tree_nonfinite4(a, p, sq, g, node, 4 * ch, x);
-                const float f = off[r];
+                const float f = noff[r];
                 x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
                 if (whole) tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch, x);
                 else *reinterpret_cast<float4 *>(part + (row0 + r) * D + 4 * ch) = x;
             }
-            // -- one small tile: the last of the CTAs that share the item joins the parts here --
+            // -- small tiles: the last of the CTAs that share the item joins the parts here --
             if (C::JOINS && !whole) {
                 const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.kt - 1);
-                group_sync(1, 128);
+                group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
                 if (threadIdx.x == 0) {
                     const bool is_last = atom_add_acq_rel_gpu(tickets + c0, 1u) == (unsigned)(c1 - c0);
                     if (is_last) atomicExch(tickets + c0, 0u);
                     *s_last = is_last;
                 }
-                group_sync(1, 128);
+                group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
                 if (*(volatile int *)s_last) {
-                    for (int e = threadIdx.x; e < min(R, live) * (D / 4); e += 128) {
+                    for (int e = threadIdx.x; e < min(R, live + row0) * (D / 4); e += 128 * NWG) {
                         const int r = e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
                         tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch,
                                     tree_join4(w, parts, C::PART, R, D, g.first, c0, c1, r, ch));
@@ -582,7 +646,7 @@ __global__ void __launch_bounds__(128) fattn_tree_join_kernel(const __grid_const
     const int c0 = blockIdx.x / (R / 16), r0 = blockIdx.x % (R / 16) * 16;
     const int end = tree_start(w, c0 + 1);
     if (c0 + 1 >= w.ctas || end <= tree_start(w, c0)) return;
-    const TreeSeg g = tree_locate(a, sq, page, R, end - 1, w.total);
+    const TreeSeg g = tree_locate(a, sq, w, page, R, end - 1, w.total);
     const int live = g.n * a.group.d - g.rt * R - r0;
     if (g.k1 - 1 == g.k0 || live <= 0 || tree_owner(w, g.first) != c0) return;  // ends here, or began before
     const int c1 = tree_owner(w, g.first + g.kt - 1);
@@ -646,7 +710,7 @@ static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvS
     const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RW, NWG, QF16>, dim3(grid), dim3(C::NT), C::SMEM, mk, mv, a, p, s,
                                    box, least, parts, be->counters, be->err_word);
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
-    if (!C::JOINS && !a.by_item && grid > 1) {
+    if constexpr (!C::JOINS) if (!a.by_item && grid > 1) {
         // started while the attention still runs; it waits for its end
         const bool pdl = be->pdl;
         be->pdl = true;
@@ -666,7 +730,7 @@ int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p
         if (a.D == 64) return a.q_f16 ? launch_tree<64, RW, NWG, true>(be, a, p, s) : launch_tree<64, RW, NWG, false>(be, a, p, s); \
         return a.q_f16 ? launch_tree<128, RW, NWG, true>(be, a, p, s) : launch_tree<128, RW, NWG, false>(be, a, p, s);              \
     }
-    FT(16, 1) FT(32, 1) FT(64, 1) FT(64, 2)
+    FT(16, 1) FT(16, 2) FT(32, 2) FT(64, 2)
 #undef FT
     return OASR_STATUS_FAILED;
 }

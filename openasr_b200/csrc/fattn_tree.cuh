@@ -25,20 +25,29 @@ struct TreeSeg {
     int first, next;       // the item's first unit, and where this segment ends, counted from the call's first
 };
 
-// T units shared by C CTAs: the first `more` take q + 1 units, the others q.
+// T units shared by C CTAs: the first `more` take q + 1 units, the others q.  Lane l keeps what
+// sequence l has: lengths, units, and the units of the sequences up to it.
 struct TreeUnits {
     int total, ctas, q, more;
+    int past, n, mine, run;
 };
 
-// Lane l of every warp: lengths of sequence s0 + l, its units and items (below 2^31: the launch
-// checks).  Runs of whole items count the items.
-static __device__ __forceinline__ int tree_lane_units(const TreeAttn &a, const KvSeqs &q, int page, int R, int s, int &past,
-                                                      int &n, bool &ok) {
-    ok = true;
+// Lane l of every warp: lengths and units of sequence s (below 2^31: the launch checks); runs of
+// whole items count the items.  `run`: the sum over the lanes up to this one.
+static __device__ __forceinline__ bool tree_lane_units(const TreeAttn &a, const KvSeqs &q, int page, int R, int s, int &past,
+                                                       int &n, int &mine, int &run) {
+    const int lane = threadIdx.x & 31;
+    bool ok = true;
     past = n = 0;
     if (s < a.S) ok = seq_lengths(q, s, page, past, n);
-    if (n == 0) return 0;
-    return (n * a.group.d + R - 1) / R * a.HKV * (a.by_item ? 1 : (past + n + TREE_BKV - 1) / TREE_BKV);
+    mine = n == 0 ? 0 : (n * a.group.d + R - 1) / R * a.HKV * (a.by_item ? 1 : (past + n + TREE_BKV - 1) / TREE_BKV);
+    run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += up;
+    }
+    return ok;
 }
 
 // All warps: the call's units and their split; a CTA gets at least `least` units where there are
@@ -46,15 +55,15 @@ static __device__ __forceinline__ int tree_lane_units(const TreeAttn &a, const K
 static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int least,
                                                        int ctas, int *err) {
     const int lane = threadIdx.x & 31;
-    int sum = 0;
-    for (int s0 = 0; s0 < a.S; s0 += 32) {
-        int past, n;
-        bool ok;
-        sum += tree_lane_units(a, q, page, R, s0 + lane, past, n, ok);
-        if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
-    }
     TreeUnits w;
-    w.total = __reduce_add_sync(0xffffffffu, sum);
+    bool ok = tree_lane_units(a, q, page, R, lane, w.past, w.n, w.mine, w.run);
+    w.total = __shfl_sync(0xffffffffu, w.run, 31);
+    for (int s0 = 32; s0 < a.S; s0 += 32) {
+        int past, n, mine, run;
+        ok &= tree_lane_units(a, q, page, R, s0 + lane, past, n, mine, run);
+        w.total += __shfl_sync(0xffffffffu, run, 31);
+    }
+    if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
     w.ctas = max(1, min(ctas, w.total / least));
     w.q = w.total / w.ctas;
     w.more = w.total - w.q * w.ctas;
@@ -75,20 +84,12 @@ static __device__ __forceinline__ int tree_slot(const TreeUnits &w, int c, int i
 }
 
 // All lanes: the segment that starts at unit u (u < total) and ends before `end`.
-static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, int page, int R, int u, int end) {
+static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, const TreeUnits &w, int page, int R,
+                                                      int u, int end) {
     const int lane = threadIdx.x & 31;
-    int base = 0;
+    int base = 0, past = w.past, n = w.n, mine = w.mine, run = w.run;
     TreeSeg g = {};
-    for (int s0 = 0; s0 < a.S; s0 += 32) {
-        int past, n;
-        bool ok;
-        const int mine = tree_lane_units(a, q, page, R, s0 + lane, past, n, ok);
-        int run = mine;  // inclusive prefix sum over the lanes
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += up;
-        }
+    for (int s0 = 0;;) {
         const unsigned hit = __ballot_sync(0xffffffffu, u < base + run);
         if (hit) {
             const int l = __ffs(hit) - 1;
@@ -99,6 +100,8 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
             break;
         }
         base += __shfl_sync(0xffffffffu, run, 31);
+        if ((s0 += 32) >= a.S) break;  // not for u < total
+        tree_lane_units(a, q, page, R, s0 + lane, past, n, mine, run);
     }
     g.T = g.past + g.n;
     g.kt = (g.T + TREE_BKV - 1) / TREE_BKV;
@@ -199,6 +202,34 @@ static __device__ __forceinline__ float tree_exp2(float x) {
     return y;
 }
 
+// Two f32 in one register pair: one instruction for both.
+typedef unsigned long long f32x2;
+static __device__ __forceinline__ f32x2 pack2(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+static __device__ __forceinline__ float2 unpack2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+static __device__ __forceinline__ f32x2 fma2(f32x2 x, f32x2 y, f32x2 z) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+static __device__ __forceinline__ f32x2 add2(f32x2 x, f32x2 y) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+static __device__ __forceinline__ f32x2 mul2(f32x2 x, f32x2 y) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
 // x = hi + lo, both f16: 22 bits of an f32
 static __device__ __forceinline__ void tree_split2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -240,6 +271,16 @@ static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const fl
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     return make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+}
+
+// The same for weights up to 2^15, the upper half cut at 11 bits instead of rounded (exact as f16
+// from 2^-14 on; below that the halves keep 2^-25, against a largest weight of 2^7).
+static __device__ __forceinline__ void tree_cut2(f32x2 w, uint32_t &hi, uint32_t &lo) {
+    const f32x2 h = w & 0xFFFFE000FFFFE000ull;
+    const float2 x = unpack2(h), y = unpack2(fma2(h, pack2(-1.0f, -1.0f), w));
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(y.x, y.y);
+    hi = *reinterpret_cast<const uint32_t *>(&a);
+    lo = *reinterpret_cast<const uint32_t *>(&b);
 }
 
 // 4-D tensor map over pages [D, page, H_kv, n_pages]: boxes of 64 values x `rows` positions,
