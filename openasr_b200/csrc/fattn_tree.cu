@@ -36,39 +36,44 @@ template <int D_, int RW_, int NWG_, bool QF16_>
 struct TreeTc {
     static constexpr int D = D_, RW = RW_, NWG = NWG_, R = RW * NWG;
     static constexpr bool QF16 = QF16_;
-    // up to 32 rows the halves of Q, and those of P, are 2 R columns of one product (half the
-    // instructions: at these sizes an instruction costs the same for 32 columns as for 16);
-    // beyond that they are two products into the same R columns
-    static constexpr bool WIDE = R <= 32;
-    static constexpr int SCOLS = WIDE && !QF16 ? 2 * R : R, OCOLS = WIDE ? 2 * R : R;
+    // The halves of P are 2 RW columns of one product, and so are those of Q up to 64 rows: K and V
+    // are fetched from shared memory once for both.  Beyond that the halves of Q are two products
+    // into the same columns (TMEM has 512).
+    static constexpr bool QWIDE = !QF16 && R <= 64;
+    static constexpr int SCOLS = QWIDE ? 2 * R : R;
+    // A group's rows go through weights and product in NB blocks of BR rows, with PB blocks under
+    // way: while one is multiplied the next one's weights are made.
+    static constexpr int PB = NWG == 1 ? 1 : 2, NB = RW == 64 ? 2 : 1, BR = RW / NB;
     static constexpr int HALF = TREE_BKV * 128;          // 128 positions x 64 values
     static constexpr int TILE = HALF * (D / 64);         // one K or V tile
     static constexpr int QROWS = QF16 ? R : 2 * R;       // rows of Q hi, then of Q lo
     static constexpr int QHALF = QROWS * 128;            // they x 64 values
     static constexpr int QBYTES = QHALF * (D / 64);
-    static constexpr int PBYTES = TREE_BKV * R * 2;      // P hi, then lo
+    static constexpr int PBYTES = TREE_BKV * BR * 2;     // a block's P hi, its P lo follows
+    static constexpr int PGROUP = PB * 2 * PBYTES;       // a group's blocks
     static constexpr int CTAS = NWG == 1 ? 2 : 1;
     static constexpr int MISC = CTAS == 2 ? 1024 : 3072;
-    static constexpr int FIXED = QBYTES + 2 * PBYTES + MISC;
+    static constexpr int FIXED = QBYTES + NWG * PGROUP + MISC;
     static constexpr int MOST = (CTAS == 2 ? 115712 : 232448) - FIXED;
     static constexpr int NS = MOST / TILE > 8 ? 8 : MOST / TILE;  // tiles in flight
     static_assert(NS >= 3, "K of the next unit and K, V of this one");
     static constexpr int OFF_Q = NS * TILE;
     static constexpr int OFF_P = OFF_Q + QBYTES;
-    static constexpr int OFF_MISC = OFF_P + 2 * PBYTES;
+    static constexpr int OFF_MISC = OFF_P + NWG * PGROUP;
     // misc: off[R], see[NWG][4][RW], barriers, flags
     static constexpr int OFF_SEE = OFF_MISC + 4 * R;
     static constexpr int OFF_BAR = OFF_SEE + 16 * R;
-    static constexpr int NBAR = 2 * NS + 6;
+    static constexpr int NBAR = 2 * NS + 4 + 2 * NWG * PB;
     static constexpr int OFF_FLAG = OFF_BAR + 8 * NBAR;
     static constexpr int SMEM = OFF_MISC + MISC;
     static_assert(OFF_FLAG + 32 <= SMEM, "misc");
+    static_assert(RW * D * 4 <= PGROUP, "a group's output rows fit its P");
     static constexpr int SW = 4 * NWG;                   // softmax warps
     // 64 rows per thread want more than the 168 registers that 10 warps leave: the other two
-    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 216 + 4 x 72)
+    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 232 + 4 x 40)
     static constexpr bool MOVE_REGS = RW == 64;
     static constexpr int NT = 32 * (SW + (MOVE_REGS ? 4 : 2));
-    static constexpr int COLS = 2 * SCOLS + 2 * OCOLS;   // S twice, O twice
+    static constexpr int COLS = 2 * SCOLS + NWG * PB * 2 * BR;  // S twice, O of the blocks
     static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int PART = R * (D + 2);             // floats of an unfinished segment
     static constexpr bool JOINS = R <= 32;               // the last CTA joins them (else fattn_tree_join_kernel)
@@ -76,6 +81,7 @@ struct TreeTc {
 
 constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
 constexpr float TREE_MOST = 15.0f;  // weights up to 2^15 stay below f16's 65504
+
 
 // K-major operand, 128-byte swizzle: sw128_desc.  M- or N-major operand in the same swizzle
 // (64 values of M contiguous per position): 8-position groups 1024 bytes apart, 64-value blocks
@@ -135,21 +141,25 @@ static __device__ __forceinline__ float warp_max_f32(float x) {
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
     return r;
 }
-// lane l gets the sum over the lanes of v[l] (N = 16: lanes l and l + 16 both)
-template <int N>
-static __device__ __forceinline__ float lane_sums(float (&v)[N]) {
+// Lane l gets the sum (or maximum) over the lanes of v[l]: at each step a lane passes on the half
+// that its partner keeps.  With 16 values lanes l and l + 16 get the same.
+template <int N, bool MAX>
+static __device__ __forceinline__ float lane_reduce(float (&v)[N]) {
     const int lane = threadIdx.x & 31;
     if (N == 16) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+        for (int i = 0; i < 16; ++i) {
+            const float x = __shfl_xor_sync(0xffffffffu, v[i], 16);
+            v[i] = MAX ? fmaxf(v[i], x) : v[i] + x;
+        }
     }
 #pragma unroll
     for (int o = N / 2; o > 0; o >>= 1) {
         const bool up = lane & o;
 #pragma unroll
         for (int i = 0; i < o; ++i) {
-            const float keep = up ? v[i + o] : v[i], give = up ? v[i] : v[i + o];
-            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            const float keep = up ? v[i + o] : v[i], x = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + o], o);
+            v[i] = MAX ? fmaxf(keep, x) : keep + x;
         }
     }
     return v[0];
@@ -161,7 +171,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                       const __grid_constant__ TreeAttn a, const __grid_constant__ KvPages p,
                       const __grid_constant__ KvSeqs sq, int box, int least, float *parts, unsigned int *tickets, int *err) {
     using C = TreeTc<D, RW, NWG, QF16>;
-    constexpr int R = C::R, NS = C::NS;
+    constexpr int R = C::R, NS = C::NS, NB = C::NB, BR = C::BR;
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
     griddep_wait();
@@ -171,7 +181,8 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     }
     float *s_off = (float *)(smem + C::OFF_MISC);
     uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + NS;
-    uint64_t *s_full = empty + NS /* [2] */, *p_full = s_full + 2, *o_full = p_full + 1, *q_full = o_full + 1,
+    uint64_t *s_full = empty + NS /* [2] */, *p_full = s_full + 2 /* [NWG][PB] */, *o_full = p_full + NWG * C::PB /* the same */,
+             *q_full = o_full + NWG * C::PB,
              *done = q_full + 1;
     volatile int *abort_flag = (volatile int *)(smem + C::OFF_FLAG);
     uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_FLAG + 4);
@@ -179,7 +190,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     int *s_last = (int *)(smem + C::OFF_FLAG + 12);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int G = a.group.d;
-    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
+    if (warp == C::SW + 1) tmem_alloc(tmem_slot, C::TMEM);
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 1);
@@ -187,17 +198,19 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         }
         mbar_init(&s_full[0], 1);
         mbar_init(&s_full[1], 1);
-        mbar_init(p_full, 128 * NWG);
-        mbar_init(o_full, 1);
+        for (int i = 0; i < NWG * C::PB; ++i) {
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_full[i], 1);
+        }
         mbar_init(q_full, 128 * NWG);
         mbar_init(done, 1);
         *abort_flag = 0;
         *s_bad = 0;
         fence_mbar_init();
     }
-    if (warp == C::SW + 1) tmem_alloc(tmem_slot, C::TMEM);
     if (warp == C::SW && lane < 2)
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &tm_v : &tm_k) : "memory");
+    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
     const int u0 = tree_start(w, blockIdx.x), u1 = tree_start(w, blockIdx.x + 1);
     tc_fence_before();
     __syncthreads();
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     const uint32_t tmem = *tmem_slot, tm_s = tmem, tm_o = tmem + 2 * C::SCOLS;
 
     if (warp >= C::SW) {
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == C::SW) {
             // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
             constexpr int HALVES = D / 64;
@@ -258,7 +271,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         } else if (warp == C::SW + 1) {
             // ---- MMA: the warp stays together, one elected lane issues ----
             constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, C::SCOLS);
-            constexpr uint32_t id_o = idesc_f16_f32(D, C::OCOLS) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
+            constexpr uint32_t id_o = idesc_f16_f32(D, 2 * C::BR) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
             const uint64_t dk = sw128_desc(smem_u32(smem)), dq = sw128_desc(smem_u32(smem + C::OFF_Q));
             const uint64_t dv = mn_sw128_desc(smem_u32(smem), D == 128 ? C::HALF : 16);
             const uint64_t dp = mn_plain_desc(smem_u32(smem + C::OFF_P), 128, TREE_BKV * 16);
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                         const uint64_t k = dk + slot * (C::TILE >> 4);
                         const uint32_t to = tm_s + (uint32_t)(j & 1) * C::SCOLS;
 #pragma unroll
-                        for (int part = 0; part < (QF16 || C::WIDE ? 1 : 2); ++part)
+                        for (int part = 0; part < (QF16 || C::QWIDE ? 1 : 2); ++part)
 #pragma unroll
                             for (int x = 0; x < D / 16; ++x)
                                 umma_f16(to, k + (x >> 2) * (C::HALF >> 4) + 2 * (x & 3),
@@ -296,24 +309,25 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     if (j + 1 < it + n) scores(j + 1);
                     const int slot = q % NS;
                     ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
-                    ok = ok && mbar_wait(p_full, (uint32_t)j & 1u, abort_flag, err);
-                    ok = __all_sync(0xffffffffu, ok);
-                    ++q;
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t v = dv + slot * (C::TILE >> 4);
-                        const uint32_t to = tm_o + (uint32_t)(j & 1) * C::OCOLS;
 #pragma unroll
-                        for (int part = 0; part < (C::WIDE ? 1 : 2); ++part)
+                    for (int i = 0; i < C::NB * NWG; ++i) {  // blocks, and in a block the groups
+                        const int b = j * C::NB + i / NWG, at = i % NWG * C::PB + b % C::PB;
+                        ok = ok && mbar_wait(&p_full[at], (uint32_t)(b / C::PB) & 1u, abort_flag, err);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t v = dv + slot * (C::TILE >> 4), pg = dp + at * (2 * C::PBYTES >> 4);
 #pragma unroll
                             for (int x = 0; x < TREE_BKV / 16; ++x)
-                                umma_f16(to, v + x * (2048 >> 4), dp + part * (C::PBYTES >> 4) + x * (256 >> 4), id_o,
-                                         part + x != 0);
-                        umma_commit(o_full);
-                        umma_commit(&empty[slot]);
+                                umma_f16(tm_o + at * 2 * C::BR, v + x * (2048 >> 4), pg + x * (256 >> 4), id_o, x != 0);
+                            umma_commit(&o_full[at]);
+                            if (i == C::NB * NWG - 1) umma_commit(&empty[slot]);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    ++q;
+                    if (!ok) break;
                 }
                 it += n;
                 u = g.next;
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         }
     } else {
         // ---- softmax: thread = position for the weights, = value of D for the output ----
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         tree_zero_padding(a, sq, p.page, (int64_t)blockIdx.x * C::SW + warp, (int64_t)gridDim.x * C::SW);
         const int wg = warp / 4, tid = threadIdx.x & 127;
         const int row0 = wg * RW;                                  // the group's first row of the tile
@@ -338,10 +352,8 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         const bool has_d = D == 128 || lane < 16;
         float *noff = s_off + row0;  // minus the offsets
         uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0;  // [4][RW]: bits of the unit's positions, by row
-        // the group's part of P, while it is free: maxima and sums [4][RW], then the output rows,
-        // RW / 2 in the place of the high halves and RW / 2 in that of the low ones
-        uint8_t *own_p = smem + C::OFF_P + row0 / 8 * (TREE_BKV * 16);
-        float *red = (float *)own_p, *fac = red;
+        // the group's part of P; while it is free, maxima and sums, then its output rows
+        uint8_t *own_p = smem + C::OFF_P + wg * C::PGROUP;
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
             const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
@@ -378,6 +390,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 for (int x = 0; x < 2 * QC; ++x)
                     m = fmaxf(m, fmaxf(fmaxf(fabsf(v[x].x), fabsf(v[x].y)), fmaxf(fabsf(v[x].z), fabsf(v[x].w))));
                 m = warp_max_f32(m);
+                float *red = (float *)own_p;
                 if (lane == 0) red[warp & 3] = m;
                 group_sync(1 + wg, 128);
                 m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -398,7 +411,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;
                 }
             }
-            if (tid < RW) noff[tid] = INFINITY;
+            if (tid < RW) noff[tid] = -TREE_NONE;
             fence_proxy_async_smem();
             mbar_arrive(q_full);
             group_sync(1 + wg, 128);
@@ -407,23 +420,26 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             f32x2 o[RW / 2], l[RW / 2];
 #pragma unroll
             for (int r = 0; r < RW / 2; ++r) o[r] = l[r] = 0ull;
-            // O^T of unit j from TMEM to the running output
-            auto drain = [&](int j) {
-                mbar_wait(o_full, (uint32_t)j & 1u, abort_flag, err);
+            // O^T of block b, the `half`-th of its unit, from TMEM to the running output: the products
+            // of both halves of P
+            auto drain = [&](int b, int half) {
+                const int at = wg * C::PB + b % C::PB;
+                mbar_wait(&o_full[at], (uint32_t)(b / C::PB) & 1u, abort_flag, err);
                 tc_fence_after();
-                const uint32_t from = tm_o + lanes + (uint32_t)(j & 1) * C::OCOLS + row0;
-                constexpr int N = RW < 32 ? RW : 32;
+                constexpr int N = BR < 32 ? BR : 32;
 #pragma unroll
-                for (int x = 0; x < C::OCOLS / R; ++x)
+                for (int x = 0; x < 2 * BR / N; ++x) {
+                    f32x2 v[N / 2];
+                    tmem_load<N>(tm_o + lanes + at * 2 * BR + x * N, v);
 #pragma unroll
-                    for (int y = 0; y < RW / N; ++y) {
-                        f32x2 v[N / 2];
-                        tmem_load<N>(from + x * R + y * N, v);
-#pragma unroll
-                        for (int i = 0; i < N / 2; ++i) o[y * N / 2 + i] = add2(o[y * N / 2 + i], v[i]);
+                    for (int i = 0; i < N / 2; ++i) {
+                        f32x2 &to = o[half * BR / 2 + x * N % BR / 2 + i];
+                        to = add2(to, v[i]);
                     }
+                }
             };
             const int n = g.k1 - g.k0, it0 = it;
+            int due = it * NB;  // the first block that is still to be drained
             for (int k = g.k0; k < g.k1; ++k, ++it) {
                 const int t = k * TREE_BKV + tid;             // this thread's position
                 const bool tail = (k + 1) * TREE_BKV > g.past;  // nodes among the positions, or the end
@@ -439,142 +455,153 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 mbar_wait(&s_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, err);
                 tc_fence_after();
                 const uint32_t ts = tm_s + lanes + (uint32_t)(it & 1) * C::SCOLS + row0;
-                // scores plus `add` (times c)
-                auto load = [&](f32x2 (&z)[RW / 2], bool offsets) {
-                    tmem_load<RW>(ts, z);
+#pragma unroll
+                for (int half = 0; half < NB; ++half) {
+                    const int b = it * NB + half;
+                    float *noff_b = noff + half * BR;
+                    const uint32_t *bits_b = bits + half * BR;
+                    uint8_t *p_b = own_p + b % C::PB * (2 * C::PBYTES);
+                    f32x2 y[BR / 2];  // scores in powers of two
+                    tmem_load<BR>(ts + half * BR, y);
                     if (C::SCOLS != R) {
-                        f32x2 lo[RW / 2];
-                        tmem_load<RW>(ts + R, lo);
+                        f32x2 lo[BR / 2];
+                        tmem_load<BR>(ts + R + half * BR, lo);
 #pragma unroll
-                        for (int i = 0; i < RW / 2; ++i) z[i] = add2(z[i], lo[i]);
+                        for (int i = 0; i < BR / 2; ++i) y[i] = add2(y[i], lo[i]);
                     }
 #pragma unroll
-                    for (int i = 0; i < RW / 2; i += 2) {
-                        const ulonglong2 f = offsets ? *reinterpret_cast<const ulonglong2 *>(noff + 2 * i) : make_ulonglong2(0, 0);
-                        z[i] = fma2(z[i], c2, f.x);
-                        z[i + 1] = fma2(z[i + 1], c2, f.y);
-                    }
+                    for (int i = 0; i < BR / 2; ++i) y[i] = mul2(y[i], c2);
                     if (tail) {
 #pragma unroll
-                        for (int i = 0; i < RW / 2; ++i) {
-                            float2 x = unpack2(z[i]);
-                            if (!(bits[2 * i] >> lane & 1u)) x.x = -INFINITY;
-                            if (!(bits[2 * i + 1] >> lane & 1u)) x.y = -INFINITY;
-                            z[i] = pack2(x.x, x.y);
+                        for (int i = 0; i < BR / 2; ++i) {
+                            float2 x = unpack2(y[i]);
+                            if (!(bits_b[2 * i] >> lane & 1u)) x.x = -INFINITY;
+                            if (!(bits_b[2 * i + 1] >> lane & 1u)) x.y = -INFINITY;
+                            y[i] = pack2(x.x, x.y);
                         }
                     }
-                };
-                f32x2 z[RW / 2];
-                const bool fresh = it == it0;
-                float top = INFINITY;
-                if (!fresh) {
-                    load(z, true);
-                    top = -INFINITY;
+                    const bool fresh = it == it0;
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < RW / 2; ++i) {
-                        const float2 x = unpack2(z[i]);
-                        top = fmaxf(top, fmaxf(x.x, x.y));
+                    for (int i = 0; i < BR / 2; i += 2) {
+                        const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff_b + 2 * i);
+                        const float2 x = unpack2(add2(y[i], f.x)), z = unpack2(add2(y[i + 1], f.y));
+                        top = fmaxf(fmaxf(top, fmaxf(x.x, x.y)), fmaxf(z.x, z.y));
                     }
-                }
-                if (group_any(1 + wg, top > TREE_MOST)) {
-                    // -- new maxima: of the unit's 128 positions, then with what was --
-                    if (!fresh) drain(it - 1);
-                    load(z, false);
-                    float keep[RW / 16] = {};
+                    const bool rescale = group_any(1 + wg, top > TREE_MOST);
+                    // the block that had this one's place; with it its part of P is free
+                    if (due <= b - C::PB) drain(due++, half);
+                    if (rescale) {
+                        // -- new maxima: of the unit's 128 positions, then with what was --
+                        if (NB == 1 && due < b) drain(due++, half);  // the rows' sums are complete
+                        float *red = (float *)p_b, *fac = red;       // [4][BR]
+                        constexpr int N = BR < 32 ? BR : 32;
 #pragma unroll
-                    for (int i = 0; i < RW / 2; ++i) {
-                        const float2 x = unpack2(z[i]);
-                        const float m0 = warp_max_f32(x.x), m1 = warp_max_f32(x.y);
-                        if (lane == (2 * i) % 16) keep[i / 8] = m0;
-                        if (lane == (2 * i + 1) % 16) keep[i / 8] = m1;
-                    }
+                        for (int x = 0; x < BR / N; ++x) {
+                            float v[N];
 #pragma unroll
-                    for (int x = 0; x < RW / 16; ++x)
-                        if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = keep[x];
-                    group_sync(1 + wg, 128);
-                    if (tid < RW) {
-                        const float old = -noff[tid];
-                        const float m = fmaxf(fmaxf(red[tid], red[RW + tid]), fmaxf(red[2 * RW + tid], red[3 * RW + tid]));
-                        const float now = fmaxf(old, m - TREE_EXP);
-                        noff[tid] = -now;
-                        fac[tid] = now == -INFINITY ? 1.0f : tree_exp2(old - now);
-                    }
-                    group_sync(1 + wg, 128);
-                    if (!fresh) {
-#pragma unroll
-                        for (int r = 0; r < RW / 2; r += 2) {
-                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
-                            o[r] = mul2(o[r], f.x), o[r + 1] = mul2(o[r + 1], f.y);
-                            l[r] = mul2(l[r], f.x), l[r + 1] = mul2(l[r + 1], f.y);
-                        }
-                    }
-                    load(z, true);
-                    group_sync(1 + wg, 128);  // the factors lie where the weights go
-                } else {
-                    drain(it - 1);  // also: P of the last unit has been read
-                }
-                // -- weights: 16 bytes per 8 rows into the N-major P tiles --
-#pragma unroll
-                for (int x = 0; x < RW / 8; ++x) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 e = unpack2(z[4 * x + i]);
-                        const f32x2 wt = pack2(tree_exp2(e.x), tree_exp2(e.y));
-                        l[4 * x + i] = add2(l[4 * x + i], wt);
-                        tree_cut2(wt, hi[i], lo[i]);
-                    }
-                    uint8_t *dst = own_p + x * (TREE_BKV * 16) + tid * 16;
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                }
-                if (tail && wg == 0) {
-                    // values of nodes and past the end that are infinite or NaN would make NaN of zero
-                    // weights: zeros here, and what was visible is added at the end
-                    const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
-                    mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
-                    uint8_t *vt = smem + qi % NS * C::TILE;
-                    if (t >= g.past) {
-                        uint32_t any = 0;
-#pragma unroll
-                        for (int ch = 0; ch < D / 8; ++ch) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
-                            any |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
-                                   ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
-                        }
-                        if (any & 0x80008000u) {  // an exponent of all ones
-                            for (int ch = 0; ch < D / 8; ++ch) {
-                                uint32_t *v = reinterpret_cast<uint32_t *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
-                                for (int x = 0; x < 4; ++x) v[x] &= ~__vcmpeq2(v[x] & 0x7C007C00u, 0x7C007C00u);
+                            for (int i = 0; i < N / 2; ++i) {
+                                const float2 e = unpack2(y[x * N / 2 + i]);
+                                v[2 * i] = e.x, v[2 * i + 1] = e.y;
                             }
-                            if (t < g.T) *s_bad = 1u;
+                            const float m = lane_reduce<N, true>(v);
+                            if (lane < N) red[(warp & 3) * BR + N * x + lane] = m;
+                        }
+                        group_sync(1 + wg, 128);
+                        if (tid < BR) {
+                            const float old = -noff_b[tid];
+                            const float m = fmaxf(fmaxf(red[tid], red[BR + tid]), fmaxf(red[2 * BR + tid], red[3 * BR + tid]));
+                            const float now = fmaxf(old, m - TREE_EXP);
+                            noff_b[tid] = -now;
+                            fac[tid] = tree_exp2(old - now);
+                        }
+                        group_sync(1 + wg, 128);
+                        if (!fresh) {
+#pragma unroll
+                            for (int r = 0; r < BR / 2; r += 2) {
+                                const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
+                                f32x2 *ob = o + half * BR / 2, *lb = l + half * BR / 2;
+                                ob[r] = mul2(ob[r], f.x), ob[r + 1] = mul2(ob[r + 1], f.y);
+                                lb[r] = mul2(lb[r], f.x), lb[r + 1] = mul2(lb[r + 1], f.y);
+                            }
+                            group_sync(1 + wg, 128);  // the factors lie where the weights go
                         }
                     }
+                    // -- weights: 16 bytes per 8 rows into the N-major P tiles --
+#pragma unroll
+                    for (int x = 0; x < BR / 8; ++x) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) {
+                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff_b + 8 * x + 2 * i);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float2 e = unpack2(add2(y[4 * x + i + h], h ? f.y : f.x));
+                                const f32x2 wt = pack2(tree_exp2(e.x), tree_exp2(e.y));
+                                f32x2 &sum = l[half * BR / 2 + 4 * x + i + h];
+                                sum = add2(sum, wt);
+                                tree_cut2(wt, hi[i + h], lo[i + h]);
+                            }
+                        }
+                        uint8_t *dst = p_b + x * (TREE_BKV * 16) + tid * 16;
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                    if (tail && wg == 0 && half == 0) {
+                        // values of nodes and past the end that are infinite or NaN would make NaN of zero
+                        // weights: zeros here, and what was visible is added at the end
+                        const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
+                        mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
+                        uint8_t *vt = smem + qi % NS * C::TILE;
+                        if (t >= g.past) {
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int ch = 0; ch < D / 8; ++ch) {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
+                                any |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
+                                       ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
+                            }
+                            if (any & 0x80008000u) {  // an exponent of all ones
+                                for (int ch = 0; ch < D / 8; ++ch) {
+                                    uint32_t *v = reinterpret_cast<uint32_t *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
+                                    for (int x = 0; x < 4; ++x) v[x] &= ~__vcmpeq2(v[x] & 0x7C007C00u, 0x7C007C00u);
+                                }
+                                if (t < g.T) *s_bad = 1u;
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    fence_proxy_async_smem();
+                    mbar_arrive(&p_full[wg * C::PB + b % C::PB]);
                 }
-                tc_fence_before();
-                fence_proxy_async_smem();
-                mbar_arrive(p_full);
             }
-            drain(it - 1);
+#pragma unroll
+            for (int x = 0; x < C::PB; ++x)
+                if (due < it * NB) drain(due++, NB == 1 ? 0 : x);
             tc_fence_before();
             q += 2 * n;
 
             // -- sums of the weights over the group's positions --
+            {
+                float *red = (float *)own_p;  // [4][RW]
+                constexpr int N = RW < 32 ? RW : 32;
 #pragma unroll
-            for (int x = 0; x < RW / 16; ++x) {
-                float v[16];
+                for (int x = 0; x < RW / N; ++x) {
+                    float v[N];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 y = unpack2(l[8 * x + i]);
-                    v[2 * i] = y.x, v[2 * i + 1] = y.y;
+                    for (int i = 0; i < N / 2; ++i) {
+                        const float2 e = unpack2(l[x * N / 2 + i]);
+                        v[2 * i] = e.x, v[2 * i + 1] = e.y;
+                    }
+                    const float sum = lane_reduce<N, false>(v);
+                    if (lane < N) red[(warp & 3) * RW + N * x + lane] = sum;
                 }
-                const float sum = lane_sums<16>(v);
-                if (lane < 16) red[(warp & 3) * RW + 16 * x + lane] = sum;
             }
             group_sync(1 + wg, 128);
             const bool whole = g.k0 == 0 && g.k1 == g.kt;
             float *part = parts + (int64_t)tree_slot(w, blockIdx.x, g.first) * C::PART;
             if (tid < RW) {
+                const float *red = (const float *)own_p;
                 const float L = (red[tid] + red[RW + tid]) + (red[2 * RW + tid] + red[3 * RW + tid]);
                 if (!whole) reinterpret_cast<float2 *>(part + R * D)[row0 + tid] = make_float2(-noff[tid], L);
                 noff[tid] = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;  // the rows' factors from here on
@@ -587,14 +614,15 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
 #pragma unroll
                 for (int r = 0; r < RW; ++r) {
                     const float2 y = unpack2(o[r / 2]);
-                    reinterpret_cast<float *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * D + d] = r & 1 ? y.y : y.x;
+                    reinterpret_cast<float *>(own_p)[r * D + d] = r & 1 ? y.y : y.x;
                 }
             }
             group_sync(1 + wg, 128);
+#pragma unroll 4
             for (int e = tid; e < min(RW, live) * (D / 4); e += 128) {
                 const int r = e / (D / 4), ch = e % (D / 4);
                 const int gr = g.rt * R + row0 + r, node = a.group(gr);
-                float4 x = reinterpret_cast<const float4 *>(own_p + (r < RW / 2 ? 0 : C::PBYTES))[(r % (RW / 2)) * (D / 4) + ch];
+                float4 x = reinterpret_cast<const float4 *>(own_p)[e];
                 if (anybad) x = tree_nonfinite4(a, p, sq, g, node, 4 * ch, x);
                 const float f = noff[r];
                 x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
@@ -635,26 +663,23 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     }
 }
 
-// Joins the items that several CTAs of fattn_tree_kernel shared: block (c, rows) takes 16 rows of
-// the item whose last unit of CTA c's range is not the item's last.
+// Joins the items that several CTAs of fattn_tree_kernel shared: block (c, rows) takes 8 rows of
+// the item whose last unit in CTA c's range is not the item's last, four columns per thread.
 template <int D, int R>
-__global__ void __launch_bounds__(128) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, KvSeqs sq, int page,
-                                                              int ctas, int least, const float *parts) {
+__global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, KvSeqs sq, int page,
+                                                                int ctas, int least, const float *parts) {
     griddep_launch_dependents();
     griddep_wait();
     const TreeUnits w = tree_count(a, sq, page, R, least, ctas, nullptr);
-    const int c0 = blockIdx.x / (R / 16), r0 = blockIdx.x % (R / 16) * 16;
+    const int c0 = blockIdx.x / (R / 8), r = blockIdx.x % (R / 8) * 8 + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4);
     const int end = tree_start(w, c0 + 1);
     if (c0 + 1 >= w.ctas || end <= tree_start(w, c0)) return;
     const TreeSeg g = tree_locate(a, sq, w, page, R, end - 1, w.total);
-    const int live = g.n * a.group.d - g.rt * R - r0;
-    if (g.k1 - 1 == g.k0 || live <= 0 || tree_owner(w, g.first) != c0) return;  // ends here, or began before
-    const int c1 = tree_owner(w, g.first + g.kt - 1);
-    for (int e = threadIdx.x; e < min(16, live) * (D / 4); e += 128) {
-        const int r = r0 + e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
-        tree_store4(a, g.s, g.hk * a.group.d + gr - node * a.group.d, node, 4 * ch,
-                    tree_join4(w, parts, R * (D + 2), R, D, g.first, c0, c1, r, ch));
-    }
+    const int gr = g.rt * R + r;
+    if (g.k1 - 1 == g.k0 || gr >= g.n * a.group.d || tree_owner(w, g.first) != c0) return;  // ends here, or began before
+    const int node = a.group(gr);
+    tree_store4(a, g.s, g.hk * a.group.d + gr - node * a.group.d, node, 4 * ch,
+                tree_join4(w, parts, R * (D + 2), R, D, g.first, c0, tree_owner(w, g.first + g.kt - 1), r, ch));
 }
 
 bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2, int64_t nb3, int D, int page, int HKV,
@@ -714,7 +739,7 @@ static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvS
         // started while the attention still runs; it waits for its end
         const bool pdl = be->pdl;
         be->pdl = true;
-        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 16)), dim3(128), 0, a, s, p.page,
+        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 8)), dim3(2 * D), 0, a, s, p.page,
                                         grid, least, (const float *)parts);
         be->pdl = pdl;
         if (je != cudaSuccess) return oasr_internal_cuda_fail(be, je, "flash_attn_tree join launch", __LINE__);

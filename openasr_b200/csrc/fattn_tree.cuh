@@ -17,6 +17,7 @@
 namespace oasr {
 
 constexpr int TREE_BKV = 128;  // positions per unit
+constexpr float TREE_NONE = -1.7e38f;  // maximum of a row that has seen nothing (finite: -inf minus it is -inf)
 
 struct TreeSeg {
     int s, hk, rt;         // sequence, K/V head, row tile
@@ -243,15 +244,15 @@ static __device__ __forceinline__ void tree_split2(float x, float y, uint32_t &h
 // is R rows of D sums, then R pairs (maximum, sum of weights).
 static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const float *parts, int size, int R, int D, int first,
                                                     int c0, int c1, int r, int ch) {
-    float M = -INFINITY, L = 0.0f;
+    float M = TREE_NONE, L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int U = 6;  // parts loaded before any is used
+    constexpr int U = 8;  // parts loaded before any is used
     for (int x = c0; x <= c1; x += U) {
         float2 ml[U];
         float4 y[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            ml[i] = make_float2(-INFINITY, 0.0f);
+            ml[i] = make_float2(M, 0.0f);
             y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (x + i <= c1) {
                 const float *pt = parts + (int64_t)tree_slot(w, x + i, first) * size;
@@ -261,7 +262,6 @@ static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const fl
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            if (ml[i].x == -INFINITY) continue;  // nothing seen
             const float m = fmaxf(M, ml[i].x), f = tree_exp2(M - m), k = tree_exp2(ml[i].x - m);
             L = fmaf(L, f, ml[i].y * k);
             v.x = fmaf(v.x, f, y[i].x * k); v.y = fmaf(v.y, f, y[i].y * k);
