@@ -169,7 +169,7 @@ template <int D, int RW, int NWG, bool QF16>
 __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NWG, QF16>::CTAS)
     fattn_tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ TreeAttn a, const __grid_constant__ KvPages p,
-                      const __grid_constant__ KvSeqs sq, int box, int least, float *parts, unsigned int *tickets, int *err) {
+                      const __grid_constant__ KvSeqs sq, int box, float *parts, TreeJoin *joins, unsigned int *tickets, int *err) {
     using C = TreeTc<D, RW, NWG, QF16>;
     constexpr int R = C::R, NS = C::NS, NB = C::NB, BR = C::BR;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     }
     if (warp == C::SW && lane < 2)
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &tm_v : &tm_k) : "memory");
-    const TreeUnits w = tree_count(a, sq, p.page, R, least, gridDim.x, err);
+    const TreeUnits w = tree_count(a, sq, p.page, R, gridDim.x, err);
     const int u0 = tree_start(w, blockIdx.x), u1 = tree_start(w, blockIdx.x + 1);
     tc_fence_before();
     __syncthreads();
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 }
                 u = g.next;
             }
+            tree_zero_padding(a, sq, p.page, blockIdx.x, gridDim.x);
             // every copy lands before the block ends, also when the others gave up
             for (int i = max(0, q - NS); i < q; ++i) {
                 const long long t0 = clock64();
@@ -343,7 +344,6 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     } else {
         // ---- softmax: thread = position for the weights, = value of D for the output ----
         if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        tree_zero_padding(a, sq, p.page, (int64_t)blockIdx.x * C::SW + warp, (int64_t)gridDim.x * C::SW);
         const int wg = warp / 4, tid = threadIdx.x & 127;
         const int row0 = wg * RW;                                  // the group's first row of the tile
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0;  // [4][RW]: bits of the unit's positions, by row
         // the group's part of P; while it is free, maxima and sums, then its output rows
         uint8_t *own_p = smem + C::OFF_P + wg * C::PGROUP;
+        if (!C::JOINS && threadIdx.x == 0) joins[blockIdx.x].live = 0;
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
             const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
@@ -629,9 +630,12 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 if (whole) tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch, x);
                 else *reinterpret_cast<float4 *>(part + (row0 + r) * D + 4 * ch) = x;
             }
+            if (!C::JOINS && !whole && g.k0 == 0 && threadIdx.x == 0)
+                joins[blockIdx.x] = TreeJoin{tree_owner(w, g.first + g.per - 1), tree_slot(w, blockIdx.x, g.first), g.s, g.hk,
+                                             g.rt * R, min(R, live)};
             // -- small tiles: the last of the CTAs that share the item joins the parts here --
             if (C::JOINS && !whole) {
-                const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.kt - 1);
+                const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.per - 1);
                 group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
                 if (threadIdx.x == 0) {
                     const bool is_last = atom_add_acq_rel_gpu(tickets + c0, 1u) == (unsigned)(c1 - c0);
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     for (int e = threadIdx.x; e < min(R, live + row0) * (D / 4); e += 128 * NWG) {
                         const int r = e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
                         tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch,
-                                    tree_join4(w, parts, C::PART, R, D, g.first, c0, c1, r, ch));
+                                    tree_join4(parts, R, D, c0, c1, tree_slot(w, c0, g.first), r, ch));
                     }
                 }
             }
@@ -664,22 +668,18 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
 }
 
 // Joins the items that several CTAs of fattn_tree_kernel shared: block (c, rows) takes 8 rows of
-// the item whose last unit in CTA c's range is not the item's last, four columns per thread.
+// the one that begins in CTA c, four columns per thread.
 template <int D, int R>
-__global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, KvSeqs sq, int page,
-                                                                int ctas, int least, const float *parts) {
+__global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, const float *parts,
+                                                                const TreeJoin *joins) {
     griddep_launch_dependents();
     griddep_wait();
-    const TreeUnits w = tree_count(a, sq, page, R, least, ctas, nullptr);
     const int c0 = blockIdx.x / (R / 8), r = blockIdx.x % (R / 8) * 8 + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4);
-    const int end = tree_start(w, c0 + 1);
-    if (c0 + 1 >= w.ctas || end <= tree_start(w, c0)) return;
-    const TreeSeg g = tree_locate(a, sq, w, page, R, end - 1, w.total);
-    const int gr = g.rt * R + r;
-    if (g.k1 - 1 == g.k0 || gr >= g.n * a.group.d || tree_owner(w, g.first) != c0) return;  // ends here, or began before
-    const int node = a.group(gr);
-    tree_store4(a, g.s, g.hk * a.group.d + gr - node * a.group.d, node, 4 * ch,
-                tree_join4(w, parts, R * (D + 2), R, D, g.first, c0, tree_owner(w, g.first + g.kt - 1), r, ch));
+    const TreeJoin g = joins[c0];
+    if (r >= g.live) return;
+    const int node = a.group(g.row + r);
+    tree_store4(a, g.s, g.hk * a.group.d + g.row + r - node * a.group.d, node, 4 * ch,
+                tree_join4(parts, R, D, c0, g.c1, g.slot, r, ch));
 }
 
 bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2, int64_t nb3, int D, int page, int HKV,
@@ -720,27 +720,26 @@ static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvS
         if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
         attr_set = true;
     }
-    const int least = 1;
     a.group = FastDiv(a.H / a.HKV);
     a.page = FastDiv(p.page);
-    a.by_item = (int64_t)s.MP * p.page <= 4 * TREE_BKV;
     const int64_t tiles = ((int64_t)s.N * (a.H / a.HKV) + C::R - 1) / C::R;
-    const int64_t most = tiles * a.HKV * a.S * (a.by_item ? 1 : ((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
+    const int64_t most = tiles * a.HKV * a.S * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
     if (most > INT32_MAX / 2 || (int64_t)s.N * (a.H / a.HKV) > INT32_MAX / 2)
         return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * C::CTAS));
     int st = 0;
-    float *parts = (float *)oasr_internal_scratch(be, (size_t)grid * 2 * C::PART * 4, &st);
+    float *parts = (float *)oasr_internal_scratch(be, (size_t)grid * (2 * C::PART * 4 + sizeof(TreeJoin)), &st);
     if (st) return st;
+    TreeJoin *joins = (TreeJoin *)(parts + (size_t)grid * 2 * C::PART);
     const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RW, NWG, QF16>, dim3(grid), dim3(C::NT), C::SMEM, mk, mv, a, p, s,
-                                   box, least, parts, be->counters, be->err_word);
+                                   box, parts, joins, be->counters, be->err_word);
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
-    if constexpr (!C::JOINS) if (!a.by_item && grid > 1) {
+    if constexpr (!C::JOINS) if (grid > 1 && (int64_t)s.MP * p.page > TREE_BKV) {
         // started while the attention still runs; it waits for its end
         const bool pdl = be->pdl;
         be->pdl = true;
-        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 8)), dim3(2 * D), 0, a, s, p.page,
-                                        grid, least, (const float *)parts);
+        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 8)), dim3(2 * D), 0, a,
+                                        (const float *)parts, (const TreeJoin *)joins);
         be->pdl = pdl;
         if (je != cudaSuccess) return oasr_internal_cuda_fail(be, je, "flash_attn_tree join launch", __LINE__);
     }

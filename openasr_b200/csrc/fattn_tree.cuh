@@ -3,12 +3,14 @@
 //
 // Work is counted in units: 128 positions of one item, an item being (sequence, K/V head, tile of
 // R rows) and a row one query head of one node (row = node * G + head in the group).  The lengths
-// are in device memory, so every warp counts the units itself and each CTA takes an equal run of
-// them: ragged batches balance without the host knowing them, and one long sequence spreads over
-// all SMs.  A CTA's range is a list of segments, each within one item; a segment that is not the
-// whole of it leaves (maximum, sum, output) in the scratch, and the parts are joined in the order
-// of the positions, so the bits do not depend on which CTA came first.  Where the page table has
-// room for a few units only, the runs are of whole items instead: nothing is left to join.
+// are in device memory, so every warp works the split out itself, one of two:
+//   - pieces: each item in equal pieces of at most t units, one piece per CTA, with the t that ends
+//     first (a short call: a CTA has one start and one end);
+//   - runs: CTA c takes the c-th of equal runs of units, across items (a long call, or more items
+//     than CTAs: ragged batches balance to the unit).
+// A segment is what a CTA does of one item.  One that is not the whole item leaves (maximum, sum,
+// output) in the scratch, and the parts are joined in the order of the positions, so the bits do
+// not depend on which CTA came first.
 #pragma once
 
 #include "pages.cuh"
@@ -23,49 +25,82 @@ struct TreeSeg {
     int s, hk, rt;         // sequence, K/V head, row tile
     int past, n, T, kt;    // committed positions, live nodes, past + n, units of the item
     int k0, k1;            // units of this segment
-    int first, next;       // the item's first unit, and where this segment ends, counted from the call's first
+    int first, per, next;  // the item's first step, its steps, and where this segment ends
 };
 
-// T units shared by C CTAs: the first `more` take q + 1 units, the others q.  Lane l keeps what
-// sequence l has: lengths, units, and the units of the sequences up to it.
+// The call's steps (units in runs, pieces otherwise) over the CTAs: the first `more` CTAs take
+// q + 1, the others q.  Lane l keeps what sequence l has: lengths, steps, and the steps of the
+// sequences up to it.
 struct TreeUnits {
     int total, ctas, q, more;
+    int piece;  // most units of a piece, or 0: runs
     int past, n, mine, run;
 };
 
-// Lane l of every warp: lengths and units of sequence s (below 2^31: the launch checks); runs of
-// whole items count the items.  `run`: the sum over the lanes up to this one.
-static __device__ __forceinline__ bool tree_lane_units(const TreeAttn &a, const KvSeqs &q, int page, int R, int s, int &past,
-                                                       int &n, int &mine, int &run) {
-    const int lane = threadIdx.x & 31;
-    bool ok = true;
+static __device__ __forceinline__ int tree_units(int past, int n) { return (past + n + TREE_BKV - 1) / TREE_BKV; }
+static __device__ __forceinline__ int tree_items(const TreeAttn &a, int n, int R) {
+    return (n * a.group.d + R - 1) / R * a.HKV;
+}
+
+// Lane l of every warp: lengths of sequence s.
+static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, const KvSeqs &q, int page, int s, int &past,
+                                                         int &n) {
     past = n = 0;
-    if (s < a.S) ok = seq_lengths(q, s, page, past, n);
-    mine = n == 0 ? 0 : (n * a.group.d + R - 1) / R * a.HKV * (a.by_item ? 1 : (past + n + TREE_BKV - 1) / TREE_BKV);
+    return s >= a.S || seq_lengths(q, s, page, past, n);
+}
+
+// Its steps (below 2^31: the launch checks) and the sum of those of the lanes up to this one.
+static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int piece, int R, int past, int n, int &mine, int &run) {
+    const int lane = threadIdx.x & 31, kt = tree_units(past, n);
+    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? (kt + piece - 1) / piece : kt);
     run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, run, o);
         if (lane >= o) run += up;
     }
-    return ok;
 }
 
-// All warps: the call's units and their split; a CTA gets at least `least` units where there are
-// that many.  A sequence with lengths out of range counts none (reported).
-static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int least,
-                                                       int ctas, int *err) {
+// The start and the end of a segment cost as much as so many units.
+constexpr int TREE_SEGMENT = 5;
+
+// All warps: the call's split.  A sequence with lengths out of range counts nothing (reported).
+static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int ctas, int *err) {
     const int lane = threadIdx.x & 31;
     TreeUnits w;
-    bool ok = tree_lane_units(a, q, page, R, lane, w.past, w.n, w.mine, w.run);
+    bool ok = tree_lane_lengths(a, q, page, lane, w.past, w.n);
+    w.piece = 0;
+    tree_lane_steps(a, 0, R, w.past, w.n, w.mine, w.run);
     w.total = __shfl_sync(0xffffffffu, w.run, 31);
+    if (a.S <= 32) {
+        // lane l tries pieces of t units, t spread from an even share of all units to the longest item
+        const int kt = tree_units(w.past, w.n), items = w.n ? tree_items(a, w.n, R) : 0;
+        const int most = __reduce_max_sync(0xffffffffu, w.n ? kt : 0), even = min(most, (w.total + ctas - 1) / ctas);
+        const int t = max(1, even + (most - even) * lane / 31);
+        int pieces = 0;
+        for (int s = 0; s < a.S; ++s)
+            pieces += __shfl_sync(0xffffffffu, items, s) * ((__shfl_sync(0xffffffffu, kt, s) + t - 1) / t);
+        // runs: an even share, and one more segment than pieces have
+        const int best = (int)__reduce_min_sync(0xffffffffu, pieces <= ctas ? (unsigned)t : 0x7fffffffu);
+        if (best <= even + TREE_SEGMENT) {
+            w.piece = best;
+            tree_lane_steps(a, best, R, w.past, w.n, w.mine, w.run);
+            w.total = __shfl_sync(0xffffffffu, w.run, 31);
+            w.ctas = max(1, w.total);
+            w.q = min(w.total, 1);
+            w.more = 0;
+            if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
+            return w;
+        }
+    }
     for (int s0 = 32; s0 < a.S; s0 += 32) {
         int past, n, mine, run;
-        ok &= tree_lane_units(a, q, page, R, s0 + lane, past, n, mine, run);
+        ok &= tree_lane_lengths(a, q, page, s0 + lane, past, n);
+        tree_lane_steps(a, 0, R, past, n, mine, run);
         w.total += __shfl_sync(0xffffffffu, run, 31);
     }
     if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
-    w.ctas = max(1, min(ctas, w.total / least));
+    w.ctas = max(1, min(ctas, w.total));
     w.q = w.total / w.ctas;
     w.more = w.total - w.q * w.ctas;
     return w;
@@ -74,7 +109,7 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
 static __device__ __forceinline__ int tree_start(const TreeUnits &w, int c) {
     return c >= w.ctas ? w.total : c * w.q + min(c, w.more);
 }
-// the CTA whose range holds unit u
+// the CTA whose range holds step u
 static __device__ __forceinline__ int tree_owner(const TreeUnits &w, int u) {
     const int big = w.more * (w.q + 1);
     return u < big ? u / (w.q + 1) : w.more + (u - big) / w.q;
@@ -84,7 +119,7 @@ static __device__ __forceinline__ int tree_slot(const TreeUnits &w, int c, int i
     return 2 * c + (item_first > tree_start(w, c) ? 1 : 0);
 }
 
-// All lanes: the segment that starts at unit u (u < total) and ends before `end`.
+// All lanes: the segment that starts at step u (u < total) and ends before `end`.
 static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, const TreeUnits &w, int page, int R,
                                                       int u, int end) {
     const int lane = threadIdx.x & 31;
@@ -102,18 +137,21 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
         }
         base += __shfl_sync(0xffffffffu, run, 31);
         if ((s0 += 32) >= a.S) break;  // not for u < total
-        tree_lane_units(a, q, page, R, s0 + lane, past, n, mine, run);
+        tree_lane_lengths(a, q, page, s0 + lane, past, n);
+        tree_lane_steps(a, w.piece, R, past, n, mine, run);
     }
     g.T = g.past + g.n;
-    g.kt = (g.T + TREE_BKV - 1) / TREE_BKV;
-    const int rts = (g.n * a.group.d + R - 1) / R, per = a.by_item ? 1 : g.kt;
-    const int item = (u - g.first) / per;
+    g.kt = tree_units(g.past, g.n);
+    g.per = w.piece ? (g.kt + w.piece - 1) / w.piece : g.kt;
+    const int rts = (g.n * a.group.d + R - 1) / R;
+    const int item = (u - g.first) / g.per;
     g.hk = item / rts;
     g.rt = item - g.hk * rts;
-    g.first += item * per;
-    g.next = min(g.first + per, end);
-    g.k0 = a.by_item ? 0 : u - g.first;
-    g.k1 = a.by_item ? g.kt : g.next - g.first;
+    g.first += item * g.per;
+    g.next = min(g.first + g.per, end);
+    const int p0 = u - g.first, p1 = g.next - g.first;
+    g.k0 = w.piece ? (int)((int64_t)p0 * g.kt / g.per) : p0;
+    g.k1 = w.piece ? (int)((int64_t)p1 * g.kt / g.per) : p1;
     return g;
 }
 
@@ -149,13 +187,13 @@ static __device__ __forceinline__ uint32_t tree_sees32(const TreeAttn &a, const 
 
 // Rows of padding nodes of every sequence: zeros.  Each of the `warps` warps of the grid, this
 // one being number w, takes every warps-th node.
-static __device__ __forceinline__ void tree_zero_padding(const TreeAttn &a, const KvSeqs &q, int page, int64_t w,
-                                                         int64_t warps) {
+static __device__ __forceinline__ void tree_zero_padding(const TreeAttn &a, const KvSeqs &q, int page, int w,
+                                                         int warps) {
     if (!q.n_nodes) return;
     const int lane = threadIdx.x & 31;
     const int per = a.D * (a.d_f16 ? 2 : 4) / 16;  // 16-byte pieces of a row
-    for (int64_t e = w; e < (int64_t)a.S * q.N; e += warps) {
-        const int s = (int)(e / q.N), i = (int)(e % q.N);
+    for (int e = w; e < a.S * q.N; e += warps) {
+        const int s = e / q.N, i = e % q.N;
         int past, n;
         seq_lengths(q, s, page, past, n);
         if (i < n) continue;
@@ -240,10 +278,15 @@ static __device__ __forceinline__ void tree_split2(float x, float y, uint32_t &h
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// The parts of an item in CTAs c0 .. c1, joined at row r and the four columns from 4 ch: each part
-// is R rows of D sums, then R pairs (maximum, sum of weights).
-static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const float *parts, int size, int R, int D, int first,
-                                                    int c0, int c1, int r, int ch) {
+// An item that CTAs c0 .. c1 share, left by c0 for the join: its rows from `row` on (`live` of
+// them), and where c0's part is (the others are in slots 2 c).  live = 0: nothing to join.
+struct TreeJoin {
+    int c1, slot, s, hk, row, live;
+};
+
+// Its parts joined at row r and the four columns from 4 ch: a part is R rows of D sums, then R
+// pairs (maximum, sum of weights).
+static __device__ __forceinline__ float4 tree_join4(const float *parts, int R, int D, int c0, int c1, int slot, int r, int ch) {
     float M = TREE_NONE, L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     constexpr int U = 8;  // parts loaded before any is used
@@ -255,7 +298,7 @@ static __device__ __forceinline__ float4 tree_join4(const TreeUnits &w, const fl
             ml[i] = make_float2(M, 0.0f);
             y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (x + i <= c1) {
-                const float *pt = parts + (int64_t)tree_slot(w, x + i, first) * size;
+                const float *pt = parts + (int64_t)(x + i == c0 ? slot : 2 * (x + i)) * (R * (D + 2));
                 ml[i] = __ldcg(reinterpret_cast<const float2 *>(pt + R * D) + r);
                 y[i] = __ldcg(reinterpret_cast<const float4 *>(pt + r * D) + ch);
             }

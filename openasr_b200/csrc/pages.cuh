@@ -74,7 +74,6 @@ struct TreeAttn {
     float scale;
     bool q_f16, d_f16;
     FastDiv group, page;          // H / HKV, positions per page
-    bool by_item;                 // whole (sequence, K/V head, row tile) items per CTA
 };
 int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s);
 
