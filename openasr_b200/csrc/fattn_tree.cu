@@ -70,7 +70,7 @@ struct TreeTc {
     static_assert(RW * D * 4 <= PGROUP, "a group's output rows fit its P");
     static constexpr int SW = 4 * NWG;                   // softmax warps
     // 64 rows per thread want more than the 168 registers that 10 warps leave: the other two
-    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 232 + 4 x 40)
+    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 216 + 4 x 72)
     static constexpr bool MOVE_REGS = RW == 64;
     static constexpr int NT = 32 * (SW + (MOVE_REGS ? 4 : 2));
     static constexpr int COLS = 2 * SCOLS + NWG * PB * 2 * BR;  // S twice, O of the blocks
@@ -190,43 +190,58 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     int *s_last = (int *)(smem + C::OFF_FLAG + 12);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int G = a.group.d;
-    if (warp == C::SW + 1) tmem_alloc(tmem_slot, C::TMEM);
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
-        mbar_init(&s_full[0], 1);
-        mbar_init(&s_full[1], 1);
-        for (int i = 0; i < NWG * C::PB; ++i) {
-            mbar_init(&p_full[i], 128);
-            mbar_init(&o_full[i], 1);
-        }
-        mbar_init(q_full, 128 * NWG);
-        mbar_init(done, 1);
-        *abort_flag = 0;
-        *s_bad = 0;
-        fence_mbar_init();
-    }
+    // Each role does what it can before the one block-wide barrier: the TMA warp makes the
+    // mbarriers and starts the first K tile, the MMA warp gets TMEM, the others bring Q.
     if (warp == C::SW && lane < 2)
         asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &tm_v : &tm_k) : "memory");
+    else if (warp < C::SW) tree_prefetch(a, sq);
     const TreeUnits w = tree_count(a, sq, p.page, R, gridDim.x, err);
     const int u0 = tree_start(w, blockIdx.x), u1 = tree_start(w, blockIdx.x + 1);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot, tm_s = tmem, tm_o = tmem + 2 * C::SCOLS;
+    TreeSeg g = {};
+    if (u0 < u1) g = tree_locate(a, sq, w, p.page, R, u0, u1);
+    bool begun = false;
+    uint32_t tmem = 0, tm_s = 0, tm_o = 0;
+    auto begin = [&]() {
+        tc_fence_before();
+        // not barrier 0: the TMA warp only arrives here, and may come to the last barrier first
+        group_sync(4, C::NT);
+        tc_fence_after();
+        tmem = *(volatile uint32_t *)tmem_slot;
+        tm_s = tmem, tm_o = tmem + 2 * C::SCOLS;
+        begun = true;
+    };
 
     if (warp >= C::SW) {
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == C::SW) {
             // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
             constexpr int HALVES = D / 64;
             const int b = lane / HALVES, half = lane % HALVES;
             const bool mine = b < TREE_BKV / box;
             int q = 0;  // tiles issued
+            if (lane == 0) {
+                for (int i = 0; i < NS; ++i) {
+                    mbar_init(&full[i], 1);
+                    mbar_init(&empty[i], 1);
+                }
+                mbar_init(&s_full[0], 1);
+                mbar_init(&s_full[1], 1);
+                for (int i = 0; i < NWG * C::PB; ++i) {
+                    mbar_init(&p_full[i], 128);
+                    mbar_init(&o_full[i], 1);
+                }
+                mbar_init(q_full, 128 * NWG);
+                mbar_init(done, 1);
+                *abort_flag = 0;
+                *s_bad = 0;
+                fence_mbar_init();
+                fence_proxy_async_smem();
+            }
+            __syncwarp();
+            asm volatile("barrier.cta.arrive 4, %0;" ::"n"(C::NT) : "memory");  // it waits for nothing itself
+            begun = true;
             for (int u = u0; u < u1;) {
-                const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
+                if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
                 const int *row = sq.table + g.s * sq.table_ld;
                 auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
                     const int t = k * TREE_BKV + b * box;
@@ -269,7 +284,11 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
                 }
             }
-        } else if (warp == C::SW + 1) {
+        } else if (warp > C::SW + 1) {
+            begin();  // only there to hand its registers over
+        } else {
+            tmem_alloc(tmem_slot, C::TMEM);
+            begin();
             // ---- MMA: the warp stays together, one elected lane issues ----
             constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, C::SCOLS);
             constexpr uint32_t id_o = idesc_f16_f32(D, 2 * C::BR) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
@@ -279,7 +298,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             int q = 0, it = 0, seg = 0;
             bool ok = true;
             for (int u = u0; u < u1; ++seg) {
-                const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
+                if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
                 const int n = g.k1 - g.k0;
                 auto scores = [&](int j) {
                     const int slot = q % NS;
@@ -343,7 +362,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         }
     } else {
         // ---- softmax: thread = position for the weights, = value of D for the output ----
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int wg = warp / 4, tid = threadIdx.x & 127;
         const int row0 = wg * RW;                                  // the group's first row of the tile
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -357,7 +376,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         if (!C::JOINS && threadIdx.x == 0) joins[blockIdx.x].live = 0;
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
-            const TreeSeg g = tree_locate(a, sq, w, p.page, R, u, u1);
+            if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
             const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
             // -- Q: 16 bytes of f16 per thread and step --
             float c = a.scale * 1.4426950408889634f;
@@ -414,8 +433,9 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             }
             if (tid < RW) noff[tid] = -TREE_NONE;
             fence_proxy_async_smem();
+            if (!begun) begin();
+            else group_sync(1 + wg, 128);
             mbar_arrive(q_full);
-            group_sync(1 + wg, 128);
 
             const f32x2 c2 = pack2(c, c);
             f32x2 o[RW / 2], l[RW / 2];
@@ -605,7 +625,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 const float *red = (const float *)own_p;
                 const float L = (red[tid] + red[RW + tid]) + (red[2 * RW + tid] + red[3 * RW + tid]);
                 if (!whole) reinterpret_cast<float2 *>(part + R * D)[row0 + tid] = make_float2(-noff[tid], L);
-                noff[tid] = whole ? (L == 0.0f ? 0.0f : 1.0f / L) : 1.0f;  // the rows' factors from here on
+                noff[tid] = L == 0.0f ? 0.0f : 1.0f / L;  // the rows' factors from here on
             }
             // V was cleaned by the first group for both
             group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
@@ -619,16 +639,23 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 }
             }
             group_sync(1 + wg, 128);
+            const int chunks = min(RW, live) * (D / 4);
+            float4 *rows = reinterpret_cast<float4 *>(own_p);
+            if (anybad) {
+                for (int e = tid; e < chunks; e += 128)
+                    rows[e] = tree_nonfinite4(a, p, sq, g, a.group(g.rt * R + row0 + e / (D / 4)), e % (D / 4) * 4, rows[e]);
+            }
+            if (whole) {
 #pragma unroll 4
-            for (int e = tid; e < min(RW, live) * (D / 4); e += 128) {
-                const int r = e / (D / 4), ch = e % (D / 4);
-                const int gr = g.rt * R + row0 + r, node = a.group(gr);
-                float4 x = reinterpret_cast<const float4 *>(own_p)[e];
-                if (anybad) x = tree_nonfinite4(a, p, sq, g, node, 4 * ch, x);
-                const float f = noff[r];
-                x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-                if (whole) tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch, x);
-                else *reinterpret_cast<float4 *>(part + (row0 + r) * D + 4 * ch) = x;
+                for (int e = tid; e < chunks; e += 128) {
+                    const int r = e / (D / 4), gr = g.rt * R + row0 + r, node = a.group(gr);
+                    const float4 x = rows[e];
+                    const float f = noff[r];
+                    tree_store4(a, g.s, g.hk * G + gr - node * G, node, e % (D / 4) * 4, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+                }
+            } else {
+#pragma unroll 4
+                for (int e = tid; e < chunks; e += 128) reinterpret_cast<float4 *>(part)[row0 * (D / 4) + e] = rows[e];
             }
             if (!C::JOINS && !whole && g.k0 == 0 && threadIdx.x == 0)
                 joins[blockIdx.x] = TreeJoin{tree_owner(w, g.first + g.per - 1), tree_slot(w, blockIdx.x, g.first), g.s, g.hk,
@@ -647,7 +674,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     for (int e = threadIdx.x; e < min(R, live + row0) * (D / 4); e += 128 * NWG) {
                         const int r = e / (D / 4), ch = e % (D / 4), gr = g.rt * R + r, node = a.group(gr);
                         tree_store4(a, g.s, g.hk * G + gr - node * G, node, 4 * ch,
-                                    tree_join4(parts, R, D, c0, c1, tree_slot(w, c0, g.first), r, ch));
+                                    tree_join4<8>(parts, R, D, c0, c1, tree_slot(w, c0, g.first), r, ch));
                     }
                 }
             }
@@ -659,6 +686,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             }
         }
     }
+    if (!begun) begin();
     tc_fence_before();
     __syncthreads();
     if (warp == C::SW + 1) {
@@ -679,7 +707,7 @@ __global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_con
     if (r >= g.live) return;
     const int node = a.group(g.row + r);
     tree_store4(a, g.s, g.hk * a.group.d + g.row + r - node * a.group.d, node, 4 * ch,
-                tree_join4(parts, R, D, c0, g.c1, g.slot, r, ch));
+                tree_join4<16>(parts, R, D, c0, g.c1, g.slot, r, ch));
 }
 
 bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2, int64_t nb3, int D, int page, int HKV,

@@ -42,6 +42,10 @@ static __device__ __forceinline__ int tree_items(const TreeAttn &a, int n, int R
     return (n * a.group.d + R - 1) / R * a.HKV;
 }
 
+// ceil(kt / t) for kt, t < 32768 by a reciprocal r = 1 / t: (kt + t - 1/2) / t is 1 / (2 t) or more
+// away from every integer, the product less than 2^-7 / t off.
+static __device__ __forceinline__ int tree_pieces(int kt, int t, float r) { return (int)(((float)(kt + t) - 0.5f) * r); }
+
 // Lane l of every warp: lengths of sequence s.
 static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, const KvSeqs &q, int page, int s, int &past,
                                                          int &n) {
@@ -52,7 +56,7 @@ static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, cons
 // Its steps (below 2^31: the launch checks) and the sum of those of the lanes up to this one.
 static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int piece, int R, int past, int n, int &mine, int &run) {
     const int lane = threadIdx.x & 31, kt = tree_units(past, n);
-    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? (kt + piece - 1) / piece : kt);
+    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? tree_pieces(kt, piece, __frcp_rn((float)piece)) : kt);
     run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -61,8 +65,8 @@ static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int pi
     }
 }
 
-// The start and the end of a segment cost as much as so many units.
-constexpr int TREE_SEGMENT = 5;
+// What the start and the end of a segment cost, and the join of an item's parts, in units.
+constexpr int TREE_SEGMENT = 5, TREE_JOIN = 3;
 
 // All warps: the call's split.  A sequence with lengths out of range counts nothing (reported).
 static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int ctas, int *err) {
@@ -72,17 +76,22 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
     w.piece = 0;
     tree_lane_steps(a, 0, R, w.past, w.n, w.mine, w.run);
     w.total = __shfl_sync(0xffffffffu, w.run, 31);
-    if (a.S <= 32) {
+    const int most = __reduce_max_sync(0xffffffffu, w.n ? tree_units(w.past, w.n) : 0);
+    if (a.S <= 32 && most < 32768) {  // (products of two unit counts fit 31 bits)
         // lane l tries pieces of t units, t spread from an even share of all units to the longest item
         const int kt = tree_units(w.past, w.n), items = w.n ? tree_items(a, w.n, R) : 0;
-        const int most = __reduce_max_sync(0xffffffffu, w.n ? kt : 0), even = min(most, (w.total + ctas - 1) / ctas);
+        const int even = min(most, (w.total + ctas - 1) / ctas);
         const int t = max(1, even + (most - even) * lane / 31);
+        const float r = __frcp_rn((float)t);
         int pieces = 0;
+#pragma unroll 4
         for (int s = 0; s < a.S; ++s)
-            pieces += __shfl_sync(0xffffffffu, items, s) * ((__shfl_sync(0xffffffffu, kt, s) + t - 1) / t);
-        // runs: an even share, and one more segment than pieces have
-        const int best = (int)__reduce_min_sync(0xffffffffu, pieces <= ctas ? (unsigned)t : 0x7fffffffu);
-        if (best <= even + TREE_SEGMENT) {
+            pieces += __shfl_sync(0xffffffffu, items, s) * tree_pieces(__shfl_sync(0xffffffffu, kt, s), t, r);
+        const unsigned cost = pieces <= ctas ? (unsigned)(t < most ? t + TREE_JOIN : t) : 65535u;
+        const unsigned least = __reduce_min_sync(0xffffffffu, cost << 16 | (unsigned)t);
+        const int best = (int)(least & 65535u);
+        // runs: an even share, a join, and one more segment than pieces have
+        if ((int)(least >> 16) <= even + TREE_JOIN + TREE_SEGMENT) {
             w.piece = best;
             tree_lane_steps(a, best, R, w.past, w.n, w.mine, w.run);
             w.total = __shfl_sync(0xffffffffu, w.run, 31);
@@ -142,7 +151,7 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
     }
     g.T = g.past + g.n;
     g.kt = tree_units(g.past, g.n);
-    g.per = w.piece ? (g.kt + w.piece - 1) / w.piece : g.kt;
+    g.per = w.piece ? tree_pieces(g.kt, w.piece, __frcp_rn((float)w.piece)) : g.kt;
     const int rts = (g.n * a.group.d + R - 1) / R;
     const int item = (u - g.first) / g.per;
     g.hk = item / rts;
@@ -150,9 +159,24 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
     g.first += item * g.per;
     g.next = min(g.first + g.per, end);
     const int p0 = u - g.first, p1 = g.next - g.first;
-    g.k0 = w.piece ? (int)((int64_t)p0 * g.kt / g.per) : p0;
-    g.k1 = w.piece ? (int)((int64_t)p1 * g.kt / g.per) : p1;
+    g.k0 = w.piece ? p0 * g.kt / g.per : p0;
+    g.k1 = w.piece ? p1 * g.kt / g.per : p1;
     return g;
+}
+
+// What is read through two more dependent loads starts on its way to L2 with the lengths: the page
+// table and the queries, spread over the grid.
+static __device__ __forceinline__ void tree_prefetch(const TreeAttn &a, const KvSeqs &q) {
+    const int step = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + threadIdx.x;
+    const int lines = (q.MP + 31) / 32;  // of 128 bytes per row of the table
+    for (int s = me / lines, l = me % lines; s < a.S; s += step / lines + 1)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(q.table + s * q.table_ld + l * 32));
+    const int bytes = a.D * (a.q_f16 ? 2 : 4);
+    for (unsigned e = me; e < (unsigned)(a.S * q.N) * (unsigned)a.H; e += step) {
+        const unsigned i = e / (unsigned)a.H, h = e % (unsigned)a.H, s = i / (unsigned)q.N;
+        const char *row = a.q + (i - s * q.N) * a.q_nb1 + h * a.q_nb2 + s * a.q_nb3;
+        for (int x = 0; x < bytes; x += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + x));
+    }
 }
 
 // Whether the row of a live node sees position t < T.
@@ -286,10 +310,10 @@ struct TreeJoin {
 
 // Its parts joined at row r and the four columns from 4 ch: a part is R rows of D sums, then R
 // pairs (maximum, sum of weights).
+template <int U>  // parts loaded before any is used
 static __device__ __forceinline__ float4 tree_join4(const float *parts, int R, int D, int c0, int c1, int slot, int r, int ch) {
     float M = TREE_NONE, L = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int U = 8;  // parts loaded before any is used
     for (int x = c0; x <= c1; x += U) {
         float2 ml[U];
         float4 y[U];
