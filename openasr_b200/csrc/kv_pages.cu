@@ -80,84 +80,139 @@ struct NormRope {
 };
 
 // y = x / sqrt(mean(x^2) + eps) * w, then pair (i, i + D/2) turned by the angle of the node's
-// position: (a cos - b sin, b cos + a sin).  One warp per (node, head): D / 32 values per lane,
-// the pair's other half 16 lanes away.  The squares are summed in 64 bits and every product
-// rounded as the Qwen driver's own kernel does, so both give the same bits.
-template <int D, bool QF16>
-__global__ void __launch_bounds__(128) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, int *err) {
+// position: (a cos - b sin, b cos + a sin).  A warp takes U heads of one node, D / 32 values per
+// lane, the pair's other half 16 lanes away; what depends on the node alone (lengths, page,
+// angles, gains) is fetched once for all of them.  The squares are summed in 64 bits and every
+// product rounded as the Qwen driver's own kernel does, so both give the same bits; the sums of
+// four heads share one butterfly (at each step a lane passes on the heads its partner keeps),
+// 12 shuffles instead of 40.  Bound by HBM for prompts: eight prompts of 512 rows (97 MB) take
+// 29 us; for a step's few rows by three dependent loads and the launch.
+template <int D, int U, bool QF16>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page,
+                                                           int groups, int *err) {
     constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31;
+    static_assert(U == 1 || U == 4, "heads per warp");
+    griddep_launch_dependents();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int HH = a.H + 2 * a.HKV;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= (int64_t)a.S * sq.N * HH) return;
-    const int h = (int)(unit % HH);
-    const int i = (int)(unit / HH % sq.N), s = (int)(unit / HH / sq.N);
+    const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (8 * U) + warp;
+    const int s = nodes(token), i = token - s * sq.N;
+    float v[U][V];
+    const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + 4 * V * lane;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int h = h0 + 8 * u;
+        if (h < HH) {
+            if (V == 4) *reinterpret_cast<float4 *>(v[u]) = *reinterpret_cast<const float4 *>(x + h * a.x_nb1);
+            else *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(x + h * a.x_nb1);
+        }
+    }
     int past, n;
-    if (!seq_lengths(sq, s, p.page, past, n) && lane == 0) atomicOr(err, ERR_BAD_INDEX);
-    float v[V];
-    {
-        const float *x = reinterpret_cast<const float *>(a.x + h * a.x_nb1 + i * a.x_nb2 + s * a.x_nb3) + V * lane;
-        if (V == 4) *reinterpret_cast<float4 *>(v) = *reinterpret_cast<const float4 *>(x);
-        else *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(x);
-    }
+    if (!seq_lengths(sq, s, p.page, past, n) && threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
     const bool live = i < n;
-    if (!live) {
-        if (h >= a.H) return;
+    char *q = a.q + i * a.q_nb2 + s * a.q_nb3 + (QF16 ? 2 : 4) * V * lane;
+    if (!live) {  // padding nodes leave zeros in q, nothing in the cache
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = 0.0f;  // padding nodes leave zeros in q, nothing in the cache
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + 8 * u;
+            if (h >= a.H) break;
+            if (QF16 && V == 4) *reinterpret_cast<uint2 *>(q + h * a.q_nb1) = make_uint2(0, 0);
+            else if (QF16) *reinterpret_cast<uint32_t *>(q + h * a.q_nb1) = 0;
+            else if (V == 4) *reinterpret_cast<float4 *>(q + h * a.q_nb1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            else *reinterpret_cast<float2 *>(q + h * a.q_nb1) = make_float2(0.0f, 0.0f);
+        }
+        return;
     }
-    const float *w = h < a.H ? a.q_norm : h < a.H + a.HKV ? a.k_norm : nullptr;
-    if (live && w) {
-        double ss = 0.0;
+    // this lane's V gains and angles
+    float wq[V], wk[V], cs[2 * V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) ss += (double)__fmul_rn(v[j], v[j]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(ss / (double)D), a.eps)));
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], scale), w[V * lane + j]);
+    for (int j = 0; j < V; ++j) {
+        wq[j] = a.q_norm ? a.q_norm[V * lane + j] : 1.0f;
+        wk[j] = a.k_norm ? a.k_norm[V * lane + j] : 1.0f;
     }
-    if (live && a.rope && h < a.H + a.HKV) {
+    if (a.rope) {
         int t = a.pos ? a.pos[s * a.pos_ld + i] : past + i;
         if (t < 0 || t >= a.n_pos) {
             if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
             t = 0;
         }
-        const float2 *cs = reinterpret_cast<const float2 *>(a.rope) + (int64_t)t * (D / 2) + V * (lane & 15);
+        const float *from = a.rope + (int64_t)t * D + 2 * V * (lane & 15);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
-            const float2 c = cs[j];
-            v[j] = lane < 16 ? __fsub_rn(__fmul_rn(v[j], c.x), __fmul_rn(other, c.y))
-                             : __fadd_rn(__fmul_rn(other, c.y), __fmul_rn(v[j], c.x));
+        for (int j = 0; j < V; j += 2) {
+            const float2 c0 = *reinterpret_cast<const float2 *>(from + 2 * j), c1 = *reinterpret_cast<const float2 *>(from + 2 * j + 2);
+            cs[2 * j] = c0.x, cs[2 * j + 1] = c0.y, cs[2 * j + 2] = c1.x, cs[2 * j + 3] = c1.y;
         }
     }
-    if (h < a.H && !QF16) {
-        float *q = reinterpret_cast<float *>(a.q + h * a.q_nb1 + i * a.q_nb2 + s * a.q_nb3) + V * lane;
-        if (V == 4) *reinterpret_cast<float4 *>(q) = *reinterpret_cast<const float4 *>(v);
-        else *reinterpret_cast<float2 *>(q) = *reinterpret_cast<const float2 *>(v);
-        return;
+    const int at = past + i, pj = page(at);
+    const int64_t off = at - pj * p.page;
+    int pg = sq.table[s * sq.table_ld + pj];
+    if (pg < 0 || pg >= p.n_pages) {
+        if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
+        pg = -1;
     }
-    char *dst;
-    if (h < a.H) {
-        dst = a.q + h * a.q_nb1 + i * a.q_nb2 + s * a.q_nb3;
-    } else {
-        const int at = past + i;
-        const int pg = sq.table[s * sq.table_ld + at / p.page];
-        if (pg < 0 || pg >= p.n_pages) {
-            if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
-            return;
-        }
-        const bool is_k = h < a.H + a.HKV;
-        const int64_t off = at % p.page;
-        dst = is_k ? p.k + pg * p.k_nb3 + (h - a.H) * p.k_nb2 + off * p.k_nb1
-                   : p.v + pg * p.v_nb3 + (h - a.H - a.HKV) * p.v_nb2 + off * p.v_nb1;
-    }
-    __half2 o[V / 2];
+    // sums of squares; lane group (lane >> 3) & 3 ends with head u = 2 (bit 4) + (bit 3) of its lane
+    float scale = 0.0f;
+    {
+        double ss[U];
 #pragma unroll
-    for (int j = 0; j < V; j += 2) o[j / 2] = __floats2half2_rn(v[j], v[j + 1]);
-    if (V == 4) *reinterpret_cast<uint2 *>(dst + 8 * lane) = *reinterpret_cast<const uint2 *>(o);
-    else *reinterpret_cast<uint32_t *>(dst + 4 * lane) = *reinterpret_cast<const uint32_t *>(o);
+        for (int u = 0; u < U; ++u) {
+            ss[u] = 0.0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) ss[u] += h0 + 8 * u < HH ? (double)__fmul_rn(v[u][j], v[u][j]) : 0.0;
+        }
+        double t;
+        if (U == 4) {
+            const bool b4 = lane & 16, b3 = lane & 8;
+            const double k0 = b4 ? ss[2] : ss[0], k1 = b4 ? ss[3 % U] : ss[1 % U];
+            const double x0 = k0 + __shfl_xor_sync(0xffffffffu, b4 ? ss[0] : ss[2 % U], 16);
+            const double x1 = k1 + __shfl_xor_sync(0xffffffffu, b4 ? ss[1 % U] : ss[3 % U], 16);
+            t = (b3 ? x1 : x0) + __shfl_xor_sync(0xffffffffu, b3 ? x0 : x1, 8);
+        } else {
+            t = ss[0] + __shfl_xor_sync(0xffffffffu, ss[0], 16);
+            t += __shfl_xor_sync(0xffffffffu, t, 8);
+        }
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(t / (double)D), a.eps)));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int h = h0 + 8 * u;
+        if (h >= HH) break;
+        const bool isq = h < a.H, isk = !isq && h < a.H + a.HKV;
+        const float sc = U == 4 ? __shfl_sync(0xffffffffu, scale, 8 * u) : scale;
+        if (isq ? a.q_norm != nullptr : isk && a.k_norm) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[u][j] = __fmul_rn(__fmul_rn(v[u][j], sc), isq ? wq[j] : wk[j]);
+        }
+        if (a.rope && (isq || isk)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float other = __shfl_xor_sync(0xffffffffu, v[u][j], 16);
+                v[u][j] = lane < 16 ? __fsub_rn(__fmul_rn(v[u][j], cs[2 * j]), __fmul_rn(other, cs[2 * j + 1]))
+                                    : __fadd_rn(__fmul_rn(other, cs[2 * j + 1]), __fmul_rn(v[u][j], cs[2 * j]));
+            }
+        }
+        if (isq && !QF16) {
+            if (V == 4) *reinterpret_cast<float4 *>(q + h * a.q_nb1) = *reinterpret_cast<const float4 *>(v[u]);
+            else *reinterpret_cast<float2 *>(q + h * a.q_nb1) = *reinterpret_cast<const float2 *>(v[u]);
+            continue;
+        }
+        char *dst = q + h * a.q_nb1;
+        if (!isq) {
+            if (pg < 0) continue;
+            dst = isk ? p.k + pg * p.k_nb3 + (h - a.H) * p.k_nb2 + off * p.k_nb1
+                      : p.v + pg * p.v_nb3 + (h - a.H - a.HKV) * p.v_nb2 + off * p.v_nb1;
+            dst += 2 * V * lane;
+        }
+        __half2 o[V / 2];
+#pragma unroll
+        for (int j = 0; j < V; j += 2) o[j / 2] = __floats2half2_rn(v[u][j], v[u][j + 1]);
+        if (V == 4) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
+        else *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(o);
+    }
 }
 
 // ---- acceptance and compaction -------------------------------------------------------------
@@ -177,7 +232,9 @@ struct Commit {
 // so a thread that moves its 16 bytes of every row in path order, a few rows loaded before they
 // are stored, never overwrites a row that it has still to read.  Each CTA repeats the walk and
 // moves 256 columns of 16 bytes of (layer, K or V, head).
-__global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, KvSeqs sq, int *err) {
+__global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, KvSeqs sq, FastDiv page, int *err) {
+    griddep_launch_dependents();
+    griddep_wait();
     __shared__ int s_next[TREE_MAX_NODES], s_path[TREE_MAX_NODES], s_tgt[TREE_MAX_NODES];
     __shared__ int s_len, s_bad;
     const int s = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
@@ -211,14 +268,17 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, K
         }
         __syncthreads();
     }
-    // (page << 32 | offset) of the rows: source replaces the path entry, destination the link
-    __shared__ int s_spg[TREE_MAX_NODES];
+    // page and offset of the rows: their sources, and where they go
+    __shared__ int s_spg[TREE_MAX_NODES], s_soff[TREE_MAX_NODES], s_doff[TREE_MAX_NODES];
     for (int c = threadIdx.x; c < len; c += blockDim.x) {
         const int from = past + s_path[c], to = past + c;
-        const int fp = sq.table[s * sq.table_ld + from / p.page], tp = sq.table[s * sq.table_ld + to / p.page];
+        const int fj = page(from), tj = page(to);
+        const int fp = sq.table[s * sq.table_ld + fj], tp = sq.table[s * sq.table_ld + tj];
         if (fp < 0 || fp >= p.n_pages || tp < 0 || tp >= p.n_pages) s_bad = 1;
         s_spg[c] = fp;
+        s_soff[c] = from - fj * p.page;
         s_next[c] = tp;
+        s_doff[c] = to - tj * p.page;
     }
     __syncthreads();
     if (s_bad) {
@@ -231,17 +291,17 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, K
     const int c16 = col % cpr, h = col / cpr % a.HKV, kv = col / cpr / a.HKV % 2, l = col / cpr / a.HKV / 2;
     const int64_t nb1 = kv ? p.v_nb1 : p.k_nb1, nb3 = kv ? p.v_nb3 : p.k_nb3;
     char *base = (kv ? p.v : p.k) + (int64_t)l * p.n_pages * nb3 + h * (kv ? p.v_nb2 : p.k_nb2) + 16 * c16;
-    constexpr int U = 4;
+    constexpr int U = 8;
     for (int b = 1; b < len; b += U) {
         uint4 r[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (b + u < len && s_path[b + u] != b + u)
-                r[u] = *reinterpret_cast<const uint4 *>(base + s_spg[b + u] * nb3 + (past + s_path[b + u]) % p.page * nb1);
+                r[u] = *reinterpret_cast<const uint4 *>(base + s_spg[b + u] * nb3 + s_soff[b + u] * nb1);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (b + u < len && s_path[b + u] != b + u)
-                *reinterpret_cast<uint4 *>(base + s_next[b + u] * nb3 + (past + b + u) % p.page * nb1) = r[u];
+                *reinterpret_cast<uint4 *>(base + s_next[b + u] * nb3 + s_doff[b + u] * nb1) = r[u];
     }
 }
 
@@ -251,6 +311,8 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, K
 template <bool FLAT>
 __global__ void __launch_bounds__(256) kv_pages_copy_kernel(const int *pairs, int64_t pair_ld, KvPages p, int L, int HKV,
                                                             int cpr, int chunks, int *err) {
+    griddep_launch_dependents();
+    griddep_wait();
     constexpr int U = 4;
     const int64_t b = blockIdx.x;
     const int ch = (int)(b % chunks), kv = (int)(b / chunks % 2), l = (int)(b / chunks / 2 % L);
@@ -332,7 +394,6 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     if (units == 0) return OASR_STATUS_SUCCESS;
     if (!qkv->data || !q->data) return fail_op(be, op, "null argument");
     if (!rows16(qkv) || !rows16(q)) return fail_op(be, op, "rows must be 16-byte aligned");
-    if (units > ((int64_t)1 << 32)) return fail_op(be, op, "too many rows");
     a.x = (const char *)qkv->data;
     a.x_nb1 = qkv->nb[1], a.x_nb2 = qkv->nb[2], a.x_nb3 = qkv->nb[3];
     a.q = (char *)q->data;
@@ -345,13 +406,22 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.pos_ld = pos ? pos->nb[1] / 4 : 0;
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
-    const dim3 grid((unsigned)((units + 3) / 4));
+    // four heads per warp share what belongs to the node, as long as that leaves every SM some
+    // blocks; below that one head per warp, so that a step's few rows start at once
+    const int64_t HH = qkv->ne[1], few = (HH + 7) / 8, many = (HH + 31) / 32;
+    const bool share = S * N * many >= 2 * be->sm_count;
+    const int groups = (int)(share ? many : few);
+    if (S * N * groups > INT32_MAX) return fail_op(be, op, "too many rows");
+    const dim3 grid((unsigned)(S * N * groups));
+    const FastDiv nodes((int)N), page(p.page);
     const bool f16 = q->type == OASR_TYPE_F16;
-    cudaError_t e;
-    if (D == 128) e = f16 ? launch_k(be, qk_norm_rope_kernel<128, true>, grid, dim3(128), 0, a, p, sq, be->err_word)
-                          : launch_k(be, qk_norm_rope_kernel<128, false>, grid, dim3(128), 0, a, p, sq, be->err_word);
-    else e = f16 ? launch_k(be, qk_norm_rope_kernel<64, true>, grid, dim3(128), 0, a, p, sq, be->err_word)
-                 : launch_k(be, qk_norm_rope_kernel<64, false>, grid, dim3(128), 0, a, p, sq, be->err_word);
+    cudaError_t e = cudaSuccess;
+#define NR(DD, UU, F)                       \
+    if (D == DD && share == (UU == 4) && f16 == F) \
+    e = launch_k(be, qk_norm_rope_kernel<DD, UU, F>, grid, dim3(256), 0, a, p, sq, nodes, page, groups, be->err_word)
+    NR(64, 1, false); NR(64, 1, true); NR(64, 4, false); NR(64, 4, true);
+    NR(128, 1, false); NR(128, 1, true); NR(128, 4, false); NR(128, 4, true);
+#undef NR
     return launched(be, e, op);
 }
 
@@ -434,7 +504,8 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
     if (cols > INT32_MAX / 2) return fail_op(be, op, "too many layers");
     a.groups = (int)((cols + 255) / 256);
     if (S * a.groups > INT32_MAX) return fail_op(be, op, "too many sequences");
-    return launched(be, launch_k(be, tree_commit_kernel, dim3((unsigned)(S * a.groups)), dim3(256), 0, a, p, sq, be->err_word), op);
+    return launched(be, launch_k(be, tree_commit_kernel, dim3((unsigned)(S * a.groups)), dim3(256), 0, a, p, sq, FastDiv(p.page),
+                                 be->err_word), op);
 }
 
 int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
