@@ -77,6 +77,7 @@ struct NormRope {
     int64_t pos_ld;
     int S, H, HKV;
     float eps;
+    bool gains16;  // both gains there, and 16-byte aligned
 };
 
 // y = x / sqrt(mean(x^2) + eps) * w, then pair (i, i + D/2) turned by the angle of the node's
@@ -84,25 +85,23 @@ struct NormRope {
 // lane, the pair's other half 16 lanes away; what depends on the node alone (lengths, page,
 // angles, gains) is fetched once for all of them.  The squares are summed in 64 bits and every
 // product rounded as the Qwen driver's own kernel does, so both give the same bits; the sums of
-// four heads share one butterfly (at each step a lane passes on the heads its partner keeps),
-// 12 shuffles instead of 40.  Bound by HBM for prompts: eight prompts of 512 rows (97 MB) take
-// 29 us; for a step's few rows by three dependent loads and the launch.
+// U heads share one butterfly (at each step a lane passes on the heads its partner keeps).  Bound by HBM for prompts: eight prompts of 512 rows (97 MB) take
+// 28 us (29 with eight heads per warp, 34 with two); for a step's few rows by three dependent loads and the launch.
 template <int D, int U, bool QF16>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page,
+__global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page,
                                                            int groups, int *err) {
-    constexpr int V = D / 32;
-    static_assert(U == 1 || U == 4, "heads per warp");
+    constexpr int V = D / 32, W = U == 1 ? 8 : 4;  // values per lane, warps per block
     griddep_launch_dependents();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int HH = a.H + 2 * a.HKV;
-    const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (8 * U) + warp;
+    const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (W * U) + warp;
     const int s = nodes(token), i = token - s * sq.N;
     float v[U][V];
     const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + 4 * V * lane;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int h = h0 + 8 * u;
+        const int h = h0 + W * u;
         if (h < HH) {
             if (V == 4) *reinterpret_cast<float4 *>(v[u]) = *reinterpret_cast<const float4 *>(x + h * a.x_nb1);
             else *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(x + h * a.x_nb1);
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(NormRope a, KvPages p
     if (!live) {  // padding nodes leave zeros in q, nothing in the cache
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = h0 + 8 * u;
+            const int h = h0 + W * u;
             if (h >= a.H) break;
             if (QF16 && V == 4) *reinterpret_cast<uint2 *>(q + h * a.q_nb1) = make_uint2(0, 0);
             else if (QF16) *reinterpret_cast<uint32_t *>(q + h * a.q_nb1) = 0;
@@ -126,10 +125,20 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(NormRope a, KvPages p
     }
     // this lane's V gains and angles
     float wq[V], wk[V], cs[2 * V];
+    if (a.gains16) {
+        if (V == 4) {
+            *reinterpret_cast<float4 *>(wq) = reinterpret_cast<const float4 *>(a.q_norm)[lane];
+            *reinterpret_cast<float4 *>(wk) = reinterpret_cast<const float4 *>(a.k_norm)[lane];
+        } else {
+            *reinterpret_cast<float2 *>(wq) = reinterpret_cast<const float2 *>(a.q_norm)[lane];
+            *reinterpret_cast<float2 *>(wk) = reinterpret_cast<const float2 *>(a.k_norm)[lane];
+        }
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        wq[j] = a.q_norm ? a.q_norm[V * lane + j] : 1.0f;
-        wk[j] = a.k_norm ? a.k_norm[V * lane + j] : 1.0f;
+        for (int j = 0; j < V; ++j) {
+            wq[j] = a.q_norm ? a.q_norm[V * lane + j] : 1.0f;
+            wk[j] = a.k_norm ? a.k_norm[V * lane + j] : 1.0f;
+        }
     }
     if (a.rope) {
         int t = a.pos ? a.pos[s * a.pos_ld + i] : past + i;
@@ -151,38 +160,35 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(NormRope a, KvPages p
         if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
         pg = -1;
     }
-    // sums of squares; lane group (lane >> 3) & 3 ends with head u = 2 (bit 4) + (bit 3) of its lane
+    // sums of squares: lane l ends with that of head u = l / (32 / U)
     float scale = 0.0f;
     {
         double ss[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             ss[u] = 0.0;
+            if (h0 + W * u < a.H + a.HKV) {  // value heads have no norm
 #pragma unroll
-            for (int j = 0; j < V; ++j) ss[u] += h0 + 8 * u < HH ? (double)__fmul_rn(v[u][j], v[u][j]) : 0.0;
+                for (int j = 0; j < V; ++j) ss[u] += (double)__fmul_rn(v[u][j], v[u][j]);
+            }
         }
-        double t;
-        if (U == 4) {
-            const bool b4 = lane & 16, b3 = lane & 8;
-            const double k0 = b4 ? ss[2] : ss[0], k1 = b4 ? ss[3 % U] : ss[1 % U];
-            const double x0 = k0 + __shfl_xor_sync(0xffffffffu, b4 ? ss[0] : ss[2 % U], 16);
-            const double x1 = k1 + __shfl_xor_sync(0xffffffffu, b4 ? ss[1 % U] : ss[3 % U], 16);
-            t = (b3 ? x1 : x0) + __shfl_xor_sync(0xffffffffu, b3 ? x0 : x1, 8);
-        } else {
-            t = ss[0] + __shfl_xor_sync(0xffffffffu, ss[0], 16);
-            t += __shfl_xor_sync(0xffffffffu, t, 8);
+#pragma unroll
+        for (int o = 16, m = U / 2; o > 0; o >>= 1, m >>= 1) {
+            const bool up = lane & o;
+            if (m == 0) ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], o);
+#pragma unroll
+            for (int k = 0; k < m; ++k)
+                ss[k] = (up ? ss[k + m] : ss[k]) + __shfl_xor_sync(0xffffffffu, up ? ss[k] : ss[k + m], o);
         }
-        t += __shfl_xor_sync(0xffffffffu, t, 4);
-        t += __shfl_xor_sync(0xffffffffu, t, 2);
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        const double t = ss[0];
         scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(t / (double)D), a.eps)));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int h = h0 + 8 * u;
+        const int h = h0 + W * u;
         if (h >= HH) break;
         const bool isq = h < a.H, isk = !isq && h < a.H + a.HKV;
-        const float sc = U == 4 ? __shfl_sync(0xffffffffu, scale, 8 * u) : scale;
+        const float sc = U == 1 ? scale : __shfl_sync(0xffffffffu, scale, 32 / U * u);
         if (isq ? a.q_norm != nullptr : isk && a.k_norm) {
 #pragma unroll
             for (int j = 0; j < V; ++j) v[u][j] = __fmul_rn(__fmul_rn(v[u][j], sc), isq ? wq[j] : wk[j]);
@@ -406,10 +412,11 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.pos_ld = pos ? pos->nb[1] / 4 : 0;
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
+    a.gains16 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 15) == 0;
     // four heads per warp share what belongs to the node, as long as that leaves every SM some
     // blocks; below that one head per warp, so that a step's few rows start at once
-    const int64_t HH = qkv->ne[1], few = (HH + 7) / 8, many = (HH + 31) / 32;
-    const bool share = S * N * many >= 2 * be->sm_count;
+    const int64_t HH = qkv->ne[1], few = (HH + 7) / 8, many = (HH + 15) / 16;
+    const bool share = S * N * many >= 4 * be->sm_count;
     const int groups = (int)(share ? many : few);
     if (S * N * groups > INT32_MAX) return fail_op(be, op, "too many rows");
     const dim3 grid((unsigned)(S * N * groups));
@@ -418,7 +425,7 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     cudaError_t e = cudaSuccess;
 #define NR(DD, UU, F)                       \
     if (D == DD && share == (UU == 4) && f16 == F) \
-    e = launch_k(be, qk_norm_rope_kernel<DD, UU, F>, grid, dim3(256), 0, a, p, sq, nodes, page, groups, be->err_word)
+    e = launch_k(be, qk_norm_rope_kernel<DD, UU, F>, grid, dim3(UU == 1 ? 256 : 128), 0, a, p, sq, nodes, page, groups, be->err_word)
     NR(64, 1, false); NR(64, 1, true); NR(64, 4, false); NR(64, 4, true);
     NR(128, 1, false); NR(128, 1, true); NR(128, 4, false); NR(128, 4, true);
 #undef NR
