@@ -17,6 +17,11 @@ import struct
 
 import numpy as np
 
+try:
+    from . import _describe
+except ImportError:  # not built: descriptors are made in Python
+    _describe = None
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liboasr_b200.so")
 
@@ -255,6 +260,7 @@ def _counted(call, item_type):
 # every symbol include/oasr_b200.h declares, with (argtypes, restype)
 _P, _I32, _I64, _U64, _F, _SZ = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float, ctypes.c_size_t
 _TP = ctypes.POINTER(OasrTensor)
+
 SIGNATURES = {
     "oasr_b200_device_count": ([ctypes.POINTER(_I32)], ctypes.c_int),
     "oasr_b200_init": ([_I32, ctypes.POINTER(_P)], ctypes.c_int),
@@ -284,10 +290,10 @@ SIGNATURES = {
     "oasr_b200_flash_attn_causal": ([_P, _TP, _TP, _TP, _F, _I32, _TP], ctypes.c_int),
     "oasr_b200_set_rows": ([_P, _TP, _TP, _TP], ctypes.c_int),
     "oasr_b200_argmax_first": ([_P, _TP, _TP], ctypes.c_int),
-    "oasr_b200_qk_norm_rope": ([_P, _TP, _TP, _TP, _F, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP], ctypes.c_int),
-    "oasr_b200_flash_attn_tree": ([_P, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _F, _TP], ctypes.c_int),
-    "oasr_b200_tree_commit": ([_P, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _TP, _I32, _TP, _TP, _TP, _TP], ctypes.c_int),
-    "oasr_b200_kv_pages_copy": ([_P, _TP, _TP, _I32, _TP], ctypes.c_int),
+    "oasr_b200_qk_norm_rope": ([_P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _P], ctypes.c_int),
+    "oasr_b200_flash_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _P, _F, _P], ctypes.c_int),
+    "oasr_b200_tree_commit": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _P], ctypes.c_int),
+    "oasr_b200_kv_pages_copy": ([_P, _P, _P, _I32, _P], ctypes.c_int),
     "oasr_b200_tree_mask": ([_P, _I32, _P], ctypes.c_int),
     "oasr_b200_whisper_load": ([_P, ctypes.POINTER(OasrWhisperConfig), ctypes.POINTER(OasrNamedTensor), _I32,
                                 ctypes.POINTER(_P)], ctypes.c_int),
@@ -365,16 +371,18 @@ def synth_normal(seed: int, n: int, mean: float = 0.0, std: float = 1.0, offset:
 # ---- tensor descriptors -----------------------------------------------------------------
 _TORCH_TYPES = None  # torch dtype -> (ggml type, element size), filled at the first use
 _DESC_PACK = struct.Struct("=iiQ8q").pack  # the fields of OasrTensor
-_ELEMENT = {F32: 4, F16: 2, I32: 4, I64: 8}
 
 
-def _torch_type(t) -> int:
+def _torch_types() -> dict:
     global _TORCH_TYPES
-    if _TORCH_TYPES is None:
-        import torch
+    import torch
 
-        _TORCH_TYPES = {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int64: I64}
-    ty = _TORCH_TYPES.get(t.dtype)
+    _TORCH_TYPES = {torch.float32: (F32, 4), torch.float16: (F16, 2), torch.int32: (I32, 4), torch.int64: (I64, 8)}
+    return _TORCH_TYPES
+
+
+def _torch_type(t) -> tuple:
+    ty = (_TORCH_TYPES or _torch_types()).get(t.dtype)
     if ty is None:
         raise UnsupportedInputs(STATUS_FAILED, f"unsupported tensor dtype {t.dtype}")
     return ty
@@ -386,8 +394,7 @@ def describe(t, ggml_type: int | None = None) -> OasrTensor:
     if type(t) is OasrTensor:
         return t
     if ggml_type is None:
-        ggml_type = _torch_type(t)
-        es = _ELEMENT[ggml_type]
+        ggml_type, es = _torch_type(t)
     else:
         es = t.element_size()
     ne, nb = t.shape, t.stride()
@@ -414,9 +421,17 @@ def describe(t, ggml_type: int | None = None) -> OasrTensor:
     return OasrTensor.from_buffer_copy(_DESC_PACK(ggml_type, 0, t.data_ptr(), *ne[:4], *nb[:4]))
 
 
-def _opt(t):
-    """descriptor of an optional tensor"""
-    return None if t is None else describe(t)
+def _arg(t):
+    """What a C call with void pointers takes for a tensor (the descriptor's bytes), a
+    descriptor or None."""
+    if t is None:
+        return None
+    if _describe is None or type(t) is OasrTensor:
+        return ctypes.byref(describe(t))
+    try:
+        return _describe.describe(t, _TORCH_TYPES or _torch_types())
+    except KeyError as e:
+        raise UnsupportedInputs(STATUS_FAILED, e.args[0]) from None
 
 
 class Weight:
@@ -657,29 +672,29 @@ class Backend:
         f16 [P, H_kv, page, D].  q_norm / k_norm f32 [D], rope f32 [n_pos, D / 2, 2], pos and
         n_nodes may be None (see the C header)."""
         self._check(lib().oasr_b200_qk_norm_rope(
-            self.handle, describe(qkv), _opt(q_norm), _opt(k_norm), eps, _opt(rope), _opt(pos), describe(page_table),
-            describe(n_past), _opt(n_nodes), describe(q), describe(k_pages), describe(v_pages)))
+            self.handle, _arg(qkv), _arg(q_norm), _arg(k_norm), eps, _arg(rope), _arg(pos), _arg(page_table),
+            _arg(n_past), _arg(n_nodes), _arg(q), _arg(k_pages), _arg(v_pages)))
 
     def flash_attn_tree(self, q, k_pages, v_pages, page_table, n_past, n_nodes, tree, scale: float, out) -> None:
         """Attention of the nodes q f32|f16 [S, H, n, D] over the pages -> out f32|f16 [S, n, H, D];
         tree i32 [S, n, ceil(n / 32)] of visible nodes, or None for a chain."""
         self._check(lib().oasr_b200_flash_attn_tree(
-            self.handle, describe(q), describe(k_pages), describe(v_pages), describe(page_table), describe(n_past),
-            _opt(n_nodes), _opt(tree), scale, describe(out)))
+            self.handle, _arg(q), _arg(k_pages), _arg(v_pages), _arg(page_table), _arg(n_past),
+            _arg(n_nodes), _arg(tree), scale, _arg(out)))
 
     def tree_commit(self, tokens, parents, target, n_nodes, n_past, page_table, k_pages, v_pages, n_layers: int, path,
                     n_accept, next_token, n_past_out) -> None:
         """Accept the drafted path that agrees with target (all i32 [S, n]) and compact its K/V rows
         in pages f16 [n_layers * P, H_kv, page, D]; path [S, n], the others [S]."""
         self._check(lib().oasr_b200_tree_commit(
-            self.handle, describe(tokens), describe(parents), describe(target), _opt(n_nodes), describe(n_past),
-            describe(page_table), describe(k_pages), describe(v_pages), n_layers, describe(path), describe(n_accept),
-            describe(next_token), describe(n_past_out)))
+            self.handle, _arg(tokens), _arg(parents), _arg(target), _arg(n_nodes), _arg(n_past),
+            _arg(page_table), _arg(k_pages), _arg(v_pages), n_layers, _arg(path), _arg(n_accept),
+            _arg(next_token), _arg(n_past_out)))
 
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
-        self._check(lib().oasr_b200_kv_pages_copy(self.handle, describe(k_pages), describe(v_pages), n_layers,
-                                                  describe(pairs)))
+        self._check(lib().oasr_b200_kv_pages_copy(self.handle, _arg(k_pages), _arg(v_pages), n_layers,
+                                                  _arg(pairs)))
 
 
 def tree_mask(parents) -> np.ndarray:

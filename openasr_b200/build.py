@@ -8,11 +8,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liboasr_b200.so")
+DESCRIBE = os.path.join(HERE, "_describe.so")  # tensor descriptors of the Python binding (csrc/describe_py.c)
 ROOT = os.path.dirname(HERE)
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
@@ -52,8 +54,23 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_describe() -> None:
+    """The CPython module behind backend.describe; without Python's headers the binding
+    describes tensors in Python (slower, the same bytes)."""
+    src, inc = os.path.join(CSRC, "describe_py.c"), sysconfig.get_path("include")
+    if not os.path.exists(os.path.join(inc, "Python.h")):
+        return
+    if os.path.exists(DESCRIBE) and os.path.getmtime(DESCRIBE) >= max(os.path.getmtime(src), _headers_mtime()):
+        return
+    cmd = [HOST_CXX, "-x", "c", "-O2", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", inc, src, "-o", DESCRIBE]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
+    _build_describe()
     cu, cpp = _sources()
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), cu + cpp))
