@@ -329,6 +329,30 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
  * with a negative page is left out. */
 int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
                             const oasr_tensor *pairs);
+/* Which sequence holds which pages (host only, one thread at a time; needs no device).
+ * Sequences share pages by reference: a fork copies nothing until one of the two writes.
+ * open / fork return the new sequence's number (0 .. max_seqs - 1), OASR_STATUS_ALLOC_FAILED
+ * when all are in use.  extend makes positions [from, to) writable, from at most what the
+ * sequence holds: it takes new pages, and pages of its own in the place of shared ones;
+ * where the rows before `from` of such a page have to come along, the (source,
+ * destination) pair for oasr_b200_kv_pages_copy goes to pairs [max_pairs][2] (at most one
+ * per call).  It returns the number of pairs, or OASR_STATUS_ALLOC_FAILED with nothing
+ * changed when the pool has too few free pages.  truncate gives the pages past position
+ * n_pos back (after a commit, or to drop a draft); close gives all of them back.  table
+ * writes the sequence's row of the page table, row[max_pages], -1 past its pages, and
+ * returns how many it has. */
+typedef struct oasr_kv_pool oasr_kv_pool;
+int oasr_b200_kv_pool_create(int32_t n_pages, int32_t page, int32_t max_pages, int32_t max_seqs, oasr_kv_pool **out);
+int oasr_b200_kv_pool_free(oasr_kv_pool *pool);
+int32_t oasr_b200_kv_pool_pages_free(const oasr_kv_pool *pool);
+int32_t oasr_b200_kv_pool_open(oasr_kv_pool *pool);
+int32_t oasr_b200_kv_pool_fork(oasr_kv_pool *pool, int32_t seq);
+int oasr_b200_kv_pool_close(oasr_kv_pool *pool, int32_t seq);
+int32_t oasr_b200_kv_pool_extend(oasr_kv_pool *pool, int32_t seq, int32_t from, int32_t to, int32_t *pairs,
+                                 int32_t max_pairs);
+int oasr_b200_kv_pool_truncate(oasr_kv_pool *pool, int32_t seq, int32_t n_pos);
+int32_t oasr_b200_kv_pool_table(const oasr_kv_pool *pool, int32_t seq, int32_t *row);
+
 /* Host helper: the tree words of one sequence from parents[n] (-1 for the root, otherwise
  * an earlier node): words [n][ceil(n / 32)], each node seeing itself and its ancestors.
  * OASR_STATUS_FAILED for a parent that does not come first, or n > 1024. */
@@ -645,6 +669,20 @@ int oasr_b200_qwen_decode_step(oasr_qwen *m, const int32_t *tokens, int32_t n_se
 int oasr_b200_qwen_generate(oasr_qwen *m, const float *emb, int32_t emb_on_device, int32_t n_seq, int32_t n_tok,
                             int32_t n_new, int32_t eos, int32_t stop_at_eos, int32_t *tokens_out,
                             int32_t tokens_on_device);
+/* Verify a tree of n drafted tokens per sequence in one pass over the model (no reference
+ * counterpart): tokens and parents [n_seq][n] (host), node 0 the token that the last call
+ * selected for the sequence (parent -1) and every other node's parent before it; pos
+ * [n_seq] the sequences' positions (tokens in the cache).  Through the four operators of
+ * the paged cache on the model's own caches, each sequence's slot being one page.  path
+ * [n_seq][n] gets the accepted nodes, then -1; n_accept [n_seq] their number; next [n_seq]
+ * the token after the last (all host).  The accepted rows are in the caches at pos, pos +
+ * 1, ...; the sequence is then at pos + n_accept with next as its input, also for
+ * oasr_b200_qwen_decode_step (at one position for all).  n_seq * n <= max_batch *
+ * max_prefill, n <= 1024, pos + n <= max_pos, and max_pos a multiple of 8.  The accepted
+ * tokens are the greedy ones of decode steps, except where two logits are nearer than the
+ * attentions' roundings (the tree attention sums on the tensor cores). */
+int oasr_b200_qwen_verify_tree(oasr_qwen *m, const int32_t *tokens, const int32_t *parents, int32_t n_seq, int32_t n,
+                               const int32_t *pos, int32_t *path, int32_t *n_accept, int32_t *next);
 /* Copy positions [0, n_pos) of one layer's f16 K and V cache rows of sequence seq
  * to host [n_kv_heads][n_pos][head_dim] (either output may be NULL). */
 int oasr_b200_qwen_read_kv(oasr_qwen *m, int32_t layer, int32_t seq, int32_t n_pos, uint16_t *k_out,

@@ -295,6 +295,15 @@ SIGNATURES = {
     "oasr_b200_tree_commit": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_kv_pages_copy": ([_P, _P, _P, _I32, _P], ctypes.c_int),
     "oasr_b200_tree_mask": ([_P, _I32, _P], ctypes.c_int),
+    "oasr_b200_kv_pool_create": ([_I32, _I32, _I32, _I32, ctypes.POINTER(_P)], ctypes.c_int),
+    "oasr_b200_kv_pool_free": ([_P], ctypes.c_int),
+    "oasr_b200_kv_pool_pages_free": ([_P], _I32),
+    "oasr_b200_kv_pool_open": ([_P], _I32),
+    "oasr_b200_kv_pool_fork": ([_P, _I32], _I32),
+    "oasr_b200_kv_pool_close": ([_P, _I32], ctypes.c_int),
+    "oasr_b200_kv_pool_extend": ([_P, _I32, _I32, _I32, _P, _I32], _I32),
+    "oasr_b200_kv_pool_truncate": ([_P, _I32, _I32], ctypes.c_int),
+    "oasr_b200_kv_pool_table": ([_P, _I32, _P], _I32),
     "oasr_b200_whisper_load": ([_P, ctypes.POINTER(OasrWhisperConfig), ctypes.POINTER(OasrNamedTensor), _I32,
                                 ctypes.POINTER(_P)], ctypes.c_int),
     "oasr_b200_whisper_free": ([_P], ctypes.c_int),
@@ -315,6 +324,7 @@ SIGNATURES = {
     "oasr_b200_qwen_prefill": ([_P, _P, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     "oasr_b200_qwen_decode_step": ([_P, _P, _I32, _I32, _P, _P], ctypes.c_int),
     "oasr_b200_qwen_generate": ([_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32], ctypes.c_int),
+    "oasr_b200_qwen_verify_tree": ([_P, _P, _P, _I32, _I32, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_qwen_read_kv": ([_P, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     "oasr_b200_row_size": ([_I32, _I64], _I64),
     "oasr_b200_quantize_chunk": ([_I32, _P, _P, _I64, _I64, _I64], _I64),
@@ -695,6 +705,56 @@ class Backend:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
         self._check(lib().oasr_b200_kv_pages_copy(self.handle, _arg(k_pages), _arg(v_pages), n_layers,
                                                   _arg(pairs)))
+
+
+class KvPool:
+    """Which sequence holds which pages of a paged K/V cache (host accounting; see the C header)."""
+
+    def __init__(self, n_pages: int, page: int, max_pages: int, max_seqs: int):
+        h = ctypes.c_void_p()
+        rc = lib().oasr_b200_kv_pool_create(n_pages, page, max_pages, max_seqs, ctypes.byref(h))
+        self._check(rc, "kv_pool_create")
+        self.handle, self.page, self.max_pages = h, page, max_pages
+
+    @staticmethod
+    def _check(rc: int, what: str) -> int:
+        if rc < 0:
+            raise _ERRORS.get(rc, GgmlBackendError)(rc, f"{what}: out of pages or sequences" if rc == STATUS_ALLOC_FAILED
+                                                    else f"{what}: bad arguments")
+        return rc
+
+    def close_pool(self) -> None:
+        if self.handle:
+            lib().oasr_b200_kv_pool_free(self.handle)
+            self.handle = ctypes.c_void_p(0)
+
+    def pages_free(self) -> int:
+        return self._check(lib().oasr_b200_kv_pool_pages_free(self.handle), "pages_free")
+
+    def open(self) -> int:
+        return self._check(lib().oasr_b200_kv_pool_open(self.handle), "open")
+
+    def fork(self, seq: int) -> int:
+        return self._check(lib().oasr_b200_kv_pool_fork(self.handle, seq), "fork")
+
+    def close(self, seq: int) -> None:
+        self._check(lib().oasr_b200_kv_pool_close(self.handle, seq), "close")
+
+    def extend(self, seq: int, start: int, end: int) -> np.ndarray:
+        """make positions [start, end) writable -> pairs [n, 2] of pages to copy first"""
+        pairs = np.empty((1, 2), np.int32)
+        n = self._check(lib().oasr_b200_kv_pool_extend(self.handle, seq, start, end, pairs.ctypes.data, 1), "extend")
+        return pairs[:n]
+
+    def truncate(self, seq: int, n_pos: int) -> None:
+        self._check(lib().oasr_b200_kv_pool_truncate(self.handle, seq, n_pos), "truncate")
+
+    def table(self, seqs) -> np.ndarray:
+        """page table rows int32 [len(seqs), max_pages]"""
+        rows = np.empty((len(seqs), self.max_pages), np.int32)
+        for i, s in enumerate(seqs):
+            self._check(lib().oasr_b200_kv_pool_table(self.handle, s, rows[i].ctypes.data), "table")
+        return rows
 
 
 def tree_mask(parents) -> np.ndarray:

@@ -64,6 +64,12 @@ struct oasr_qwen {
     int mask_tok;
     // decode activations, max_batch rows
     float *dx, *dqkv, *dq, *dattn, *dt, *dgu, *logits;
+    // K and V caches of all layers, one after the other (the layers' k_cache / v_cache point here)
+    __half *k_all, *v_all;
+    // drafted trees, made at the first verify_tree: logits of tree_chunk nodes, and per node or
+    // sequence the inputs and results (one buffer of int32)
+    float *tree_logits;
+    int *tree_ints;
     void *dqa;
     int *tokens, *pos, *nkv, *history;
     int family;
@@ -410,6 +416,88 @@ int prefill_from(oasr_qwen *m, const float *emb, bool on_device, int n, int T) {
     return launch_decode_advance(m->be, m->tokens, m->pos, m->nkv, m->history, n, m->P);
 }
 
+// ---- drafted trees ---------------------------------------------------------------------------
+constexpr int TREE_CHUNK = 128;  // nodes whose logits exist at a time
+
+// device int32 buffers of a verification: rows of n per sequence, then one value per sequence
+struct TreeInts {
+    int *tokens, *parents, *target, *path, *pos, *words;  // [n_seq][n] (words: [n_seq][n][W])
+    int *n_past, *accept, *next, *past_out, *table;       // [n_seq]
+};
+
+TreeInts tree_ints(oasr_qwen *m, int n_seq, int n) {
+    const int64_t rows = (int64_t)n_seq * n;
+    int *p = m->tree_ints;
+    TreeInts t;
+    for (int **q : {&t.tokens, &t.parents, &t.target, &t.path, &t.pos}) { *q = p; p += rows; }
+    for (int **q : {&t.n_past, &t.accept, &t.next, &t.past_out, &t.table}) { *q = p; p += n_seq; }
+    t.words = p;
+    return t;
+}
+
+oasr_tensor ints(const int *p, int64_t ne0, int64_t ne1) {
+    return make_tensor(OASR_TYPE_I32, p, ne0, ne1, 1, 1, ne0 * 4, ne0 * ne1 * 4, ne0 * ne1 * 4);
+}
+
+// The model over n_seq trees of n nodes (inputs in the device buffers): K and V of the nodes go to
+// positions n_past + i of the caches, taken as pages of max_pos positions, one per sequence.
+int run_tree(oasr_qwen *m, const TreeInts &t, int n_seq, int n) {
+    oasr_backend *be = m->be;
+    const int d = m->d, fam = m->family, H = m->H, HKV = m->HKV, D = m->D, P = m->P, W = (n + 31) / 32;
+    const int64_t M = (int64_t)n_seq * n, qkvw = m->qw + 2 * m->kvw, n_pos = m->P;
+    const ActPlanes qd = act_planes_at(m->qa, fam, M, d);
+    const ActPlanes qq = act_planes_at(m->qa, fam, M, m->qw);
+    const ActPlanes qf = act_planes_at(m->qa, fam, M, m->ffn);
+    const oasr_tensor past = ints(t.n_past, n_seq, 1), table = ints(t.table, 1, n_seq), pos = ints(t.pos, n, n_seq);
+    const oasr_tensor words = make_tensor(OASR_TYPE_I32, t.words, W, n, n_seq, 1, W * 4, (int64_t)W * n * 4, (int64_t)W * M * 4);
+    const oasr_tensor rope = make_tensor(OASR_TYPE_F32, m->rope, 2, D / 2, n_pos, 1, 8, D * 4, n_pos * D * 4);
+    const oasr_tensor qkv = make_tensor(OASR_TYPE_F32, m->qkv, D, H + 2 * HKV, n, n_seq, D * 4, qkvw * 4, qkvw * n * 4);
+    const int64_t qrow = (int64_t)m->qw * 4, row = D * 2, head = row * P, slot = head * HKV;
+    oasr_tensor q_out = make_tensor(OASR_TYPE_F32, m->q, D, H, n, n_seq, D * 4, qrow, qrow * n);
+    const oasr_tensor q_in = make_tensor(OASR_TYPE_F32, m->q, D, n, H, n_seq, qrow, D * 4, qrow * n);
+    oasr_tensor out = make_tensor(OASR_TYPE_F32, m->attn, D, H, n, n_seq, D * 4, qrow, qrow * n);
+    Q_TRY(launch_embed_q8_0(be, m->tok_emb, t.tokens, (int)M, nullptr, nullptr, P, m->x));
+    Q_TRY(launch_resid_norm_quant(be, m->x, nullptr, nullptr, M, d, m->cfg.rms_eps, true, m->layers[0].attn_norm,
+                                  nullptr, nullptr, &qd, fam));
+    for (size_t l = 0; l < m->layers.size(); ++l) {
+        const QLayer &L = m->layers[l];
+        const oasr_tensor qn = make_tensor(OASR_TYPE_F32, L.q_norm, D, 1, 1, 1, D * 4, D * 4, D * 4);
+        const oasr_tensor kn = make_tensor(OASR_TYPE_F32, L.k_norm, D, 1, 1, 1, D * 4, D * 4, D * 4);
+        oasr_tensor k = make_tensor(OASR_TYPE_F16, L.k_cache, D, P, HKV, m->B, row, head, slot);
+        oasr_tensor v = make_tensor(OASR_TYPE_F16, L.v_cache, D, P, HKV, m->B, row, head, slot);
+        Q_TRY(mul_mat_planes(be, L.qkv, qd, M, m->qkv, qkvw));
+        Q_TRY(oasr_b200_qk_norm_rope(be, &qkv, &qn, &kn, m->cfg.rms_eps, &rope, &pos, &table, &past, nullptr, &q_out, &k, &v));
+        Q_TRY(oasr_b200_flash_attn_tree(be, &q_in, &k, &v, &table, &past, nullptr, &words, 1.0f / sqrtf((float)D), &out));
+        oasr_tensor at = make_tensor(OASR_TYPE_F32, m->attn, m->qw, M, 1, 1, qrow, qrow * M, qrow * M);
+        Q_TRY(launch_quantize_act(be, &at, fam, qq));
+        Q_TRY(mul_mat_planes(be, L.o, qq, M, m->t, d));
+        Q_TRY(launch_resid_norm_quant(be, m->x, m->t, nullptr, M, d, m->cfg.rms_eps, true, L.ffn_norm, nullptr, nullptr,
+                                      &qd, fam));
+        Q_TRY(mul_mat_planes(be, L.gu, qd, M, m->gu, 2 * m->ffn));
+        Q_TRY(launch_swiglu_quant(be, m->gu, M, m->ffn, 2 * m->ffn, nullptr, &qf, fam));
+        Q_TRY(mul_mat_planes(be, L.down, qf, M, m->t, d));
+        if (l + 1 < m->layers.size())
+            Q_TRY(launch_resid_norm_quant(be, m->x, m->t, nullptr, M, d, m->cfg.rms_eps, true,
+                                          m->layers[l + 1].attn_norm, nullptr, nullptr, &qd, fam));
+    }
+    const int lfam = weight_family(m->out_w);
+    for (int64_t r = 0; r < M; r += TREE_CHUNK) {  // the choice after every node
+        const int rows = (int)std::min<int64_t>(TREE_CHUNK, M - r);
+        const ActPlanes ql = act_planes_at(m->qa, lfam, rows, d);
+        Q_TRY(launch_resid_norm_quant(be, m->x + r * d, m->t + r * d, nullptr, rows, d, m->cfg.rms_eps, true, m->out_norm,
+                                      nullptr, nullptr, &ql, lfam));
+        Q_TRY(mul_mat_planes(be, m->out_w, ql, rows, m->tree_logits, m->cfg.n_vocab));
+        Q_TRY(launch_argmax_rows(be, m->tree_logits, m->cfg.n_vocab, m->cfg.n_vocab, rows, t.target + r));
+    }
+    const int64_t layers = (int64_t)m->layers.size();
+    oasr_tensor k = make_tensor(OASR_TYPE_F16, m->k_all, D, P, HKV, layers * m->B, row, head, slot);
+    oasr_tensor v = make_tensor(OASR_TYPE_F16, m->v_all, D, P, HKV, layers * m->B, row, head, slot);
+    const oasr_tensor tok = ints(t.tokens, n, n_seq), par = ints(t.parents, n, n_seq), tgt = ints(t.target, n, n_seq);
+    oasr_tensor path = ints(t.path, n, n_seq), acc = ints(t.accept, n_seq, 1), nxt = ints(t.next, n_seq, 1),
+                pout = ints(t.past_out, n_seq, 1);
+    return oasr_b200_tree_commit(be, &tok, &par, &tgt, nullptr, &past, &table, &k, &v, (int32_t)layers, &path, &acc, &nxt, &pout);
+}
+
 bool prefill_args_ok(oasr_qwen *m, const float *emb, int n_seq, int n_tok) {
     return m && emb && n_seq >= 1 && n_seq <= m->B && n_tok >= 1 && n_tok <= m->Tmax && n_tok < m->P;
 }
@@ -510,12 +598,17 @@ int oasr_b200_qwen_load(oasr_backend *be, const oasr_qwen_config *cfg, const oas
         L_TRY(upload_vec(m, T_(p + "ffn_norm.weight"), d, &L.ffn_norm, p + "ffn_norm.weight"));
         L_TRY(upload_vec(m, T_(p + "attn_q_norm.weight"), D, &L.q_norm, p + "attn_q_norm.weight"));
         L_TRY(upload_vec(m, T_(p + "attn_k_norm.weight"), D, &L.k_norm, p + "attn_k_norm.weight"));
-        const size_t cache = (size_t)B * HKV * P * D * 2;
-        L_TRY(qalloc(m, &L.k_cache, cache));
-        L_TRY(qalloc(m, &L.v_cache, cache));
-        // zeroed like the reference's KV arena (allocate_zeroed_llm_resident_kv_arena)
-        if (cudaMemset(L.k_cache, 0, cache) != cudaSuccess || cudaMemset(L.v_cache, 0, cache) != cudaSuccess)
-            return fail(qfail(m, "KV cache zeroing failed"));
+        const size_t cache = (size_t)B * HKV * P * D;
+        if (l == 0) {
+            const size_t all = cache * cfg->n_layers * 2;
+            L_TRY(qalloc(m, &m->k_all, all));
+            L_TRY(qalloc(m, &m->v_all, all));
+            // zeroed like the reference's KV arena (allocate_zeroed_llm_resident_kv_arena)
+            if (cudaMemset(m->k_all, 0, all) != cudaSuccess || cudaMemset(m->v_all, 0, all) != cudaSuccess)
+                return fail(qfail(m, "KV cache zeroing failed"));
+        }
+        L.k_cache = m->k_all + cache * l;
+        L.v_cache = m->v_all + cache * l;
         m->layers.push_back(L);
     }
     m->family = weight_family(m->layers[0].qkv);
@@ -642,6 +735,61 @@ int oasr_b200_qwen_generate(oasr_qwen *m, const float *emb, int32_t emb_on_devic
         return oasr_b200_synchronize(m->be);
     }
     return oasr_internal_launch_check(m->be, "qwen_generate");
+}
+
+int oasr_b200_qwen_verify_tree(oasr_qwen *m, const int32_t *tokens, const int32_t *parents, int32_t n_seq, int32_t n,
+                               const int32_t *pos, int32_t *path, int32_t *n_accept, int32_t *next) {
+    if (!m) return OASR_STATUS_FAILED;
+    if (!tokens || !parents || !pos || !path || !n_accept || !next || n_seq < 1 || n_seq > m->B || n < 1 || n > 1024 ||
+        (int64_t)n_seq * n > (int64_t)m->B * m->Tmax || m->P % 8)
+        return qfail(m, "verify_tree: bad arguments");
+    int st = oasr_internal_precheck(m->be);
+    if (st) return st;
+    const int W = (n + 31) / 32;
+    const size_t rows = (size_t)n_seq * n;
+    // inputs, in the order of the device buffer up to the tables, and the words after it
+    std::vector<int32_t> rowsv(2 * rows), posv(rows), seqv(5 * (size_t)n_seq), words(rows * W);
+    for (int s = 0; s < n_seq; ++s) {
+        if (pos[s] < 0 || (int64_t)pos[s] + n > m->P) return qfail(m, "verify_tree: a tree does not fit the context");
+        if (parents[(size_t)s * n] != -1 || oasr_b200_tree_mask(parents + (size_t)s * n, n, words.data() + (size_t)s * n * W))
+            return qfail(m, "verify_tree: parents must come before their children, node 0 is the root");
+        seqv[s] = pos[s];
+        seqv[4 * (size_t)n_seq + s] = s;  // page s of the caches
+        for (int i = 0; i < n; ++i) {
+            const size_t r = (size_t)s * n + i;
+            if (tokens[r] < 0 || tokens[r] >= m->cfg.n_vocab) return qfail(m, "verify_tree: token out of range");
+            rowsv[r] = tokens[r];
+            rowsv[rows + r] = parents[r];
+            posv[r] = parents[r] < 0 ? pos[s] : posv[(size_t)s * n + parents[r]] + 1;  // pos + depth
+        }
+    }
+    QStreamScope sc(m);
+    if (!m->tree_logits) {
+        const size_t most = (size_t)m->B * m->Tmax;
+        Q_TRY(qalloc(m, &m->tree_logits, (size_t)TREE_CHUNK * m->cfg.n_vocab * 4));
+        Q_TRY(qalloc(m, &m->tree_ints, (most * (5 + 32) + (size_t)m->B * 5) * 4));
+    }
+    const TreeInts t = tree_ints(m, n_seq, n);
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(t.tokens, rowsv.data(), rowsv.size() * 4, cudaMemcpyHostToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(t.pos, posv.data(), posv.size() * 4, cudaMemcpyHostToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(t.n_past, seqv.data(), seqv.size() * 4, cudaMemcpyHostToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(t.words, words.data(), words.size() * 4, cudaMemcpyHostToDevice, m->stream));
+    Q_TRY(run_tree(m, t, n_seq, n));
+    std::vector<int32_t> got(3 * (size_t)n_seq);  // accept, next, past_out lie side by side
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(path, t.path, rows * 4, cudaMemcpyDeviceToHost, m->stream));
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(got.data(), t.accept, got.size() * 4, cudaMemcpyDeviceToHost, m->stream));
+    // the decode state moves on: next inputs, positions, lengths
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(m->tokens, t.next, n_seq * 4, cudaMemcpyDeviceToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(m->pos, t.past_out, n_seq * 4, cudaMemcpyDeviceToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaStreamSynchronize(m->stream));
+    for (int s = 0; s < n_seq; ++s) {
+        n_accept[s] = got[s];
+        next[s] = got[(size_t)n_seq + s];
+        ++got[2 * (size_t)n_seq + s];
+    }
+    OASR_CUDA_TRY(m->be, cudaMemcpyAsync(m->nkv, got.data() + 2 * (size_t)n_seq, n_seq * 4, cudaMemcpyHostToDevice, m->stream));
+    OASR_CUDA_TRY(m->be, cudaStreamSynchronize(m->stream));
+    return oasr_b200_synchronize(m->be);
 }
 
 int oasr_b200_qwen_read_kv(oasr_qwen *m, int32_t layer, int32_t seq, int32_t n_pos, uint16_t *k_out, uint16_t *v_out) {

@@ -33,6 +33,15 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_get_stream),
     OASR_ENTRY(oasr_b200_init),
     OASR_ENTRY(oasr_b200_kv_pages_copy),
+    OASR_ENTRY(oasr_b200_kv_pool_close),
+    OASR_ENTRY(oasr_b200_kv_pool_create),
+    OASR_ENTRY(oasr_b200_kv_pool_extend),
+    OASR_ENTRY(oasr_b200_kv_pool_fork),
+    OASR_ENTRY(oasr_b200_kv_pool_free),
+    OASR_ENTRY(oasr_b200_kv_pool_open),
+    OASR_ENTRY(oasr_b200_kv_pool_pages_free),
+    OASR_ENTRY(oasr_b200_kv_pool_table),
+    OASR_ENTRY(oasr_b200_kv_pool_truncate),
     OASR_ENTRY(oasr_b200_last_error),
     OASR_ENTRY(oasr_b200_mem_stats),
     OASR_ENTRY(oasr_b200_memory_get_api_v1),
@@ -48,6 +57,7 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_qwen_load),
     OASR_ENTRY(oasr_b200_qwen_prefill),
     OASR_ENTRY(oasr_b200_qwen_read_kv),
+    OASR_ENTRY(oasr_b200_qwen_verify_tree),
     OASR_ENTRY(oasr_b200_reserve_scratch),
     OASR_ENTRY(oasr_b200_row_size),
     OASR_ENTRY(oasr_b200_serve_batch_vram_cap),

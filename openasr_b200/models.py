@@ -359,6 +359,52 @@ class QwenModel:
         self.backend._check(bk.lib().oasr_b200_qwen_generate(self.handle, emb_dev.data_ptr(), 1, n_seq, n_tok, n_new,
                                                              QWEN_EOS, 0, tokens_dev.data_ptr(), 1))
 
+    def verify_tree(self, tokens, parents, pos):
+        """Drafted trees tokens / parents [n_seq][n] (node 0: the token selected last, parent -1) at
+        positions pos [n_seq] -> (accepted nodes [n_seq][n] with -1 after them, their number
+        [n_seq], the token after them [n_seq])"""
+        tk, par, ps = (np.ascontiguousarray(x, np.int32) for x in (tokens, parents, pos))
+        if tk.ndim != 2 or par.shape != tk.shape or ps.shape != (tk.shape[0],):
+            raise bk.UnsupportedInputs(bk.STATUS_FAILED, "verify_tree: tokens and parents [n_seq][n], pos [n_seq]")
+        path, acc, nxt = np.empty_like(tk), np.empty(len(ps), np.int32), np.empty(len(ps), np.int32)
+        self.backend._check(bk.lib().oasr_b200_qwen_verify_tree(
+            self.handle, tk.ctypes.data, par.ctypes.data, tk.shape[0], tk.shape[1], ps.ctypes.data, path.ctypes.data,
+            acc.ctypes.data, nxt.ctypes.data))
+        return path, acc, nxt
+
+    def generate_speculative(self, emb: np.ndarray, draft, n_new: int = 256):
+        """prefill + n_new greedy tokens per sequence, several per pass: before each pass
+        draft(s, tokens so far) returns (tokens, parents) of the nodes after the last token of
+        sequence s -- parent -1: the last token itself, else an earlier node of the list --, and
+        the model keeps the longest branch that it would have chosen.  Returns
+        ([n_seq][n_new] tokens, number of passes)."""
+        _, nxt = self.prefill(emb)
+        n, T = emb.shape[0], emb.shape[1]
+        out = [[int(t)] for t in nxt]
+        done, passes = n_new - 1, 0
+        pos = np.full(n, T, np.int32)
+        while min(len(o) for o in out) <= done:
+            trees = [draft(s, out[s]) if len(out[s]) <= done else ([], []) for s in range(n)]
+            room = self.cfg.max_pos - int(pos.max())
+            if room < 1:
+                raise bk.UnsupportedInputs(bk.STATUS_FAILED, "generate_speculative: the context is full")
+            width = min(1 + max(len(t[0]) for t in trees), room)
+            # nodes past a sequence's own draft repeat its root's token under nobody (-1): never accepted
+            tokens, parents = np.zeros((n, width), np.int32), np.full((n, width), -1, np.int32)
+            for s, (tk, par) in enumerate(trees):
+                k = min(len(tk), width - 1)
+                tokens[s] = out[s][-1]
+                tokens[s, 1:1 + k] = tk[:k]
+                parents[s, 1:1 + k] = np.asarray(par[:k], np.int32) + 1
+            path, acc, nxt = self.verify_tree(tokens, parents, pos)
+            passes += 1
+            for s in range(n):
+                if len(out[s]) > done:
+                    continue  # finished: its position stays, the pass's rows for it are dropped
+                out[s] += [int(tokens[s, j]) for j in path[s, 1:acc[s]]] + [int(nxt[s])]
+                pos[s] += acc[s]
+        return np.array([o[:n_new] for o in out], np.int32), passes
+
     def read_kv(self, layer: int, seq: int, n_pos: int):
         """(K, V) f16 [n_kv_heads][n_pos][head_dim] of one layer and sequence"""
         c = self.cfg
