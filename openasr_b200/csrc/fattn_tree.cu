@@ -36,21 +36,18 @@ template <int D_, int RW_, int NWG_, bool QF16_>
 struct TreeTc {
     static constexpr int D = D_, RW = RW_, NWG = NWG_, R = RW * NWG;
     static constexpr bool QF16 = QF16_;
-    // The halves of P are 2 RW columns of one product, and so are those of Q up to 64 rows: K and V
-    // are fetched from shared memory once for both.  Beyond that the halves of Q are two products
-    // into the same columns (TMEM has 512).
-    static constexpr bool QWIDE = !QF16 && R <= 64;
-    static constexpr int SCOLS = QWIDE ? 2 * R : R;
-    // A group's rows go through weights and product in NB blocks of BR rows, with PB blocks under
-    // way: while one is multiplied the next one's weights are made.
-    static constexpr int PB = NWG == 1 ? 1 : 2, NB = RW == 64 ? 2 : 1, BR = RW / NB;
+    // The halves of P are 2 RW columns of one product, and so are those of Q: K and V are fetched
+    // from shared memory once for both.
+    static constexpr int SCOLS = QF16 ? R : 2 * R;
+    // A group has the weights of PB units under way: while one is multiplied the next one's are made.
+    static constexpr int PB = NWG == 1 ? 1 : 2;
     static constexpr int HALF = TREE_BKV * 128;          // 128 positions x 64 values
     static constexpr int TILE = HALF * (D / 64);         // one K or V tile
     static constexpr int QROWS = QF16 ? R : 2 * R;       // rows of Q hi, then of Q lo
     static constexpr int QHALF = QROWS * 128;            // they x 64 values
     static constexpr int QBYTES = QHALF * (D / 64);
-    static constexpr int PBYTES = TREE_BKV * BR * 2;     // a block's P hi, its P lo follows
-    static constexpr int PGROUP = PB * 2 * PBYTES;       // a group's blocks
+    static constexpr int PBYTES = TREE_BKV * RW * 2;     // a group's P hi, its P lo follows
+    static constexpr int PGROUP = PB * 2 * PBYTES;       // a group's units
     static constexpr int CTAS = NWG == 1 ? 2 : 1;
     static constexpr int MISC = CTAS == 2 ? 1024 : 3072;
     static constexpr int FIXED = QBYTES + NWG * PGROUP + MISC;
@@ -69,32 +66,13 @@ struct TreeTc {
     static_assert(OFF_FLAG + 32 <= SMEM, "misc");
     static_assert(RW * D * 4 <= PGROUP, "a group's output rows fit its P");
     static constexpr int SW = 4 * NWG;                   // softmax warps
-    // 64 rows per thread want more than the 168 registers that 10 warps leave: the other two
-    // warps become a group of four that hands registers over (12 warps x 168 = 8 x 216 + 4 x 72)
-    static constexpr bool MOVE_REGS = RW == 64;
-    static constexpr int NT = 32 * (SW + (MOVE_REGS ? 4 : 2));
-    static constexpr int COLS = 2 * SCOLS + NWG * PB * 2 * BR;  // S twice, O of the blocks
+    static constexpr int NT = 32 * (SW + 2);
+    static constexpr int COLS = 2 * SCOLS + NWG * PB * 2 * RW;  // S twice, O of the groups' units
     static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static constexpr int PART = R * (D + 2);             // floats of an unfinished segment
     static constexpr bool JOINS = R <= 32;               // the last CTA joins them (else fattn_tree_join_kernel)
 };
 
-constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
-constexpr float TREE_MOST = 15.0f;  // weights up to 2^15 stay below f16's 65504
-
-
-// K-major operand, 128-byte swizzle: sw128_desc.  M- or N-major operand in the same swizzle
-// (64 values of M contiguous per position): 8-position groups 1024 bytes apart, 64-value blocks
-// `block` bytes apart.
-static __device__ __forceinline__ uint64_t mn_sw128_desc(uint32_t addr, uint32_t block) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(block >> 4) << 16;
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= (uint64_t)1u << 46;
-    d |= (uint64_t)2u << 61;
-    return d;
-}
 // N-major operand without swizzle: 8 x 8 blocks of 128 bytes (8 values of N contiguous, 8
 // positions), `kgroup` bytes to the next 8 positions, `nblock` to the next 8 values of N.
 static __device__ __forceinline__ uint64_t mn_plain_desc(uint32_t addr, uint32_t kgroup, uint32_t nblock) {
@@ -104,42 +82,6 @@ static __device__ __forceinline__ uint64_t mn_plain_desc(uint32_t addr, uint32_t
     d |= (uint64_t)(nblock >> 4) << 32;
     d |= (uint64_t)1u << 46;
     return d;
-}
-static __device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
-}
-// N columns of this warp's 32 lanes (16 at a time, one wait)
-template <int N>
-static __device__ __forceinline__ void tmem_load(uint32_t addr, f32x2 (&v)[N / 2]) {
-    uint32_t r[N / 16][16];
-#pragma unroll
-    for (int x = 0; x < N / 16; ++x) tmem_ld16(addr + 16 * x, r[x]);
-    // the first wait is for all; the others keep the uses of their registers behind it
-#pragma unroll
-    for (int x = 0; x < N / 16; ++x) tmem_ld_wait(r[x]);
-#pragma unroll
-    for (int x = 0; x < N / 2; ++x) v[x] = pack2(__uint_as_float(r[x / 8][2 * (x % 8)]), __uint_as_float(r[x / 8][2 * (x % 8) + 1]));
-}
-// any of the group's 128 threads
-static __device__ __forceinline__ bool group_any(int id, bool x) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
-        "barrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"(id), "r"((uint32_t)x)
-        : "memory");
-    return r != 0;
-}
-static __device__ __forceinline__ void group_sync(int id, int threads) {
-    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-static __device__ __forceinline__ float warp_max_f32(float x) {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
-    return r;
 }
 // Lane l gets the sum (or maximum) over the lanes of v[l]: at each step a lane passes on the half
 // that its partner keeps.  With 16 values lanes l and l + 16 get the same.
@@ -171,7 +113,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                       const __grid_constant__ TreeAttn a, const __grid_constant__ KvPages p,
                       const __grid_constant__ KvSeqs sq, int box, float *parts, TreeJoin *joins, unsigned int *tickets, int *err) {
     using C = TreeTc<D, RW, NWG, QF16>;
-    constexpr int R = C::R, NS = C::NS, NB = C::NB, BR = C::BR;
+    constexpr int R = C::R, NS = C::NS;
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
     griddep_wait();
@@ -212,13 +154,8 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
     };
 
     if (warp >= C::SW) {
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == C::SW) {
-            // ---- TMA: K0, then K(j+1), V(j); lane = (box, half of D) ----
-            constexpr int HALVES = D / 64;
-            const int b = lane / HALVES, half = lane % HALVES;
-            const bool mine = b < TREE_BKV / box;
-            int q = 0;  // tiles issued
+            // ---- TMA: K0, then K(j+1), V(j) ----
             if (lane == 0) {
                 for (int i = 0; i < NS; ++i) {
                     mbar_init(&full[i], 1);
@@ -240,58 +177,13 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             __syncwarp();
             asm volatile("barrier.cta.arrive 4, %0;" ::"n"(C::NT) : "memory");  // it waits for nothing itself
             begun = true;
-            for (int u = u0; u < u1;) {
-                if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
-                const int *row = sq.table + g.s * sq.table_ld;
-                auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
-                    const int t = k * TREE_BKV + b * box;
-                    int pg = p.n_pages;
-                    if (mine && t < g.T) {
-                        pg = __ldg(row + a.page(t));
-                        if (pg < 0 || pg >= p.n_pages) {
-                            atomicOr(err, ERR_BAD_INDEX);
-                            pg = p.n_pages;
-                        }
-                    }
-                    return pg;
-                };
-                auto issue = [&](const CUtensorMap *map, int k, int pg) {
-                    const int slot = q % NS, t = k * TREE_BKV + b * box;
-                    if (mbar_wait(&empty[slot], (uint32_t)(q / NS & 1) ^ 1u, abort_flag, err)) {
-                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], C::TILE);
-                        __syncwarp();
-                        if (mine)
-                            tma_load_4d(smem + slot * C::TILE + half * C::HALF + b * box * 128, map, &full[slot], 64 * half,
-                                        t - a.page(t) * p.page, g.hk, pg);
-                        ++q;
-                    }
-                    __syncwarp();
-                };
-                int pg = page_of(g.k0);
-                issue(&tm_k, g.k0, pg);
-                for (int k = g.k0; k < g.k1; ++k) {
-                    const int next = k + 1 < g.k1 ? page_of(k + 1) : 0;
-                    if (k + 1 < g.k1) issue(&tm_k, k + 1, next);
-                    issue(&tm_v, k, pg);
-                    pg = next;
-                }
-                u = g.next;
-            }
-            tree_zero_padding(a, sq, p.page, blockIdx.x, gridDim.x);
-            // every copy lands before the block ends, also when the others gave up
-            for (int i = max(0, q - NS); i < q; ++i) {
-                const long long t0 = clock64();
-                while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
-                }
-            }
-        } else if (warp > C::SW + 1) {
-            begin();  // only there to hand its registers over
+            tree_stream<D, NS>(&tm_k, &tm_v, a, p, sq, w, g, R, u0, u1, box, smem, full, empty, abort_flag, err);
         } else {
             tmem_alloc(tmem_slot, C::TMEM);
             begin();
             // ---- MMA: the warp stays together, one elected lane issues ----
             constexpr uint32_t id_s = idesc_f16_f32(TREE_BKV, C::SCOLS);
-            constexpr uint32_t id_o = idesc_f16_f32(D, 2 * C::BR) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
+            constexpr uint32_t id_o = idesc_f16_f32(D, 2 * RW) | 1u << 15 | 1u << 16;  // V^T and P^T: M- and N-major
             const uint64_t dk = sw128_desc(smem_u32(smem)), dq = sw128_desc(smem_u32(smem + C::OFF_Q));
             const uint64_t dv = mn_sw128_desc(smem_u32(smem), D == 128 ? C::HALF : 16);
             const uint64_t dp = mn_plain_desc(smem_u32(smem + C::OFF_P), 128, TREE_BKV * 16);
@@ -311,12 +203,9 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                         const uint64_t k = dk + slot * (C::TILE >> 4);
                         const uint32_t to = tm_s + (uint32_t)(j & 1) * C::SCOLS;
 #pragma unroll
-                        for (int part = 0; part < (QF16 || C::QWIDE ? 1 : 2); ++part)
-#pragma unroll
-                            for (int x = 0; x < D / 16; ++x)
-                                umma_f16(to, k + (x >> 2) * (C::HALF >> 4) + 2 * (x & 3),
-                                         dq + part * (R * 128 >> 4) + (x >> 2) * (C::QHALF >> 4) + 2 * (x & 3), id_s,
-                                         part + x != 0);
+                        for (int x = 0; x < D / 16; ++x)
+                            umma_f16(to, k + (x >> 2) * (C::HALF >> 4) + 2 * (x & 3),
+                                     dq + (x >> 2) * (C::QHALF >> 4) + 2 * (x & 3), id_s, x != 0);
                         umma_commit(&s_full[j & 1]);
                         umma_commit(&empty[slot]);
                     }
@@ -330,9 +219,9 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     const int slot = q % NS;
                     ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
 #pragma unroll
-                    for (int i = 0; i < C::NB * NWG; ++i) {  // blocks, and in a block the groups
-                        const int b = j * C::NB + i / NWG, at = i % NWG * C::PB + b % C::PB;
-                        ok = ok && mbar_wait(&p_full[at], (uint32_t)(b / C::PB) & 1u, abort_flag, err);
+                    for (int i = 0; i < NWG; ++i) {
+                        const int at = i * C::PB + j % C::PB;
+                        ok = ok && mbar_wait(&p_full[at], (uint32_t)(j / C::PB) & 1u, abort_flag, err);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
@@ -340,9 +229,9 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                             const uint64_t v = dv + slot * (C::TILE >> 4), pg = dp + at * (2 * C::PBYTES >> 4);
 #pragma unroll
                             for (int x = 0; x < TREE_BKV / 16; ++x)
-                                umma_f16(tm_o + at * 2 * C::BR, v + x * (2048 >> 4), pg + x * (256 >> 4), id_o, x != 0);
+                                umma_f16(tm_o + at * 2 * RW, v + x * (2048 >> 4), pg + x * (256 >> 4), id_o, x != 0);
                             umma_commit(&o_full[at]);
-                            if (i == C::NB * NWG - 1) umma_commit(&empty[slot]);
+                            if (i == NWG - 1) umma_commit(&empty[slot]);
                         }
                         __syncwarp();
                     }
@@ -362,7 +251,6 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         }
     } else {
         // ---- softmax: thread = position for the weights, = value of D for the output ----
-        if (C::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int wg = warp / 4, tid = threadIdx.x & 127;
         const int row0 = wg * RW;                                  // the group's first row of the tile
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -378,59 +266,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         for (int u = u0; u < u1;) {
             if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
             const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
-            // -- Q: 16 bytes of f16 per thread and step --
-            float c = a.scale * 1.4426950408889634f;
-            constexpr int QC = RW * (D / 8) / 128;  // chunks of 8 values per thread
-            uint8_t *qs = smem + C::OFF_Q;
-            auto q_row = [&](int r) -> const char * {
-                const int gr = g.rt * R + row0 + r, node = a.group(gr);
-                return a.q + node * a.q_nb1 + (g.hk * G + gr - node * G) * a.q_nb2 + g.s * a.q_nb3;
-            };
-            if (QF16) {
-#pragma unroll
-                for (int x = 0; x < QC; ++x) {
-                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < live) v = *reinterpret_cast<const uint4 *>(q_row(r) + 16 * ch);
-                    *reinterpret_cast<uint4 *>(qs + (ch >> 3) * C::QHALF + sw128_off(row0 + r, ch & 7)) = v;
-                }
-            } else {
-                float m = 0.0f;
-                float4 v[2 * QC];
-#pragma unroll
-                for (int x = 0; x < QC; ++x) {
-                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
-                    v[2 * x] = v[2 * x + 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (r < live) {
-                        v[2 * x] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
-                        v[2 * x + 1] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < 2 * QC; ++x)
-                    m = fmaxf(m, fmaxf(fmaxf(fabsf(v[x].x), fabsf(v[x].y)), fmaxf(fabsf(v[x].z), fabsf(v[x].w))));
-                m = warp_max_f32(m);
-                float *red = (float *)own_p;
-                if (lane == 0) red[warp & 3] = m;
-                group_sync(1 + wg, 128);
-                m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-                // 2^(8 - e) and its inverse, both in the normal range
-                const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-                const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
-                c *= __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
-#pragma unroll
-                for (int x = 0; x < QC; ++x) {
-                    const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
-                    uint4 hi, lo;
-                    tree_split2(v[2 * x].x * up, v[2 * x].y * up, hi.x, lo.x);
-                    tree_split2(v[2 * x].z * up, v[2 * x].w * up, hi.y, lo.y);
-                    tree_split2(v[2 * x + 1].x * up, v[2 * x + 1].y * up, hi.z, lo.z);
-                    tree_split2(v[2 * x + 1].z * up, v[2 * x + 1].w * up, hi.w, lo.w);
-                    uint8_t *half = qs + (ch >> 3) * C::QHALF;
-                    *reinterpret_cast<uint4 *>(half + sw128_off(row0 + r, ch & 7)) = hi;
-                    *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;
-                }
-            }
+            const float c = tree_load_q<D, RW, R, QF16>(a, g, row0, live, a.scale, smem + C::OFF_Q, C::QHALF, (float *)own_p, 1 + wg);
             if (tid < RW) noff[tid] = -TREE_NONE;
             fence_proxy_async_smem();
             if (!begun) begin();
@@ -441,26 +277,21 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             f32x2 o[RW / 2], l[RW / 2];
 #pragma unroll
             for (int r = 0; r < RW / 2; ++r) o[r] = l[r] = 0ull;
-            // O^T of block b, the `half`-th of its unit, from TMEM to the running output: the products
-            // of both halves of P
-            auto drain = [&](int b, int half) {
-                const int at = wg * C::PB + b % C::PB;
-                mbar_wait(&o_full[at], (uint32_t)(b / C::PB) & 1u, abort_flag, err);
+            // O^T of unit j from TMEM to the running output: the products of both halves of P
+            auto drain = [&](int j) {
+                const int at = wg * C::PB + j % C::PB;
+                mbar_wait(&o_full[at], (uint32_t)(j / C::PB) & 1u, abort_flag, err);
                 tc_fence_after();
-                constexpr int N = BR < 32 ? BR : 32;
 #pragma unroll
-                for (int x = 0; x < 2 * BR / N; ++x) {
-                    f32x2 v[N / 2];
-                    tmem_load<N>(tm_o + lanes + at * 2 * BR + x * N, v);
+                for (int x = 0; x < 2; ++x) {
+                    f32x2 v[RW / 2];
+                    tmem_load<RW>(tm_o + lanes + (at * 2 + x) * RW, v);
 #pragma unroll
-                    for (int i = 0; i < N / 2; ++i) {
-                        f32x2 &to = o[half * BR / 2 + x * N % BR / 2 + i];
-                        to = add2(to, v[i]);
-                    }
+                    for (int i = 0; i < RW / 2; ++i) o[i] = add2(o[i], v[i]);
                 }
             };
             const int n = g.k1 - g.k0, it0 = it;
-            int due = it * NB;  // the first block that is still to be drained
+            int due = it;  // the first unit that is still to be drained
             for (int k = g.k0; k < g.k1; ++k, ++it) {
                 const int t = k * TREE_BKV + tid;             // this thread's position
                 const bool tail = (k + 1) * TREE_BKV > g.past;  // nodes among the positions, or the end
@@ -476,147 +307,114 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 mbar_wait(&s_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, err);
                 tc_fence_after();
                 const uint32_t ts = tm_s + lanes + (uint32_t)(it & 1) * C::SCOLS + row0;
+                uint8_t *p_at = own_p + it % C::PB * (2 * C::PBYTES);
+                f32x2 y[RW / 2];  // scores in powers of two
+                tmem_load<RW>(ts, y);
+                if (C::SCOLS != R) {
+                    f32x2 lo[RW / 2];
+                    tmem_load<RW>(ts + R, lo);
 #pragma unroll
-                for (int half = 0; half < NB; ++half) {
-                    const int b = it * NB + half;
-                    float *noff_b = noff + half * BR;
-                    const uint32_t *bits_b = bits + half * BR;
-                    uint8_t *p_b = own_p + b % C::PB * (2 * C::PBYTES);
-                    f32x2 y[BR / 2];  // scores in powers of two
-                    tmem_load<BR>(ts + half * BR, y);
-                    if (C::SCOLS != R) {
-                        f32x2 lo[BR / 2];
-                        tmem_load<BR>(ts + R + half * BR, lo);
-#pragma unroll
-                        for (int i = 0; i < BR / 2; ++i) y[i] = add2(y[i], lo[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < BR / 2; ++i) y[i] = mul2(y[i], c2);
-                    if (tail) {
-#pragma unroll
-                        for (int i = 0; i < BR / 2; ++i) {
-                            float2 x = unpack2(y[i]);
-                            if (!(bits_b[2 * i] >> lane & 1u)) x.x = -INFINITY;
-                            if (!(bits_b[2 * i + 1] >> lane & 1u)) x.y = -INFINITY;
-                            y[i] = pack2(x.x, x.y);
-                        }
-                    }
-                    const bool fresh = it == it0;
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < BR / 2; i += 2) {
-                        const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff_b + 2 * i);
-                        const float2 x = unpack2(add2(y[i], f.x)), z = unpack2(add2(y[i + 1], f.y));
-                        top = fmaxf(fmaxf(top, fmaxf(x.x, x.y)), fmaxf(z.x, z.y));
-                    }
-                    const bool rescale = group_any(1 + wg, top > TREE_MOST);
-                    // the block that had this one's place; with it its part of P is free
-                    if (due <= b - C::PB) drain(due++, half);
-                    if (rescale) {
-                        // -- new maxima: of the unit's 128 positions, then with what was --
-                        if (NB == 1 && due < b) drain(due++, half);  // the rows' sums are complete
-                        float *red = (float *)p_b, *fac = red;       // [4][BR]
-                        constexpr int N = BR < 32 ? BR : 32;
-#pragma unroll
-                        for (int x = 0; x < BR / N; ++x) {
-                            float v[N];
-#pragma unroll
-                            for (int i = 0; i < N / 2; ++i) {
-                                const float2 e = unpack2(y[x * N / 2 + i]);
-                                v[2 * i] = e.x, v[2 * i + 1] = e.y;
-                            }
-                            const float m = lane_reduce<N, true>(v);
-                            if (lane < N) red[(warp & 3) * BR + N * x + lane] = m;
-                        }
-                        group_sync(1 + wg, 128);
-                        if (tid < BR) {
-                            const float old = -noff_b[tid];
-                            const float m = fmaxf(fmaxf(red[tid], red[BR + tid]), fmaxf(red[2 * BR + tid], red[3 * BR + tid]));
-                            const float now = fmaxf(old, m - TREE_EXP);
-                            noff_b[tid] = -now;
-                            fac[tid] = tree_exp2(old - now);
-                        }
-                        group_sync(1 + wg, 128);
-                        if (!fresh) {
-#pragma unroll
-                            for (int r = 0; r < BR / 2; r += 2) {
-                                const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
-                                f32x2 *ob = o + half * BR / 2, *lb = l + half * BR / 2;
-                                ob[r] = mul2(ob[r], f.x), ob[r + 1] = mul2(ob[r + 1], f.y);
-                                lb[r] = mul2(lb[r], f.x), lb[r + 1] = mul2(lb[r + 1], f.y);
-                            }
-                            group_sync(1 + wg, 128);  // the factors lie where the weights go
-                        }
-                    }
-                    // -- weights: 16 bytes per 8 rows into the N-major P tiles --
-#pragma unroll
-                    for (int x = 0; x < BR / 8; ++x) {
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i += 2) {
-                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff_b + 8 * x + 2 * i);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float2 e = unpack2(add2(y[4 * x + i + h], h ? f.y : f.x));
-                                const f32x2 wt = pack2(tree_exp2(e.x), tree_exp2(e.y));
-                                f32x2 &sum = l[half * BR / 2 + 4 * x + i + h];
-                                sum = add2(sum, wt);
-                                tree_cut2(wt, hi[i + h], lo[i + h]);
-                            }
-                        }
-                        uint8_t *dst = p_b + x * (TREE_BKV * 16) + tid * 16;
-                        *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
-                    if (tail && wg == 0 && half == 0) {
-                        // values of nodes and past the end that are infinite or NaN would make NaN of zero
-                        // weights: zeros here, and what was visible is added at the end
-                        const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
-                        mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
-                        uint8_t *vt = smem + qi % NS * C::TILE;
-                        if (t >= g.past) {
-                            uint32_t any = 0;
-#pragma unroll
-                            for (int ch = 0; ch < D / 8; ++ch) {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
-                                any |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
-                                       ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
-                            }
-                            if (any & 0x80008000u) {  // an exponent of all ones
-                                for (int ch = 0; ch < D / 8; ++ch) {
-                                    uint32_t *v = reinterpret_cast<uint32_t *>(vt + (ch >> 3) * C::HALF + sw128_off(tid, ch & 7));
-                                    for (int x = 0; x < 4; ++x) v[x] &= ~__vcmpeq2(v[x] & 0x7C007C00u, 0x7C007C00u);
-                                }
-                                if (t < g.T) *s_bad = 1u;
-                            }
-                        }
-                    }
-                    tc_fence_before();
-                    fence_proxy_async_smem();
-                    mbar_arrive(&p_full[wg * C::PB + b % C::PB]);
+                    for (int i = 0; i < RW / 2; ++i) y[i] = add2(y[i], lo[i]);
                 }
+#pragma unroll
+                for (int i = 0; i < RW / 2; ++i) y[i] = mul2(y[i], c2);
+                if (tail) {
+#pragma unroll
+                    for (int i = 0; i < RW / 2; ++i) {
+                        float2 x = unpack2(y[i]);
+                        if (!(bits[2 * i] >> lane & 1u)) x.x = -INFINITY;
+                        if (!(bits[2 * i + 1] >> lane & 1u)) x.y = -INFINITY;
+                        y[i] = pack2(x.x, x.y);
+                    }
+                }
+                const bool fresh = it == it0;
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < RW / 2; i += 2) {
+                    const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff + 2 * i);
+                    const float2 x = unpack2(add2(y[i], f.x)), z = unpack2(add2(y[i + 1], f.y));
+                    top = fmaxf(fmaxf(top, fmaxf(x.x, x.y)), fmaxf(z.x, z.y));
+                }
+                const bool rescale = group_any(1 + wg, top > TREE_MOST);
+                // the unit that had this one's place; with it its part of P is free
+                if (due <= it - C::PB) drain(due++);
+                if (rescale) {
+                    // -- new maxima: of the unit's 128 positions, then with what was --
+                    if (due < it) drain(due++);  // the rows' sums are complete
+                    float *red = (float *)p_at, *fac = red;  // [4][RW]
+                    float v[RW];
+#pragma unroll
+                    for (int i = 0; i < RW / 2; ++i) {
+                        const float2 e = unpack2(y[i]);
+                        v[2 * i] = e.x, v[2 * i + 1] = e.y;
+                    }
+                    const float most = lane_reduce<RW, true>(v);
+                    if (lane < RW) red[(warp & 3) * RW + lane] = most;
+                    group_sync(1 + wg, 128);
+                    if (tid < RW) {
+                        const float old = -noff[tid];
+                        const float m = fmaxf(fmaxf(red[tid], red[RW + tid]), fmaxf(red[2 * RW + tid], red[3 * RW + tid]));
+                        const float now = fmaxf(old, m - TREE_EXP);
+                        noff[tid] = -now;
+                        fac[tid] = tree_exp2(old - now);
+                    }
+                    group_sync(1 + wg, 128);
+                    if (!fresh) {
+#pragma unroll
+                        for (int r = 0; r < RW / 2; r += 2) {
+                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
+                            o[r] = mul2(o[r], f.x), o[r + 1] = mul2(o[r + 1], f.y);
+                            l[r] = mul2(l[r], f.x), l[r + 1] = mul2(l[r + 1], f.y);
+                        }
+                        group_sync(1 + wg, 128);  // the factors lie where the weights go
+                    }
+                }
+                // -- weights: 16 bytes per 8 rows into the N-major P tiles --
+#pragma unroll
+                for (int x = 0; x < RW / 8; ++x) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2) {
+                        const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(noff + 8 * x + 2 * i);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float2 e = unpack2(add2(y[4 * x + i + h], h ? f.y : f.x));
+                            const f32x2 wt = pack2(tree_exp2(e.x), tree_exp2(e.y));
+                            f32x2 &sum = l[4 * x + i + h];
+                            sum = add2(sum, wt);
+                            tree_cut2(wt, hi[i + h], lo[i + h]);
+                        }
+                    }
+                    uint8_t *dst = p_at + x * (TREE_BKV * 16) + tid * 16;
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(dst + C::PBYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                if (tail && wg == 0) {
+                    const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1);  // V's place in the ring
+                    mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
+                    if (t >= g.past && tree_clean_v<D>(smem + qi % NS * C::TILE, tid) && t < g.T) *s_bad = 1u;
+                }
+                tc_fence_before();
+                fence_proxy_async_smem();
+                mbar_arrive(&p_full[wg * C::PB + it % C::PB]);
             }
 #pragma unroll
             for (int x = 0; x < C::PB; ++x)
-                if (due < it * NB) drain(due++, NB == 1 ? 0 : x);
+                if (due < it) drain(due++);
             tc_fence_before();
             q += 2 * n;
 
             // -- sums of the weights over the group's positions --
             {
                 float *red = (float *)own_p;  // [4][RW]
-                constexpr int N = RW < 32 ? RW : 32;
+                float v[RW];
 #pragma unroll
-                for (int x = 0; x < RW / N; ++x) {
-                    float v[N];
-#pragma unroll
-                    for (int i = 0; i < N / 2; ++i) {
-                        const float2 e = unpack2(l[x * N / 2 + i]);
-                        v[2 * i] = e.x, v[2 * i + 1] = e.y;
-                    }
-                    const float sum = lane_reduce<N, false>(v);
-                    if (lane < N) red[(warp & 3) * RW + N * x + lane] = sum;
+                for (int i = 0; i < RW / 2; ++i) {
+                    const float2 e = unpack2(l[i]);
+                    v[2 * i] = e.x, v[2 * i + 1] = e.y;
                 }
+                const float sum = lane_reduce<RW, false>(v);
+                if (lane < RW) red[(warp & 3) * RW + lane] = sum;
             }
             group_sync(1 + wg, 128);
             const bool whole = g.k0 == 0 && g.k1 == g.kt;
@@ -732,15 +530,50 @@ bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int tree_prepare(oasr_backend *be, TreeAttn &a, const KvPages &p, const KvSeqs &s, int R, int ctas_per_sm, TreeLaunch *out) {
+    // the longest run of positions, up to a unit, that never crosses a page
+    out->box = std::min(TREE_BKV, p.page & -p.page);
+    if (!tree_page_map(&out->k, p.k, p.k_nb1, p.k_nb2, p.k_nb3, a.D, p.page, a.HKV, p.n_pages, out->box) ||
+        !tree_page_map(&out->v, p.v, p.v_nb1, p.v_nb2, p.v_nb3, a.D, p.page, a.HKV, p.n_pages, out->box))
+        return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: the pages' strides make no tensor map");
+    a.group = FastDiv(a.H / a.HKV);
+    a.page = FastDiv(p.page);
+    const int64_t tiles = ((int64_t)s.N * a.group.d + R - 1) / R;
+    const int64_t most = tiles * a.HKV * a.S * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
+    if (most > INT32_MAX / 2 || (int64_t)s.N * a.group.d > INT32_MAX / 2 || (int64_t)a.S * s.N * a.H > INT32_MAX)
+        return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
+    out->grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * ctas_per_sm));
+    const size_t part = (size_t)R * (a.D + 2) * 4;
+    int st = 0;
+    out->parts = (float *)oasr_internal_scratch(be, out->grid * (2 * part + sizeof(TreeJoin)), &st);
+    out->joins = (TreeJoin *)((char *)out->parts + out->grid * 2 * part);
+    return st;
+}
+
+int tree_join(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s, int R, const TreeLaunch &l) {
+    if (l.grid == 1 || (int64_t)s.MP * p.page <= TREE_BKV) return OASR_STATUS_SUCCESS;  // no item is shared
+    // started while the attention still runs; it waits for its end
+    const bool pdl = be->pdl;
+    be->pdl = true;
+    const dim3 grid(l.grid * (R / 8)), block(2 * a.D);
+    const float *parts = l.parts;
+    const TreeJoin *joins = l.joins;
+    cudaError_t e;
+    if (R == 64) e = a.D == 64 ? launch_k(be, fattn_tree_join_kernel<64, 64>, grid, block, 0, a, parts, joins)
+                               : launch_k(be, fattn_tree_join_kernel<128, 64>, grid, block, 0, a, parts, joins);
+    else e = a.D == 64 ? launch_k(be, fattn_tree_join_kernel<64, 128>, grid, block, 0, a, parts, joins)
+                       : launch_k(be, fattn_tree_join_kernel<128, 128>, grid, block, 0, a, parts, joins);
+    be->pdl = pdl;
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree join launch", __LINE__);
+    return oasr_internal_launch_check(be, "flash_attn_tree join");
+}
+
 template <int D, int RW, int NWG, bool QF16>
 static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvSeqs &s) {
     using C = TreeTc<D, RW, NWG, QF16>;
-    // the longest run of positions, up to a unit, that never crosses a page
-    const int box = std::min(TREE_BKV, p.page & -p.page);
-    CUtensorMap mk, mv;
-    if (!tree_page_map(&mk, p.k, p.k_nb1, p.k_nb2, p.k_nb3, a.D, p.page, a.HKV, p.n_pages, box) ||
-        !tree_page_map(&mv, p.v, p.v_nb1, p.v_nb2, p.v_nb3, a.D, p.page, a.HKV, p.n_pages, box))
-        return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: the pages' strides make no tensor map");
+    TreeLaunch l;
+    const int st = tree_prepare(be, a, p, s, C::R, C::CTAS, &l);
+    if (st) return st;
     static std::atomic<bool> attr_set{false};
     if (!attr_set) {
         const cudaError_t e = cudaFuncSetAttribute(fattn_tree_kernel<D, RW, NWG, QF16>,
@@ -748,43 +581,25 @@ static int launch_tree(oasr_backend *be, TreeAttn a, const KvPages &p, const KvS
         if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
         attr_set = true;
     }
-    a.group = FastDiv(a.H / a.HKV);
-    a.page = FastDiv(p.page);
-    const int64_t tiles = ((int64_t)s.N * (a.H / a.HKV) + C::R - 1) / C::R;
-    const int64_t most = tiles * a.HKV * a.S * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
-    if (most > INT32_MAX / 2 || (int64_t)s.N * (a.H / a.HKV) > INT32_MAX / 2)
-        return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * C::CTAS));
-    int st = 0;
-    float *parts = (float *)oasr_internal_scratch(be, (size_t)grid * (2 * C::PART * 4 + sizeof(TreeJoin)), &st);
-    if (st) return st;
-    TreeJoin *joins = (TreeJoin *)(parts + (size_t)grid * 2 * C::PART);
-    const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RW, NWG, QF16>, dim3(grid), dim3(C::NT), C::SMEM, mk, mv, a, p, s,
-                                   box, parts, joins, be->counters, be->err_word);
+    const cudaError_t e = launch_k(be, fattn_tree_kernel<D, RW, NWG, QF16>, dim3(l.grid), dim3(C::NT), C::SMEM, l.k, l.v, a, p,
+                                   s, l.box, l.parts, l.joins, be->counters, be->err_word);
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
-    if constexpr (!C::JOINS) if (grid > 1 && (int64_t)s.MP * p.page > TREE_BKV) {
-        // started while the attention still runs; it waits for its end
-        const bool pdl = be->pdl;
-        be->pdl = true;
-        const cudaError_t je = launch_k(be, fattn_tree_join_kernel<D, C::R>, dim3(grid * (C::R / 8)), dim3(2 * D), 0, a,
-                                        (const float *)parts, (const TreeJoin *)joins);
-        be->pdl = pdl;
-        if (je != cudaSuccess) return oasr_internal_cuda_fail(be, je, "flash_attn_tree join launch", __LINE__);
-    }
+    if (!C::JOINS) return tree_join(be, a, p, s, C::R, l);
     return oasr_internal_launch_check(be, "flash_attn_tree");
 }
 
 int launch_flash_attn_tree(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s) {
     // the smallest tile that takes all rows of a K/V head, so that K and V are read once
     const int64_t rows = (int64_t)s.N * (a.H / a.HKV);
-#define FT(RW, NWG)                                                                                      \
-    if (rows <= RW * NWG || RW * NWG == 128) {                                                           \
-        if (a.D == 64) return a.q_f16 ? launch_tree<64, RW, NWG, true>(be, a, p, s) : launch_tree<64, RW, NWG, false>(be, a, p, s); \
-        return a.q_f16 ? launch_tree<128, RW, NWG, true>(be, a, p, s) : launch_tree<128, RW, NWG, false>(be, a, p, s);              \
-    }
-    FT(16, 1) FT(16, 2) FT(32, 2) FT(64, 2)
+    if (rows > 64) return launch_tree_wide(be, a, p, s);
+#define FT(DD, RW, NWG, Q) \
+    if (a.D == DD && a.q_f16 == Q && rows <= RW * NWG) return launch_tree<DD, RW, NWG, Q>(be, a, p, s)
+#define FTQ(DD, RW, NWG) FT(DD, RW, NWG, false); FT(DD, RW, NWG, true)
+    FTQ(64, 16, 1); FTQ(64, 16, 2); FTQ(64, 32, 2);
+    FTQ(128, 16, 1); FTQ(128, 16, 2); FTQ(128, 32, 2);
+#undef FTQ
 #undef FT
-    return OASR_STATUS_FAILED;
+    return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: head_dim must be 64 or 128");
 }
 
 }  // namespace oasr

@@ -364,4 +364,212 @@ static __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtenso
         : "memory");
 }
 
+constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
+constexpr float TREE_MOST = 15.0f;  // weights up to 2^15 stay below f16's 65504
+
+
+
+// K-major operand, 128-byte swizzle: sw128_desc.  M- or N-major operand in the same swizzle
+// (64 values of M contiguous per position): 8-position groups 1024 bytes apart, 64-value blocks
+// `block` bytes apart.
+static __device__ __forceinline__ uint64_t mn_sw128_desc(uint32_t addr, uint32_t block) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+static __device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// N columns of this warp's 32 lanes (16 at a time, one wait)
+template <int N>
+static __device__ __forceinline__ void tmem_load(uint32_t addr, f32x2 (&v)[N / 2]) {
+    uint32_t r[N / 16][16];
+#pragma unroll
+    for (int x = 0; x < N / 16; ++x) tmem_ld16(addr + 16 * x, r[x]);
+    // the first wait is for all; the others keep the uses of their registers behind it
+#pragma unroll
+    for (int x = 0; x < N / 16; ++x) tmem_ld_wait(r[x]);
+#pragma unroll
+    for (int x = 0; x < N / 2; ++x) v[x] = pack2(__uint_as_float(r[x / 8][2 * (x % 8)]), __uint_as_float(r[x / 8][2 * (x % 8) + 1]));
+}
+// any of the group's 128 threads
+static __device__ __forceinline__ bool group_any(int id, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+        "barrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"((uint32_t)x)
+        : "memory");
+    return r != 0;
+}
+static __device__ __forceinline__ void group_sync(int id, int threads) {
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+static __device__ __forceinline__ float warp_max_f32(float x) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+// The TMA warp's work: per segment K0, then K(j+1) and V(j), tiles of 128 positions through a ring
+// of NS slots.  A tile is one box per run of positions within a page and 64 values of D; lane =
+// (box, half of D).  Then the padding rows, and the end of all copies.
+template <int D, int NS>
+static __device__ __forceinline__ void tree_stream(const CUtensorMap *tm_k, const CUtensorMap *tm_v, const TreeAttn &a,
+                                                   const KvPages &p, const KvSeqs &sq, const TreeUnits &w, TreeSeg g, int R,
+                                                   int u0, int u1, int box, uint8_t *ring, uint64_t *full, uint64_t *empty,
+                                                   volatile int *abort_flag, int *err) {
+    constexpr int HALVES = D / 64, HALF = TREE_BKV * 128, TILE = HALF * HALVES;
+    const int lane = threadIdx.x & 31, b = lane / HALVES, half = lane % HALVES;
+    const bool mine = b < TREE_BKV / box;
+    int q = 0;  // tiles issued
+    bool ok = true;
+    for (int u = u0; u < u1;) {
+        if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
+        const int *row = sq.table + g.s * sq.table_ld;
+        auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
+            const int t = k * TREE_BKV + b * box;
+            int pg = p.n_pages;
+            if (mine && t < g.T) {
+                pg = __ldg(row + a.page(t));
+                if (pg < 0 || pg >= p.n_pages) {
+                    atomicOr(err, ERR_BAD_INDEX);
+                    pg = p.n_pages;
+                }
+            }
+            return pg;
+        };
+        auto issue = [&](const CUtensorMap *map, int k, int pg) {
+            const int slot = q % NS, t = k * TREE_BKV + b * box;
+            ok = ok && mbar_wait(&empty[slot], (uint32_t)(q / NS & 1) ^ 1u, abort_flag, err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            if (lane == 0) mbar_arrive_expect_tx(&full[slot], TILE);
+            __syncwarp();
+            if (mine)
+                tma_load_4d(ring + slot * TILE + half * HALF + b * box * 128, map, &full[slot], 64 * half,
+                            t - a.page(t) * p.page, g.hk, pg);
+            __syncwarp();
+            ++q;
+        };
+        int pg = page_of(g.k0);
+        issue(tm_k, g.k0, pg);
+        for (int k = g.k0; k < g.k1; ++k) {
+            const int next = k + 1 < g.k1 ? page_of(k + 1) : 0;
+            if (k + 1 < g.k1) issue(tm_k, k + 1, next);
+            issue(tm_v, k, pg);
+            pg = next;
+        }
+        u = g.next;
+    }
+    tree_zero_padding(a, sq, p.page, blockIdx.x, gridDim.x);
+    // every copy lands before the block ends, also when the others gave up
+    for (int i = max(0, q - NS); i < q; ++i) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[i % NS], (uint32_t)(i / NS & 1)) && clock64() - t0 < kMbarWaitLimit) {
+        }
+    }
+}
+
+// Row `r` (a position) of a V tile: values that are infinite or NaN would make NaN of zero weights,
+// so they become zeros, and tree_nonfinite4 adds the visible ones at the end.  True if there were any.
+template <int D>
+static __device__ __forceinline__ bool tree_clean_v(uint8_t *tile, int r) {
+    constexpr int HALF = TREE_BKV * 128;
+    uint32_t any = 0;
+#pragma unroll
+    for (int ch = 0; ch < D / 8; ++ch) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(tile + (ch >> 3) * HALF + sw128_off(r, ch & 7));
+        any |= ((v.x & 0x7C007C00u) + 0x04000400u) | ((v.y & 0x7C007C00u) + 0x04000400u) |
+               ((v.z & 0x7C007C00u) + 0x04000400u) | ((v.w & 0x7C007C00u) + 0x04000400u);
+    }
+    if (!(any & 0x80008000u)) return false;  // no exponent of all ones
+    for (int ch = 0; ch < D / 8; ++ch) {
+        uint32_t *v = reinterpret_cast<uint32_t *>(tile + (ch >> 3) * HALF + sw128_off(r, ch & 7));
+        for (int x = 0; x < 4; ++x) v[x] &= ~__vcmpeq2(v[x] & 0x7C007C00u, 0x7C007C00u);
+    }
+    return true;
+}
+
+// RW rows of a tile's queries (from row0 on, `live` of them real) as 16-bit K-major operands: f16
+// queries as they are, f32 ones times a power of two that brings the largest of the RW rows to 2^8
+// and cut into hi and lo, lo R rows after hi.  One group of 128 threads, barrier `id`; `red`: four
+// floats of shared memory.  Returns the factor that takes the products to powers of two.
+template <int D, int RW, int R, bool QF16>
+static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const TreeSeg &g, int row0, int live, float scale,
+                                                    uint8_t *qs, int qhalf, float *red, int id) {
+    constexpr int QC = RW * (D / 8) / 128;  // chunks of 8 values per thread
+    const int tid = threadIdx.x & 127, G = a.group.d;
+    float c = fabsf(scale) * 1.4426950408889634f;
+    const float sign = scale < 0.0f ? -1.0f : 1.0f;  // a negative scale turns the queries
+    auto q_row = [&](int r) -> const char * {
+        const int gr = g.rt * R + row0 + r, node = a.group(gr);
+        return a.q + node * a.q_nb1 + (g.hk * G + gr - node * G) * a.q_nb2 + g.s * a.q_nb3;
+    };
+    if (QF16) {
+        const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int x = 0; x < QC; ++x) {
+            const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < live) v = *reinterpret_cast<const uint4 *>(q_row(r) + 16 * ch);
+            *reinterpret_cast<uint4 *>(qs + (ch >> 3) * qhalf + sw128_off(row0 + r, ch & 7)) =
+                make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+        }
+        return c;
+    }
+    float m = 0.0f;
+    float4 v[2 * QC];
+#pragma unroll
+    for (int x = 0; x < QC; ++x) {
+        const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+        v[2 * x] = v[2 * x + 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < live) {
+            v[2 * x] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
+            v[2 * x + 1] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < 2 * QC; ++x)
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(v[x].x), fabsf(v[x].y)), fmaxf(fabsf(v[x].z), fabsf(v[x].w))));
+    m = warp_max_f32(m);
+    if ((threadIdx.x & 31) == 0) red[tid >> 5] = m;
+    group_sync(id, 128);
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    // 2^(8 - e) and its inverse, both in the normal range
+    const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
+    const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23) * sign;
+#pragma unroll
+    for (int x = 0; x < QC; ++x) {
+        const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+        uint4 hi, lo;
+        tree_split2(v[2 * x].x * up, v[2 * x].y * up, hi.x, lo.x);
+        tree_split2(v[2 * x].z * up, v[2 * x].w * up, hi.y, lo.y);
+        tree_split2(v[2 * x + 1].x * up, v[2 * x + 1].y * up, hi.z, lo.z);
+        tree_split2(v[2 * x + 1].z * up, v[2 * x + 1].w * up, hi.w, lo.w);
+        uint8_t *half = qs + (ch >> 3) * qhalf;
+        *reinterpret_cast<uint4 *>(half + sw128_off(row0 + r, ch & 7)) = hi;
+        *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;
+    }
+    return c * __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
+}
+
+// host: the launch that the two kernels share (fattn_tree.cu)
+struct TreeLaunch {
+    CUtensorMap k, v;
+    int box, grid;
+    float *parts;
+    TreeJoin *joins;
+};
+int tree_prepare(oasr_backend *be, TreeAttn &a, const KvPages &p, const KvSeqs &s, int R, int ctas_per_sm, TreeLaunch *out);
+int tree_join(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s, int R, const TreeLaunch &l);
+// tiles of 128 rows (fattn_tree_wide.cu)
+int launch_tree_wide(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s);
+
 }  // namespace oasr
