@@ -356,12 +356,20 @@ bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2,
                    int n_pages, int rows);
 
 static __device__ __forceinline__ void tma_load_4d(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z,
-                                                   int w) {
+                                                   int w, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
-            smem_u32(smem_dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, "
+        "%6}], [%2], %7;" ::"r"(smem_u32(smem_dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
         : "memory");
+}
+// K and V that only one tile of rows reads go through L2 first out: what every call starts with --
+// its code, lengths, page tables, queries -- stays.
+static __device__ __forceinline__ uint64_t tree_policy(bool once) {
+    uint64_t p;
+    if (once) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    else asm volatile("createpolicy.fractional.L2::evict_unchanged.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 
 constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
@@ -428,6 +436,7 @@ static __device__ __forceinline__ void tree_stream(const CUtensorMap *tm_k, cons
     constexpr int HALVES = D / 64, HALF = TREE_BKV * 128, TILE = HALF * HALVES;
     const int lane = threadIdx.x & 31, b = lane / HALVES, half = lane % HALVES;
     const bool mine = b < TREE_BKV / box;
+    const uint64_t policy = tree_policy((int64_t)sq.N * a.group.d <= R);
     int q = 0;  // tiles issued
     bool ok = true;
     for (int u = u0; u < u1;) {
@@ -454,7 +463,7 @@ static __device__ __forceinline__ void tree_stream(const CUtensorMap *tm_k, cons
             __syncwarp();
             if (mine)
                 tma_load_4d(ring + slot * TILE + half * HALF + b * box * 128, map, &full[slot], 64 * half,
-                            t - a.page(t) * p.page, g.hk, pg);
+                            t - a.page(t) * p.page, g.hk, pg, policy);
             __syncwarp();
             ++q;
         };
@@ -512,11 +521,12 @@ static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const Tre
         const int gr = g.rt * R + row0 + r, node = a.group(gr);
         return a.q + node * a.q_nb1 + (g.hk * G + gr - node * G) * a.q_nb2 + g.s * a.q_nb3;
     };
+    // short loops: at the start of a call the code itself comes from far away
     if (QF16) {
         const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-        for (int x = 0; x < QC; ++x) {
-            const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+#pragma unroll 4
+        for (int e = tid; e < 128 * QC; e += 128) {
+            const int r = e / (D / 8), ch = e % (D / 8);
             uint4 v = make_uint4(0, 0, 0, 0);
             if (r < live) v = *reinterpret_cast<const uint4 *>(q_row(r) + 16 * ch);
             *reinterpret_cast<uint4 *>(qs + (ch >> 3) * qhalf + sw128_off(row0 + r, ch & 7)) =
@@ -525,19 +535,14 @@ static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const Tre
         return c;
     }
     float m = 0.0f;
-    float4 v[2 * QC];
-#pragma unroll
-    for (int x = 0; x < QC; ++x) {
-        const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
-        v[2 * x] = v[2 * x + 1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int e = tid; e < 256 * QC; e += 128) {
+        const int r = e / (D / 4), ch = e % (D / 4);
         if (r < live) {
-            v[2 * x] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
-            v[2 * x + 1] = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
+            const float4 v = *reinterpret_cast<const float4 *>(q_row(r) + 16 * ch);
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
     }
-#pragma unroll
-    for (int x = 0; x < 2 * QC; ++x)
-        m = fmaxf(m, fmaxf(fmaxf(fabsf(v[x].x), fabsf(v[x].y)), fmaxf(fabsf(v[x].z), fabsf(v[x].w))));
     m = warp_max_f32(m);
     if ((threadIdx.x & 31) == 0) red[tid >> 5] = m;
     group_sync(id, 128);
@@ -545,14 +550,19 @@ static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const Tre
     // 2^(8 - e) and its inverse, both in the normal range
     const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
     const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23) * sign;
-#pragma unroll
-    for (int x = 0; x < QC; ++x) {
-        const int e = tid + 128 * x, r = e / (D / 8), ch = e % (D / 8);
+#pragma unroll 2
+    for (int e = tid; e < 128 * QC; e += 128) {
+        const int r = e / (D / 8), ch = e % (D / 8);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = v;
+        if (r < live) {
+            v = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
+            z = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
+        }
         uint4 hi, lo;
-        tree_split2(v[2 * x].x * up, v[2 * x].y * up, hi.x, lo.x);
-        tree_split2(v[2 * x].z * up, v[2 * x].w * up, hi.y, lo.y);
-        tree_split2(v[2 * x + 1].x * up, v[2 * x + 1].y * up, hi.z, lo.z);
-        tree_split2(v[2 * x + 1].z * up, v[2 * x + 1].w * up, hi.w, lo.w);
+        tree_split2(v.x * up, v.y * up, hi.x, lo.x);
+        tree_split2(v.z * up, v.w * up, hi.y, lo.y);
+        tree_split2(z.x * up, z.y * up, hi.z, lo.z);
+        tree_split2(z.z * up, z.w * up, hi.w, lo.w);
         uint8_t *half = qs + (ch >> 3) * qhalf;
         *reinterpret_cast<uint4 *>(half + sw128_off(row0 + r, ch & 7)) = hi;
         *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;

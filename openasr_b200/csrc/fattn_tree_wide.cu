@@ -228,27 +228,24 @@ __global__ void __launch_bounds__(384, 1)
                 if ((it & 1) != wg) continue;
                 const uint32_t phase = (uint32_t)(it >> 1) & 1u, ts = tmem + lanes + (uint32_t)wg * R;
                 const bool tail = (k + 1) * TREE_BKV > g.past;  // nodes among the positions, or the end
-                uint32_t see[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    see[x] = !tail ? 0xffffffffu : node < 0 ? 0u : tree_sees32(a, g, node, k * TREE_BKV + 32 * x);
                 mbar_wait(&s_full[wg], phase, abort_flag, err);
                 tc_fence_after();
                 auto masked = [&](int x, f32x2 (&y)[16]) {
                     tmem_load<32>(ts + 32 * x, y);
                     if (tail) {
+                        const uint32_t see = node < 0 ? 0u : tree_sees32(a, g, node, k * TREE_BKV + 32 * x);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             float2 e = unpack2(y[i]);
-                            if (!(see[x] >> (2 * i) & 1u)) e.x = -INFINITY;
-                            if (!(see[x] >> (2 * i + 1) & 1u)) e.y = -INFINITY;
+                            if (!(see >> (2 * i) & 1u)) e.x = -INFINITY;
+                            if (!(see >> (2 * i + 1) & 1u)) e.y = -INFINITY;
                             y[i] = pack2(e.x, e.y);
                         }
                     }
                 };
                 f32x2 y[16];
                 float top = -INFINITY, top2 = -INFINITY;
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < 4; ++x) {
                     masked(x, y);
 #pragma unroll
@@ -270,7 +267,7 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 // -- weights, in place of the scores --
                 const f32x2 n2 = pack2(-off, -off);
-#pragma unroll
+#pragma unroll 1
                 for (int x = 0; x < 4; ++x) {
                     masked(x, y);
                     uint32_t h[32];
