@@ -307,7 +307,9 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
  * sees the nodes 0..i; with n = 1 that is a decode step over the pages.  q F32 or F16 [D,
  * n, H, n_seq], dst F32 or F16 [D, H, n, n_seq] as in oasr_b200_flash_attn_ext, H % H_kv
  * == 0.  A row that sees nothing is zeros.  What a row does not see does not reach it: K
- * and V rows of hidden nodes and of positions past the last node may hold anything. */
+ * and V rows of hidden nodes and of positions past the last node may hold anything.  What it
+ * does see and is not finite makes its output NaN or infinite: all of the row for a query or
+ * a K value, that value of D for a V value. */
 int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages,
                               const oasr_tensor *v_pages, const oasr_tensor *page_table, const oasr_tensor *n_past,
                               const oasr_tensor *n_nodes, const oasr_tensor *tree, float scale, oasr_tensor *dst);

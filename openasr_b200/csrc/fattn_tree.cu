@@ -12,7 +12,7 @@
 // so no row of the matrix unit is padding, K and V are used in the layout of the pages, and the
 // work of the softmax threads -- one per position, R weights each -- shrinks with R.
 //
-// f32 accuracy from 16-bit operands: an f32 query (after a power of two that brings the tile's
+// f32 accuracy from 16-bit operands: an f32 query (after a power of two that brings the row's
 // largest value to 2^8) and every weight are two f16 halves, hi + lo, 22 bits; both go through
 // the same product, added in the f32 accumulator.  A unit's O^T is added to the running output
 // in registers, because the tensor cores cut off the bits below a large accumulator.
@@ -57,8 +57,9 @@ struct TreeTc {
     static constexpr int OFF_Q = NS * TILE;
     static constexpr int OFF_P = OFF_Q + QBYTES;
     static constexpr int OFF_MISC = OFF_P + NWG * PGROUP;
-    // misc: off[R], see[NWG][4][RW], barriers, flags
-    static constexpr int OFF_SEE = OFF_MISC + 4 * R;
+    // misc: off[R], query factors [R], see[NWG][4][RW], barriers, flags
+    static constexpr int OFF_FAC = OFF_MISC + 4 * R;
+    static constexpr int OFF_SEE = OFF_FAC + 4 * R;
     static constexpr int OFF_BAR = OFF_SEE + 16 * R;
     static constexpr int NBAR = 2 * NS + 4 + 2 * NWG * PB;
     static constexpr int OFF_FLAG = OFF_BAR + 8 * NBAR;
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         const int d = D == 128 ? tid : 16 * (warp & 3) + lane;
         const bool has_d = D == 128 || lane < 16;
         float *noff = s_off + row0;  // minus the offsets
+        float *fac = (float *)(smem + C::OFF_FAC) + row0;
         uint32_t *see = (uint32_t *)(smem + C::OFF_SEE) + 4 * row0;  // [4][RW]: bits of the unit's positions, by row
         // the group's part of P; while it is free, maxima and sums, then its output rows
         uint8_t *own_p = smem + C::OFF_P + wg * C::PGROUP;
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         for (int u = u0; u < u1;) {
             if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
             const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
-            const float c = tree_load_q<D, RW, R, QF16>(a, g, row0, live, a.scale, smem + C::OFF_Q, C::QHALF, (float *)own_p, 1 + wg);
+            const float c = tree_load_q<D, RW, R, QF16>(a, g, row0, live, a.scale, smem + C::OFF_Q, C::QHALF, fac);
             if (tid < RW) noff[tid] = -TREE_NONE;
             fence_proxy_async_smem();
             if (!begun) begin();
@@ -317,7 +319,10 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                     for (int i = 0; i < RW / 2; ++i) y[i] = add2(y[i], lo[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < RW / 2; ++i) y[i] = mul2(y[i], c2);
+                for (int i = 0; i < RW / 2; i += 2) {
+                    const ulonglong2 f = QF16 ? make_ulonglong2(c2, c2) : *reinterpret_cast<const ulonglong2 *>(fac + 2 * i);
+                    y[i] = mul2(y[i], f.x), y[i + 1] = mul2(y[i + 1], f.y);
+                }
                 if (tail) {
 #pragma unroll
                     for (int i = 0; i < RW / 2; ++i) {
@@ -341,7 +346,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                 if (rescale) {
                     // -- new maxima: of the unit's 128 positions, then with what was --
                     if (due < it) drain(due++);  // the rows' sums are complete
-                    float *red = (float *)p_at, *fac = red;  // [4][RW]
+                    float *red = (float *)p_at, *down = red;  // [4][RW]
                     float v[RW];
 #pragma unroll
                     for (int i = 0; i < RW / 2; ++i) {
@@ -356,13 +361,13 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                         const float m = fmaxf(fmaxf(red[tid], red[RW + tid]), fmaxf(red[2 * RW + tid], red[3 * RW + tid]));
                         const float now = fmaxf(old, m - TREE_EXP);
                         noff[tid] = -now;
-                        fac[tid] = tree_exp2(old - now);
+                        down[tid] = tree_exp2(old - now);
                     }
                     group_sync(1 + wg, 128);
                     if (!fresh) {
 #pragma unroll
                         for (int r = 0; r < RW / 2; r += 2) {
-                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(fac + 2 * r);
+                            const ulonglong2 f = *reinterpret_cast<const ulonglong2 *>(down + 2 * r);
                             o[r] = mul2(o[r], f.x), o[r + 1] = mul2(o[r + 1], f.y);
                             l[r] = mul2(l[r], f.x), l[r + 1] = mul2(l[r + 1], f.y);
                         }

@@ -13,6 +13,8 @@
 // not depend on which CTA came first.
 #pragma once
 
+#include <cfloat>
+
 #include "pages.cuh"
 #include "tc_common.cuh"
 
@@ -375,8 +377,6 @@ static __device__ __forceinline__ uint64_t tree_policy(bool once) {
 constexpr float TREE_EXP = 7.0f;    // weight of the reference maximum: 2^7
 constexpr float TREE_MOST = 15.0f;  // weights up to 2^15 stay below f16's 65504
 
-
-
 // K-major operand, 128-byte swizzle: sw128_desc.  M- or N-major operand in the same swizzle
 // (64 values of M contiguous per position): 8-position groups 1024 bytes apart, 64-value blocks
 // `block` bytes apart.
@@ -507,67 +507,59 @@ static __device__ __forceinline__ bool tree_clean_v(uint8_t *tile, int r) {
 }
 
 // RW rows of a tile's queries (from row0 on, `live` of them real) as 16-bit K-major operands: f16
-// queries as they are, f32 ones times a power of two that brings the largest of the RW rows to 2^8
-// and cut into hi and lo, lo R rows after hi.  One group of 128 threads, barrier `id`; `red`: four
-// floats of shared memory.  Returns the factor that takes the products to powers of two.
+// queries as they are, f32 ones times the scale and cut into hi and lo, lo R rows after hi, each row
+// times a power of two that brings its largest value to 2^8 (its own: a row of huge or infinite values
+// is no other row's business).  One group of 128 threads.  The products times the returned factor
+// (f16), or times the row's factor[] (f32: a power of two, so exactly), are scores in powers of two;
+// neither is ever zero, so that -inf stays -inf.
 template <int D, int RW, int R, bool QF16>
 static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const TreeSeg &g, int row0, int live, float scale,
-                                                    uint8_t *qs, int qhalf, float *red, int id) {
-    constexpr int QC = RW * (D / 8) / 128;  // chunks of 8 values per thread
-    const int tid = threadIdx.x & 127, G = a.group.d;
-    float c = fabsf(scale) * 1.4426950408889634f;
-    const float sign = scale < 0.0f ? -1.0f : 1.0f;  // a negative scale turns the queries
+                                                    uint8_t *qs, int qhalf, float *factor) {
+    const int tid = threadIdx.x & 127, lane = tid & 31, G = a.group.d;
+    const float c = scale * 1.4426950408889634f;
     auto q_row = [&](int r) -> const char * {
         const int gr = g.rt * R + row0 + r, node = a.group(gr);
         return a.q + node * a.q_nb1 + (g.hk * G + gr - node * G) * a.q_nb2 + g.s * a.q_nb3;
     };
     // short loops: at the start of a call the code itself comes from far away
-    if (QF16) {
-        const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;
+    if constexpr (QF16) {
+        const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns the queries
 #pragma unroll 4
-        for (int e = tid; e < 128 * QC; e += 128) {
+        for (int e = tid; e < RW * (D / 8); e += 128) {
             const int r = e / (D / 8), ch = e % (D / 8);
             uint4 v = make_uint4(0, 0, 0, 0);
             if (r < live) v = *reinterpret_cast<const uint4 *>(q_row(r) + 16 * ch);
             *reinterpret_cast<uint4 *>(qs + (ch >> 3) * qhalf + sw128_off(row0 + r, ch & 7)) =
                 make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
         }
-        return c;
-    }
-    float m = 0.0f;
+        return fmaxf(fabsf(c), FLT_MIN);
+    } else {
 #pragma unroll 4
-    for (int e = tid; e < 256 * QC; e += 128) {
-        const int r = e / (D / 4), ch = e % (D / 4);
-        if (r < live) {
-            const float4 v = *reinterpret_cast<const float4 *>(q_row(r) + 16 * ch);
-            m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        for (int e = tid; e < RW * (D / 4); e += 128) {  // a warp has one row, or two of D = 64
+            const int r = e / (D / 4), ch = e % (D / 4);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < live) v = *reinterpret_cast<const float4 *>(q_row(r) + 16 * ch);
+            v = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
+            float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+            if (D == 128) {
+                m = warp_max_f32(m);
+            } else {
+                const float m0 = warp_max_f32(lane < 16 ? m : 0.0f), m1 = warp_max_f32(lane < 16 ? 0.0f : m);
+                m = lane < 16 ? m0 : m1;
+            }
+            // 2^(8 - e2) and its inverse, both in the normal range
+            const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
+            const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
+            uint2 hi, lo;
+            tree_split2(v.x * up, v.y * up, hi.x, lo.x);
+            tree_split2(v.z * up, v.w * up, hi.y, lo.y);
+            uint8_t *half = qs + (ch >> 4) * qhalf + 8 * (ch & 1);
+            *reinterpret_cast<uint2 *>(half + sw128_off(row0 + r, ch >> 1 & 7)) = hi;
+            *reinterpret_cast<uint2 *>(half + sw128_off(R + row0 + r, ch >> 1 & 7)) = lo;
+            if (ch == 0) factor[r] = __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
         }
     }
-    m = warp_max_f32(m);
-    if ((threadIdx.x & 31) == 0) red[tid >> 5] = m;
-    group_sync(id, 128);
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    // 2^(8 - e) and its inverse, both in the normal range
-    const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 100);
-    const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23) * sign;
-#pragma unroll 2
-    for (int e = tid; e < 128 * QC; e += 128) {
-        const int r = e / (D / 8), ch = e % (D / 8);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f), z = v;
-        if (r < live) {
-            v = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch);
-            z = *reinterpret_cast<const float4 *>(q_row(r) + 32 * ch + 16);
-        }
-        uint4 hi, lo;
-        tree_split2(v.x * up, v.y * up, hi.x, lo.x);
-        tree_split2(v.z * up, v.w * up, hi.y, lo.y);
-        tree_split2(z.x * up, z.y * up, hi.z, lo.z);
-        tree_split2(z.z * up, z.w * up, hi.w, lo.w);
-        uint8_t *half = qs + (ch >> 3) * qhalf;
-        *reinterpret_cast<uint4 *>(half + sw128_off(row0 + r, ch & 7)) = hi;
-        *reinterpret_cast<uint4 *>(half + sw128_off(R + row0 + r, ch & 7)) = lo;
-    }
-    return c * __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
+    return 1.0f;
 }
 
 // host: the launch that the two kernels share (fattn_tree.cu)

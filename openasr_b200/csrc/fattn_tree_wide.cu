@@ -28,9 +28,9 @@ struct TreeWide {
     static constexpr int NS = MOST / TILE > 8 ? 8 : MOST / TILE;
     static_assert(NS >= 4, "K of two units, K and V of the next");
     static constexpr int OFF_Q = NS * TILE, OFF_MISC = OFF_Q + QBYTES;
-    // misc: (offset, sum) [2][R], query factors [2], barriers, flags
+    // misc: (offset, sum) [2][R], query factors [R], barriers, flags
     static constexpr int OFF_C = OFF_MISC + 16 * R;
-    static constexpr int OFF_BAR = OFF_C + 16;
+    static constexpr int OFF_BAR = OFF_C + 4 * R;
     static constexpr int OFF_FLAG = OFF_BAR + 8 * (2 * NS + 8);
     static constexpr int SMEM = OFF_MISC + MISC;
     static_assert(OFF_FLAG + 32 <= SMEM, "misc");
@@ -208,14 +208,13 @@ __global__ void __launch_bounds__(384, 1)
         for (int u = u0; u < u1;) {
             if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
             const int live = g.n * G - g.rt * R;  // rows of the tile below this are real
-            const float c_own = tree_load_q<D, 64, R, QF16>(a, g, 64 * wg, live - 64 * wg, a.scale, smem + C::OFF_Q, C::QHALF,
-                                                            (float *)(s_ml + wg * R), 1 + wg);
-            if (tid == 0) s_c[wg] = c_own;
+            const float c16 = tree_load_q<D, 64, R, QF16>(a, g, 64 * wg, live - 64 * wg, a.scale, smem + C::OFF_Q, C::QHALF,
+                                                          s_c + 64 * wg);
             fence_proxy_async_smem();
             if (!begun) begin();
             else group_sync(3, 256);
             mbar_arrive(q_full);
-            const float c = s_c[tid / 64];
+            const float c = QF16 ? c16 : s_c[tid];
             const f32x2 c2 = pack2(c, c);
             const int node = tid < live ? a.group(g.rt * R + tid) : -1;
 
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(384, 1)
                         top2 = fmaxf(top2, fmaxf(f.x, f.y));
                     }
                 }
-                top = fmaxf(top, top2) * c;  // (c is not negative: the sign of the scale is in Q)
+                top = fmaxf(top, top2) * c;  // (c is positive: the sign of the scale is in Q)
                 const bool more = top - off > TREE_MOST;
                 if (__any_sync(0xffffffffu, more)) {
                     const float now = more ? fmaxf(off, top - TREE_EXP) : off, f = tree_exp2(off - now);

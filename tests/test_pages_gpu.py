@@ -110,7 +110,7 @@ def attend64(c, q, live, sees, scale):
                 x = kk @ q[s, h, i].astype(np.float64) * scale
                 w = np.exp(x - x.max())
                 out[s, i, h] = (w / w.sum()) @ vv
-                ds = 2.0**-20 * scale * (np.abs(kk) @ np.abs(q[s, h, i].astype(np.float64))).max()
+                ds = 2.0**-20 * abs(scale) * (np.abs(kk) @ np.abs(q[s, h, i].astype(np.float64))).max()
                 tol[s, i, h] = 2 * (2 * ds + 2.0**-20) * np.abs(vv).max()
     return out, tol
 
@@ -263,6 +263,80 @@ def test_an_infinite_value_reaches_the_rows_that_see_it(be, N):
     check(got, want, tol, False)
 
 
+@pytest.mark.parametrize("S,N,H,HKV,D,page,past", [
+    (1, 12, 4, 2, 128, 64, [20000]),      # 24, 60, 63 and 200 rows over a long cache: many parts of an item
+    (2, 30, 4, 2, 64, 32, [9000, 137]),
+    (1, 9, 14, 2, 128, 16, [15001]),
+    (2, 50, 8, 2, 128, 64, [11000, 300]),
+    (1, 100, 4, 2, 64, 256, [16383]),
+])
+def test_long_caches(be, S, N, H, HKV, D, page, past):
+    rng = np.random.default_rng(N)
+    c = Cache(rng, S, N, HKV, D, page, past)
+    q = rng.standard_normal((S, H, N, D)).astype(np.float32)
+    sees = np.stack([sees_of(p) for p in random_parents(rng, S, N)])
+    want, tol = attend64(c, q, [N] * S, sees, 1 / math.sqrt(D))
+    check(run_attn(be, c, q, None, words_of(sees), 1 / math.sqrt(D)), want, tol, False)
+
+
+@pytest.mark.parametrize("S,N,H,HKV,D,page", [(33, 1, 2, 1, 128, 64), (70, 5, 4, 2, 64, 16), (40, 40, 4, 2, 128, 32)])
+def test_more_sequences_than_lanes(be, S, N, H, HKV, D, page):
+    """ragged batches, empty sequences among them"""
+    rng = np.random.default_rng(S)
+    past = [int(x) for x in rng.integers(0, 700, S)]
+    past[0], past[S - 1] = 0, 900
+    c = Cache(rng, S, N, HKV, D, page, past)
+    live = rng.integers(0, N + 1, S).astype(np.int32)
+    live[S - 1] = N
+    q = rng.standard_normal((S, H, N, D)).astype(np.float32)
+    sees = np.broadcast_to(np.tril(np.ones((N, N), bool)), (S, N, N))
+    want, tol = attend64(c, q, live, sees, 0.1)
+    check(run_attn(be, c, q, live, None, 0.1), want, tol, False)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("N", [3, 14, 30, 80])
+@pytest.mark.parametrize("scale", [-0.11, 0.0])
+def test_scales_that_are_not_positive(be, N, scale, f16):
+    rng = np.random.default_rng(20)
+    c = Cache(rng, 2, N, 2, 128, 16, [150, 0])
+    q = rng.standard_normal((2, 4, N, 128)).astype(np.float16 if f16 else np.float32)
+    sees = np.stack([sees_of(p) for p in random_parents(rng, 2, N)])
+    want, tol = attend64(c, q, [N, N], sees, scale)
+    check(run_attn(be, c, q, None, words_of(sees), scale, f16), want, tol, f16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [7, 14, 30, 80])
+def test_rows_of_very_different_queries(be, N, D):
+    """a row's accuracy goes by its own size, whatever lies beside it in a tile"""
+    rng = np.random.default_rng(21)
+    c = Cache(rng, 1, N, 2, D, 16, [300])
+    size = 2.0 ** rng.integers(-40, 4, (1, 4, N, 1))
+    size[0, 1, 2] = 2.0**90      # scores past 2^90: one weight is all that is left
+    q = (rng.standard_normal((1, 4, N, D)) * size).astype(np.float32)
+    q[0, 2, 3] = 0
+    sees = np.tril(np.ones((1, N, N), bool))
+    want, tol = attend64(c, q, [N], sees, 0.1)
+    check(run_attn(be, c, q, None, None, 0.1), want, tol, False)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("N", [7, 14, 30, 80])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_query_that_is_not_finite_spoils_its_own_row_alone(be, N, bad, f16):
+    rng = np.random.default_rng(22)
+    c = Cache(rng, 1, N, 2, 128, 16, [200])
+    q = rng.standard_normal((1, 4, N, 128)).astype(np.float16 if f16 else np.float32)
+    sees = np.tril(np.ones((1, N, N), bool))
+    want, tol = attend64(c, q, [N], sees, 0.1)
+    q[0, 1, 4, 17] = bad   # times positive and negative keys: the softmax has no value
+    got = run_attn(be, c, q, None, None, 0.1, f16)
+    assert np.isnan(got[0, 4, 1]).all()
+    got[0, 4, 1] = want[0, 4, 1]
+    check(got, want, tol, f16)
+
+
 @pytest.mark.parametrize("layout", ["head", "row"])
 @pytest.mark.parametrize("N,H,HKV", [(1, 16, 8), (12, 16, 8), (70, 4, 2)])
 def test_strides(be, layout, N, H, HKV):
@@ -342,6 +416,43 @@ def test_on_another_stream_and_in_a_captured_step(be):
         with torch.cuda.graph(g, stream=side):
             be.flash_attn_tree(qd, k, v, table, past, None, None, 0.1, out)
         for step in ([300, 200], [17, 64], [0, 299]):
+            past.copy_(torch.tensor(step, dtype=torch.int32))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            c.past = np.array(step, np.int32)
+            want, tol = attend64(c, q, [N, N], sees, 0.1)
+            check(out.cpu().double().numpy(), want, tol, False)
+        del g
+    finally:
+        be.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("N", [30, 70])
+def test_a_captured_call_with_a_join(be, N):
+    """items shared by many CTAs, replayed with other lengths: long, within a unit, long again"""
+    import torch
+
+    rng = np.random.default_rng(23)
+    c = Cache(rng, 2, N, 2, 128, 64, [4000, 2500])
+    q = rng.standard_normal((2, 4, N, 128)).astype(np.float32)
+    sees = np.broadcast_to(np.tril(np.ones((N, N), bool)), (2, N, N))
+    k, v = c.device()
+    k.nan_to_num_(0.0), v.nan_to_num_(0.0)
+    c.k, c.v = np.nan_to_num(c.k), np.nan_to_num(c.v)
+    qd, table, past = cuda(q), cuda(c.table), cuda(c.past)
+    out = torch.zeros(2, N, 4, 128, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    be.set_stream(side)
+    try:
+        be.flash_attn_tree(qd, k, v, table, past, None, None, 0.1, out)
+        be.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            be.flash_attn_tree(qd, k, v, table, past, None, None, 0.1, out)
+            be.flash_attn_tree(qd, k, v, table, past, None, None, 0.1, out)
+        for step in ([4000, 2500], [0, 5], [3999, 100]):
             past.copy_(torch.tensor(step, dtype=torch.int32))
             torch.cuda.synchronize()
             g.replay()
