@@ -77,67 +77,66 @@ struct NormRope {
     int64_t pos_ld;
     int S, H, HKV;
     float eps;
-    bool gains16;  // both gains there, and 16-byte aligned
+    bool gains8;  // both gains there, and 8-byte aligned
 };
 
 // y = x / sqrt(mean(x^2) + eps) * w, then pair (i, i + D/2) turned by the angle of the node's
-// position: (a cos - b sin, b cos + a sin).  A warp takes U heads of one node, D / 32 values per
-// lane, the pair's other half 16 lanes away; what depends on the node alone (lengths, page,
-// angles, gains) is fetched once for all of them.  The squares are summed in 64 bits and every
-// product rounded as the Qwen driver's own kernel does, so both give the same bits; the sums of
-// U heads share one butterfly (at each step a lane passes on the heads its partner keeps).  Bound by HBM for prompts: eight prompts of 512 rows (97 MB) take
-// 28 us (29 with eight heads per warp, 34 with two); for a step's few rows by three dependent loads and the launch.
+// position: (a cos - b sin, b cos + a sin).  D / 4 lanes take a head, two neighbouring values and
+// the two they turn with per lane, so that the rotation needs no other lane; a warp takes U rounds
+// of heads of one node, and what depends on the node alone (lengths, page, angles, gains) is
+// fetched once for all of them.  The squares are summed in 64 bits and every product rounded as the
+// Qwen driver's own kernel does, so both give the same bits; the sums of the U rounds share one
+// butterfly (at each step a lane passes on the heads its partner keeps).
 template <int D, int U, bool QF16>
 __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page,
                                                            int groups, int *err) {
-    constexpr int V = D / 32, W = U == 1 ? 8 : 4;  // values per lane, warps per block
+    constexpr int LPH = D / 4, HPW = 32 / LPH;  // lanes per head, heads per warp and round
+    constexpr int W = (U == 1 ? 8 : 4) * HPW;   // heads per block and round
     griddep_launch_dependents();
     griddep_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, l = lane % LPH;
     const int HH = a.H + 2 * a.HKV;
-    const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (W * U) + warp;
+    const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (W * U) + threadIdx.x / LPH;
     const int s = nodes(token), i = token - s * sq.N;
-    float v[U][V];
-    const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + 4 * V * lane;
+    float2 lo[U], hi[U];  // values 2 l, 2 l + 1 and D / 2 further
+    const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + 8 * l;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int h = h0 + W * u;
         if (h < HH) {
-            if (V == 4) *reinterpret_cast<float4 *>(v[u]) = *reinterpret_cast<const float4 *>(x + h * a.x_nb1);
-            else *reinterpret_cast<float2 *>(v[u]) = *reinterpret_cast<const float2 *>(x + h * a.x_nb1);
+            lo[u] = *reinterpret_cast<const float2 *>(x + h * a.x_nb1);
+            hi[u] = *reinterpret_cast<const float2 *>(x + h * a.x_nb1 + 2 * D);
+        } else {
+            lo[u] = hi[u] = make_float2(0.0f, 0.0f);
         }
     }
     int past, n;
     if (!seq_lengths(sq, s, p.page, past, n) && threadIdx.x == 0) atomicOr(err, ERR_BAD_INDEX);
     const bool live = i < n;
-    char *q = a.q + i * a.q_nb2 + s * a.q_nb3 + (QF16 ? 2 : 4) * V * lane;
+    char *q = a.q + i * a.q_nb2 + s * a.q_nb3 + (QF16 ? 4 : 8) * l;
+    constexpr int HALF = QF16 ? D : 2 * D;  // bytes
     if (!live) {  // padding nodes leave zeros in q, nothing in the cache
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = h0 + W * u;
             if (h >= a.H) break;
-            if (QF16 && V == 4) *reinterpret_cast<uint2 *>(q + h * a.q_nb1) = make_uint2(0, 0);
-            else if (QF16) *reinterpret_cast<uint32_t *>(q + h * a.q_nb1) = 0;
-            else if (V == 4) *reinterpret_cast<float4 *>(q + h * a.q_nb1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            else *reinterpret_cast<float2 *>(q + h * a.q_nb1) = make_float2(0.0f, 0.0f);
+            char *d = q + h * a.q_nb1;
+            if (QF16) *reinterpret_cast<uint32_t *>(d) = 0, *reinterpret_cast<uint32_t *>(d + HALF) = 0;
+            else *reinterpret_cast<uint2 *>(d) = make_uint2(0, 0), *reinterpret_cast<uint2 *>(d + HALF) = make_uint2(0, 0);
         }
         return;
     }
-    // this lane's V gains and angles
-    float wq[V], wk[V], cs[2 * V];
-    if (a.gains16) {
-        if (V == 4) {
-            *reinterpret_cast<float4 *>(wq) = reinterpret_cast<const float4 *>(a.q_norm)[lane];
-            *reinterpret_cast<float4 *>(wk) = reinterpret_cast<const float4 *>(a.k_norm)[lane];
-        } else {
-            *reinterpret_cast<float2 *>(wq) = reinterpret_cast<const float2 *>(a.q_norm)[lane];
-            *reinterpret_cast<float2 *>(wk) = reinterpret_cast<const float2 *>(a.k_norm)[lane];
-        }
-    } else {
+    // this lane's gains, and the two angles
+    float2 wq[2], wk[2], cs[2];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            wq[j] = a.q_norm ? a.q_norm[V * lane + j] : 1.0f;
-            wk[j] = a.k_norm ? a.k_norm[V * lane + j] : 1.0f;
+    for (int j = 0; j < 2; ++j) {
+        const int c = 2 * l + j * (D / 2);
+        if (a.gains8) {
+            wq[j] = *reinterpret_cast<const float2 *>(a.q_norm + c);
+            wk[j] = *reinterpret_cast<const float2 *>(a.k_norm + c);
+        } else {
+            wq[j] = a.q_norm ? make_float2(a.q_norm[c], a.q_norm[c + 1]) : make_float2(1.0f, 1.0f);
+            wk[j] = a.k_norm ? make_float2(a.k_norm[c], a.k_norm[c + 1]) : make_float2(1.0f, 1.0f);
         }
     }
     if (a.rope) {
@@ -146,12 +145,8 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
             if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
             t = 0;
         }
-        const float *from = a.rope + (int64_t)t * D + 2 * V * (lane & 15);
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-            const float2 c0 = *reinterpret_cast<const float2 *>(from + 2 * j), c1 = *reinterpret_cast<const float2 *>(from + 2 * j + 2);
-            cs[2 * j] = c0.x, cs[2 * j + 1] = c0.y, cs[2 * j + 2] = c1.x, cs[2 * j + 3] = c1.y;
-        }
+        const float2 *from = reinterpret_cast<const float2 *>(a.rope + (int64_t)t * D) + 2 * l;
+        cs[0] = from[0], cs[1] = from[1];
     }
     const int at = past + i, pj = page(at);
     const int64_t off = at - pj * p.page;
@@ -160,20 +155,19 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
         if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
         pg = -1;
     }
-    // sums of squares: lane l ends with that of head u = l / (32 / U)
+    // sums of squares: lane LPH / U * u of a head's lanes ends with that of round u
     float scale = 0.0f;
     {
         double ss[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             ss[u] = 0.0;
-            if (h0 + W * u < a.H + a.HKV) {  // value heads have no norm
-#pragma unroll
-                for (int j = 0; j < V; ++j) ss[u] += (double)__fmul_rn(v[u][j], v[u][j]);
-            }
+            if (h0 + W * u < a.H + a.HKV)  // value heads have no norm
+                ss[u] = ((double)__fmul_rn(lo[u].x, lo[u].x) + (double)__fmul_rn(lo[u].y, lo[u].y)) +
+                        ((double)__fmul_rn(hi[u].x, hi[u].x) + (double)__fmul_rn(hi[u].y, hi[u].y));
         }
 #pragma unroll
-        for (int o = 16, m = U / 2; o > 0; o >>= 1, m >>= 1) {
+        for (int o = LPH / 2, m = U / 2; o > 0; o >>= 1, m >>= 1) {
             const bool up = lane & o;
             if (m == 0) ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], o);
 #pragma unroll
@@ -186,38 +180,35 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int h = h0 + W * u;
-        if (h >= HH) break;
         const bool isq = h < a.H, isk = !isq && h < a.H + a.HKV;
-        const float sc = U == 1 ? scale : __shfl_sync(0xffffffffu, scale, 32 / U * u);
+        const float sc = U == 1 ? scale : __shfl_sync(0xffffffffu, scale, LPH / U * u, LPH);
+        if (h >= HH) continue;
         if (isq ? a.q_norm != nullptr : isk && a.k_norm) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[u][j] = __fmul_rn(__fmul_rn(v[u][j], sc), isq ? wq[j] : wk[j]);
+            const float2 w0 = isq ? wq[0] : wk[0], w1 = isq ? wq[1] : wk[1];
+            lo[u] = make_float2(__fmul_rn(__fmul_rn(lo[u].x, sc), w0.x), __fmul_rn(__fmul_rn(lo[u].y, sc), w0.y));
+            hi[u] = make_float2(__fmul_rn(__fmul_rn(hi[u].x, sc), w1.x), __fmul_rn(__fmul_rn(hi[u].y, sc), w1.y));
         }
         if (a.rope && (isq || isk)) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float other = __shfl_xor_sync(0xffffffffu, v[u][j], 16);
-                v[u][j] = lane < 16 ? __fsub_rn(__fmul_rn(v[u][j], cs[2 * j]), __fmul_rn(other, cs[2 * j + 1]))
-                                    : __fadd_rn(__fmul_rn(other, cs[2 * j + 1]), __fmul_rn(v[u][j], cs[2 * j]));
-            }
-        }
-        if (isq && !QF16) {
-            if (V == 4) *reinterpret_cast<float4 *>(q + h * a.q_nb1) = *reinterpret_cast<const float4 *>(v[u]);
-            else *reinterpret_cast<float2 *>(q + h * a.q_nb1) = *reinterpret_cast<const float2 *>(v[u]);
-            continue;
+            const float2 f = lo[u], g = hi[u];
+            lo[u] = make_float2(__fsub_rn(__fmul_rn(f.x, cs[0].x), __fmul_rn(g.x, cs[0].y)),
+                                __fsub_rn(__fmul_rn(f.y, cs[1].x), __fmul_rn(g.y, cs[1].y)));
+            hi[u] = make_float2(__fadd_rn(__fmul_rn(f.x, cs[0].y), __fmul_rn(g.x, cs[0].x)),
+                                __fadd_rn(__fmul_rn(f.y, cs[1].y), __fmul_rn(g.y, cs[1].x)));
         }
         char *dst = q + h * a.q_nb1;
+        if (isq && !QF16) {
+            *reinterpret_cast<float2 *>(dst) = lo[u];
+            *reinterpret_cast<float2 *>(dst + HALF) = hi[u];
+            continue;
+        }
         if (!isq) {
             if (pg < 0) continue;
             dst = isk ? p.k + pg * p.k_nb3 + (h - a.H) * p.k_nb2 + off * p.k_nb1
                       : p.v + pg * p.v_nb3 + (h - a.H - a.HKV) * p.v_nb2 + off * p.v_nb1;
-            dst += 2 * V * lane;
+            dst += 4 * l;
         }
-        __half2 o[V / 2];
-#pragma unroll
-        for (int j = 0; j < V; j += 2) o[j / 2] = __floats2half2_rn(v[u][j], v[u][j + 1]);
-        if (V == 4) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
-        else *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(o);
+        *reinterpret_cast<__half2 *>(dst) = __floats2half2_rn(lo[u].x, lo[u].y);
+        *reinterpret_cast<__half2 *>(dst + D) = __floats2half2_rn(hi[u].x, hi[u].y);
     }
 }
 
@@ -412,10 +403,11 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.pos_ld = pos ? pos->nb[1] / 4 : 0;
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
-    a.gains16 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 15) == 0;
-    // four heads per warp share what belongs to the node, as long as that leaves every SM some
-    // blocks; below that one head per warp, so that a step's few rows start at once
-    const int64_t HH = qkv->ne[1], few = (HH + 7) / 8, many = (HH + 15) / 16;
+    a.gains8 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 7) == 0;
+    // four rounds of heads per warp share what belongs to the node, as long as that leaves every SM
+    // some blocks; below that one round per warp, so that a step's few rows start at once
+    const int64_t HH = qkv->ne[1], per = D == 64 ? 2 : 1, few = (HH + 8 * per - 1) / (8 * per),
+                  many = (HH + 16 * per - 1) / (16 * per);
     const bool share = S * N * many >= 4 * be->sm_count;
     const int groups = (int)(share ? many : few);
     if (S * N * groups > INT32_MAX) return fail_op(be, op, "too many rows");
