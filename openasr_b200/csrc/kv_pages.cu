@@ -84,9 +84,11 @@ struct NormRope {
 // position: (a cos - b sin, b cos + a sin).  D / 4 lanes take a head, two neighbouring values and
 // the two they turn with per lane, so that the rotation needs no other lane; a warp takes U rounds
 // of heads of one node, and what depends on the node alone (lengths, page, angles, gains) is
-// fetched once for all of them.  The squares are summed in 64 bits and every product rounded as the
-// Qwen driver's own kernel does, so both give the same bits; the sums of the U rounds share one
-// butterfly (at each step a lane passes on the heads its partner keeps).
+// fetched once for all of them.  The sums of squares of the U rounds share one butterfly (at each
+// step a lane passes on the heads its partner keeps).  For prompts bound by HBM and the issue of
+// some 100 instructions per head: eight prompts of 512 rows of 16 + 16 heads (97 MB) take 24 us, 4.0
+// TB/s (30 us with two rounds per warp; 24 with eight, but then eight trees of 61 nodes of D = 64 take
+// 6.4 instead of 4.1 us).  For a step's few rows by three dependent loads and the launch: 2.5 us.
 template <int D, int U, bool QF16>
 __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page,
                                                            int groups, int *err) {
@@ -99,13 +101,14 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
     const int token = blockIdx.x / groups, h0 = (blockIdx.x - token * groups) * (W * U) + threadIdx.x / LPH;
     const int s = nodes(token), i = token - s * sq.N;
     float2 lo[U], hi[U];  // values 2 l, 2 l + 1 and D / 2 further
-    const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + 8 * l;
+    const char *x = a.x + i * a.x_nb2 + s * a.x_nb3 + h0 * a.x_nb1 + 8 * l;
+    const int64_t x_step = W * a.x_nb1;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u, x += x_step) {
         const int h = h0 + W * u;
         if (h < HH) {
-            lo[u] = *reinterpret_cast<const float2 *>(x + h * a.x_nb1);
-            hi[u] = *reinterpret_cast<const float2 *>(x + h * a.x_nb1 + 2 * D);
+            lo[u] = *reinterpret_cast<const float2 *>(x);
+            hi[u] = *reinterpret_cast<const float2 *>(x + 2 * D);
         } else {
             lo[u] = hi[u] = make_float2(0.0f, 0.0f);
         }
@@ -155,16 +158,16 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
         if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
         pg = -1;
     }
+    char *k_row = p.k + pg * p.k_nb3 + off * p.k_nb1 + 4 * l, *v_row = p.v + pg * p.v_nb3 + off * p.v_nb1 + 4 * l;
     // sums of squares: lane LPH / U * u of a head's lanes ends with that of round u
     float scale = 0.0f;
     {
-        double ss[U];
+        float ss[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ss[u] = 0.0;
+            ss[u] = 0.0f;
             if (h0 + W * u < a.H + a.HKV)  // value heads have no norm
-                ss[u] = ((double)__fmul_rn(lo[u].x, lo[u].x) + (double)__fmul_rn(lo[u].y, lo[u].y)) +
-                        ((double)__fmul_rn(hi[u].x, hi[u].x) + (double)__fmul_rn(hi[u].y, hi[u].y));
+                ss[u] = fmaf(lo[u].x, lo[u].x, lo[u].y * lo[u].y) + fmaf(hi[u].x, hi[u].x, hi[u].y * hi[u].y);
         }
 #pragma unroll
         for (int o = LPH / 2, m = U / 2; o > 0; o >>= 1, m >>= 1) {
@@ -174,8 +177,7 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
             for (int k = 0; k < m; ++k)
                 ss[k] = (up ? ss[k + m] : ss[k]) + __shfl_xor_sync(0xffffffffu, up ? ss[k] : ss[k + m], o);
         }
-        const double t = ss[0];
-        scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(t / (double)D), a.eps)));
+        scale = __frcp_rn(__fsqrt_rn(fmaf(ss[0], 1.0f / D, a.eps)));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -203,9 +205,7 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128) qk_norm_rope_kernel(NormRo
         }
         if (!isq) {
             if (pg < 0) continue;
-            dst = isk ? p.k + pg * p.k_nb3 + (h - a.H) * p.k_nb2 + off * p.k_nb1
-                      : p.v + pg * p.v_nb3 + (h - a.H - a.HKV) * p.v_nb2 + off * p.v_nb1;
-            dst += 4 * l;
+            dst = isk ? k_row + (h - a.H) * p.k_nb2 : v_row + (h - a.H - a.HKV) * p.v_nb2;
         }
         *reinterpret_cast<__half2 *>(dst) = __floats2half2_rn(lo[u].x, lo[u].y);
         *reinterpret_cast<__half2 *>(dst + D) = __floats2half2_rn(hi[u].x, hi[u].y);
@@ -404,8 +404,9 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
     a.gains8 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 7) == 0;
-    // four rounds of heads per warp share what belongs to the node, as long as that leaves every SM
-    // some blocks; below that one round per warp, so that a step's few rows start at once
+    // four rounds of heads per warp share what belongs to the node (eight prompts of 512 rows: 24 us,
+    // 30 with two), as long as that leaves every SM some blocks; below that one round per warp, so
+    // that a step's few rows start at once
     const int64_t HH = qkv->ne[1], per = D == 64 ? 2 : 1, few = (HH + 8 * per - 1) / (8 * per),
                   many = (HH + 16 * per - 1) / (16 * per);
     const bool share = S * N * many >= 4 * be->sm_count;
