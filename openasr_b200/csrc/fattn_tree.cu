@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
             for (int u = u0; u < u1; ++seg) {
                 if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
                 const int n = g.k1 - g.k0;
+                if (n == 0) break;
                 auto scores = [&](int j) {
                     const int slot = q % NS;
                     ok = ok && mbar_wait(&full[slot], (uint32_t)(q / NS & 1), abort_flag, err);
@@ -267,6 +268,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
             if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
+            if (g.k0 == g.k1) break;
             const int live = g.n * G - g.rt * R - row0;  // rows of the group below this are real
             const float c = tree_load_q<D, RW, R, QF16>(a, g, row0, live, a.scale, smem + C::OFF_Q, C::QHALF, fac);
             if (tid < RW) noff[tid] = -TREE_NONE;
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
                                              g.rt * R, min(R, live)};
             // -- small tiles: the last of the CTAs that share the item joins the parts here --
             if (C::JOINS && !whole) {
-                const int c0 = tree_owner(w, g.first), c1 = tree_owner(w, g.first + g.per - 1);
+                const int c0 = tree_owner(w, g.first + g.lead), c1 = tree_owner(w, g.first + g.per - 1);
                 group_sync(NWG == 1 ? 1 : 3, 128 * NWG);
                 if (threadIdx.x == 0) {
                     const bool is_last = atom_add_acq_rel_gpu(tickets + c0, 1u) == (unsigned)(c1 - c0);
@@ -544,8 +546,8 @@ int tree_prepare(oasr_backend *be, TreeAttn &a, const KvPages &p, const KvSeqs &
     a.group = FastDiv(a.H / a.HKV);
     a.page = FastDiv(p.page);
     const int64_t tiles = ((int64_t)s.N * a.group.d + R - 1) / R;
-    const int64_t most = tiles * a.HKV * a.S * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
-    if (most > INT32_MAX / 2 || (int64_t)s.N * a.group.d > INT32_MAX / 2 || (int64_t)a.S * s.N * a.H > INT32_MAX)
+    const int64_t items = tiles * a.HKV * a.S, most = items * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
+    if (most + items * tree_segment(R) > INT32_MAX / 2 || (int64_t)s.N * a.group.d > INT32_MAX / 2 || (int64_t)a.S * s.N * a.H > INT32_MAX)
         return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
     out->grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * ctas_per_sm));
     const size_t part = (size_t)R * (a.D + 2) * 4;

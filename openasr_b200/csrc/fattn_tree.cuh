@@ -7,7 +7,9 @@
 //   - pieces: each item in equal pieces of at most t units, one piece per CTA, with the t that ends
 //     first (a short call: a CTA has one start and one end);
 //   - runs: CTA c takes the c-th of equal runs of units, across items (a long call, or more items
-//     than CTAs: ragged batches balance to the unit).
+//     than CTAs: ragged batches balance to the unit).  An item counts tree_segment units more than
+//     it has, at its front, for the start and the end of the segment that it begins; where a run
+//     ends among those, the next one begins the item.
 // A segment is what a CTA does of one item.  One that is not the whole item leaves (maximum, sum,
 // output) in the scratch, and the parts are joined in the order of the positions, so the bits do
 // not depend on which CTA came first.
@@ -28,6 +30,7 @@ struct TreeSeg {
     int past, n, T, kt;    // committed positions, live nodes, past + n, units of the item
     int k0, k1;            // units of this segment
     int first, per, next;  // the item's first step, its steps, and where this segment ends
+    int lead;              // its steps without a unit
 };
 
 // The call's steps (units in runs, pieces otherwise) over the CTAs: the first `more` CTAs take
@@ -55,10 +58,14 @@ static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, cons
     return s >= a.S || seq_lengths(q, s, page, past, n);
 }
 
+// What the start and the end of a segment cost, and the join of an item's parts, in units.
+__host__ __device__ constexpr int tree_segment(int R) { return R == 128 ? 9 : 5; }
+constexpr int TREE_JOIN = 3;
+
 // Its steps (below 2^31: the launch checks) and the sum of those of the lanes up to this one.
 static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int piece, int R, int past, int n, int &mine, int &run) {
     const int lane = threadIdx.x & 31, kt = tree_units(past, n);
-    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? tree_pieces(kt, piece, __frcp_rn((float)piece)) : kt);
+    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? tree_pieces(kt, piece, __frcp_rn((float)piece)) : kt + tree_segment(R));
     run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -66,9 +73,6 @@ static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int pi
         if (lane >= o) run += up;
     }
 }
-
-// What the start and the end of a segment cost, and the join of an item's parts, in units.
-constexpr int TREE_SEGMENT = 5, TREE_JOIN = 3;
 
 // All warps: the call's split.  A sequence with lengths out of range counts nothing (reported).
 static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const KvSeqs &q, int page, int R, int ctas, int *err) {
@@ -82,7 +86,8 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
     if (a.S <= 32 && most < 32768) {  // (products of two unit counts fit 31 bits)
         // lane l tries pieces of t units, t spread from an even share of all units to the longest item
         const int kt = tree_units(w.past, w.n), items = w.n ? tree_items(a, w.n, R) : 0;
-        const int even = min(most, (w.total + ctas - 1) / ctas);
+        const int units = w.total - tree_segment(R) * (int)__reduce_add_sync(0xffffffffu, (unsigned)items);
+        const int run = (w.total + ctas - 1) / ctas, even = min(most, (units + ctas - 1) / ctas);
         const int t = max(1, even + (most - even) * lane / 31);
         const float r = __frcp_rn((float)t);
         int pieces = 0;
@@ -92,8 +97,7 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
         const unsigned cost = pieces <= ctas ? (unsigned)(t < most ? t + TREE_JOIN : t) : 65535u;
         const unsigned least = __reduce_min_sync(0xffffffffu, cost << 16 | (unsigned)t);
         const int best = (int)(least & 65535u);
-        // runs: an even share, a join, and one more segment than pieces have
-        if ((int)(least >> 16) <= even + TREE_JOIN + TREE_SEGMENT) {
+        if ((int)(least >> 16) <= run + TREE_JOIN) {
             w.piece = best;
             tree_lane_steps(a, best, R, w.past, w.n, w.mine, w.run);
             w.total = __shfl_sync(0xffffffffu, w.run, 31);
@@ -130,7 +134,8 @@ static __device__ __forceinline__ int tree_slot(const TreeUnits &w, int c, int i
     return 2 * c + (item_first > tree_start(w, c) ? 1 : 0);
 }
 
-// All lanes: the segment that starts at step u (u < total) and ends before `end`.
+// All lanes: the segment that starts at step u (u < total) and ends before `end`; without units only
+// if it is the last before `end`.
 static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const KvSeqs &q, const TreeUnits &w, int page, int R,
                                                       int u, int end) {
     const int lane = threadIdx.x & 31;
@@ -153,7 +158,8 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
     }
     g.T = g.past + g.n;
     g.kt = tree_units(g.past, g.n);
-    g.per = w.piece ? tree_pieces(g.kt, w.piece, __frcp_rn((float)w.piece)) : g.kt;
+    g.lead = w.piece ? 0 : tree_segment(R);
+    g.per = w.piece ? tree_pieces(g.kt, w.piece, __frcp_rn((float)w.piece)) : g.kt + tree_segment(R);
     const int rts = (g.n * a.group.d + R - 1) / R;
     const int item = (u - g.first) / g.per;
     g.hk = item / rts;
@@ -161,8 +167,8 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
     g.first += item * g.per;
     g.next = min(g.first + g.per, end);
     const int p0 = u - g.first, p1 = g.next - g.first;
-    g.k0 = w.piece ? p0 * g.kt / g.per : p0;
-    g.k1 = w.piece ? p1 * g.kt / g.per : p1;
+    g.k0 = w.piece ? p0 * g.kt / g.per : max(0, p0 - g.lead);
+    g.k1 = w.piece ? p1 * g.kt / g.per : max(0, p1 - g.lead);
     return g;
 }
 
@@ -441,6 +447,7 @@ static __device__ __forceinline__ void tree_stream(const CUtensorMap *tm_k, cons
     bool ok = true;
     for (int u = u0; u < u1;) {
         if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
+        if (g.k0 == g.k1) break;
         const int *row = sq.table + g.s * sq.table_ld;
         auto page_of = [&](int k) {  // positions past the end read page n_pages: zeros
             const int t = k * TREE_BKV + b * box;

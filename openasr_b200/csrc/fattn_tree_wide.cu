@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(384, 1)
             for (int u = u0; u < u1; ++seg) {
                 if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
                 const int n = g.k1 - g.k0;
+                if (n == 0) break;
                 auto scores = [&](int j) {
                     const int slot = q % NS;
                     const uint32_t parity = (uint32_t)(q / NS & 1);
@@ -207,6 +208,7 @@ __global__ void __launch_bounds__(384, 1)
         int it = 0, q = 0;
         for (int u = u0; u < u1;) {
             if (u != u0) g = tree_locate(a, sq, w, p.page, R, u, u1);
+            if (g.k0 == g.k1) break;
             const int live = g.n * G - g.rt * R;  // rows of the tile below this are real
             const float c16 = tree_load_q<D, 64, R, QF16>(a, g, 64 * wg, live - 64 * wg, a.scale, smem + C::OFF_Q, C::QHALF,
                                                           s_c + 64 * wg);
