@@ -501,7 +501,10 @@ __global__ void __launch_bounds__(TreeTc<D, RW, NWG, QF16>::NT, TreeTc<D, RW, NW
 }
 
 // Joins the items that several CTAs of fattn_tree_kernel shared: block (c, rows) takes 8 rows of
-// the one that begins in CTA c, four columns per thread.
+// the one that begins in CTA c, four columns per thread, six parts loaded at a time.  After runs of
+// 16 wide trees (2 or 3 parts of 66 KB each) the join costs 4 us of 96, after the pieces of two long
+// caches (37 parts of 21 KB) 4 us of 32, half of it the launch; with sixteen parts at a time 8 and 5,
+// with four 4 and 5, by the last CTA alone 6 and 10.
 template <int D, int R>
 __global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_constant__ TreeAttn a, const float *parts,
                                                                 const TreeJoin *joins) {
@@ -512,7 +515,7 @@ __global__ void __launch_bounds__(2 * D) fattn_tree_join_kernel(const __grid_con
     if (r >= g.live) return;
     const int node = a.group(g.row + r);
     tree_store4(a, g.s, g.hk * a.group.d + g.row + r - node * a.group.d, node, 4 * ch,
-                tree_join4<16>(parts, R, D, c0, g.c1, g.slot, r, ch));
+                tree_join4<6>(parts, R, D, c0, g.c1, g.slot, r, ch));
 }
 
 bool tree_page_map(CUtensorMap *map, const char *base, int64_t nb1, int64_t nb2, int64_t nb3, int D, int page, int HKV,
@@ -559,9 +562,6 @@ int tree_prepare(oasr_backend *be, TreeAttn &a, const KvPages &p, const KvSeqs &
 
 int tree_join(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeqs &s, int R, const TreeLaunch &l) {
     if (l.grid == 1 || (int64_t)s.MP * p.page <= TREE_BKV) return OASR_STATUS_SUCCESS;  // no item is shared
-    // started while the attention still runs; it waits for its end
-    const bool pdl = be->pdl;
-    be->pdl = true;
     const dim3 grid(l.grid * (R / 8)), block(2 * a.D);
     const float *parts = l.parts;
     const TreeJoin *joins = l.joins;
@@ -570,7 +570,6 @@ int tree_join(oasr_backend *be, const TreeAttn &a, const KvPages &p, const KvSeq
                                : launch_k(be, fattn_tree_join_kernel<128, 64>, grid, block, 0, a, parts, joins);
     else e = a.D == 64 ? launch_k(be, fattn_tree_join_kernel<64, 128>, grid, block, 0, a, parts, joins)
                        : launch_k(be, fattn_tree_join_kernel<128, 128>, grid, block, 0, a, parts, joins);
-    be->pdl = pdl;
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree join launch", __LINE__);
     return oasr_internal_launch_check(be, "flash_attn_tree join");
 }
