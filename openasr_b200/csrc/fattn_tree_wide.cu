@@ -12,6 +12,15 @@
 // CTA: two groups of 4 softmax warps take every other unit, each with sums of its own that are
 // joined at the end of a segment; one TMA warp, one MMA warp.  The queries of the groups' units are
 // the same 128 rows.  Accuracy, offsets and the split over the CTAs are those of fattn_tree.cu.
+// S(j + 2) overwrites P(j): the products of one thread run in the order of their issue.
+//
+// Sixteen trees of 61 nodes, 4001 to 8190 positions, 8 K/V heads of 128, f16 (411 MB): 96 us, 4.3 TB/s
+// (112 us with equal runs that did not count the segments' ends).  A unit takes a CTA 2600 clocks, of
+// which the weights are 2400 of a group's 5200 -- 32 columns at a time: a loop over 16 columns takes
+// 101 us, two rounds in one body 104, all four unrolled 102 (code is fetched more slowly than run).
+// P goes to the matrix unit by 32 positions; handed over whole it took 133 -> 141 us for four chunks of
+// 512 rows over 4000 positions.  The rest is the segments: 14000 clocks from the launch to the first
+// product, 10000 for the end of each, 4 us for the join.
 #include <algorithm>
 
 #include "fattn_tree.cuh"
@@ -31,7 +40,8 @@ struct TreeWide {
     // misc: (offset, sum) [2][R], query factors [R], barriers, flags
     static constexpr int OFF_C = OFF_MISC + 16 * R;
     static constexpr int OFF_BAR = OFF_C + 4 * R;
-    static constexpr int OFF_FLAG = OFF_BAR + 8 * (2 * NS + 8);
+    static constexpr int SPLIT = 4;  // parts of a unit's weights that are handed over one by one
+    static constexpr int OFF_FLAG = OFF_BAR + 8 * (2 * NS + 6 + 2 * SPLIT);
     static constexpr int SMEM = OFF_MISC + MISC;
     static_assert(OFF_FLAG + 32 <= SMEM, "misc");
     // 12 warps at 168 registers; the softmax warps, with a row of output each, take more
@@ -77,7 +87,7 @@ __global__ void __launch_bounds__(384, 1)
     float2 *s_ml = (float2 *)(smem + C::OFF_MISC);
     float *s_c = (float *)(smem + C::OFF_C);
     uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + NS;
-    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *q_full = o_full + 2, *done = q_full + 1;
+    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2 * C::SPLIT /* [2][SPLIT] before */, *q_full = o_full + 2, *done = q_full + 1;
     volatile int *abort_flag = (volatile int *)(smem + C::OFF_FLAG);
     uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_FLAG + 4);
     unsigned int *s_bad = (unsigned int *)(smem + C::OFF_FLAG + 8);
@@ -110,7 +120,7 @@ __global__ void __launch_bounds__(384, 1)
                 }
                 for (int i = 0; i < 2; ++i) {
                     mbar_init(&s_full[i], 1);
-                    mbar_init(&p_full[i], 128);
+                    for (int x = 0; x < C::SPLIT; ++x) mbar_init(&p_full[i * C::SPLIT + x], 128);
                     mbar_init(&o_full[i], 1);
                 }
                 mbar_init(q_full, 256);
@@ -169,21 +179,28 @@ __global__ void __launch_bounds__(384, 1)
                     const int slot = q % NS, b = j & 1;
                     const uint32_t parity = (uint32_t)(q / NS & 1);
                     ++q;
-                    if (!arrived(&full[slot], parity) || !arrived(&p_full[b], (uint32_t)(j >> 1) & 1u)) break;
-                    if (elect_one()) {
-                        const uint64_t v = dv + slot * (C::TILE >> 4);
-                        // per 32 positions 16 columns of high halves, then 16 of low ones
+                    if (!arrived(&full[slot], parity)) break;
+                    const uint64_t v = dv + slot * (C::TILE >> 4);
+                    // as the weights come: per 32 positions 16 columns of high halves, then 16 of low ones
 #pragma unroll
-                        for (int x = 0; x < TREE_BKV / 16; ++x)
+                    for (int h = 0; h < C::SPLIT; ++h) {
+                        if (!arrived(&p_full[b * C::SPLIT + h], (uint32_t)(j >> 1) & 1u)) break;
+                        if (elect_one()) {
 #pragma unroll
-                            for (int part = 0; part < 2; ++part)
-                                umma_f16_ts(tmem + C::TM_O + (uint32_t)b * R,
-                                            tmem + (uint32_t)(b * R + 32 * (x >> 1) + 8 * (x & 1) + 16 * part),
-                                            v + x * (2048 >> 4), id_o, x + part != 0);
-                        umma_commit(&o_full[b]);
-                        umma_commit(&empty[slot]);
+                            for (int x = h * (8 / C::SPLIT); x < (h + 1) * (8 / C::SPLIT); ++x)
+#pragma unroll
+                                for (int part = 0; part < 2; ++part)
+                                    umma_f16_ts(tmem + C::TM_O + (uint32_t)b * R,
+                                                tmem + (uint32_t)(b * R + 32 * (x >> 1) + 8 * (x & 1) + 16 * part),
+                                                v + x * (2048 >> 4), id_o, x + part != 0);
+                            if (h == C::SPLIT - 1) {
+                                umma_commit(&o_full[b]);
+                                umma_commit(&empty[slot]);
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     if (j + 2 < it + n) scores(j + 2);
                 }
                 it += n;
@@ -266,6 +283,12 @@ __global__ void __launch_bounds__(384, 1)
                     for (int i = 0; i < D / 2; ++i) o[i] = mul2(o[i], f2);
                     off = now;
                 }
+                if (tail) {
+                    const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1), t = k * TREE_BKV + tid;  // V's place
+                    mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
+                    if (t >= g.past && tree_clean_v<D>(smem + qi % NS * C::TILE, tid) && t < g.T) *s_bad = 1u;
+                    fence_proxy_async_smem();
+                }
                 // -- weights, in place of the scores --
                 const f32x2 n2 = pack2(-off, -off);
 #pragma unroll 1
@@ -281,16 +304,12 @@ __global__ void __launch_bounds__(384, 1)
                         tree_cut2(wt, h[i], h[16 + i]);
                     }
                     tmem_store32(ts + 32 * x, h);
+                    if ((x + 1) % (4 / C::SPLIT) == 0) {
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tc_fence_before();
+                        mbar_arrive(&p_full[wg * C::SPLIT + x / (4 / C::SPLIT)]);
+                    }
                 }
-                if (tail) {
-                    const int j = it - it0, qi = q + (j + 1 < n ? 2 + 2 * j : 2 * n - 1), t = k * TREE_BKV + tid;  // V's place
-                    mbar_wait(&full[qi % NS], (uint32_t)(qi / NS & 1), abort_flag, err);
-                    if (t >= g.past && tree_clean_v<D>(smem + qi % NS * C::TILE, tid) && t < g.T) *s_bad = 1u;
-                    fence_proxy_async_smem();
-                }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                mbar_arrive(&p_full[wg]);
                 // -- the product, when it is there --
                 mbar_wait(&o_full[wg], phase, abort_flag, err);
                 tc_fence_after();
