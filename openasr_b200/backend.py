@@ -17,11 +17,6 @@ import struct
 
 import numpy as np
 
-try:
-    from . import _describe
-except ImportError:  # not built: descriptors are made in Python
-    _describe = None
-
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "liboasr_b200.so")
 
@@ -431,17 +426,36 @@ def describe(t, ggml_type: int | None = None) -> OasrTensor:
     return OasrTensor.from_buffer_copy(_DESC_PACK(ggml_type, 0, t.data_ptr(), *ne[:4], *nb[:4]))
 
 
-def _arg(t):
-    """What a C call with void pointers takes for a tensor (the descriptor's bytes), a
-    descriptor or None."""
-    if t is None:
-        return None
-    if _describe is None or type(t) is OasrTensor:
-        return ctypes.byref(describe(t))
-    try:
-        return _describe.describe(t, _TORCH_TYPES or _torch_types())
-    except KeyError as e:
-        raise UnsupportedInputs(STATUS_FAILED, e.args[0]) from None
+def _unsupported(dtype):
+    raise UnsupportedInputs(STATUS_FAILED, f"unsupported tensor dtype {dtype}")
+
+
+class _CtypesOps:
+    """The calls of csrc/torch_ops.cc by ctypes, for a build without torch's headers."""
+
+    def __getattr__(self, name):
+        fn = getattr(lib(), "oasr_b200_" + name)
+        plain = (int, float, type(None))
+        return lambda *args: fn(*(x if isinstance(x, plain) else ctypes.byref(describe(x)) for x in args))
+
+
+_OPS = None  # the extension or _CtypesOps, from the first call
+
+
+def _ops():
+    global _OPS
+    if _OPS is None:
+        try:
+            import torch  # noqa: F401  (before the extension, which is linked against it)
+
+            from . import _torch_ops
+        except ImportError:
+            _OPS = _CtypesOps()
+        else:
+            _torch_ops.bind(_unsupported, *(ctypes.cast(getattr(lib(), "oasr_b200_" + f), ctypes.c_void_p).value for f in (
+                "qk_norm_rope", "flash_attn_tree", "tree_commit", "kv_pages_copy")))
+            _OPS = _torch_ops
+    return _OPS
 
 
 class Weight:
@@ -681,30 +695,25 @@ class Backend:
         q f32|f16 [S, n, H, D] and the K/V rows at positions n_past + i of the pages
         f16 [P, H_kv, page, D].  q_norm / k_norm f32 [D], rope f32 [n_pos, D / 2, 2], pos and
         n_nodes may be None (see the C header)."""
-        self._check(lib().oasr_b200_qk_norm_rope(
-            self.handle, _arg(qkv), _arg(q_norm), _arg(k_norm), eps, _arg(rope), _arg(pos), _arg(page_table),
-            _arg(n_past), _arg(n_nodes), _arg(q), _arg(k_pages), _arg(v_pages)))
+        self._check((_OPS or _ops()).qk_norm_rope(self.handle.value, qkv, q_norm, k_norm, eps, rope, pos, page_table, n_past,
+                                                  n_nodes, q, k_pages, v_pages))
 
     def flash_attn_tree(self, q, k_pages, v_pages, page_table, n_past, n_nodes, tree, scale: float, out) -> None:
         """Attention of the nodes q f32|f16 [S, H, n, D] over the pages -> out f32|f16 [S, n, H, D];
         tree i32 [S, n, ceil(n / 32)] of visible nodes, or None for a chain."""
-        self._check(lib().oasr_b200_flash_attn_tree(
-            self.handle, _arg(q), _arg(k_pages), _arg(v_pages), _arg(page_table), _arg(n_past),
-            _arg(n_nodes), _arg(tree), scale, _arg(out)))
+        self._check((_OPS or _ops()).flash_attn_tree(self.handle.value, q, k_pages, v_pages, page_table, n_past, n_nodes, tree,
+                                                     scale, out))
 
     def tree_commit(self, tokens, parents, target, n_nodes, n_past, page_table, k_pages, v_pages, n_layers: int, path,
                     n_accept, next_token, n_past_out) -> None:
         """Accept the drafted path that agrees with target (all i32 [S, n]) and compact its K/V rows
         in pages f16 [n_layers * P, H_kv, page, D]; path [S, n], the others [S]."""
-        self._check(lib().oasr_b200_tree_commit(
-            self.handle, _arg(tokens), _arg(parents), _arg(target), _arg(n_nodes), _arg(n_past),
-            _arg(page_table), _arg(k_pages), _arg(v_pages), n_layers, _arg(path), _arg(n_accept),
-            _arg(next_token), _arg(n_past_out)))
+        self._check((_OPS or _ops()).tree_commit(self.handle.value, tokens, parents, target, n_nodes, n_past, page_table,
+                                                 k_pages, v_pages, n_layers, path, n_accept, next_token, n_past_out))
 
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
-        self._check(lib().oasr_b200_kv_pages_copy(self.handle, _arg(k_pages), _arg(v_pages), n_layers,
-                                                  _arg(pairs)))
+        self._check((_OPS or _ops()).kv_pages_copy(self.handle.value, k_pages, v_pages, n_layers, pairs))
 
 
 class KvPool:

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -14,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "liboasr_b200.so")
-DESCRIBE = os.path.join(HERE, "_describe.so")  # tensor descriptors of the Python binding (csrc/describe_py.c)
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")  # the Python binding's short way (csrc/torch_ops.cc)
 ROOT = os.path.dirname(HERE)
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
@@ -54,15 +55,20 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
-def _build_describe() -> None:
-    """The CPython module behind backend.describe; without Python's headers the binding
-    describes tensors in Python (slower, the same bytes)."""
-    src, inc = os.path.join(CSRC, "describe_py.c"), sysconfig.get_path("include")
-    if not os.path.exists(os.path.join(inc, "Python.h")):
+def _build_torch_ops() -> None:
+    """The Python binding's extension; without torch's headers the binding goes through ctypes
+    (slower, the same calls)."""
+    spec = importlib.util.find_spec("torch")
+    torch = os.path.dirname(spec.origin) if spec and spec.origin else ""
+    src, inc = os.path.join(CSRC, "torch_ops.cc"), sysconfig.get_path("include")
+    if not (os.path.exists(os.path.join(torch, "include", "torch", "csrc", "autograd", "python_variable.h"))
+            and os.path.exists(os.path.join(inc, "Python.h"))):
         return
-    if os.path.exists(DESCRIBE) and os.path.getmtime(DESCRIBE) >= max(os.path.getmtime(src), _headers_mtime()):
+    if os.path.exists(TORCH_OPS) and os.path.getmtime(TORCH_OPS) >= max(os.path.getmtime(src), _headers_mtime()):
         return
-    cmd = [HOST_CXX, "-x", "c", "-O2", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", inc, src, "-o", DESCRIBE]
+    cmd = [HOST_CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", inc,
+           "-isystem", os.path.join(torch, "include"), src, "-o", TORCH_OPS, "-L", os.path.join(torch, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
@@ -70,7 +76,7 @@ def _build_describe() -> None:
 
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    _build_describe()
+    _build_torch_ops()
     cu, cpp = _sources()
     with cf.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), cu + cpp))

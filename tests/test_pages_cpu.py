@@ -123,3 +123,55 @@ def test_pool_refusals():
     p.close(t)
     with pytest.raises(bk.UnsupportedInputs):
         p.close(t)
+
+
+def test_the_extension_passes_what_describe_says():
+    """tensors, strided views, ready descriptors and None through the extension and through ctypes"""
+    import ctypes
+
+    import torch
+
+    from openasr_b200 import backend as bk
+
+    ext = bk._ops()
+    if isinstance(ext, bk._CtypesOps):
+        pytest.skip("built without torch's headers")
+    got = []
+
+    @ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, *[ctypes.c_void_p] * 2, ctypes.c_int32, ctypes.c_void_p)
+    def copy(be, k, v, n_layers, pairs):
+        got.append((be, n_layers, *(None if p is None else ctypes.string_at(p, ctypes.sizeof(bk.OasrTensor)) for p in (k, v, pairs))))
+        return 7
+
+    addr = ctypes.cast(copy, ctypes.c_void_p).value
+    base = torch.zeros(3, 5, 4, 16, dtype=torch.float16)
+    views = [base, base.permute(0, 2, 1, 3), base[1:, :, ::2], base[0, 0, 0], base[0, 0, 0, 0], torch.zeros(2, 0, 3),
+             torch.zeros(7, dtype=torch.int32), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(1, 1, dtype=torch.float32)]
+    try:
+        ext.bind(bk._unsupported, addr, addr, addr, addr)
+        for t in views:
+            assert ext.kv_pages_copy(5, t, None, -2, bk.describe(t)) == 7
+            want = bytes(bk.describe(t))
+            assert got.pop() == (5, -2, want, None, want)
+        with pytest.raises(bk.UnsupportedInputs, match="float64"):
+            ext.kv_pages_copy(5, torch.zeros(2, dtype=torch.float64), None, 1, None)
+        for args in ((5, "x", None, 1, None), (5, base, base, 2**31, base), (5, base), (5, base, base, 1.5, base)):
+            with pytest.raises((TypeError, OverflowError)):
+                ext.kv_pages_copy(*args)
+        assert not got
+    finally:
+        bk._OPS = None
+        bk._ops()
+
+
+def test_both_ways_refuse_alike():
+    import torch
+
+    from openasr_b200 import backend as bk
+
+    t = torch.zeros(2, 2)
+    for ops in (bk._ops(), bk._CtypesOps()):  # no backend: refused before anything is read
+        assert ops.kv_pages_copy(0, t, t, 1, t) == bk.STATUS_FAILED
+        assert ops.flash_attn_tree(0, t, t, t, t, t, None, None, 0.5, t) == bk.STATUS_FAILED
+        assert ops.qk_norm_rope(0, t, None, None, 0.5, t, t, t, t, t, t, t, t) == bk.STATUS_FAILED
+        assert ops.tree_commit(0, t, t, t, t, t, t, t, t, 1, t, t, t, t) == bk.STATUS_FAILED
