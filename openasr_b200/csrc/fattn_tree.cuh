@@ -547,29 +547,41 @@ static __device__ __forceinline__ float tree_load_q(const TreeAttn &a, const Tre
         }
         return fmaxf(fabsf(c), FLT_MIN);
     } else {
-#pragma unroll 4
-        for (int e = tid; e < RW * (D / 4); e += 128) {  // a warp has one row, or two of D = 64
-            const int r = e / (D / 4), ch = e % (D / 4);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (r < live) v = *reinterpret_cast<const float4 *>(q_row(r) + 16 * ch);
-            v = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
-            float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-            if (D == 128) {
-                m = warp_max_f32(m);
-            } else {
-                const float m0 = warp_max_f32(lane < 16 ? m : 0.0f), m1 = warp_max_f32(lane < 16 ? 0.0f : m);
-                m = lane < 16 ? m0 : m1;
+        // rows of a lane under way at once (32 trees of 43 nodes, no committed positions, 38.5 us one after
+        // the other, 32.1 with four, 31.0 with eight)
+        constexpr int B = RW * (D / 4) / 128 < 8 ? RW * (D / 4) / 128 : 8;
+        static_assert(RW * (D / 4) % (128 * B) == 0, "whole rounds");
+#pragma unroll 1
+        for (int e0 = tid; e0 < RW * (D / 4); e0 += 128 * B) {  // a warp has one row, or two of D = 64
+            float4 v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int r = (e0 + 128 * b) / (D / 4), ch = e0 % (D / 4);
+                v[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (r < live) v[b] = *reinterpret_cast<const float4 *>(q_row(r) + 16 * ch);
             }
-            // 2^(8 - e2) and its inverse, both in the normal range
-            const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
-            const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
-            uint2 hi, lo;
-            tree_split2(v.x * up, v.y * up, hi.x, lo.x);
-            tree_split2(v.z * up, v.w * up, hi.y, lo.y);
-            uint8_t *half = qs + (ch >> 4) * qhalf + 8 * (ch & 1);
-            *reinterpret_cast<uint2 *>(half + sw128_off(row0 + r, ch >> 1 & 7)) = hi;
-            *reinterpret_cast<uint2 *>(half + sw128_off(R + row0 + r, ch >> 1 & 7)) = lo;
-            if (ch == 0) factor[r] = __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int r = (e0 + 128 * b) / (D / 4), ch = e0 % (D / 4);
+                const float4 z = make_float4(v[b].x * c, v[b].y * c, v[b].z * c, v[b].w * c);
+                float m = fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w)));
+                if (D == 128) {
+                    m = warp_max_f32(m);
+                } else {
+                    const float m0 = warp_max_f32(lane < 16 ? m : 0.0f), m1 = warp_max_f32(lane < 16 ? 0.0f : m);
+                    m = lane < 16 ? m0 : m1;
+                }
+                // 2^(8 - e2) and its inverse, both in the normal range
+                const int e2 = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 127);
+                const float up = __uint_as_float((uint32_t)(127 + 8 - e2) << 23);
+                uint2 hi, lo;
+                tree_split2(z.x * up, z.y * up, hi.x, lo.x);
+                tree_split2(z.z * up, z.w * up, hi.y, lo.y);
+                uint8_t *half = qs + (ch >> 4) * qhalf + 8 * (ch & 1);
+                *reinterpret_cast<uint2 *>(half + sw128_off(row0 + r, ch >> 1 & 7)) = hi;
+                *reinterpret_cast<uint2 *>(half + sw128_off(R + row0 + r, ch >> 1 & 7)) = lo;
+                if (ch == 0) factor[r] = __uint_as_float((uint32_t)(127 + e2 - 8) << 23);
+            }
         }
     }
     return 1.0f;

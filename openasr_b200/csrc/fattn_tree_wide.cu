@@ -361,11 +361,17 @@ __global__ void __launch_bounds__(384, 1)
                     }
                 }
                 group_sync(3, 256);
+                if (anybad) {
+                    for (int e = threadIdx.x; e < min(R, live) * HC; e += 256) {
+                        const int r = e / HC, ch = e % HC;
+                        float4 &x = stage[r * HC + (ch ^ (r & (HC - 1)))];
+                        x = tree_nonfinite4(a, p, sq, g, a.group(g.rt * R + r), half * (D / 2) + 4 * ch, x);
+                    }
+                }
 #pragma unroll 4
                 for (int e = threadIdx.x; e < min(R, live) * HC; e += 256) {
                     const int r = e / HC, ch = e % HC, gr = g.rt * R + r, nd = a.group(gr), col = half * (D / 2) + 4 * ch;
-                    float4 x = stage[r * HC + (ch ^ (r & (HC - 1)))];
-                    if (anybad) x = tree_nonfinite4(a, p, sq, g, nd, col, x);
+                    const float4 x = stage[r * HC + (ch ^ (r & (HC - 1)))];
                     if (whole) tree_store4(a, g.s, g.hk * G + gr - nd * G, nd, col, x);
                     else *reinterpret_cast<float4 *>(part + r * D + col) = x;
                 }
