@@ -20,37 +20,15 @@
 
 #include "pages.cuh"
 #include "tc_common.cuh"
+#include "tree_split.h"
 
 namespace oasr {
 
-constexpr int TREE_BKV = 128;  // positions per unit
 constexpr float TREE_NONE = -1.7e38f;  // maximum of a row that has seen nothing (finite: -inf minus it is -inf)
 
-struct TreeSeg {
-    int s, hk, rt;         // sequence, K/V head, row tile
-    int past, n, T, kt;    // committed positions, live nodes, past + n, units of the item
-    int k0, k1;            // units of this segment
-    int first, per, next;  // the item's first step, its steps, and where this segment ends
-    int lead;              // its steps without a unit
-};
-
-// The call's steps (units in runs, pieces otherwise) over the CTAs: the first `more` CTAs take
-// q + 1, the others q.  Lane l keeps what sequence l has: lengths, steps, and the steps of the
-// sequences up to it.
-struct TreeUnits {
-    int total, ctas, q, more;
-    int piece;  // most units of a piece, or 0: runs
-    int past, n, mine, run;
-};
-
-static __device__ __forceinline__ int tree_units(int past, int n) { return (past + n + TREE_BKV - 1) / TREE_BKV; }
 static __device__ __forceinline__ int tree_items(const TreeAttn &a, int n, int R) {
     return (n * a.group.d + R - 1) / R * a.HKV;
 }
-
-// ceil(kt / t) for kt, t < 32768 by a reciprocal r = 1 / t: (kt + t - 1/2) / t is 1 / (2 t) or more
-// away from every integer, the product less than 2^-7 / t off.
-static __device__ __forceinline__ int tree_pieces(int kt, int t, float r) { return (int)(((float)(kt + t) - 0.5f) * r); }
 
 // Lane l of every warp: lengths of sequence s.
 static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, const KvSeqs &q, int page, int s, int &past,
@@ -59,18 +37,10 @@ static __device__ __forceinline__ bool tree_lane_lengths(const TreeAttn &a, cons
     return s >= a.S || seq_lengths(q, s, page, past, n);
 }
 
-// What the start and the end of a segment cost, and the join of an item's parts, in units: measured
-// best of 1, 3, 5, 7 for tiles up to 64 rows (69.6, 69.2, 69.1, 69.1 us for 16 x 16 rows, 16 x 64 86.8,
-// 84.7, 84.0, 85.1), of 7, 9, 12, 16 for 128 (16 trees of 61 nodes 100.8, 100.3, 103.6, 109).  A join:
-// 8 sequences of one token of 20 heads of 64 take 13.3, 13.8, 11.5, 11.5 us with 1, 2, 3, 5, one token
-// alone 8.8, 8.8, 8.8, 9.9.
-__host__ __device__ constexpr int tree_segment(int R) { return R == 128 ? 9 : 5; }
-constexpr int TREE_JOIN = 3;
-
 // Its steps (below 2^31: the launch checks) and the sum of those of the lanes up to this one.
 static __device__ __forceinline__ void tree_lane_steps(const TreeAttn &a, int piece, int R, int past, int n, int &mine, int &run) {
     const int lane = threadIdx.x & 31, kt = tree_units(past, n);
-    mine = n == 0 ? 0 : tree_items(a, n, R) * (piece ? tree_pieces(kt, piece, __frcp_rn((float)piece)) : kt + tree_segment(R));
+    mine = n == 0 ? 0 : tree_steps(tree_items(a, n, R), kt, piece, R);
     run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -89,26 +59,23 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
     w.total = __shfl_sync(0xffffffffu, w.run, 31);
     const int most = __reduce_max_sync(0xffffffffu, w.n ? tree_units(w.past, w.n) : 0);
     if (a.S <= 32 && most < 32768) {  // (products of two unit counts fit 31 bits)
-        // lane l tries pieces of t units, t spread from an even share of all units to the longest item
         const int kt = tree_units(w.past, w.n), items = w.n ? tree_items(a, w.n, R) : 0;
         const int units = w.total - tree_segment(R) * (int)__reduce_add_sync(0xffffffffu, (unsigned)items);
         const int run = (w.total + ctas - 1) / ctas, even = min(most, (units + ctas - 1) / ctas);
-        const int t = max(1, even + (most - even) * lane / 31);
-        const float r = __frcp_rn((float)t);
+        const int t = tree_try(even, most, lane);
+        const float r = tree_rcp(t);
         int pieces = 0;
 #pragma unroll 4
         for (int s = 0; s < a.S; ++s)
             pieces += __shfl_sync(0xffffffffu, items, s) * tree_pieces(__shfl_sync(0xffffffffu, kt, s), t, r);
-        const unsigned cost = pieces <= ctas ? (unsigned)(t < most ? t + TREE_JOIN : t) : 65535u;
+        const unsigned cost = tree_piece_cost(pieces, ctas, t, most);
         const unsigned least = __reduce_min_sync(0xffffffffu, cost << 16 | (unsigned)t);
         const int best = (int)(least & 65535u);
-        if ((int)(least >> 16) <= run + TREE_JOIN) {
+        if (tree_in_pieces(least >> 16, run)) {
             w.piece = best;
             tree_lane_steps(a, best, R, w.past, w.n, w.mine, w.run);
             w.total = __shfl_sync(0xffffffffu, w.run, 31);
-            w.ctas = max(1, w.total);
-            w.q = min(w.total, 1);
-            w.more = 0;
+            tree_set_pieces(w);
             if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
             return w;
         }
@@ -120,23 +87,8 @@ static __device__ __forceinline__ TreeUnits tree_count(const TreeAttn &a, const 
         w.total += __shfl_sync(0xffffffffu, run, 31);
     }
     if (!ok && err && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(err, ERR_BAD_INDEX);
-    w.ctas = max(1, min(ctas, w.total));
-    w.q = w.total / w.ctas;
-    w.more = w.total - w.q * w.ctas;
+    tree_set_runs(w, ctas);
     return w;
-}
-
-static __device__ __forceinline__ int tree_start(const TreeUnits &w, int c) {
-    return c >= w.ctas ? w.total : c * w.q + min(c, w.more);
-}
-// the CTA whose range holds step u
-static __device__ __forceinline__ int tree_owner(const TreeUnits &w, int u) {
-    const int big = w.more * (w.q + 1);
-    return u < big ? u / (w.q + 1) : w.more + (u - big) / w.q;
-}
-// A CTA leaves at most two unfinished segments: its first (slot 2c) and its last (2c + 1).
-static __device__ __forceinline__ int tree_slot(const TreeUnits &w, int c, int item_first) {
-    return 2 * c + (item_first > tree_start(w, c) ? 1 : 0);
 }
 
 // All lanes: the segment that starts at step u (u < total) and ends before `end`; without units only
@@ -161,19 +113,7 @@ static __device__ __forceinline__ TreeSeg tree_locate(const TreeAttn &a, const K
         tree_lane_lengths(a, q, page, s0 + lane, past, n);
         tree_lane_steps(a, w.piece, R, past, n, mine, run);
     }
-    g.T = g.past + g.n;
-    g.kt = tree_units(g.past, g.n);
-    g.lead = w.piece ? 0 : tree_segment(R);
-    g.per = w.piece ? tree_pieces(g.kt, w.piece, __frcp_rn((float)w.piece)) : g.kt + tree_segment(R);
-    const int rts = (g.n * a.group.d + R - 1) / R;
-    const int item = (u - g.first) / g.per;
-    g.hk = item / rts;
-    g.rt = item - g.hk * rts;
-    g.first += item * g.per;
-    g.next = min(g.first + g.per, end);
-    const int p0 = u - g.first, p1 = g.next - g.first;
-    g.k0 = w.piece ? p0 * g.kt / g.per : max(0, p0 - g.lead);
-    g.k1 = w.piece ? p1 * g.kt / g.per : max(0, p1 - g.lead);
+    tree_cut(g, w.piece, g.n * a.group.d, R, u, end);
     return g;
 }
 

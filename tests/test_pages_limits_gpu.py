@@ -1,0 +1,64 @@
+"""The paged cache's operators at the ends of their ranges: calls of very many steps, long chains, mixed
+types, lengths near 2^31.  Tolerances as in test_pages_gpu.py; where a sum has very many terms, n
+additions in 32 bits add 8 sqrt(n) 2^-24 of it (roundings are as often up as down)."""
+import math
+
+import numpy as np
+import pytest
+
+from test_pages_gpu import Cache, attend64, be, check, cuda, run_attn, words_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def attend_pool(pool_k, pool_v, q, counts, scale):
+    """Rows q [N, H, D] over one K/V head's pool rows [R, D], row r seen counts[N, R] times -> [N, H, D]
+    in 64 bits, and the largest sum |q| |k| of a visible position."""
+    import torch
+
+    k, v, q = pool_k.double(), pool_v.double(), q.double()
+    x = torch.einsum("nhd,rd->nhr", q, k) * scale
+    seen = (counts > 0)[:, None]
+    w = torch.exp(x - x.masked_fill(~seen, -math.inf).amax(-1, keepdim=True)) * counts[:, None]
+    o = torch.einsum("nhr,rd->nhd", w, v) / w.sum(-1, keepdim=True)
+    return o, torch.einsum("nhd,rd->nhr", q.abs(), k.abs()).max()
+
+
+def repeated_pages(seed, page, pages, D, past, N):
+    """One sequence over a pool of few pages (reads may share them) -> K, V, its table row, and how
+    often node i sees each of the pool's rows"""
+    import torch
+
+    g = torch.Generator("cuda")
+    g.manual_seed(seed)
+    k, v = (torch.randn(pages, 1, page, D, generator=g, device="cuda").half() for _ in range(2))
+    MP = -(-(past + N) // page)
+    order = torch.arange(MP, device="cuda") * 7 % pages
+    p = torch.arange(past + N, device="cuda")
+    row = order[p // page] * page + p % page
+    base = torch.bincount(row[:past], minlength=pages * page)
+    own = torch.nn.functional.one_hot(row[past:], pages * page).cumsum(0)
+    return k, v, order.int()[None], (base[None] + own).double()
+
+
+@pytest.mark.parametrize("past,N,H,D,page,f16", [
+    (1000000, 4968, 32, 64, 64, True),   # 1242 tiles of 128 rows, 7822 steps each: 66000 steps to a CTA
+])
+def test_long_chains(be, past, N, H, D, page, f16):  # noqa: F811
+    import torch
+
+    k, v, table, counts = repeated_pages(N, page, 15, D, past, N)
+    g = torch.Generator("cuda")
+    g.manual_seed(N + 1)
+    dt = torch.float16 if f16 else torch.float32
+    q = torch.randn(1, N, H, D, generator=g, device="cuda").to(dt)
+    out = torch.full((1, N, H, D), 7.0, dtype=dt, device="cuda")
+    scale = 1 / math.sqrt(D)
+    be.flash_attn_tree(q.permute(0, 2, 1, 3), k, v, table, cuda(np.array([past], np.int32)), None, None, scale, out)
+    be.synchronize()
+    units = -(-(past + N) // 128)
+    for n0 in range(0, N, 512):
+        want, big = attend_pool(k[:, 0].reshape(-1, D), v[:, 0].reshape(-1, D), q[0, n0:n0 + 512], counts[n0:n0 + 512], scale)
+        ds = 2.0**-20 * scale * float(big)
+        tol = (2 * (2 * ds + 2.0**-20) + 8 * math.sqrt(128 * units) * 2.0**-24) * float(v.abs().max())
+        check(out[0, n0:n0 + 512].double().cpu().numpy(), want.cpu().numpy(), tol, f16)
