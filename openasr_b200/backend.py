@@ -695,25 +695,25 @@ class Backend:
         q f32|f16 [S, n, H, D] and the K/V rows at positions n_past + i of the pages
         f16 [P, H_kv, page, D].  q_norm / k_norm f32 [D], rope f32 [n_pos, D / 2, 2], pos and
         n_nodes may be None (see the C header)."""
-        self._check((_OPS or _ops()).qk_norm_rope(self.handle.value, qkv, q_norm, k_norm, eps, rope, pos, page_table, n_past,
+        self._check((_OPS or _ops()).qk_norm_rope(self.handle.value or 0, qkv, q_norm, k_norm, eps, rope, pos, page_table, n_past,
                                                   n_nodes, q, k_pages, v_pages))
 
     def flash_attn_tree(self, q, k_pages, v_pages, page_table, n_past, n_nodes, tree, scale: float, out) -> None:
         """Attention of the nodes q f32|f16 [S, H, n, D] over the pages -> out f32|f16 [S, n, H, D];
         tree i32 [S, n, ceil(n / 32)] of visible nodes, or None for a chain."""
-        self._check((_OPS or _ops()).flash_attn_tree(self.handle.value, q, k_pages, v_pages, page_table, n_past, n_nodes, tree,
+        self._check((_OPS or _ops()).flash_attn_tree(self.handle.value or 0, q, k_pages, v_pages, page_table, n_past, n_nodes, tree,
                                                      scale, out))
 
     def tree_commit(self, tokens, parents, target, n_nodes, n_past, page_table, k_pages, v_pages, n_layers: int, path,
                     n_accept, next_token, n_past_out) -> None:
         """Accept the drafted path that agrees with target (all i32 [S, n]) and compact its K/V rows
         in pages f16 [n_layers * P, H_kv, page, D]; path [S, n], the others [S]."""
-        self._check((_OPS or _ops()).tree_commit(self.handle.value, tokens, parents, target, n_nodes, n_past, page_table,
+        self._check((_OPS or _ops()).tree_commit(self.handle.value or 0, tokens, parents, target, n_nodes, n_past, page_table,
                                                  k_pages, v_pages, n_layers, path, n_accept, next_token, n_past_out))
 
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
-        self._check((_OPS or _ops()).kv_pages_copy(self.handle.value, k_pages, v_pages, n_layers, pairs))
+        self._check((_OPS or _ops()).kv_pages_copy(self.handle.value or 0, k_pages, v_pages, n_layers, pairs))
 
 
 class KvPool:

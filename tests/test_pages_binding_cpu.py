@@ -1,0 +1,39 @@
+"""What the Python calls of the paged cache's operators refuse before anything reaches a device."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from openasr_b200 import backend as bk  # noqa: E402
+
+
+def calls(be, t):
+    """the four calls with tensor t everywhere"""
+    return (lambda: be.kv_pages_copy(t, t, 1, t), lambda: be.flash_attn_tree(t, t, t, t, t, None, None, 0.5, t),
+            lambda: be.qk_norm_rope(t, None, None, 0.5, t, t, t, t, t, t, t, t),
+            lambda: be.tree_commit(t, t, t, t, t, t, t, t, 1, t, t, t, t))
+
+
+@pytest.fixture(params=["extension", "ctypes"])
+def ops(request, monkeypatch):
+    if request.param == "ctypes":
+        monkeypatch.setattr(bk, "_OPS", bk._CtypesOps())
+    elif isinstance(bk._ops(), bk._CtypesOps):
+        pytest.skip("built without torch's headers")
+    return request.param
+
+
+def closed_backend():
+    be = bk.Backend.__new__(bk.Backend)
+    be.handle, be.ordinal = ctypes.c_void_p(0), 0
+    return be
+
+
+def test_a_closed_backend_is_the_librarys_error(ops):
+    """as for the other operators: a status of the library, not a TypeError of the binding"""
+    be = closed_backend()
+    t = bk.describe(torch.zeros(2, 2))
+    for call in calls(be, t):
+        with pytest.raises(bk.GgmlBackendError, match="null backend"):
+            call()
