@@ -426,17 +426,31 @@ def describe(t, ggml_type: int | None = None) -> OasrTensor:
     return OasrTensor.from_buffer_copy(_DESC_PACK(ggml_type, 0, t.data_ptr(), *ne[:4], *nb[:4]))
 
 
-def _unsupported(dtype):
-    raise UnsupportedInputs(STATUS_FAILED, f"unsupported tensor dtype {dtype}")
+def _unsupported(what, reason=None):
+    raise UnsupportedInputs(STATUS_FAILED, f"{reason or 'unsupported tensor dtype'} {what}")
 
 
 class _CtypesOps:
-    """The calls of csrc/torch_ops.cc by ctypes, for a build without torch's headers."""
+    """The calls of csrc/torch_ops.cc by ctypes, for a build without torch's headers; the same checks."""
 
     def __getattr__(self, name):
         fn = getattr(lib(), "oasr_b200_" + name)
-        plain = (int, float, type(None))
-        return lambda *args: fn(*(x if isinstance(x, plain) else ctypes.byref(describe(x)) for x in args))
+
+        def call(be, *args):
+            be, device = be if isinstance(be, tuple) else (be, -1)
+            return fn(be, *(x if isinstance(x, (int, float, type(None))) else ctypes.byref(self.take(x, device)) for x in args))
+
+        return call
+
+    @staticmethod
+    def take(t, device: int) -> OasrTensor:
+        if type(t) is not OasrTensor:
+            _torch_type(t)
+            if device >= 0 and t.numel() and not (t.is_cuda and t.device.index == device):
+                _unsupported(t.device, "a tensor on another device than the backend's:")
+            if t.dim() > 4:
+                _unsupported(t.dim(), "a tensor has at most 4 dimensions, not")
+        return describe(t)
 
 
 _OPS = None  # the extension or _CtypesOps, from the first call
@@ -688,32 +702,34 @@ class Backend:
         self._check(lib().oasr_b200_argmax_first(self.handle, ctypes.byref(describe(logits)), ctypes.byref(describe(out))))
 
 
-    # -- paged K/V cache and drafted trees (shapes below are torch's: slowest dimension first) --
+    # -- paged K/V cache and drafted trees (shapes below are torch's: slowest dimension first; all
+    # tensors on the backend's device) --
     def qk_norm_rope(self, qkv, q_norm, k_norm, eps: float, rope, pos, page_table, n_past, n_nodes, q, k_pages,
                      v_pages) -> None:
         """Norms, rotation and the cache write of new nodes: qkv f32 [S, n, H + 2 H_kv, D] ->
         q f32|f16 [S, n, H, D] and the K/V rows at positions n_past + i of the pages
         f16 [P, H_kv, page, D].  q_norm / k_norm f32 [D], rope f32 [n_pos, D / 2, 2], pos and
         n_nodes may be None (see the C header)."""
-        self._check((_OPS or _ops()).qk_norm_rope(self.handle.value or 0, qkv, q_norm, k_norm, eps, rope, pos, page_table, n_past,
-                                                  n_nodes, q, k_pages, v_pages))
+        self._check((_OPS or _ops()).qk_norm_rope((self.handle.value or 0, self.ordinal), qkv, q_norm, k_norm, eps, rope, pos,
+                                                  page_table, n_past, n_nodes, q, k_pages, v_pages))
 
     def flash_attn_tree(self, q, k_pages, v_pages, page_table, n_past, n_nodes, tree, scale: float, out) -> None:
         """Attention of the nodes q f32|f16 [S, H, n, D] over the pages -> out f32|f16 [S, n, H, D];
         tree i32 [S, n, ceil(n / 32)] of visible nodes, or None for a chain."""
-        self._check((_OPS or _ops()).flash_attn_tree(self.handle.value or 0, q, k_pages, v_pages, page_table, n_past, n_nodes, tree,
-                                                     scale, out))
+        self._check((_OPS or _ops()).flash_attn_tree((self.handle.value or 0, self.ordinal), q, k_pages, v_pages, page_table,
+                                                     n_past, n_nodes, tree, scale, out))
 
     def tree_commit(self, tokens, parents, target, n_nodes, n_past, page_table, k_pages, v_pages, n_layers: int, path,
                     n_accept, next_token, n_past_out) -> None:
         """Accept the drafted path that agrees with target (all i32 [S, n]) and compact its K/V rows
         in pages f16 [n_layers * P, H_kv, page, D]; path [S, n], the others [S]."""
-        self._check((_OPS or _ops()).tree_commit(self.handle.value or 0, tokens, parents, target, n_nodes, n_past, page_table,
-                                                 k_pages, v_pages, n_layers, path, n_accept, next_token, n_past_out))
+        self._check((_OPS or _ops()).tree_commit((self.handle.value or 0, self.ordinal), tokens, parents, target, n_nodes,
+                                                 n_past, page_table, k_pages, v_pages, n_layers, path, n_accept, next_token,
+                                                 n_past_out))
 
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
-        self._check((_OPS or _ops()).kv_pages_copy(self.handle.value or 0, k_pages, v_pages, n_layers, pairs))
+        self._check((_OPS or _ops()).kv_pages_copy((self.handle.value or 0, self.ordinal), k_pages, v_pages, n_layers, pairs))
 
 
 class KvPool:

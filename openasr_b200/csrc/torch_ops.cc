@@ -12,7 +12,7 @@
 
 namespace {
 
-PyObject *s_unsupported;  // callable(dtype): raises
+PyObject *s_unsupported;  // callable(what, reason or None for a dtype): raises
 decltype(&oasr_b200_qk_norm_rope) s_qk_norm_rope;
 decltype(&oasr_b200_flash_attn_tree) s_flash_attn_tree;
 decltype(&oasr_b200_tree_commit) s_tree_commit;
@@ -20,11 +20,20 @@ decltype(&oasr_b200_kv_pages_copy) s_kv_pages_copy;
 
 // The descriptor of a torch tensor (ne = reversed sizes, nb = reversed byte strides), of a ready
 // one (any object whose buffer is an oasr_tensor), or nothing for None.
+//
+// The kernels read all of them on the backend's device: a tensor elsewhere (a page table still on the
+// host) would be an illegal access there, so it is refused here.
 struct Arg {
     oasr_tensor d;
     oasr_tensor *p = nullptr;
 
-    bool take(PyObject *o) {
+    static bool refuse(PyObject *what, const char *reason) {
+        if (what) Py_XDECREF(PyObject_CallFunction(s_unsupported, "Oz", what, reason));
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "unsupported tensor");
+        return false;
+    }
+
+    bool take(PyObject *o, int device) {
         if (o == Py_None) return true;
         p = &d;
         if (!THPVariable_Check(o)) {
@@ -45,14 +54,26 @@ struct Arg {
             case at::kLong: d.type = OASR_TYPE_I64, size = 8; break;
             default: {
                 PyObject *dtype = PyObject_GetAttrString(o, "dtype");
-                if (dtype) Py_XDECREF(PyObject_CallOneArg(s_unsupported, dtype));
+                const bool taken = refuse(dtype, nullptr);
                 Py_XDECREF(dtype);
-                return false;
+                return taken;
             }
+        }
+        if (device >= 0 && t.numel() != 0 && !(t.is_cuda() && t.get_device() == device)) {
+            PyObject *where = PyObject_GetAttrString(o, "device");
+            const bool taken = refuse(where, "a tensor on another device than the backend's:");
+            Py_XDECREF(where);
+            return taken;
         }
         try {
             const auto sizes = t.sizes(), strides = t.strides();
             const int64_t dims = t.dim();
+            if (dims > 4) {
+                PyObject *n = PyLong_FromLongLong(dims);
+                const bool taken = refuse(n, "a tensor has at most 4 dimensions, not");
+                Py_XDECREF(n);
+                return taken;
+            }
             for (int i = 0; i < 4; ++i) {
                 d.ne[i] = i < dims ? sizes[dims - 1 - i] : 1;
                 d.nb[i] = i < dims ? strides[dims - 1 - i] * size : i ? d.nb[i - 1] * d.ne[i - 1] : size;
@@ -72,11 +93,26 @@ bool count(Py_ssize_t n, Py_ssize_t want) {
     return n == want;
 }
 
-// args[from + i] to t[i]
+// The backend: its address, or (address, device) to have the tensors' device checked.
+struct Where {
+    oasr_backend *be = nullptr;
+    int device = -1;
+
+    explicit Where(PyObject *o) {
+        if (PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2) {
+            device = (int)PyLong_AsLong(PyTuple_GET_ITEM(o, 1));
+            o = PyTuple_GET_ITEM(o, 0);
+        }
+        if (!PyErr_Occurred()) be = static_cast<oasr_backend *>(PyLong_AsVoidPtr(o));
+    }
+};
+
+// args[i] to t[i]
 template <int N>
-bool take(Arg (&t)[N], PyObject *const *args) {
+bool take(Arg (&t)[N], PyObject *const *args, const Where &at) {
+    if (PyErr_Occurred()) return false;
     for (int i = 0; i < N; ++i)
-        if (!t[i].take(args[i])) return false;
+        if (!t[i].take(args[i], at.device)) return false;
     return true;
 }
 
@@ -91,23 +127,25 @@ PyObject *status(F &&call) {
 
 PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Arg x[3], y[8];
-    if (!count(n, 13) || !take(x, a + 1) || !take(y, a + 5)) return nullptr;
-    auto *be = static_cast<oasr_backend *>(PyLong_AsVoidPtr(a[0]));
+    if (!count(n, 13)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !take(y, a + 5, at)) return nullptr;
     const float eps = (float)PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) return nullptr;
     return status([&] {
-        return s_qk_norm_rope(be, x[0].p, x[1].p, x[2].p, eps, y[0].p, y[1].p, y[2].p, y[3].p, y[4].p, y[5].p, y[6].p, y[7].p);
+        return s_qk_norm_rope(at.be, x[0].p, x[1].p, x[2].p, eps, y[0].p, y[1].p, y[2].p, y[3].p, y[4].p, y[5].p, y[6].p, y[7].p);
     });
 }
 
 PyObject *flash_attn_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Arg x[7], y[1];
-    if (!count(n, 10) || !take(x, a + 1) || !take(y, a + 9)) return nullptr;
-    auto *be = static_cast<oasr_backend *>(PyLong_AsVoidPtr(a[0]));
+    if (!count(n, 10)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !take(y, a + 9, at)) return nullptr;
     const float scale = (float)PyFloat_AsDouble(a[8]);
     if (PyErr_Occurred()) return nullptr;
     return status([&] {
-        return s_flash_attn_tree(be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, scale, y[0].p);
+        return s_flash_attn_tree(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, scale, y[0].p);
     });
 }
 
@@ -125,11 +163,11 @@ bool int32(PyObject *o, int32_t *v) {
 PyObject *tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Arg x[8], y[4];
     int32_t layers;
-    if (!count(n, 14) || !take(x, a + 1) || !int32(a[9], &layers) || !take(y, a + 10)) return nullptr;
-    auto *be = static_cast<oasr_backend *>(PyLong_AsVoidPtr(a[0]));
-    if (PyErr_Occurred()) return nullptr;
+    if (!count(n, 14)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !int32(a[9], &layers) || !take(y, a + 10, at)) return nullptr;
     return status([&] {
-        return s_tree_commit(be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, layers, y[0].p, y[1].p, y[2].p,
+        return s_tree_commit(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, layers, y[0].p, y[1].p, y[2].p,
                              y[3].p);
     });
 }
@@ -137,10 +175,10 @@ PyObject *tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *kv_pages_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Arg x[2], y[1];
     int32_t layers;
-    if (!count(n, 5) || !take(x, a + 1) || !int32(a[3], &layers) || !take(y, a + 4)) return nullptr;
-    auto *be = static_cast<oasr_backend *>(PyLong_AsVoidPtr(a[0]));
-    if (PyErr_Occurred()) return nullptr;
-    return status([&] { return s_kv_pages_copy(be, x[0].p, x[1].p, layers, y[0].p); });
+    if (!count(n, 5)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !int32(a[3], &layers) || !take(y, a + 4, at)) return nullptr;
+    return status([&] { return s_kv_pages_copy(at.be, x[0].p, x[1].p, layers, y[0].p); });
 }
 
 // bind(unsupported, addresses of the four C functions in the order below)

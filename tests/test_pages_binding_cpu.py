@@ -37,3 +37,25 @@ def test_a_closed_backend_is_the_librarys_error(ops):
     for call in calls(be, t):
         with pytest.raises(bk.GgmlBackendError, match="null backend"):
             call()
+
+
+def test_a_tensor_on_the_host_is_refused(ops):
+    """the kernels would read it at an address that the device does not have"""
+    be = closed_backend()
+    for call in calls(be, torch.zeros(2, 2)):
+        with pytest.raises(bk.UnsupportedInputs, match="another device than the backend's: cpu"):
+            call()
+    ready = bk.describe(torch.zeros(2, 2))
+    for a in ((torch.zeros(2, 2), ready, 1, ready), (ready, ready, 1, torch.zeros(1, 2, dtype=torch.int32))):
+        with pytest.raises(bk.UnsupportedInputs, match="another device"):
+            be.kv_pages_copy(*a)
+    with pytest.raises(bk.GgmlBackendError, match="null backend"):  # nothing to read: as far as the library
+        be.kv_pages_copy(ready, ready, 1, torch.zeros(0, 2, dtype=torch.int32))
+
+
+def test_a_tensor_of_five_dimensions_is_refused(ops):
+    """[layers, pages, heads, positions, D] is no pool of pages: its first layer alone would be taken"""
+    be = closed_backend()
+    ready = bk.describe(torch.zeros(2, 2))
+    with pytest.raises(bk.UnsupportedInputs, match="at most 4 dimensions, not 5"):
+        bk._ops().kv_pages_copy(be.handle.value or 0, torch.zeros(2, 3, 2, 8, 64, dtype=torch.float16), ready, 1, ready)
