@@ -319,7 +319,8 @@ int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr
  * (oasr_b200_argmax_first of its logits).  Node 0 is accepted; after node c the lowest node
  * j > c with parents[j] == c and tokens[j] == target[c].  path I32 [n, n_seq] gets the
  * accepted nodes, then -1; n_accept their number; next_token the choice after the last (-1
- * for a sequence without nodes); n_past_out = n_past + n_accept (not the n_past tensor).
+ * for a sequence without nodes); n_past_out = n_past + n_accept.  None of the four may
+ * overlap an input or another of them: the inputs are still read while they are written.
  * The K and V rows of the accepted nodes move to positions n_past, n_past + 1, ... in each
  * of the n_layers layers; the rows after them are undefined. */
 int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oasr_tensor *parents,

@@ -5,6 +5,7 @@
 // The cache of one layer is a pool of pages [D, page, n_kv_heads, n_pages] f16; a sequence
 // owns positions through its row of the page table.  Node i of sequence s sits at position
 // n_past[s] + i; lengths live in device memory, so a step can be captured once and replayed.
+#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
@@ -356,6 +357,26 @@ bool is_rows_i32(const oasr_tensor *t, int64_t N, int64_t S) {
            (t->nb[0] == 4 || N <= 1) && t->nb[1] % 4 == 0;
 }
 
+// Rows of I32 on the device: `n` rows of `width` values, `ld` values apart.
+struct IntRows {
+    const int *at;
+    int64_t n, width, ld;
+};
+IntRows int_rows(const oasr_tensor *t) { return {(const int *)t->data, t->ne[1], t->ne[0], t->ne[1] > 1 ? t->nb[1] / 4 : 0}; }
+
+// Whether the two have a value in common (rows side by side in one buffer have none).
+bool share_values(const IntRows &a, const IntRows &b) {
+    auto row = [](const IntRows &r, int64_t i) { return r.at + (r.ld < 0 ? r.n - 1 - i : i) * r.ld; };  // ascending
+    if (row(a, a.n - 1) + a.width <= row(b, 0) || row(b, b.n - 1) + b.width <= row(a, 0)) return false;
+    for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
+        const int *x = row(a, i), *y = row(b, j);
+        if (x + a.width <= y) ++i;
+        else if (y + b.width <= x) ++j;
+        else return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -493,8 +514,18 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
         return fail_op(be, op, "tokens, parents, target and path must be I32 [n, n_seq]");
     if (!is_vec_i32(n_accept, S) || !is_vec_i32(next_token, S) || !is_vec_i32(n_past_out, S))
         return fail_op(be, op, "n_accept, next_token and n_past_out must be I32 [n_seq]");
-    if (n_past_out->data == n_past->data)
-        return fail_op(be, op, "n_past_out must not be n_past (it is still read while n_past_out is written)");
+    // every CTA of a sequence walks its tree, while the first of them writes the results
+    const oasr_tensor *outs[] = {path, n_accept, next_token, n_past_out}, *ins[] = {tokens, parents, target, n_past, page_table, n_nodes};
+    if (S > 1 && llabs(path->nb[1] / 4) < N) return fail_op(be, op, "path's rows must not overlap");
+    for (int i = 0; i < 4; ++i) {
+        for (const oasr_tensor *t : ins)
+            if (t && share_values(int_rows(outs[i]), int_rows(t)))
+                return fail_op(be, op, "path, n_accept, next_token and n_past_out must not overlap an input (it is still read "
+                                       "while they are written)");
+        for (int j = 0; j < i; ++j)
+            if (share_values(int_rows(outs[i]), int_rows(outs[j])))
+                return fail_op(be, op, "path, n_accept, next_token and n_past_out must not overlap one another");
+    }
     Commit a;
     a.tokens = (const int *)tokens->data, a.tok_ld = tokens->nb[1] / 4;
     a.parents = (const int *)parents->data, a.par_ld = parents->nb[1] / 4;

@@ -62,3 +62,54 @@ def test_long_chains(be, past, N, H, D, page, f16):  # noqa: F811
         ds = 2.0**-20 * scale * float(big)
         tol = (2 * (2 * ds + 2.0**-20) + 8 * math.sqrt(128 * units) * 2.0**-24) * float(v.abs().max())
         check(out[0, n0:n0 + 512].double().cpu().numpy(), want.cpu().numpy(), tol, f16)
+
+
+# ---- what tree_commit writes must not be what it reads ------------------------------------------
+def commit_args(S=3, N=5):
+    import torch
+
+    i32 = dict(dtype=torch.int32, device="cuda")
+    pages = [torch.zeros(4 * S, 2, 8, 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    table = torch.arange(2 * S, **i32).view(S, 2)
+    parents = torch.arange(-1, N - 1, **i32).repeat(S, 1)
+    return dict(tokens=torch.zeros(S, N, **i32), parents=parents, target=torch.zeros(S, N, **i32), n_nodes=torch.full((S,), N, **i32),
+                n_past=torch.arange(S, **i32), table=table, k=pages[0], v=pages[1], layers=1, path=torch.zeros(S, N, **i32),
+                n_accept=torch.zeros(S, **i32), next=torch.zeros(S, **i32), past_out=torch.zeros(S, **i32))
+
+
+def test_tree_commit_refuses_results_over_its_inputs(be):  # noqa: F811
+    import torch
+
+    import openasr_b200 as ob
+
+    ok = commit_args()
+    be.tree_commit(*ok.values())
+    be.synchronize()
+    wide = torch.zeros(3, 12, dtype=torch.int32, device="cuda")
+    for kw in (*(dict(path=ok[x]) for x in ("tokens", "parents", "target")), dict(n_accept=ok["n_nodes"]), dict(n_accept=ok["n_past"]),
+               dict(next=ok["n_past"]), dict(next=ok["n_nodes"]), dict(past_out=ok["n_past"]), dict(past_out=ok["n_nodes"]),
+               dict(n_accept=ok["parents"].view(-1)[6:9]), dict(next=ok["table"].view(-1)[3:6]),       # a part of one
+               dict(tokens=wide[:, 1:6], path=wide[:, 5:10]), dict(next=ok["n_accept"]), dict(past_out=ok["next"]),
+               dict(n_accept=ok["path"].view(-1)[12:15]), dict(path=torch.zeros(1, 5, dtype=torch.int32, device="cuda").expand(3, 5))):
+        with pytest.raises(ob.backend.UnsupportedInputs, match="overlap"):
+            be.tree_commit(*{**ok, **kw}.values())
+            be.synchronize()
+
+
+def test_tree_commit_takes_rows_side_by_side_in_one_buffer(be):  # noqa: F811
+    """inputs may be one tensor, and results may lie between them, as long as no value is both"""
+    import torch
+
+    a = commit_args()
+    want = {**a, **{x: a[x].clone() for x in ("path", "n_accept", "next", "past_out")}}
+    be.tree_commit(*want.values())
+    all_ = torch.zeros(3, 10, dtype=torch.int32, device="cuda")
+    vec = torch.zeros(12, dtype=torch.int32, device="cuda")
+    vec[:3] = a["n_past"]
+    got = {**a, "tokens": all_[:, :5], "target": all_[:, :5], "path": all_[:, 5:], "n_past": vec[:3], "n_accept": vec[3:6],
+           "next": vec[6:9], "past_out": vec[9:]}
+    be.tree_commit(*got.values())
+    be.synchronize()
+    for x in ("path", "n_accept", "next", "past_out"):
+        assert torch.equal(got[x], want[x])
+    assert want["n_accept"].tolist() == [5] * 3
