@@ -143,6 +143,7 @@ int oasr_internal_cuda_fail(oasr_backend *be, cudaError_t e, const char *what, i
     char buf[512];
     snprintf(buf, sizeof buf, "%s failed at backend.cu:%d: %s", what, line, cudaGetErrorString(e));
     int st = e == cudaErrorMemoryAllocation ? OASR_STATUS_ALLOC_FAILED : OASR_STATUS_EXECUTION_FAILED;
+    (void)cudaGetLastError();  // reported here: the next call's launch check must not find it again
     if (be) be->last_native_error = (int64_t)e;
     if (e == cudaErrorIllegalAddress || e == cudaErrorLaunchFailure || e == cudaErrorIllegalInstruction ||
         e == cudaErrorMisalignedAddress || e == cudaErrorHardwareStackError || e == cudaErrorECCUncorrectable ||

@@ -113,3 +113,24 @@ def test_tree_commit_takes_rows_side_by_side_in_one_buffer(be):  # noqa: F811
     for x in ("path", "n_accept", "next", "past_out"):
         assert torch.equal(got[x], want[x])
     assert want["n_accept"].tolist() == [5] * 3
+
+
+def test_an_allocation_that_failed_is_reported_once():
+    """the call after it is not refused for the same error"""
+    import torch
+
+    import openasr_b200 as ob
+    from openasr_b200 import backend as bk
+
+    b = ob.Backend(0)
+    try:
+        b.set_stream(torch.cuda.current_stream())
+        with pytest.raises(bk.AllocFailed):
+            b.reserve_scratch(1 << 50)
+        c = Cache(np.random.default_rng(1), 1, 2, 1, 64, 8, [20])
+        q = np.random.default_rng(2).standard_normal((1, 2, 2, 64)).astype(np.float32)
+        sees = np.tril(np.ones((1, 2, 2), bool))
+        want, tol = attend64(c, q, [2], sees, 0.1)
+        check(run_attn(b, c, q, None, None, 0.1), want, tol, False)
+    finally:
+        b.close()
