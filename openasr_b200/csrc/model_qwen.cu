@@ -764,10 +764,10 @@ int oasr_b200_qwen_verify_tree(oasr_qwen *m, const int32_t *tokens, const int32_
         }
     }
     QStreamScope sc(m);
-    if (!m->tree_logits) {
-        const size_t most = (size_t)m->B * m->Tmax;
-        Q_TRY(qalloc(m, &m->tree_logits, (size_t)TREE_CHUNK * m->cfg.n_vocab * 4));
-        Q_TRY(qalloc(m, &m->tree_ints, (most * (5 + 32) + (size_t)m->B * 5) * 4));
+    if (!m->tree_ints) {  // one allocation: both are there or neither is
+        const size_t logits = align256((size_t)TREE_CHUNK * m->cfg.n_vocab * 4), most = (size_t)m->B * m->Tmax;
+        Q_TRY(qalloc(m, &m->tree_logits, logits + (most * (5 + 32) + (size_t)m->B * 5) * 4));
+        m->tree_ints = (int *)((char *)m->tree_logits + logits);
     }
     const TreeInts t = tree_ints(m, n_seq, n);
     OASR_CUDA_TRY(m->be, cudaMemcpyAsync(t.tokens, rowsv.data(), rowsv.size() * 4, cudaMemcpyHostToDevice, m->stream));
