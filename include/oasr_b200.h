@@ -283,6 +283,7 @@ int oasr_b200_argmax_first(oasr_backend *be, const oasr_tensor *logits, oasr_ten
  *                     position n_past[s] + i
  *   n_nodes           I32 [n_seq] or NULL (= n): live nodes; the rest of the n rows is
  *                     padding, whose outputs are zeros
+ * n_past + n_nodes is at most max_pages * page, and at most 2^31 - 129.
  * All of them live in device memory and are read when the kernel runs, so a captured step
  * can be replayed while the sequences grow.  Page ids and lengths are checked by the
  * kernels: one out of range makes oasr_b200_synchronize return

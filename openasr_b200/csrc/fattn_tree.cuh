@@ -20,7 +20,6 @@
 
 #include "pages.cuh"
 #include "tc_common.cuh"
-#include "tree_split.h"
 
 namespace oasr {
 

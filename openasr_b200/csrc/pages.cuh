@@ -2,6 +2,7 @@
 #pragma once
 
 #include "kernels.cuh"
+#include "tree_split.h"
 
 namespace oasr {
 
@@ -33,7 +34,7 @@ struct KvSeqs {
 static __device__ __forceinline__ bool seq_lengths(const KvSeqs &q, int s, int page, int &past, int &n) {
     past = q.n_past[s];
     n = q.n_nodes ? q.n_nodes[s] : q.N;
-    if (past < 0 || n < 0 || n > q.N || (int64_t)past + n > (int64_t)q.MP * page) {
+    if (!kv_lengths_fit(past, n, q.N, q.MP, page)) {
         past = n = 0;
         return false;
     }

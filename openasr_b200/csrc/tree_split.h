@@ -2,6 +2,8 @@
 // arithmetic alone, for the kernels and for a host that checks it.
 #pragma once
 
+#include <stdint.h>
+
 #include <algorithm>
 
 #ifdef __CUDACC__
@@ -13,6 +15,12 @@
 namespace oasr {
 
 constexpr int TREE_BKV = 128;  // positions per unit
+
+// Whether a sequence's committed positions and live nodes fit its MP pages and the N rows of the
+// tensors; positions are 32-bit numbers, also those at the end of the last unit.
+OASR_HD bool kv_lengths_fit(int past, int n, int N, int MP, int page) {
+    return past >= 0 && n >= 0 && n <= N && (int64_t)past + n <= (int64_t)MP * page && (int64_t)past + n <= INT32_MAX - TREE_BKV;
+}
 
 struct TreeSeg {
     int s, hk, rt;         // sequence, K/V head, row tile

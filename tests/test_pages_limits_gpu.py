@@ -134,3 +134,47 @@ def test_an_allocation_that_failed_is_reported_once():
         check(run_attn(b, c, q, None, None, 0.1), want, tol, False)
     finally:
         b.close()
+
+
+def test_positions_up_to_2_31(be):  # noqa: F811
+    """Two pages of 2^20 positions, repeated 4096 times: the longest cache that 32-bit positions allow is
+    read whole, one position more is reported by every operator."""
+    import torch
+
+    import openasr_b200 as ob
+
+    D, page, MP, T = 64, 1 << 20, 4096, (1 << 31) - 129
+    g = torch.Generator("cuda")
+    g.manual_seed(7)
+    k = torch.randn(2, 1, page, D, generator=g, device="cuda").half()
+    # the first half of the cache has values about 1, the second about 3
+    v = (torch.randn(2, 1, page, D, generator=g, device="cuda") / 4 + torch.tensor([1.0, 3.0], device="cuda").view(2, 1, 1, 1)).half()
+    table = (torch.arange(MP, device="cuda") >= MP // 4).int()[None]
+    q = torch.randn(1, 1, 2, D, generator=g, device="cuda")
+    out = torch.full((1, 1, 2, D), 7.0, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    be.flash_attn_tree(q.permute(0, 2, 1, 3), k, v, table, torch.tensor([T - 1], **i32), None, None, 0.125, out)
+    be.synchronize()
+    p = page * torch.tensor([MP // 4, MP // 4], dtype=torch.int64)  # positions 0 .. T - 1: the last page lacks 129
+    counts = torch.full((1, 2 * page), MP // 4, dtype=torch.float64, device="cuda")
+    counts[0, -129:] -= 1
+    assert int(counts.sum()) == T and int(p.sum()) == T + 129
+    want, big = attend_pool(k[:, 0].reshape(-1, D), v[:, 0].reshape(-1, D), q[0], counts, 0.125)
+    # per sum: 2^24 units in 296 CTAs one after the other, then the 296 parts
+    ds = 2.0**-20 * 0.125 * float(big)
+    tol = (2 * (2 * ds + 2.0**-20) + 8 * math.sqrt(2.0**24 / 296 + 296) * 2.0**-24) * float(v.abs().max())
+    check(out[0].double().cpu().numpy(), want.cpu().numpy(), tol, False)
+
+    x = torch.randn(1, 2, 4, D, generator=g, device="cuda")
+    z2, z1 = torch.zeros(1, 2, **i32), [torch.zeros(1, **i32) for _ in range(4)]
+    before = k.clone()
+    for past, n in ((T - 1, 2), (2**31 - 1, 1), (2**31 - 2, 2)):
+        lens = torch.tensor([past], **i32), torch.tensor([n], **i32)
+        o2 = torch.zeros(1, 2, 2, D, device="cuda")
+        for call in (lambda: be.flash_attn_tree(x[:, :, :2].permute(0, 2, 1, 3), k, v, table, *lens, None, 0.125, o2),
+                     lambda: be.qk_norm_rope(x, None, None, 0.0, None, None, table, *lens, o2, k, v),
+                     lambda: be.tree_commit(z2, z2 - 1, z2, lens[1], lens[0], table, k, v, 1, z2.clone(), z1[0], z1[1], z1[2])):
+            with pytest.raises(ob.backend.ExecutionFailed):
+                call()
+                be.synchronize()
+    assert torch.equal(before, k)

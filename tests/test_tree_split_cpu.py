@@ -59,6 +59,8 @@ static TreeUnits count(int S, const int *past, const int *n, int G, int HKV, int
     return w;
 }
 
+extern "C" int fits(int past, int n, int N, int MP, int page) { return kv_lengths_fit(past, n, N, MP, page); }
+
 // 0: right, else a number that says what is not
 extern "C" int check(int S, const int *past, const int *n, int G, int HKV, int R, int grid, int *in_pieces) {
     std::vector<int> steps;
@@ -151,3 +153,14 @@ def test_every_unit_is_done_once_over_the_whole_range(lib):
         assert rc == 0, (past, n, G, HKV, R, grid)
         pieces += piece > 0
     assert pieces > 300
+
+
+@pytest.mark.parametrize("past,n,N,MP,page,want", [
+    (0, 0, 1, 1, 8, True), (7, 1, 1, 1, 8, True), (8, 1, 1, 1, 8, False), (7, 2, 1, 1, 8, False), (-1, 1, 1, 1, 8, False),
+    (3, -1, 1, 1, 8, False), (-2**31, 1, 1, 1, 8, False), (2**31 - 1, 1, 1, 4096, 2**20, False), (2**31 - 1, 1024, 1024, 2**24, 2**24, False),
+    (2**31 - 1 - 128, 0, 5, 4096, 2**20, True), (2**31 - 1 - 129, 1, 1, 4096, 2**20, True), (2**31 - 1 - 128, 1, 1, 4096, 2**20, False),
+])
+def test_positions_stay_32_bit_numbers(lib, past, n, N, MP, page, want):
+    """a cache of 2^31 positions and more (pages shared by many entries of a table) is in bounds, its last
+    positions are not numbers that a kernel can hold"""
+    assert bool(lib.fits(past, n, N, MP, page)) == want
