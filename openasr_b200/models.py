@@ -384,23 +384,28 @@ class QwenModel:
         done, passes = n_new - 1, 0
         pos = np.full(n, T, np.int32)
         while min(len(o) for o in out) <= done:
-            trees = [draft(s, out[s]) if len(out[s]) <= done else ([], []) for s in range(n)]
-            room = self.cfg.max_pos - int(pos.max())
+            live = [s for s in range(n) if len(out[s]) <= done]
+            trees = {s: draft(s, out[s]) for s in live}
+            room = self.cfg.max_pos - int(pos[live].max())
             if room < 1:
                 raise bk.UnsupportedInputs(bk.STATUS_FAILED, "generate_speculative: the context is full")
-            width = min(1 + max(len(t[0]) for t in trees), room)
+            width = min(1 + max(len(t[0]) for t in trees.values()), room)
             # nodes past a sequence's own draft repeat its root's token under nobody (-1): never accepted
             tokens, parents = np.zeros((n, width), np.int32), np.full((n, width), -1, np.int32)
-            for s, (tk, par) in enumerate(trees):
-                k = min(len(tk), width - 1)
-                tokens[s] = out[s][-1]
-                tokens[s, 1:1 + k] = tk[:k]
-                parents[s, 1:1 + k] = np.asarray(par[:k], np.int32) + 1
-            path, acc, nxt = self.verify_tree(tokens, parents, pos)
-            passes += 1
+            at = np.minimum(pos, self.cfg.max_pos - width)
             for s in range(n):
-                if len(out[s]) > done:
-                    continue  # finished: its position stays, the pass's rows for it are dropped
+                if s in trees:
+                    tk = trees[s][0][:width - 1]
+                    par = trees[s][1][:len(tk)]
+                else:  # finished: where the context ends short of the others' trees, its last tokens once more
+                    tk = out[s][at[s] - T + 1:][:width - 1]
+                    par = range(-1, len(tk) - 1)
+                tokens[s] = out[s][at[s] - T]
+                tokens[s, 1:1 + len(tk)] = tk
+                parents[s, 1:1 + len(tk)] = np.asarray(par, np.int32) + 1
+            path, acc, nxt = self.verify_tree(tokens, parents, at)
+            passes += 1
+            for s in live:
                 out[s] += [int(tokens[s, j]) for j in path[s, 1:acc[s]]] + [int(nxt[s])]
                 pos[s] += acc[s]
         return np.array([o[:n_new] for o in out], np.int32), passes
