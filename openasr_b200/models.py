@@ -376,8 +376,9 @@ class QwenModel:
         """prefill + n_new greedy tokens per sequence, several per pass: before each pass
         draft(s, tokens so far) returns (tokens, parents) of the nodes after the last token of
         sequence s -- parent -1: the last token itself, else an earlier node of the list --, and
-        the model keeps the longest branch that it would have chosen.  Returns
-        ([n_seq][n_new] tokens, number of passes)."""
+        the model keeps the longest branch that it would have chosen; of a draft wider than a pass
+        (verify_tree) or than the context the first nodes count.  Returns ([n_seq][n_new] tokens,
+        number of passes)."""
         _, nxt = self.prefill(emb)
         n, T = emb.shape[0], emb.shape[1]
         out = [[int(t)] for t in nxt]
@@ -389,7 +390,8 @@ class QwenModel:
             room = self.cfg.max_pos - int(pos[live].max())
             if room < 1:
                 raise bk.UnsupportedInputs(bk.STATUS_FAILED, "generate_speculative: the context is full")
-            width = min(1 + max(len(t[0]) for t in trees.values()), room)
+            fits = min(1024, self.cfg.max_batch * self.cfg.max_prefill // n)  # nodes of a sequence that a pass takes
+            width = min(1 + max(len(t[0]) for t in trees.values()), room, fits)
             # nodes past a sequence's own draft repeat its root's token under nobody (-1): never accepted
             tokens, parents = np.zeros((n, width), np.int32), np.full((n, width), -1, np.int32)
             at = np.minimum(pos, self.cfg.max_pos - width)

@@ -90,3 +90,16 @@ def test_the_context_is_full_only_for_a_sequence_that_goes_on():
     m = Decoder(20)
     with pytest.raises(bk.UnsupportedInputs, match="context is full"):
         m.generate_speculative(np.zeros((1, 10, 4), np.float32), drafter(10, lambda s, made: 0), 30)
+
+
+@pytest.mark.parametrize("max_prefill,max_batch,n,most", [(8, 2, 2, 8), (5, 3, 2, 7), (1, 4, 3, 1), (2000, 2, 1, 1024)])
+def test_drafts_wider_than_a_pass_are_cut(max_prefill, max_batch, n, most):
+    """a pass takes max_batch * max_prefill nodes in all and 1024 of a sequence; the rest of a draft waits"""
+    T, n_new = 1, 1100
+    m = Decoder(4000, max_prefill, max_batch)
+    if most < 100:
+        n_new = 30
+    draft = drafter(T, lambda s, made: n_new)
+    got, passes = m.generate_speculative(np.zeros((n, T, 4), np.float32), draft, n_new)
+    assert got.tolist() == [greedy_tokens(s, T, n_new) for s in range(n)]
+    assert max(m.widths) == most and passes == -(-(n_new - 1) // most)
