@@ -375,13 +375,11 @@ static cudaError_t launch_fa_tc(oasr_backend *be, dim3 grid, const CUtensorMap &
                                 const CUtensorMap &mv, int NQ, int NKV, int H, int HKV, float scale_log2,
                                 const oasr_tensor *dst) {
     using C = FaTc<D>;
-    static std::atomic<bool> attr_set{false};  // per instantiation, same for every device of this build
-    if (!attr_set) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(fattn_tc_kernel<D, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
-        if (e != cudaSuccess) return e;
-        attr_set = true;
-    }
+    static OncePerDevice smem;
+    const cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(fattn_tc_kernel<D, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    });
+    if (e != cudaSuccess) return e;
     fattn_tc_kernel<D, CAUSAL><<<grid, C::NTHREADS, C::SMEM_BYTES, be->stream>>>(
         mq, mk, mv, NQ, NKV, H, HKV, scale_log2, (char *)dst->data, dst->nb[1], dst->nb[2], dst->nb[3], be->err_word);
     return cudaGetLastError();

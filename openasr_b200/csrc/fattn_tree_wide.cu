@@ -402,14 +402,12 @@ static int launch_wide(oasr_backend *be, TreeAttn a, const KvPages &p, const KvS
     TreeLaunch l;
     const int st = tree_prepare(be, a, p, s, C::R, 1, &l);
     if (st) return st;
-    static std::atomic<bool> attr_set{false};
-    if (!attr_set) {
-        const cudaError_t e = cudaFuncSetAttribute(fattn_tree_wide_kernel<D, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   C::SMEM);
-        if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
-        attr_set = true;
-    }
-    const cudaError_t e = launch_k(be, fattn_tree_wide_kernel<D, QF16>, dim3(l.grid), dim3(C::NT), C::SMEM, l.k, l.v, a, p, s, l.box,
+    static OncePerDevice smem;
+    cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(fattn_tree_wide_kernel<D, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    });
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree attribute", __LINE__);
+    e = launch_k(be, fattn_tree_wide_kernel<D, QF16>, dim3(l.grid), dim3(C::NT), C::SMEM, l.k, l.v, a, p, s, l.box,
                                    l.parts, l.joins, be->err_word);
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "flash_attn_tree launch", __LINE__);
     return tree_join(be, a, p, s, C::R, l);

@@ -164,11 +164,11 @@ int launch_gemm_f16(oasr_backend *be, const __half *A, int64_t lda, const __half
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return oasr_internal_fail(be, OASR_STATUS_FAILED, "gemm_f16: tensor map encoding failed");
-    static std::atomic<bool> attr_set{false};  // idempotent set-up; concurrent first calls set the same attribute
-    if (!attr_set) {
-        cudaFuncSetAttribute(gemm_f16_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gf16::SMEM_BYTES);
-        attr_set = true;
-    }
+    static OncePerDevice smem;
+    const cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(gemm_f16_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gf16::SMEM_BYTES);
+    });
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "gemm_f16_tc attribute", __LINE__);
     dim3 grid((unsigned)((N + gf16::BN - 1) / gf16::BN), (unsigned)((M + gf16::BM - 1) / gf16::BM));
     gemm_f16_tc_kernel<<<grid, gf16::NTHREADS, gf16::SMEM_BYTES, be->stream>>>(
         ma, mb, M, N, K, y, y_ld, bias, gelu ? be->gelu_table : nullptr, be->err_word);

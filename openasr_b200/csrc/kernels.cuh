@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "once_per_device.h"
 
 namespace oasr {
 

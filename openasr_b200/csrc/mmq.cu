@@ -660,11 +660,11 @@ static int launch_q4k_tc(oasr_backend *be, const oasr_weight *w, int64_t slice, 
     st = encode_2d(be, &map_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, w->h16 + slice * N * K, K, N, (uint64_t)K * 2, 64, 128,
                    CU_TENSOR_MAP_SWIZZLE_128B);
     if (st) return st;
-    static std::atomic<bool> attr_set{false};  // idempotent set-up; concurrent first calls set the same attribute
-    if (!attr_set) {
-        cudaFuncSetAttribute(mmq_q4k_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q4k::SMEM_BYTES);
-        attr_set = true;
-    }
+    static OncePerDevice smem;
+    const cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(mmq_q4k_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q4k::SMEM_BYTES);
+    });
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "mmq_q4k_tc attribute", __LINE__);
     const int64_t meta_sb = Np * q4k::META_COL;
     const float *meta = w->k_meta + slice * (K / 256) * meta_sb;
     dim3 grid((unsigned)((N + q4k::BN - 1) / q4k::BN), (unsigned)((M + q4k::BM - 1) / q4k::BM));
@@ -692,11 +692,11 @@ static int launch_q80_tc(oasr_backend *be, const oasr_weight *w, int64_t slice, 
     st = encode_2d(be, &map_dw, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, w->dT + slice * (int64_t)(K / 32) * N, N, K / 32,
                    (uint64_t)N * 4, 128, 4, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (st) return st;
-    static std::atomic<bool> attr_set{false};  // idempotent set-up; concurrent first calls set the same attribute
-    if (!attr_set) {
-        cudaFuncSetAttribute(mmq_q80_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q80::SMEM_BYTES);
-        attr_set = true;
-    }
+    static OncePerDevice smem;
+    const cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(mmq_q80_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, q80::SMEM_BYTES);
+    });
+    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "mmq_q80_tc attribute", __LINE__);
     dim3 grid((unsigned)((N + q80::BN - 1) / q80::BN), (unsigned)((M + q80::BM - 1) / q80::BM));
     mmq_q80_tc_kernel<<<grid, q80::NTHREADS, q80::SMEM_BYTES, be->stream>>>(map_a, map_w, map_dw, (int)N, a.d, (int)M,
                                                                             K, y, y_ld, be->err_word);
