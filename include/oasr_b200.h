@@ -297,7 +297,9 @@ int oasr_b200_argmax_first(oasr_backend *be, const oasr_tensor *logits, oasr_ten
  * head with gains q_norm / k_norm F32 [D] (NULL: none), then the NeoX rotation of the
  * pairs (i, i + D/2) by rope F32 [2, D/2, n_pos] = (cos, sin) per position (NULL: none)
  * at pos I32 [n, n_seq] (NULL: n_past + i; a tree passes n_past + depth).  Queries go to q
- * F32 or F16 [D, H, n, n_seq], keys and values to their rows of the pages. */
+ * F32 or F16 [D, H, n, n_seq], keys and values to their rows of the pages.  Squares are
+ * rounded to 32 bits and summed in 64, as in ggml's RMSNorm and the decoders here: the same
+ * head gives the same bits in all of them. */
 int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_tensor *q_norm,
                            const oasr_tensor *k_norm, float eps, const oasr_tensor *rope, const oasr_tensor *pos,
                            const oasr_tensor *page_table, const oasr_tensor *n_past, const oasr_tensor *n_nodes,

@@ -85,11 +85,14 @@ struct NormRope {
 // position: (a cos - b sin, b cos + a sin).  D / 4 lanes take a head, two neighbouring values and
 // the two they turn with per lane, so that the rotation needs no other lane; a warp takes U rounds
 // of heads of one node, and what depends on the node alone (lengths, page, angles, gains) is
-// fetched once for all of them.  The sums of squares of the U rounds share one butterfly (at each
-// step a lane passes on the heads its partner keeps).  For prompts bound by HBM and the issue of
-// some 100 instructions per head: eight prompts of 512 rows of 16 + 16 heads (97 MB) take 24 us, 4.0
-// TB/s (30 us with two rounds per warp; 24 with eight, but then eight trees of 61 nodes of D = 64 take
-// 6.4 instead of 4.1 us).  For a step's few rows by three dependent loads and the launch: 2.5 us.
+// fetched once for all of them.  The squares are summed in 64 bits and every product is rounded as in
+// the decoders' own norm (qwen_qkv_post_kernel), so that a verification pass writes the bits that a
+// decode step writes; the sums of the U rounds share one butterfly (at each step a lane passes on the
+// heads its partner keeps).  For prompts bound by HBM and the issue of some 100 instructions per head:
+// eight prompts of 512 rows of 16 + 16 heads (97 MB) take 26.0 us, 3.7 TB/s, and eight trees of 61 nodes
+// of D = 64 4.6 us.  Sums in 32 bits took 24.5 and 4.2 (with them, two rounds per warp took 30 us for the
+// prompts; eight 24, but then the trees 6.4) and left one K value in some 200 heads a bit apart.  For a
+// step's few rows by three dependent loads and the launch: 2.5 us.
 template <int D, int U, bool QF16>
 __global__ void __launch_bounds__(U == 1 ? 256 : 128)
     qk_norm_rope_kernel(NormRope a, KvPages p, KvSeqs sq, FastDiv nodes, FastDiv page, int groups, int *err) {
@@ -163,12 +166,13 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128)
     // sums of squares: lane LPH / U * u of a head's lanes ends with that of round u
     float scale = 0.0f;
     {
-        float ss[U];
+        double ss[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ss[u] = 0.0f;
+            ss[u] = 0.0;
             if (h0 + W * u < a.H + a.HKV)  // value heads have no norm
-                ss[u] = fmaf(lo[u].x, lo[u].x, lo[u].y * lo[u].y) + fmaf(hi[u].x, hi[u].x, hi[u].y * hi[u].y);
+                ss[u] = ((double)__fmul_rn(lo[u].x, lo[u].x) + (double)__fmul_rn(lo[u].y, lo[u].y)) +
+                        ((double)__fmul_rn(hi[u].x, hi[u].x) + (double)__fmul_rn(hi[u].y, hi[u].y));
         }
 #pragma unroll
         for (int o = LPH / 2, m = U / 2; o > 0; o >>= 1, m >>= 1) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(U == 1 ? 256 : 128)
             for (int k = 0; k < m; ++k)
                 ss[k] = (up ? ss[k + m] : ss[k]) + __shfl_xor_sync(0xffffffffu, up ? ss[k] : ss[k + m], o);
         }
-        scale = __frcp_rn(__fsqrt_rn(fmaf(ss[0], 1.0f / D, a.eps)));
+        scale = __frcp_rn(__fsqrt_rn(__fadd_rn((float)(ss[0] / (double)D), a.eps)));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -429,8 +433,8 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
     a.gains8 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 7) == 0;
-    // four rounds of heads per warp share what belongs to the node (eight prompts of 512 rows: 24 us,
-    // 30 with two), as long as that leaves every SM some blocks; below that one round per warp, so
+    // four rounds of heads per warp share what belongs to the node (eight prompts of 512 rows: 26 us;
+    // 24 against 30 with two when the sums were in 32 bits), as long as that leaves every SM some blocks; below that one round per warp, so
     // that a step's few rows start at once
     const int64_t HH = qkv->ne[1], per = D == 64 ? 2 : 1, few = (HH + 8 * per - 1) / (8 * per),
                   many = (HH + 16 * per - 1) / (16 * per);
