@@ -339,10 +339,10 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * Sequences share pages by reference: a fork copies nothing until one of the two writes.
  * open / fork return the new sequence's number (0 .. max_seqs - 1), OASR_STATUS_ALLOC_FAILED
  * when all are in use.  extend makes positions [from, to) writable, from at most what the
- * sequence holds: it takes new pages, and pages of its own in the place of shared ones;
+ * sequence's pages hold: it takes new pages, and pages of its own in the place of shared ones;
  * where the rows before `from` of such a page have to come along, the (source,
  * destination) pair for oasr_b200_kv_pages_copy goes to pairs [max_pairs][2] (at most one
- * per call).  It returns the number of pairs, or OASR_STATUS_ALLOC_FAILED with nothing
+ * per call); what shared pages held from `from` on does not.  It returns the number of pairs, or OASR_STATUS_ALLOC_FAILED with nothing
  * changed when the pool has too few free pages.  truncate gives the pages past position
  * n_pos back (after a commit, or to drop a draft); close gives all of them back.  table
  * writes the sequence's row of the page table, row[max_pages], -1 past its pages, and

@@ -120,7 +120,8 @@ int32_t oasr_b200_kv_pool_extend(oasr_kv_pool *pool, int32_t seq, int32_t from, 
     return guarded([&]() -> int32_t {
         std::vector<int32_t> &own = pool->seqs[(size_t)seq].pages;
         const int32_t first = from / pool->page, last = (int32_t)(((int64_t)to + pool->page - 1) / pool->page), held = (int32_t)own.size();
-        if (last > pool->max_pages || first > held) return OASR_STATUS_FAILED;  // positions before `from` have to be held
+        // positions before `from` have to be held, in whole pages
+        if (last > pool->max_pages || from > (int64_t)held * pool->page) return OASR_STATUS_FAILED;
         // what it takes: new pages, and own ones in the place of shared pages that are written
         int32_t need = std::max(0, last - held), copies = 0;
         for (int32_t j = first; j < std::min(last, held); ++j)
