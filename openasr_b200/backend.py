@@ -784,7 +784,9 @@ class KvPool:
 
 def tree_mask(parents) -> np.ndarray:
     """int32 words [n, ceil(n / 32)] of a drafted tree: each node sees itself and its ancestors."""
-    par = np.ascontiguousarray(parents, np.int32)
+    par = np.asarray(parents, np.int32, order="C")
+    if par.ndim != 1:
+        raise UnsupportedInputs(STATUS_FAILED, "tree_mask: parents [n] of one sequence")
     words = np.zeros((len(par), (len(par) + 31) // 32), np.int32)
     rc = lib().oasr_b200_tree_mask(par.ctypes.data, len(par), words.ctypes.data)
     if rc != 0:

@@ -59,3 +59,11 @@ def test_a_tensor_of_five_dimensions_is_refused(ops):
     ready = bk.describe(torch.zeros(2, 2))
     with pytest.raises(bk.UnsupportedInputs, match="at most 4 dimensions, not 5"):
         bk._ops().kv_pages_copy(be.handle.value or 0, torch.zeros(2, 3, 2, 8, 64, dtype=torch.float16), ready, 1, ready)
+
+
+def test_tree_mask_takes_one_sequence():
+    """of a table of sequences the first column's length was taken as the number of nodes"""
+    for bad in ([[-1, 0, 1], [-1, 0, 0]], -1, [[]]):
+        with pytest.raises(bk.UnsupportedInputs):
+            bk.tree_mask(bad)
+    assert bk.tree_mask([]).shape == (0, 0) and bk.tree_mask([-1, 0]).tolist() == [[1], [3]]
