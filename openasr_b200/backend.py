@@ -784,8 +784,8 @@ class KvPool:
 
 def tree_mask(parents) -> np.ndarray:
     """int32 words [n, ceil(n / 32)] of a drafted tree: each node sees itself and its ancestors."""
-    par = np.asarray(parents, np.int32, order="C")
-    if par.ndim != 1:
+    par = np.ascontiguousarray(parents, np.int32)
+    if par.size != len(par):
         raise UnsupportedInputs(STATUS_FAILED, "tree_mask: parents [n] of one sequence")
     words = np.zeros((len(par), (len(par) + 31) // 32), np.int32)
     rc = lib().oasr_b200_tree_mask(par.ctypes.data, len(par), words.ctypes.data)

@@ -63,7 +63,8 @@ def test_a_tensor_of_five_dimensions_is_refused(ops):
 
 def test_tree_mask_takes_one_sequence():
     """of a table of sequences the first column's length was taken as the number of nodes"""
-    for bad in ([[-1, 0, 1], [-1, 0, 0]], -1, [[]]):
+    for bad in ([[-1, 0, 1], [-1, 0, 0]], [[]]):
         with pytest.raises(bk.UnsupportedInputs):
             bk.tree_mask(bad)
     assert bk.tree_mask([]).shape == (0, 0) and bk.tree_mask([-1, 0]).tolist() == [[1], [3]]
+    assert bk.tree_mask([[-1], [0]]).tolist() == [[1], [3]] and bk.tree_mask(-1).tolist() == [[1]], "as before"
