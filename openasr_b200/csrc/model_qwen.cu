@@ -25,6 +25,7 @@
 #include <string.h>
 
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -738,7 +739,7 @@ int oasr_b200_qwen_generate(oasr_qwen *m, const float *emb, int32_t emb_on_devic
 }
 
 int oasr_b200_qwen_verify_tree(oasr_qwen *m, const int32_t *tokens, const int32_t *parents, int32_t n_seq, int32_t n,
-                               const int32_t *pos, int32_t *path, int32_t *n_accept, int32_t *next) {
+                               const int32_t *pos, int32_t *path, int32_t *n_accept, int32_t *next) try {
     if (!m) return OASR_STATUS_FAILED;
     if (!tokens || !parents || !pos || !path || !n_accept || !next || n_seq < 1 || n_seq > m->B || n < 1 || n > 1024 ||
         (int64_t)n_seq * n > (int64_t)m->B * m->Tmax || m->P % 8)
@@ -790,6 +791,8 @@ int oasr_b200_qwen_verify_tree(oasr_qwen *m, const int32_t *tokens, const int32_
     OASR_CUDA_TRY(m->be, cudaMemcpyAsync(m->nkv, got.data() + 2 * (size_t)n_seq, n_seq * 4, cudaMemcpyHostToDevice, m->stream));
     OASR_CUDA_TRY(m->be, cudaStreamSynchronize(m->stream));
     return oasr_b200_synchronize(m->be);
+} catch (const std::bad_alloc &) {  // nothing may be thrown through the C boundary
+    return OASR_STATUS_ALLOC_FAILED;
 }
 
 int oasr_b200_qwen_read_kv(oasr_qwen *m, int32_t layer, int32_t seq, int32_t n_pos, uint16_t *k_out, uint16_t *v_out) {

@@ -51,3 +51,54 @@ def test_prompt_and_tokens_may_fill_the_context(gpu_backend):
             m.generate(emb, n_new=n_new + 1)
     finally:
         m.close()
+
+
+WITHOUT_HOST_MEMORY = """
+import ctypes, resource
+import numpy as np
+import openasr_b200 as ob
+from openasr_b200 import backend as bk, models as om
+
+cfg = om.QWEN3_ASR_0_6B.replace(n_layers=1, n_vocab=4096, max_pos=1040, max_prefill=1024, max_batch=8)
+be = ob.Backend(0)
+m = om.QwenModel(be, cfg, om.qwen_synthetic_pack(cfg, seed=0x0A5A0003))
+_, first = m.prefill(om.qwen_synthetic_prefix(0x0A5A3000, 8, 8, cfg.d_model))
+tokens = np.tile(first[:, None], (1, 1024)).astype(np.int32)
+parents = np.tile(np.arange(-1, 1023, dtype=np.int32), (8, 1))
+pos, path, acc, nxt = np.full(8, 8, np.int32), np.empty_like(tokens), np.zeros(8, np.int32), np.zeros(8, np.int32)
+args = (m.handle, tokens.ctypes.data, parents.ctypes.data, 8, 1024, pos.ctypes.data, path.ctypes.data, acc.ctypes.data, nxt.ctypes.data)
+verify = bk.lib().oasr_b200_qwen_verify_tree
+libc = ctypes.CDLL(None)
+libc.malloc.restype, libc.malloc.argtypes, libc.free.argtypes = ctypes.c_void_p, [ctypes.c_size_t], [ctypes.c_void_p]
+held, size = [], 1 << 20
+pages = int(open("/proc/self/statm").read().split()[0])
+_, hard = resource.getrlimit(resource.RLIMIT_AS)
+resource.setrlimit(resource.RLIMIT_AS, (pages * 4096, hard))
+while size >= 1 << 17:  # the masks of the trees alone take a megabyte
+    p = libc.malloc(size)
+    if p:
+        held.append(p)
+    else:
+        size >>= 1
+rc = verify(*args)
+resource.setrlimit(resource.RLIMIT_AS, (hard, hard))
+for p in held:
+    libc.free(p)
+assert rc == bk.STATUS_ALLOC_FAILED, rc
+rc = verify(*args)
+assert rc == 0 and (acc >= 1).all(), rc
+m.close()
+be.close()
+print("passed")
+"""
+
+
+def test_a_pass_without_host_memory_is_a_status(gpu_backend):
+    """not an exception through the C entry, which would end the process"""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(ob.__file__)))
+    r = subprocess.run([sys.executable, "-c", WITHOUT_HOST_MEMORY], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.endswith("passed\n"), r.stderr[-2000:]
