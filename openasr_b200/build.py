@@ -56,22 +56,38 @@ def _compile(src: str, verbose: bool) -> str:
 
 
 def _build_torch_ops() -> None:
-    """The Python binding's extension; without torch's headers the binding goes through ctypes
-    (slower, the same calls)."""
+    """The Python binding's extension, for the torch that is installed.  Without torch's headers, or
+    where they do not compile, there is none and the binding goes through ctypes (slower, the same calls)."""
     spec = importlib.util.find_spec("torch")
     torch = os.path.dirname(spec.origin) if spec and spec.origin else ""
     src, inc = os.path.join(CSRC, "torch_ops.cc"), sysconfig.get_path("include")
+    stamp = TORCH_OPS + ".for"  # which torch and Python it was built for: another one's may not be loaded
     if not (os.path.exists(os.path.join(torch, "include", "torch", "csrc", "autograd", "python_variable.h"))
             and os.path.exists(os.path.join(inc, "Python.h"))):
+        _remove(TORCH_OPS, stamp)
         return
-    if os.path.exists(TORCH_OPS) and os.path.getmtime(TORCH_OPS) >= max(os.path.getmtime(src), _headers_mtime()):
+    with open(os.path.join(torch, "version.py")) as f:
+        wants = f"{sys.version}\n{torch}\n{f.read()}"
+    if os.path.exists(TORCH_OPS) and os.path.getmtime(TORCH_OPS) >= max(os.path.getmtime(src), _headers_mtime()) and \
+            os.path.exists(stamp) and open(stamp).read() == wants:
         return
+    _remove(TORCH_OPS, stamp)
     cmd = [HOST_CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I", inc,
            "-isystem", os.path.join(torch, "include"), src, "-o", TORCH_OPS, "-L", os.path.join(torch, "lib"),
            "-ltorch_python", "-ltorch_cpu", "-lc10"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        _remove(TORCH_OPS)
+        sys.stderr.write(f"the Python binding's extension does not compile, its calls go through ctypes: {' '.join(cmd)}\n{r.stderr}")
+        return
+    with open(stamp, "w") as f:
+        f.write(wants)
+
+
+def _remove(*paths: str) -> None:
+    for p in paths:
+        if os.path.exists(p):
+            os.remove(p)
 
 
 def build(verbose: bool = False) -> str:
