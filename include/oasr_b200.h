@@ -285,7 +285,11 @@ int oasr_b200_argmax_first(oasr_backend *be, const oasr_tensor *logits, oasr_ten
  *                     padding, whose outputs are zeros
  * n_past + n_nodes is at most max_pages * page, and at most 2^31 - 129.
  * All of them live in device memory and are read when the kernel runs, so a captured step
- * can be replayed while the sequences grow.  Page ids and lengths are checked by the
+ * can be replayed while the sequences grow.  The attention's unfinished sums lie in the
+ * backend's scratch, whose address a capture keeps: reserve before the capture what the
+ * largest later call of the backend takes (oasr_b200_reserve_scratch), and capture again
+ * after a call that made the scratch grow (oasr_b200_mem_stats) or after the memory API's
+ * trim -- a replay would write to memory that is no longer the backend's.  Page ids and lengths are checked by the
  * kernels: one out of range makes oasr_b200_synchronize return
  * OASR_STATUS_EXECUTION_FAILED, nothing outside the pages is touched, and the call's
  * outputs for that sequence are undefined.  Pages that a call writes must belong to one
