@@ -315,8 +315,10 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
  * n, H, n_seq], dst F32 or F16 [D, H, n, n_seq] as in oasr_b200_flash_attn_ext, H % H_kv
  * == 0.  A row that sees nothing is zeros.  What a row does not see does not reach it: K
  * and V rows of hidden nodes and of positions past the last node may hold anything.  What it
- * does see and is not finite makes its output NaN or infinite: all of the row for a query or
- * a K value, that value of D for a V value. */
+ * does see and is not finite reaches it: a query makes its row NaN (zeros, if every score is
+ * -inf), a V value that value of D NaN or infinite, a K value the row NaN -- or, where its
+ * score is -inf, the position's weight zero (with F32 queries one or the other: they are
+ * multiplied in two parts). */
 int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages,
                               const oasr_tensor *v_pages, const oasr_tensor *page_table, const oasr_tensor *n_past,
                               const oasr_tensor *n_nodes, const oasr_tensor *tree, float scale, oasr_tensor *dst);
@@ -346,11 +348,11 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * sequence's pages hold: it takes new pages, and pages of its own in the place of shared ones;
  * where the rows before `from` of such a page have to come along, the (source,
  * destination) pair for oasr_b200_kv_pages_copy goes to pairs [max_pairs][2] (at most one
- * per call); what shared pages held from `from` on does not.  It returns the number of pairs, or OASR_STATUS_ALLOC_FAILED with nothing
- * changed when the pool has too few free pages.  truncate gives the pages past position
- * n_pos back (after a commit, or to drop a draft); close gives all of them back.  table
- * writes the sequence's row of the page table, row[max_pages], -1 past its pages, and
- * returns how many it has. */
+ * per call); what shared pages held from `from` on does not.  It returns the number of
+ * pairs, or OASR_STATUS_ALLOC_FAILED with nothing changed when the pool has too few free
+ * pages.  truncate gives the pages past position n_pos back (after a commit, or to drop a
+ * draft); close gives all of them back.  table writes the sequence's row of the page table,
+ * row[max_pages], -1 past its pages, and returns how many it has. */
 typedef struct oasr_kv_pool oasr_kv_pool;
 int oasr_b200_kv_pool_create(int32_t n_pages, int32_t page, int32_t max_pages, int32_t max_seqs, oasr_kv_pool **out);
 int oasr_b200_kv_pool_free(oasr_kv_pool *pool);

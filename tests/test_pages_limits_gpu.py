@@ -43,6 +43,8 @@ def repeated_pages(seed, page, pages, D, past, N):
 
 @pytest.mark.parametrize("past,N,H,D,page,f16", [
     (1000000, 4968, 32, 64, 64, True),   # 1242 tiles of 128 rows, 7822 steps each: 66000 steps to a CTA
+    (0, 1500, 3, 128, 16, False),        # a chain longer than a tree may be
+    (70, 1100, 1, 64, 40, False),
 ])
 def test_long_chains(be, past, N, H, D, page, f16):  # noqa: F811
     import torch
@@ -178,3 +180,59 @@ def test_positions_up_to_2_31(be):  # noqa: F811
                 call()
                 be.synchronize()
     assert torch.equal(before, k)
+
+
+@pytest.mark.parametrize("N,H,HKV,D", [(1, 4, 2, 128), (7, 6, 6, 64), (20, 8, 2, 128), (61, 4, 2, 128), (150, 2, 1, 64)])
+@pytest.mark.parametrize("q16,o16", [(False, True), (True, False)])
+def test_queries_and_outputs_of_different_types(be, N, H, HKV, D, q16, o16):  # noqa: F811
+    import torch
+
+    rng = np.random.default_rng(N + D)
+    c = Cache(rng, 2, N, HKV, D, 16, [130, 9])
+    q = rng.standard_normal((2, H, N, D)).astype(np.float16 if q16 else np.float32)
+    sees = np.broadcast_to(np.tril(np.ones((N, N), bool)), (2, N, N))
+    live = np.array([N, max(1, N // 2)], np.int32)
+    want, tol = attend64(c, q, live, sees, 0.09)
+    k, v = c.device()
+    out = torch.full((2, N, H, D), 7.0, dtype=torch.float16 if o16 else torch.float32, device="cuda")
+    be.flash_attn_tree(cuda(q), k, v, cuda(c.table), cuda(c.past), cuda(live), None, 0.09, out)
+    be.synchronize()
+    check(out.cpu().double().numpy(), want, tol, o16)
+
+
+@pytest.mark.parametrize("N", [3, 14, 30, 80])
+@pytest.mark.parametrize("f16", [False, True])
+def test_a_key_whose_score_is_minus_infinity(be, N, f16):  # noqa: F811
+    """f16 queries: the position has no weight; f32 ones: that, or the row is NaN"""
+    rng = np.random.default_rng(N)
+    c = Cache(rng, 1, N, 2, 128, 16, [150])
+    q = rng.standard_normal((1, 4, N, 128)).astype(np.float16 if f16 else np.float32)
+    q[..., 5] = -np.abs(q[..., 5]) - np.float16(0.5)
+    c.k[c.table[0, 1], :, 4, 5] = np.inf  # position 20
+    sees = np.tril(np.ones((1, N, N), bool))
+    without = Cache(rng, 1, N, 2, 128, 16, [149])
+    for name in ("k", "v"):
+        rows = np.delete(c.rows(getattr(c, name), 0, 150 + N), 20, axis=1)
+        at = np.arange(149 + N)
+        getattr(without, name)[without.table[0, at // 16], :, at % 16] = rows.transpose(1, 0, 2)
+    want, tol = attend64(without, q, [N], sees, 0.1)
+    got = run_attn(be, c, q, None, None, 0.1, f16)
+    if not f16:
+        assert np.isnan(got).all(-1)[np.isnan(got).any(-1)].all()
+        got = np.where(np.isnan(got), want, got)
+    check(got, want, tol, f16)
+
+
+def test_calls_of_too_many_steps_are_refused(be):  # noqa: F811
+    """rows and positions that 31 bits do not count (views of little memory: nothing is read)"""
+    import torch
+
+    import openasr_b200 as ob
+
+    k, v = (torch.zeros(1, 1, 4096, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    past = torch.zeros(1, dtype=torch.int32, device="cuda")
+    row = torch.zeros(1, 1, 1, 64, device="cuda")
+    table = torch.zeros(1, 1 << 22, dtype=torch.int32, device="cuda")
+    for N, H, MP in ((1 << 24, 128, 1), (1 << 24, 1, 1 << 18), (1 << 17, 1, 1 << 22)):
+        with pytest.raises(ob.backend.UnsupportedInputs, match="too many"):
+            be.flash_attn_tree(row.expand(1, H, N, 64), k, v, table[:, :MP], past, None, None, 0.1, row.expand(1, N, H, 64))
