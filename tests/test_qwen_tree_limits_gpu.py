@@ -102,3 +102,29 @@ def test_a_pass_without_host_memory_is_a_status(gpu_backend):
     root = os.path.dirname(os.path.dirname(os.path.abspath(ob.__file__)))
     r = subprocess.run([sys.executable, "-c", WITHOUT_HOST_MEMORY], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.endswith("passed\n"), r.stderr[-2000:]
+
+
+def test_a_pass_over_all_layers(gpu_backend):
+    """28 layers: every token that a pass selects is within what the decoder's tensor-core prompt pass is
+    held to at full depth (4e-2 of the largest logit, test_qwen_gpu.py) of a decode step's best"""
+    bound, T, steps, n = 4e-2, 60, 20, 3
+    cfg = om.QWEN3_ASR_0_6B.replace(n_vocab=4096, max_pos=128, max_prefill=64, max_batch=4)
+    m = om.QwenModel(gpu_backend, cfg, om.qwen_synthetic_pack(cfg, seed=0x0A5A0003))
+    try:
+        emb = om.qwen_synthetic_prefix(0x0A5A5000, n, T, cfg.d_model)
+        serial = m.generate(emb, n_new=steps)
+
+        def draft(s, tokens):  # two right tokens, beside them a wrong one with a child
+            tk = serial[s, len(tokens):len(tokens) + 2].tolist()
+            return tk + [(tokens[-1] + 1) % cfg.n_vocab, 7], list(range(-1, len(tk) - 1)) + [-1, len(tk)]
+
+        got, passes = m.generate_speculative(emb, draft, steps)
+        assert passes < steps - 1
+        logits, _ = m.prefill(emb)
+        for i in range(steps):
+            if i:
+                logits, _ = m.decode_step(got[:, i - 1], T + i - 1)
+            below = logits.max(1) - logits[np.arange(n), got[:, i]]
+            assert (below <= bound * np.abs(logits).max(1)).all(), i
+    finally:
+        m.close()
