@@ -14,8 +14,9 @@
 // the same 128 rows.  Accuracy, offsets and the split over the CTAs are those of fattn_tree.cu.
 // S(j + 2) overwrites P(j): the products of one thread run in the order of their issue.
 //
-// Sixteen trees of 61 nodes, 4001 to 8190 positions, 8 K/V heads of 128, f16 (411 MB): 96 us, 4.3 TB/s
-// (112 us with equal runs that did not count the segments' ends).  A unit takes a CTA 2600 clocks, of
+// Sixteen trees of 61 nodes, 4001 to 8190 positions, 8 K/V heads of 128, f16 (411 MB): 97 us, 4.2 TB/s
+// at 1965 MHz (112 us with equal runs that did not count the segments' ends); back to back for a third
+// of a second the power cap holds the SM clock near 1650 MHz and a call takes 107 to 119 us.  A unit takes a CTA 2600 clocks, of
 // which the weights are 2400 of a group's 5200 -- 32 columns at a time: a loop over 16 columns takes
 // 101 us, two rounds in one body 104, all four unrolled 102 (code is fetched more slowly than run).
 // P goes to the matrix unit by 32 positions; handed over whole it took 133 -> 141 us for four chunks of

@@ -88,9 +88,9 @@ struct NormRope {
 // fetched once for all of them.  The squares are summed in 64 bits and every product is rounded as in
 // the decoders' own norm (qwen_qkv_post_kernel), so that a verification pass writes the bits that a
 // decode step writes; the sums of the U rounds share one butterfly (at each step a lane passes on the
-// heads its partner keeps).  For prompts bound by HBM and the issue of some 100 instructions per head:
-// eight prompts of 512 rows of 16 + 16 heads (97 MB) take 26.0 us, 3.7 TB/s, and eight trees of 61 nodes
-// of D = 64 4.6 us.  Sums in 32 bits took 24.5 and 4.2 (with them, two rounds per warp took 30 us for the
+// heads its partner keeps).  For prompts bound by HBM and the issue of some 140 instructions per head:
+// eight prompts of 512 rows of 16 + 16 heads (97 MB) take 25.7 us, 3.8 TB/s, and eight trees of 61 nodes
+// of D = 64 4.5 us.  Sums in 32 bits took 24.3 and 4.2 (with them, two rounds per warp took 30 us for the
 // prompts; eight 24, but then the trees 6.4) and left one K value in some 200 heads a bit apart.  For a
 // step's few rows by three dependent loads and the launch: 2.5 us.
 template <int D, int U, bool QF16>
@@ -236,7 +236,8 @@ struct Commit {
 // moves 256 columns of 16 bytes of (layer, K or V, head).  Bound by HBM's rate for 256-byte rows
 // from all over the pages: 32 trees, 13 rows each, 28 layers of 8 heads of 128 (88 MB) take 22 us, 4.0
 // TB/s; more CTAs per SM (5 to 7 in the place of 4) take 23 to 25 us, twelve rows at a time 25, four
-// 22.  4 us of it, and all of a small call, are the dependent loads up to the first row.
+// 22.  4 us of it, and all of a small call, are the dependent loads up to the first row; those 896 CTAs
+// are one and a half waves, and the second wave has them once more.
 __global__ void __launch_bounds__(256) tree_commit_kernel(Commit a, KvPages p, KvSeqs sq, FastDiv page, int *err) {
     griddep_launch_dependents();
     griddep_wait();

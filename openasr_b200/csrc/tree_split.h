@@ -43,7 +43,8 @@ struct TreeUnits {
 // best of 1, 3, 5, 7 for tiles up to 64 rows (69.6, 69.2, 69.1, 69.1 us for 16 x 16 rows, 16 x 64 86.8,
 // 84.7, 84.0, 85.1), of 7, 9, 12, 16 for 128 (16 trees of 61 nodes 100.8, 100.3, 103.6, 109).  A join:
 // 8 sequences of one token of 20 heads of 64 take 13.3, 13.8, 11.5, 11.5 us with 1, 2, 3, 5, one token
-// alone 8.8, 8.8, 8.8, 9.9.
+// alone 8.8, 8.8, 8.8, 9.9.  The segments' figures are of D = 128; a unit of D = 64 is half the bytes,
+// for which no other values were measured.
 OASR_HD constexpr int tree_segment(int R) { return R == 128 ? 9 : 5; }
 constexpr int TREE_JOIN = 3;
 
