@@ -16,9 +16,12 @@ using namespace oasr;
 
 namespace oasr {
 
+// 4-byte values that are read and written as such
+static bool aligned4(const oasr_tensor *t) { return ((uintptr_t)t->data & 3) == 0; }
+
 static bool is_vec_i32(const oasr_tensor *t, int64_t n) {
-    return t && t->type == OASR_TYPE_I32 && t->data && t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 && t->ne[3] == 1 &&
-           (t->nb[0] == 4 || n <= 1);
+    return t && t->type == OASR_TYPE_I32 && t->data && aligned4(t) && t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 &&
+           t->ne[3] == 1 && (t->nb[0] == 4 || n <= 1);
 }
 
 static int fail_op(oasr_backend *be, const char *op, const char *what) {
@@ -51,8 +54,8 @@ int seqs_check(oasr_backend *be, const char *op, const oasr_tensor *table, const
                const oasr_tensor *n_nodes, int64_t S, int64_t N, KvSeqs *out) {
     if (!table || !n_past) return fail_op(be, op, "null argument");
     if (S > (1 << 20) || N > (1 << 24) || S * N > INT32_MAX) return fail_op(be, op, "too many sequences or nodes");
-    if (table->type != OASR_TYPE_I32 || !table->data || table->ne[1] != S || table->ne[2] != 1 || table->ne[3] != 1 ||
-        table->ne[0] < 1 || table->ne[0] > (1 << 24) || (table->nb[0] != 4 && table->ne[0] > 1) || table->nb[1] % 4)
+    if (table->type != OASR_TYPE_I32 || !table->data || !aligned4(table) || table->ne[1] != S || table->ne[2] != 1 ||
+        table->ne[3] != 1 || table->ne[0] < 1 || table->ne[0] > (1 << 24) || (table->nb[0] != 4 && table->ne[0] > 1) || table->nb[1] % 4)
         return fail_op(be, op, "page_table must be I32 [max_pages, n_seq]");
     if (!is_vec_i32(n_past, S)) return fail_op(be, op, "n_past must be I32 [n_seq]");
     if (n_nodes && !is_vec_i32(n_nodes, S)) return fail_op(be, op, "n_nodes must be I32 [n_seq]");
@@ -358,8 +361,8 @@ bool rows16(const oasr_tensor *t) {
 
 // I32 [N, S] with contiguous rows
 bool is_rows_i32(const oasr_tensor *t, int64_t N, int64_t S) {
-    return t && t->type == OASR_TYPE_I32 && t->data && t->ne[0] == N && t->ne[1] == S && t->ne[2] == 1 && t->ne[3] == 1 &&
-           (t->nb[0] == 4 || N <= 1) && t->nb[1] % 4 == 0;
+    return t && t->type == OASR_TYPE_I32 && t->data && aligned4(t) && t->ne[0] == N && t->ne[1] == S && t->ne[2] == 1 &&
+           t->ne[3] == 1 && (t->nb[0] == 4 || N <= 1) && t->nb[1] % 4 == 0;
 }
 
 // Rows of I32 on the device: `n` rows of `width` values, `ld` values apart.
@@ -405,8 +408,8 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     if ((q->type != OASR_TYPE_F32 && q->type != OASR_TYPE_F16) || q->ne[0] != D || q->ne[1] != H || q->ne[2] != N || q->ne[3] != S)
         return fail_op(be, op, "q must be F32 or F16 [D, H, n, n_seq]");
     for (const oasr_tensor *w : {q_norm, k_norm})
-        if (w && (w->type != OASR_TYPE_F32 || !w->data || w->ne[0] != D || w->ne[1] != 1 || w->ne[2] != 1 || w->ne[3] != 1 ||
-                  w->nb[0] != 4))
+        if (w && (w->type != OASR_TYPE_F32 || !w->data || !aligned4(w) || w->ne[0] != D || w->ne[1] != 1 || w->ne[2] != 1 ||
+                  w->ne[3] != 1 || w->nb[0] != 4))
             return fail_op(be, op, "q_norm and k_norm must be F32 [D]");
     if ((q_norm || k_norm) && !(eps >= 0.0f)) return fail_op(be, op, "eps must not be negative");
     if (rope && (rope->type != OASR_TYPE_F32 || !rope->data || rope->ne[0] != 2 || rope->ne[1] != D / 2 || rope->ne[2] < 1 ||
@@ -434,9 +437,9 @@ int oasr_b200_qk_norm_rope(oasr_backend *be, const oasr_tensor *qkv, const oasr_
     a.S = (int)S, a.H = (int)H, a.HKV = (int)HKV;
     a.eps = eps;
     a.gains8 = a.q_norm && a.k_norm && (((uintptr_t)a.q_norm | (uintptr_t)a.k_norm) & 7) == 0;
-    // four rounds of heads per warp share what belongs to the node (eight prompts of 512 rows: 26 us;
-    // 24 against 30 with two when the sums were in 32 bits), as long as that leaves every SM some blocks; below that one round per warp, so
-    // that a step's few rows start at once
+    // four rounds of heads per warp share what belongs to the node (eight prompts of 512 rows: 26 us; 24
+    // against 30 with two when the sums were in 32 bits), as long as that leaves every SM some blocks;
+    // below that one round per warp, so that a step's few rows start at once
     const int64_t HH = qkv->ne[1], per = D == 64 ? 2 : 1, few = (HH + 8 * per - 1) / (8 * per),
                   many = (HH + 16 * per - 1) / (16 * per);
     const bool share = S * N * many >= 4 * be->sm_count;
@@ -477,8 +480,8 @@ int oasr_b200_flash_attn_tree(oasr_backend *be, const oasr_tensor *q, const oasr
     if (!(scale == scale)) return fail_op(be, op, "scale must be a number");
     st = seqs_check(be, op, page_table, n_past, n_nodes, S, N, &sq);
     if (st) return st;
-    if (tree && (tree->type != OASR_TYPE_I32 || tree->ne[0] != (N + 31) / 32 || tree->ne[1] != N || tree->ne[2] != S ||
-                 tree->ne[3] != 1 || (tree->nb[0] != 4 && tree->ne[0] > 1) || tree->nb[1] % 4 || tree->nb[2] % 4))
+    if (tree && (tree->type != OASR_TYPE_I32 || !aligned4(tree) || tree->ne[0] != (N + 31) / 32 || tree->ne[1] != N ||
+                 tree->ne[2] != S || tree->ne[3] != 1 || (tree->nb[0] != 4 && tree->ne[0] > 1) || tree->nb[1] % 4 || tree->nb[2] % 4))
         return fail_op(be, op, "tree must be I32 [ceil(n / 32), n, n_seq]");
     if (tree && N > TREE_MAX_NODES) return fail_op(be, op, "a tree has at most 1024 nodes");
     if (N == 0 || S == 0) return OASR_STATUS_SUCCESS;
@@ -520,7 +523,8 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
     if (!is_vec_i32(n_accept, S) || !is_vec_i32(next_token, S) || !is_vec_i32(n_past_out, S))
         return fail_op(be, op, "n_accept, next_token and n_past_out must be I32 [n_seq]");
     // every CTA of a sequence walks its tree, while the first of them writes the results
-    const oasr_tensor *outs[] = {path, n_accept, next_token, n_past_out}, *ins[] = {tokens, parents, target, n_past, page_table, n_nodes};
+    const oasr_tensor *outs[] = {path, n_accept, next_token, n_past_out};
+    const oasr_tensor *ins[] = {tokens, parents, target, n_past, page_table, n_nodes};
     if (S > 1 && llabs(path->nb[1] / 4) < N) return fail_op(be, op, "path's rows must not overlap");
     for (int i = 0; i < 4; ++i) {
         for (const oasr_tensor *t : ins)
@@ -556,8 +560,8 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
     KvPages p;
     st = pages_check(be, op, k_pages, v_pages, n_layers, &p);
     if (st) return st;
-    if (!pairs || pairs->type != OASR_TYPE_I32 || pairs->ne[0] != 2 || pairs->ne[2] != 1 || pairs->ne[3] != 1 ||
-        pairs->nb[0] != 4 || pairs->nb[1] % 4)
+    if (!pairs || pairs->type != OASR_TYPE_I32 || !aligned4(pairs) || pairs->ne[0] != 2 || pairs->ne[2] != 1 ||
+        pairs->ne[3] != 1 || pairs->nb[0] != 4 || pairs->nb[1] % 4)
         return fail_op(be, op, "pairs must be I32 [2, n]");
     if (pairs->ne[1] == 0) return OASR_STATUS_SUCCESS;
     if (!pairs->data) return fail_op(be, op, "null argument");

@@ -236,3 +236,37 @@ def test_calls_of_too_many_steps_are_refused(be):  # noqa: F811
     for N, H, MP in ((1 << 24, 128, 1), (1 << 24, 1, 1 << 18), (1 << 17, 1, 1 << 22)):
         with pytest.raises(ob.backend.UnsupportedInputs, match="too many"):
             be.flash_attn_tree(row.expand(1, H, N, 64), k, v, table[:, :MP], past, None, None, 0.1, row.expand(1, N, H, 64))
+
+
+def test_addresses_that_are_not_aligned_are_refused(be):  # noqa: F811
+    """descriptors whose 4-byte values lie two bytes off (a tensor of torch cannot); nothing is launched"""
+    import torch
+
+    import openasr_b200 as ob
+
+    def off(t):
+        d = ob.describe(t)
+        d.data += 2
+        return d
+
+    a = commit_args()
+    S, N, H, D = 3, 5, 4, 64
+    f32 = dict(device="cuda")
+    x, q = torch.zeros(S, N, H + 4, D, **f32), torch.zeros(S, N, H, D, **f32)
+    gain, tree = torch.ones(D, **f32), torch.zeros(S, N, 1, dtype=torch.int32, device="cuda")
+    pairs = torch.full((2, 2), -1, dtype=torch.int32, device="cuda")
+    norm = dict(x=x, wq=gain, wk=gain, eps=1e-6, rope=None, pos=a["tokens"], table=a["table"], past=a["n_past"], nodes=a["n_nodes"],
+                q=q, k=a["k"], v=a["v"])
+    attn = dict(q=q.permute(0, 2, 1, 3), k=a["k"], v=a["v"], table=a["table"], past=a["n_past"], nodes=a["n_nodes"], tree=tree,
+                scale=0.1, out=q.clone())
+    for call, args, names in ((be.tree_commit, a, ("tokens", "parents", "target", "n_nodes", "n_past", "table", "path", "n_accept",
+                                                   "next", "past_out")),
+                              (be.qk_norm_rope, norm, ("wq", "wk", "pos", "table", "past", "nodes")),
+                              (be.flash_attn_tree, attn, ("table", "past", "nodes", "tree"))):
+        call(*args.values())
+        for name in names:
+            with pytest.raises(ob.backend.UnsupportedInputs):
+                call(*{**args, name: off(args[name])}.values())
+    with pytest.raises(ob.backend.UnsupportedInputs):
+        be.kv_pages_copy(a["k"], a["v"], 1, off(pairs))
+    be.synchronize()
