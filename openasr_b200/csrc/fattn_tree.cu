@@ -556,7 +556,9 @@ int tree_prepare(oasr_backend *be, TreeAttn &a, const KvPages &p, const KvSeqs &
     a.page = FastDiv(p.page);
     const int64_t tiles = ((int64_t)s.N * a.group.d + R - 1) / R;
     const int64_t items = tiles * a.HKV * a.S, most = items * (((int64_t)s.MP * p.page + TREE_BKV - 1) / TREE_BKV);
-    if (most + items * tree_segment(R) > INT32_MAX / 2 || (int64_t)s.N * a.group.d > INT32_MAX / 2 || (int64_t)a.S * s.N * a.H > INT32_MAX)
+    // (rows are counted in steps of the grid's warps, which must not pass 31 bits either)
+    if (most + items * tree_segment(R) > INT32_MAX / 2 || (int64_t)s.N * a.group.d > INT32_MAX / 2 ||
+        (int64_t)a.S * s.N * a.H > INT32_MAX - 65536)
         return oasr_internal_fail(be, OASR_STATUS_FAILED, "flash_attn_tree: too many rows and positions");
     out->grid = (int)std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)be->sm_count * ctas_per_sm));
     const size_t part = (size_t)R * (a.D + 2) * 4;

@@ -233,9 +233,10 @@ def test_calls_of_too_many_steps_are_refused(be):  # noqa: F811
     past = torch.zeros(1, dtype=torch.int32, device="cuda")
     row = torch.zeros(1, 1, 1, 64, device="cuda")
     table = torch.zeros(1, 1 << 22, dtype=torch.int32, device="cuda")
-    for N, H, MP in ((1 << 24, 128, 1), (1 << 24, 1, 1 << 18), (1 << 17, 1, 1 << 22)):
+    for S, N, H, MP in ((1, 1 << 24, 128, 1), (1, 1 << 24, 1, 1 << 18), (1, 1 << 17, 1, 1 << 22), (128, (1 << 24) - 1, 1, 1)):
         with pytest.raises(ob.backend.UnsupportedInputs, match="too many"):
-            be.flash_attn_tree(row.expand(1, H, N, 64), k, v, table[:, :MP], past, None, None, 0.1, row.expand(1, N, H, 64))
+            be.flash_attn_tree(row.expand(S, H, N, 64), k, v, table[:, :MP].expand(S, MP), past.repeat(S), None, None, 0.1,
+                               row.expand(S, N, H, 64))
 
 
 def test_addresses_that_are_not_aligned_are_refused(be):  # noqa: F811
