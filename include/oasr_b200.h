@@ -77,6 +77,7 @@ enum oasr_op {
     OASR_OP_FLASH_ATTN_TREE = 6, /* src0 = q, src1 = k_pages */
     OASR_OP_TREE_COMMIT = 7,     /* src0 = tokens, src1 = k_pages */
     OASR_OP_KV_PAGES_COPY = 8,   /* src0 = k_pages */
+    OASR_OP_TREE_SAMPLE = 9,     /* src0 = logits */
 };
 
 /* GGML_BACKEND_GRAPH_CANCEL_* mechanisms and observation granularities -- ffi.rs:118-124 */
@@ -336,6 +337,32 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
                           const oasr_tensor *target, const oasr_tensor *n_nodes, const oasr_tensor *n_past,
                           const oasr_tensor *page_table, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
                           oasr_tensor *path, oasr_tensor *n_accept, oasr_tensor *next_token, oasr_tensor *n_past_out);
+/* The token after each node, drawn from the model's probabilities instead of its first maximum
+ * (oasr_b200_argmax_first): a target for oasr_b200_tree_commit, or, with one node per sequence
+ * and without a draft, a step of sampling.  logits F32 [n_vocab, n, n_seq], rows contiguous.
+ * temperature F32 [n_seq] (NULL: 1): p(x) = exp((l(x) - max) / T) / Z over the finite logits; a
+ * sequence at 0 takes the first maximum, as argmax_first does.  uniforms F32 [2, n, n_seq], each
+ * in [0, 1).  target I32 [n, n_seq] gets the smallest x whose running sum of p passes
+ * uniforms[1] of the node; logprob F32 [n, n_seq] (NULL: none) the natural logarithm of that
+ * token's p (0 at temperature 0).  Padding nodes (n_nodes, NULL: none) get -1 and 0, and so does
+ * a row without a finite logit.
+ * draft_probs F32 [n_vocab, n, n_seq], given with tokens and parents I32 [n, n_seq] (all NULL
+ * without a draft; n <= 1024 with one): row c holds the probabilities, not negative and finite,
+ * that the children of node c were drawn from, one after the other and each on its own.  They
+ * are then accepted by rejection: with r = p, child j in ascending order becomes the target
+ * if uniforms[0] of j times draft_probs[tokens[j]] is less than r(tokens[j]); otherwise r becomes
+ * max(r - draft_probs, 0) over its sum (p, if that sum is 0).  When all children are rejected the
+ * target is drawn from r as from p above, and is none of their tokens.  So the tokens that
+ * tree_commit then accepts are distributed as if each had been sampled from the model alone.
+ * (A draft without probabilities needs none of this: a child is accepted if it is the token
+ * drawn.)  Sums are of 64 bits.  What cannot be drawn from -- a temperature or a uniform number
+ * out of range, a child's token outside the vocabulary -- makes oasr_b200_synchronize return
+ * OASR_STATUS_EXECUTION_FAILED, and the node's outputs are undefined.  target and logprob may not
+ * overlap an input or one another. */
+int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits, const oasr_tensor *temperature,
+                          const oasr_tensor *uniforms, const oasr_tensor *tokens, const oasr_tensor *parents,
+                          const oasr_tensor *draft_probs, const oasr_tensor *n_nodes, oasr_tensor *target,
+                          oasr_tensor *logprob);
 /* Copy pages in each of the n_layers layers, K and V: pairs I32 [2, n] = (source,
  * destination) page.  Destinations are distinct and no source is a destination; a pair
  * with a negative page is left out. */

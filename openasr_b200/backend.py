@@ -24,6 +24,7 @@ F32, F16, Q4_0, Q8_0, Q4_K, I32, I64 = 0, 1, 2, 8, 12, 26, 27
 PREC_DEFAULT, PREC_F32 = 0, 10
 OP_MUL_MAT, OP_FLASH_ATTN_EXT, OP_SET_ROWS, OP_ARGMAX_FIRST = 1, 2, 3, 4
 OP_QK_NORM_ROPE, OP_FLASH_ATTN_TREE, OP_TREE_COMMIT, OP_KV_PAGES_COPY = 5, 6, 7, 8
+OP_TREE_SAMPLE = 9
 
 STATUS_ALLOC_FAILED, STATUS_FAILED, STATUS_SUCCESS = -2, -1, 0
 STATUS_ABORTED, STATUS_EXECUTION_FAILED, STATUS_DEVICE_LOST, STATUS_BACKEND_POISONED = 1, 2, 3, 4
@@ -289,6 +290,7 @@ SIGNATURES = {
     "oasr_b200_flash_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _P, _F, _P], ctypes.c_int),
     "oasr_b200_tree_commit": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_kv_pages_copy": ([_P, _P, _P, _I32, _P], ctypes.c_int),
+    "oasr_b200_tree_sample": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_tree_mask": ([_P, _I32, _P], ctypes.c_int),
     "oasr_b200_kv_pool_create": ([_I32, _I32, _I32, _I32, ctypes.POINTER(_P)], ctypes.c_int),
     "oasr_b200_kv_pool_free": ([_P], ctypes.c_int),
@@ -467,7 +469,7 @@ def _ops():
             _OPS = _CtypesOps()
         else:
             _torch_ops.bind(_unsupported, *(ctypes.cast(getattr(lib(), "oasr_b200_" + f), ctypes.c_void_p).value for f in (
-                "qk_norm_rope", "flash_attn_tree", "tree_commit", "kv_pages_copy")))
+                "qk_norm_rope", "flash_attn_tree", "tree_commit", "kv_pages_copy", "tree_sample")))
             _OPS = _torch_ops
     return _OPS
 
@@ -726,6 +728,15 @@ class Backend:
         self._check((_OPS or _ops()).tree_commit((self.handle.value or 0, self.ordinal), tokens, parents, target, n_nodes,
                                                  n_past, page_table, k_pages, v_pages, n_layers, path, n_accept, next_token,
                                                  n_past_out))
+
+    def tree_sample(self, logits, temperature, uniforms, tokens, parents, draft_probs, n_nodes, target, logprob=None) -> None:
+        """The token after each node, drawn from softmax(logits f32 [S, n, V] / temperature f32 [S]) with
+        uniforms f32 [S, n, 2] -> target i32 [S, n] (for tree_commit) and its logprob f32 [S, n] or
+        None.  tokens / parents i32 [S, n] with draft_probs f32 [S, n, V]: children drawn from the
+        draft's probabilities are accepted by rejection first; all three None without (see the C
+        header).  temperature and n_nodes may be None."""
+        self._check((_OPS or _ops()).tree_sample((self.handle.value or 0, self.ordinal), logits, temperature, uniforms, tokens,
+                                                 parents, draft_probs, n_nodes, target, logprob))
 
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""

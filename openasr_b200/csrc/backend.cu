@@ -567,6 +567,7 @@ int oasr_b200_supports_op(oasr_backend *be, int32_t op, const oasr_tensor *src0,
     case OASR_OP_SET_ROWS:
         return src0->type == OASR_TYPE_F16 || src0->type == OASR_TYPE_F32;
     case OASR_OP_ARGMAX_FIRST:
+    case OASR_OP_TREE_SAMPLE:
         return src0->type == OASR_TYPE_F32;
     case OASR_OP_QK_NORM_ROPE:
     case OASR_OP_FLASH_ATTN_TREE:

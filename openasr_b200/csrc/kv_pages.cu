@@ -10,23 +10,12 @@
 
 #include <algorithm>
 
+#include "op_checks.cuh"
 #include "pages.cuh"
 
 using namespace oasr;
 
 namespace oasr {
-
-// 4-byte values that are read and written as such
-static bool aligned4(const oasr_tensor *t) { return ((uintptr_t)t->data & 3) == 0; }
-
-static bool is_vec_i32(const oasr_tensor *t, int64_t n) {
-    return t && t->type == OASR_TYPE_I32 && t->data && aligned4(t) && t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 &&
-           t->ne[3] == 1 && (t->nb[0] == 4 || n <= 1);
-}
-
-static int fail_op(oasr_backend *be, const char *op, const char *what) {
-    return oasr_internal_fail(be, OASR_STATUS_FAILED, std::string(op) + ": " + what);
-}
 
 int pages_check(oasr_backend *be, const char *op, const oasr_tensor *k, const oasr_tensor *v, int layers, KvPages *out) {
     if (!k || !v) return fail_op(be, op, "null argument");
@@ -348,41 +337,6 @@ __global__ void __launch_bounds__(256) kv_pages_copy_kernel(const int *pairs, in
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (e0 + 256 * u < total) *reinterpret_cast<uint4 *>(layer + dst * nb3 + off[u]) = r[u];
-}
-
-int launched(oasr_backend *be, cudaError_t e, const char *what) {
-    if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, what, __LINE__);
-    return oasr_internal_launch_check(be, what);
-}
-
-bool rows16(const oasr_tensor *t) {
-    return ((uintptr_t)t->data & 15) == 0 && t->nb[1] % 16 == 0 && t->nb[2] % 16 == 0 && t->nb[3] % 16 == 0;
-}
-
-// I32 [N, S] with contiguous rows
-bool is_rows_i32(const oasr_tensor *t, int64_t N, int64_t S) {
-    return t && t->type == OASR_TYPE_I32 && t->data && aligned4(t) && t->ne[0] == N && t->ne[1] == S && t->ne[2] == 1 &&
-           t->ne[3] == 1 && (t->nb[0] == 4 || N <= 1) && t->nb[1] % 4 == 0;
-}
-
-// Rows of I32 on the device: `n` rows of `width` values, `ld` values apart.
-struct IntRows {
-    const int *at;
-    int64_t n, width, ld;
-};
-IntRows int_rows(const oasr_tensor *t) { return {(const int *)t->data, t->ne[1], t->ne[0], t->ne[1] > 1 ? t->nb[1] / 4 : 0}; }
-
-// Whether the two have a value in common (rows side by side in one buffer have none).
-bool share_values(const IntRows &a, const IntRows &b) {
-    auto row = [](const IntRows &r, int64_t i) { return r.at + (r.ld < 0 ? r.n - 1 - i : i) * r.ld; };  // ascending
-    if (row(a, a.n - 1) + a.width <= row(b, 0) || row(b, b.n - 1) + b.width <= row(a, 0)) return false;
-    for (int64_t i = 0, j = 0; i < a.n && j < b.n;) {
-        const int *x = row(a, i), *y = row(b, j);
-        if (x + a.width <= y) ++i;
-        else if (y + b.width <= x) ++j;
-        else return true;
-    }
-    return false;
 }
 
 }  // namespace

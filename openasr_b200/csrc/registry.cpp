@@ -72,6 +72,7 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_synth_normal),
     OASR_ENTRY(oasr_b200_tree_commit),
     OASR_ENTRY(oasr_b200_tree_mask),
+    OASR_ENTRY(oasr_b200_tree_sample),
     OASR_ENTRY(oasr_b200_weight_download),
     OASR_ENTRY(oasr_b200_weight_free),
     OASR_ENTRY(oasr_b200_weight_info),

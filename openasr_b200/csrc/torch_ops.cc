@@ -17,6 +17,7 @@ decltype(&oasr_b200_qk_norm_rope) s_qk_norm_rope;
 decltype(&oasr_b200_flash_attn_tree) s_flash_attn_tree;
 decltype(&oasr_b200_tree_commit) s_tree_commit;
 decltype(&oasr_b200_kv_pages_copy) s_kv_pages_copy;
+decltype(&oasr_b200_tree_sample) s_tree_sample;
 
 // The descriptor of a torch tensor (ne = reversed sizes, nb = reversed byte strides), of a ready
 // one (any object whose buffer is an oasr_tensor), or nothing for None.
@@ -181,11 +182,22 @@ PyObject *kv_pages_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return status([&] { return s_kv_pages_copy(at.be, x[0].p, x[1].p, layers, y[0].p); });
 }
 
-// bind(unsupported, addresses of the four C functions in the order below)
+PyObject *tree_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Arg x[9];
+    if (!count(n, 10)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at)) return nullptr;
+    return status([&] {
+        return s_tree_sample(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, x[8].p);
+    });
+}
+
+// bind(unsupported, addresses of the C functions in the order below)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    if (!count(n, 5)) return nullptr;
-    void *f[4];
-    for (int i = 0; i < 4; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
+    constexpr int N = 5;
+    if (!count(n, 1 + N)) return nullptr;
+    void *f[N];
+    for (int i = 0; i < N; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(a[0]);
     Py_XSETREF(s_unsupported, a[0]);
@@ -193,11 +205,13 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     s_flash_attn_tree = reinterpret_cast<decltype(s_flash_attn_tree)>(f[1]);
     s_tree_commit = reinterpret_cast<decltype(s_tree_commit)>(f[2]);
     s_kv_pages_copy = reinterpret_cast<decltype(s_kv_pages_copy)>(f[3]);
+    s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
     Py_RETURN_NONE;
 }
 
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(bind), FAST(qk_norm_rope), FAST(flash_attn_tree), FAST(tree_commit), FAST(kv_pages_copy),
+                         FAST(tree_sample),
                          {nullptr, nullptr, 0, nullptr}};
 #undef FAST
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
