@@ -78,6 +78,8 @@ enum oasr_op {
     OASR_OP_TREE_COMMIT = 7,     /* src0 = tokens, src1 = k_pages */
     OASR_OP_KV_PAGES_COPY = 8,   /* src0 = k_pages */
     OASR_OP_TREE_SAMPLE = 9,     /* src0 = logits */
+    OASR_OP_ATTN_WEIGHTS = 10,   /* src0 = q, src1 = k_pages */
+    OASR_OP_KV_EVICT = 11,       /* src0 = weights, src1 = k_pages */
 };
 
 /* GGML_BACKEND_GRAPH_CANCEL_* mechanisms and observation granularities -- ffi.rs:118-124 */
@@ -368,6 +370,36 @@ int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits, const oas
  * with a negative page is left out. */
 int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
                             const oasr_tensor *pairs);
+/* A bounded cache: how much attention each cached position gets, and eviction by it.  weights F32
+ * [page, H_kv, n_pages] lies beside the pages (rows contiguous, other strides free): entry (j, h,
+ * page id) belongs to that page's row of K/V head h.
+ *
+ * oasr_b200_attn_weights: q F32 or F16 [D, n, H, n_seq] as in oasr_b200_flash_attn_tree, the nodes
+ * being a chain (node i sees the positions up to n_past + i).  To a position's entry it adds the
+ * softmax weights that the position gets from all live nodes and all query heads of its K/V head,
+ * after the old value was multiplied by decay; with decay 0, and for the positions from n_past on,
+ * which are new, the old value is not read.  Entries of positions past the last node stay as they are.
+ * One call per layer and step, with the queries and the lengths of that layer's flash_attn_tree; or
+ * one after the prompt with its last rows and decay 0, which scores all of it.  A row with something
+ * that is not finite (a query, a K row that it sees) makes the entries of what it sees NaN; a position
+ * whose score is -inf gets nothing.
+ *
+ * oasr_b200_kv_evict: of each sequence with more than n_keep I32 [n_seq] of its n_past positions, every
+ * K/V head of every layer keeps the first n_sink, the last n_recent and, of those between, the ones
+ * with the greatest weights (of equal ones the first; NaN after all others) to n_keep in all.  Their K
+ * and V rows and weights move to positions 0, 1, ... in their order; n_past_out I32 [n_seq] is n_keep
+ * for those sequences and n_past for the others, which stay as they are.  What pages hold from n_keep
+ * on stays as it was; oasr_b200_kv_pool_truncate gives those pages back.  Keys keep the rotation of the
+ * positions that they had: later nodes pass pos to oasr_b200_qk_norm_rope, counting on from there.
+ * weights has the pages of all layers along ne[2], as k_pages along ne[3].  n_keep of a longer sequence
+ * must be n_sink + n_recent or more (checked on the device like the lengths).  n_past_out may not overlap
+ * an input. */
+int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages,
+                           const oasr_tensor *page_table, const oasr_tensor *n_past, const oasr_tensor *n_nodes,
+                           float scale, float decay, oasr_tensor *weights);
+int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const oasr_tensor *page_table, const oasr_tensor *n_past,
+                       const oasr_tensor *n_keep, int32_t n_sink, int32_t n_recent, oasr_tensor *k_pages,
+                       oasr_tensor *v_pages, int32_t n_layers, oasr_tensor *n_past_out);
 /* Which sequence holds which pages (host only, one thread at a time; needs no device).
  * Sequences share pages by reference: a fork copies nothing until one of the two writes.
  * open / fork return the new sequence's number (0 .. max_seqs - 1), OASR_STATUS_ALLOC_FAILED

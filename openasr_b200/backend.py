@@ -24,7 +24,7 @@ F32, F16, Q4_0, Q8_0, Q4_K, I32, I64 = 0, 1, 2, 8, 12, 26, 27
 PREC_DEFAULT, PREC_F32 = 0, 10
 OP_MUL_MAT, OP_FLASH_ATTN_EXT, OP_SET_ROWS, OP_ARGMAX_FIRST = 1, 2, 3, 4
 OP_QK_NORM_ROPE, OP_FLASH_ATTN_TREE, OP_TREE_COMMIT, OP_KV_PAGES_COPY = 5, 6, 7, 8
-OP_TREE_SAMPLE = 9
+OP_TREE_SAMPLE, OP_ATTN_WEIGHTS, OP_KV_EVICT = 9, 10, 11
 
 STATUS_ALLOC_FAILED, STATUS_FAILED, STATUS_SUCCESS = -2, -1, 0
 STATUS_ABORTED, STATUS_EXECUTION_FAILED, STATUS_DEVICE_LOST, STATUS_BACKEND_POISONED = 1, 2, 3, 4
@@ -290,6 +290,8 @@ SIGNATURES = {
     "oasr_b200_flash_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _P, _F, _P], ctypes.c_int),
     "oasr_b200_tree_commit": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_kv_pages_copy": ([_P, _P, _P, _I32, _P], ctypes.c_int),
+    "oasr_b200_attn_weights": ([_P, _P, _P, _P, _P, _P, _F, _F, _P], ctypes.c_int),
+    "oasr_b200_kv_evict": ([_P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _P], ctypes.c_int),
     "oasr_b200_tree_sample": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P], ctypes.c_int),
     "oasr_b200_tree_mask": ([_P, _I32, _P], ctypes.c_int),
     "oasr_b200_kv_pool_create": ([_I32, _I32, _I32, _I32, ctypes.POINTER(_P)], ctypes.c_int),
@@ -469,7 +471,8 @@ def _ops():
             _OPS = _CtypesOps()
         else:
             _torch_ops.bind(_unsupported, *(ctypes.cast(getattr(lib(), "oasr_b200_" + f), ctypes.c_void_p).value for f in (
-                "qk_norm_rope", "flash_attn_tree", "tree_commit", "kv_pages_copy", "tree_sample")))
+                "qk_norm_rope", "flash_attn_tree", "tree_commit", "kv_pages_copy", "tree_sample",
+                "attn_weights", "kv_evict")))
             _OPS = _torch_ops
     return _OPS
 
@@ -741,6 +744,20 @@ class Backend:
     def kv_pages_copy(self, k_pages, v_pages, n_layers: int, pairs) -> None:
         """Copy page pairs[i, 0] to pairs[i, 1] (i32 [n, 2]) in every layer, K and V."""
         self._check((_OPS or _ops()).kv_pages_copy((self.handle.value or 0, self.ordinal), k_pages, v_pages, n_layers, pairs))
+
+    def attn_weights(self, q, k_pages, page_table, n_past, n_nodes, scale: float, decay: float, weights) -> None:
+        """Add the attention that each position gets from the nodes q f32|f16 [S, H, n, D] (a chain) to its
+        entry of weights f32 [P, H_kv, page], old entries times decay (0: not read)."""
+        self._check((_OPS or _ops()).attn_weights((self.handle.value or 0, self.ordinal), q, k_pages, page_table, n_past,
+                                                  n_nodes, scale, decay, weights))
+
+    def kv_evict(self, weights, page_table, n_past, n_keep, n_sink: int, n_recent: int, k_pages, v_pages, n_layers: int,
+                 n_past_out) -> None:
+        """Keep n_keep i32 [S] positions of each longer sequence -- the first n_sink, the last n_recent and
+        the greatest weights f32 [n_layers * P, H_kv, page] between -- and move their rows to the front of
+        pages f16 [n_layers * P, H_kv, page, D], every layer and head for itself; n_past_out i32 [S]."""
+        self._check((_OPS or _ops()).kv_evict((self.handle.value or 0, self.ordinal), weights, page_table, n_past, n_keep, n_sink,
+                                              n_recent, k_pages, v_pages, n_layers, n_past_out))
 
 
 class KvPool:

@@ -572,6 +572,8 @@ int oasr_b200_supports_op(oasr_backend *be, int32_t op, const oasr_tensor *src0,
     case OASR_OP_QK_NORM_ROPE:
     case OASR_OP_FLASH_ATTN_TREE:
     case OASR_OP_TREE_COMMIT:
+    case OASR_OP_ATTN_WEIGHTS:
+    case OASR_OP_KV_EVICT:
     case OASR_OP_KV_PAGES_COPY: {
         // F16 pages [D, page, H_kv, n_pages] in src1 (the page copy has them in src0)
         const oasr_tensor *k = op == OASR_OP_KV_PAGES_COPY ? src0 : src1;
@@ -579,10 +581,11 @@ int oasr_b200_supports_op(oasr_backend *be, int32_t op, const oasr_tensor *src0,
             k->ne[2] < 1)
             return 0;
         if (op == OASR_OP_TREE_COMMIT) return src0->type == OASR_TYPE_I32;
+        if (op == OASR_OP_KV_EVICT) return src0->type == OASR_TYPE_F32 && src0->ne[0] == k->ne[1] && src0->ne[1] == k->ne[2];
         if (op == OASR_OP_QK_NORM_ROPE)
             return src0->type == OASR_TYPE_F32 && src0->ne[0] == k->ne[0] && src0->ne[1] > 2 * k->ne[2] &&
                    src0->ne[1] % k->ne[2] == 0;
-        if (op == OASR_OP_FLASH_ATTN_TREE)
+        if (op == OASR_OP_FLASH_ATTN_TREE || op == OASR_OP_ATTN_WEIGHTS)
             return (src0->type == OASR_TYPE_F32 || src0->type == OASR_TYPE_F16) && src0->ne[0] == k->ne[0] &&
                    src0->ne[2] >= 1 && src0->ne[2] % k->ne[2] == 0;
         return 1;

@@ -23,6 +23,7 @@ const Entry kEntries[] = {
     {"ggml_backend_memory_get_api_v1", reinterpret_cast<void *>(&oasr_b200_memory_get_api_v1)},
     OASR_ENTRY(oasr_b200_act_bytes),
     OASR_ENTRY(oasr_b200_argmax_first),
+    OASR_ENTRY(oasr_b200_attn_weights),
     OASR_ENTRY(oasr_b200_device_count),
     OASR_ENTRY(oasr_b200_flash_attn_causal),
     OASR_ENTRY(oasr_b200_flash_attn_ext),
@@ -32,6 +33,7 @@ const Entry kEntries[] = {
     OASR_ENTRY(oasr_b200_get_proc_address),
     OASR_ENTRY(oasr_b200_get_stream),
     OASR_ENTRY(oasr_b200_init),
+    OASR_ENTRY(oasr_b200_kv_evict),
     OASR_ENTRY(oasr_b200_kv_pages_copy),
     OASR_ENTRY(oasr_b200_kv_pool_close),
     OASR_ENTRY(oasr_b200_kv_pool_create),

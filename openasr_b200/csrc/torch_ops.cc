@@ -18,6 +18,8 @@ decltype(&oasr_b200_flash_attn_tree) s_flash_attn_tree;
 decltype(&oasr_b200_tree_commit) s_tree_commit;
 decltype(&oasr_b200_kv_pages_copy) s_kv_pages_copy;
 decltype(&oasr_b200_tree_sample) s_tree_sample;
+decltype(&oasr_b200_attn_weights) s_attn_weights;
+decltype(&oasr_b200_kv_evict) s_kv_evict;
 
 // The descriptor of a torch tensor (ne = reversed sizes, nb = reversed byte strides), of a ready
 // one (any object whose buffer is an oasr_tensor), or nothing for None.
@@ -192,9 +194,30 @@ PyObject *tree_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+PyObject *attn_weights(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Arg x[5], y[1];
+    if (!count(n, 9)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !take(y, a + 8, at)) return nullptr;
+    const float scale = (float)PyFloat_AsDouble(a[6]), decay = (float)PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    return status([&] { return s_attn_weights(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, scale, decay, y[0].p); });
+}
+
+PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Arg x[4], y[2], z[1];
+    int32_t sink, recent, layers;
+    if (!count(n, 11)) return nullptr;
+    const Where at(a[0]);
+    if (!take(x, a + 1, at) || !int32(a[5], &sink) || !int32(a[6], &recent) || !take(y, a + 7, at) || !int32(a[9], &layers) ||
+        !take(z, a + 10, at))
+        return nullptr;
+    return status([&] { return s_kv_evict(at.be, x[0].p, x[1].p, x[2].p, x[3].p, sink, recent, y[0].p, y[1].p, layers, z[0].p); });
+}
+
 // bind(unsupported, addresses of the C functions in the order below)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    constexpr int N = 5;
+    constexpr int N = 7;
     if (!count(n, 1 + N)) return nullptr;
     void *f[N];
     for (int i = 0; i < N; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
@@ -206,12 +229,14 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     s_tree_commit = reinterpret_cast<decltype(s_tree_commit)>(f[2]);
     s_kv_pages_copy = reinterpret_cast<decltype(s_kv_pages_copy)>(f[3]);
     s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
+    s_attn_weights = reinterpret_cast<decltype(s_attn_weights)>(f[5]);
+    s_kv_evict = reinterpret_cast<decltype(s_kv_evict)>(f[6]);
     Py_RETURN_NONE;
 }
 
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(bind), FAST(qk_norm_rope), FAST(flash_attn_tree), FAST(tree_commit), FAST(kv_pages_copy),
-                         FAST(tree_sample),
+                         FAST(tree_sample), FAST(attn_weights), FAST(kv_evict),
                          {nullptr, nullptr, 0, nullptr}};
 #undef FAST
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
