@@ -9,7 +9,7 @@
 //
 // The borders of that running sum are V numbers in [0, 1): an error e of it gives another token once in
 // 1 / (V e) draws, so that with V = 152k sums in 32 bits (e = 1e-7 to 1e-6) would miss in some percent of
-// the draws.  Weights and sums are therefore 64-bit, from an exponential made for it (exp16).
+// the draws.  Weights and sums are therefore 64-bit, from an exponential made for it (exp_of).
 #include <cooperative_groups.h>
 
 #include "once_per_device.h"
@@ -19,6 +19,7 @@
 using namespace oasr;
 
 namespace {
+
 
 constexpr int NT = 256, NW = NT / 32;
 
@@ -41,44 +42,72 @@ struct Sample {
 };
 
 // ---- the exponential --------------------------------------------------------------------------
-// 2^(t / 16) = 2^e 2^(j / 16) 2^(r / 16), k = 16 e + j the integer nearest to t, |r| <= 1/2: the Taylor
-// polynomial of degree 5 of 2^(r / 16) (remainder (ln 2 / 32)^6 / 720 = 1.4e-13), 2^(j / 16) from a table
-// of 16 (one 8-byte value per pair of banks: no conflicts), 2^e added to its exponent field.  Adding
-// 1.5 * 2^52 leaves k in the low word.
+// With t = (l - ref) 256 log2(e) / T, exp((l - ref) / T) = 2^(t / 256) = 2^e 2^(j / 256) 2^(r / 256), k = 256 e + j
+// the integer nearest to t and |r| <= 1/2: the Taylor polynomial of degree 3 of 2^(r / 256) (remainder
+// (ln 2 / 512)^4 / 24 = 1.4e-13), 2^(j / 256) from a table in shared memory, 2^e added to its exponent field.
+// Adding 1.5 * 2^52 to t in one multiply-add rounds it and leaves k in the low word, another one gives r.  That
+// is seven operations of 64 bits per value; a table of 16 takes two more terms (in a
+// loop of nothing else 3.6 values per clock and SM instead of 4.4).
+// The table has a copy for each pair of banks, so that the 16 lanes of an access never meet (32 KB).
 constexpr double MAGIC = 6755399441055744.0;
-constexpr double LN2_16 = 0.69314718055994530942 / 16, LOG2E_16 = 16 / 0.69314718055994530942;
-constexpr double T_LOW = -16000.0;   // below: a weight under 2^-1000 of the reference's
-constexpr double T_HIGH = 13000.0;   // above: a new reference is taken
-constexpr double B_MOST = 131072.0;  // most |reference / T| (in 1/16 octaves) for l / T in one multiply-add
+constexpr int STEPS = 256, COPIES = 16;
+constexpr double LN2 = 0.69314718055994530942;
+constexpr double LOW = 1000 * STEPS;   // steps below the reference: a weight under 2^-1000, left out
+constexpr double HIGH = 800 * STEPS;   // steps above it: a new reference is taken
+constexpr double ROOM = 300 * STEPS;
+constexpr double MOST = 1e6 * STEPS;   // reference / T in steps up to which numbers of 32 bits are fine enough to hold the reference less 1000 T
 
-// 2^(j / 16) with j << 16 taken off its high word, so that adding k << 16 = (16 e + j) << 16 adds e alone
-__device__ __forceinline__ double table_entry(int j) {
-    const double v = exp2((double)j / 16.0);
-    return __hiloint2double(__double2hiint(v) - (j << 16), __double2loint(v));
+struct Table {
+    double v[STEPS][COPIES];
+    // 2^(j / 256) with j << 12 taken off its high word, so that adding k << 12 = (256 e + j) << 12 adds e alone
+    __device__ __forceinline__ void fill() {
+        for (int j = threadIdx.x; j < STEPS; j += blockDim.x) {
+            const double x = exp2((double)j / STEPS), y = __hiloint2double(__double2hiint(x) - (j << 12), __double2loint(x));
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c) v[j][(c + j) % COPIES] = y;
+        }
+    }
+};
+
+// acc[i] += 2^(d[i] C / 256), step by step for all N: each step waits for the one before
+template <int N>
+__device__ __forceinline__ void exp_add(const double (&d)[N], double C, uint32_t tab, double (&acc)[N]) {
+    constexpr double A1 = LN2 / STEPS, A2 = A1 * A1 / 2, A3 = A2 * A1 / 3;
+    double z[N], v[N], r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = fma(d[i], C, MAGIC);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        asm("ld.shared.f64 %0, [%1];" : "=d"(v[i]) : "r"((__double2loint(z[i]) & (STEPS - 1)) * (COPIES * 8) + tab));
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = MAGIC - z[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = fma(d[i], C, r[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __hiloint2double(__double2hiint(v[i]) + (__double2loint(z[i]) << 12), __double2loint(v[i]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = fma(A3, r[i], A2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = fma(z[i], r[i], A1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = fma(z[i], r[i], 1.0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fma(v[i], z[i], acc[i]);
 }
 
-__device__ __forceinline__ void exp16_parts(double t, const double *tab, double &scale, double &poly) {
-    const double z = t + MAGIC;
-    const int k = __double2loint(z);
-    const double r = t - (z - MAGIC);
-    constexpr double A1 = LN2_16, A2 = A1 * LN2_16 / 2, A3 = A2 * LN2_16 / 3, A4 = A3 * LN2_16 / 4, A5 = A4 * LN2_16 / 5;
-    poly = fma(fma(fma(fma(fma(A5, r, A4), r, A3), r, A2), r, A1), r, 1.0);
-    const double v = tab[k & 15];
-    scale = __hiloint2double(__double2hiint(v) + (k << 16), __double2loint(v));
-}
-
-// for T_LOW <= t <= 16000; 0 below
-__device__ __forceinline__ double exp16(double t, const double *tab) {
-    if (!(t >= T_LOW)) return 0.0;
-    double scale, poly;
-    exp16_parts(t, tab, scale, poly);
-    return scale * poly;
+// 2^(d C / 256), d C at most 1000 octaves; 0 from 1000 octaves under 1 on
+__device__ __forceinline__ double exp_of(double d, double C, uint32_t tab) {
+    if (!(d * C > -LOW)) return 0.0;
+    const double x[1] = {d};
+    double y[1] = {0.0};
+    exp_add(x, C, tab, y);
+    return y[0];
 }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-__device__ __forceinline__ double weight(float v, float ref, double C, const double *tab) {
-    return finite(v) ? exp16(((double)v - (double)ref) * C, tab) : 0.0;
+__device__ __forceinline__ double weight(float v, float ref, double C, uint32_t tab) {
+    return finite(v) ? exp_of((double)v - (double)ref, C, tab) : 0.0;
 }
 
 // ---- a warp's share of a row ------------------------------------------------------------------
@@ -92,11 +121,12 @@ struct Row {
         end = off + V;
     }
     __device__ __forceinline__ int vectors() const { return (end + 3) >> 2; }
-    __device__ __forceinline__ float4 load(int j) const {
-        if (4 * j >= off && 4 * j + 4 <= end) {
-            const int4 r = ldg_stream(base + 4 * (int64_t)j);
-            return make_float4(__int_as_float(r.x), __int_as_float(r.y), __int_as_float(r.z), __int_as_float(r.w));
-        }
+    __device__ __forceinline__ float4 whole(int j) const {
+        const int4 r = ldg_stream(base + 4 * (int64_t)j);
+        return make_float4(__int_as_float(r.x), __int_as_float(r.y), __int_as_float(r.z), __int_as_float(r.w));
+    }
+    __device__ __forceinline__ float4 load(int j) const {  // -inf where the row has no value
+        if (4 * j >= off && 4 * j + 4 <= end) return whole(j);
         float v[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = 4 * j + c >= off && 4 * j + c < end ? __ldg(base + 4 * (int64_t)j + c) : -INFINITY;
@@ -117,99 +147,165 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-constexpr int U = 4;  // vectors of a lane in flight
-
-__device__ __forceinline__ void load_tile(float4 (&b)[U], const Row &row, int j0, int j1, int lane) {
+// a warp's tile: U vectors per lane
+template <int U>
+__device__ __forceinline__ void load_tile(float4 (&b)[U], const Row &row, int j, int j1, int lane) {
+    if (4 * j >= row.off && j + 32 * U <= j1 && 4 * (j + 32 * U) <= row.end) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int j = j0 + 32 * u + lane;
-        b[u] = j < j1 ? row.load(j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int u = 0; u < U; ++u) b[u] = row.whole(j + 32 * u + lane);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            b[u] = j + 32 * u + lane < j1 ? row.load(j + 32 * u + lane) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
 }
 
-// any values: the maximum first, then the sum, values that are not finite left out
-__device__ __noinline__ Part range_sum_any(Row row, int j0, int j1, double C, const double *tab) {
+// A warp's run of vectors [j0, j1) in at most 32 stretches of `step` vectors (a multiple of 256: whole
+// pairs of tiles); lane i keeps the sum of stretch i, so that a drawn value is then looked for in one of
+// them alone.
+struct Run {
+    int j0, j1, step;
+    __device__ __forceinline__ int from(int i) const { return min(j0 + i * step, j1); }
+};
+
+__device__ __forceinline__ double scaled(double sum, float from, float to, double C, uint32_t tab) {
+    return from == to ? sum : from == -INFINITY ? 0.0 : sum * exp_of((double)from - (double)to, C, tab);
+}
+
+// any values: the maximum first, then the sums, values that are not finite left out
+__device__ __noinline__ Part run_sum_any(Row row, Run run, double C, uint32_t tab) {
     const int lane = threadIdx.x & 31;
     float m = -INFINITY;
-    for (int j = j0 + lane; j < j1; j += 32) {
+    for (int j = run.j0 + lane; j < run.j1; j += 32) {
         const float4 v = row.load(j);
         for (float f : {v.x, v.y, v.z, v.w})
             if (finite(f)) m = fmaxf(m, f);
     }
     m = warp_max(m);
-    double s = 0.0;
+    Part mine{0.0, m, 0};
     if (m > -INFINITY)
-        for (int j = j0 + lane; j < j1; j += 32) {
-            const float4 v = row.load(j);
-            for (float f : {v.x, v.y, v.z, v.w}) s += weight(f, m, C, tab);
+        for (int i = 0; run.from(i) < run.j1; ++i) {
+            double s = 0.0;
+            for (int j = run.from(i) + lane; j < run.from(i + 1); j += 32) {
+                const float4 v = row.load(j);
+                for (float f : {v.x, v.y, v.z, v.w}) s += weight(f, m, C, tab);
+            }
+            s = warp_sum(s);
+            if (lane == i) mine.sum = s;
         }
-    return Part{warp_sum(s), m, 0};
+    return mine;
 }
 
-// Vectors [j0, j1) by one warp in one pass.  The reference is the first tile's maximum; a value far above
-// it (T_HIGH) makes a new one, so that no maximum has to be known first.  l / T - ref / T is one
-// multiply-add of 64 bits.  -inf falls below T_LOW; +inf, NaN and a reference too large for that
-// multiply-add (a temperature of some 1e-4 and less) are left to range_sum_any.
-__device__ __forceinline__ Part range_sum(const Row &row, int j0, int j1, double C, const double *tab) {
+__device__ __forceinline__ float abs_max3(float a, float b, float c) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+    return m;
+}
+
+// The run in one pass, relative to exp(ref / T); ref is 0 as long as the row's values are of the common
+// size (ROOM), so that no maximum has to be known first, the runs' sums need no scaling to one another,
+// and the subtraction is left out.  A value far above it makes the tile's maximum the reference.  Values
+// 1000 octaves below it and -inf count as 2^-1000; +inf, NaN and a reference too large (a temperature of
+// some 1e-5 and less) are left to run_sum_any.  The next tile is on its way while one is summed.
+template <int U>
+__device__ __forceinline__ Part run_sum(const Row &row, const Run &run, float4 (&a)[U], float ref, double C, uint32_t tab) {
     const int lane = threadIdx.x & 31;
-    float ref = -INFINITY, high = -INFINITY;
-    double B = 0.0, acc[4] = {0.0, 0.0, 0.0, 0.0};
-    bool plain = true;
-    float4 next[U];
-    load_tile(next, row, j0, j1, lane);
-    for (int j = j0; j < j1; j += 32 * U) {
-        float4 cur[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) cur[u] = next[u];
-        if (j + 32 * U < j1) load_tile(next, row, j + 32 * U, j1, lane);
-        float m = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(fmaxf(cur[u].x, cur[u].y), fmaxf(cur[u].z, cur[u].w)));
-        if (__any_sync(0xffffffffu, m > high)) {
-            m = warp_max(m);
-            plain = finite(m) && fabs((double)m * C) <= B_MOST;
-            if (!plain) break;
-            const double f = exp16(((double)ref - (double)m) * C, tab);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] *= f;
-            ref = m;
-            B = -(double)m * C;
-            high = (float)((double)m + T_HIGH / C);
-        }
-        if (ref == -INFINITY) continue;  // nothing finite so far
+    constexpr int G = 4;    // values at a time
+    float low, high, calm;  // between -calm and calm lies nothing under low or over high
+    double acc[G] = {};
+    auto refer = [&](float m) {
+        ref = m;
+        low = (float)((double)m - LOW / C);
+        high = m == -INFINITY ? m : fminf((float)((double)m + HIGH / C), 3.402823466e38f);
+        calm = fminf(high, -low);
+    };
+    refer(ref);
+    bool plain = ref == -INFINITY || fabs((double)ref * C) <= MOST;
+    auto add = [&](float4 (&b)[U]) {
+        float m = 0.0f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float v[4] = {cur[u].x, cur[u].y, cur[u].z, cur[u].w};
+            m = abs_max3(m, b[u].x, b[u].y);
+            m = abs_max3(m, b[u].z, b[u].w);
+        }
+        if (__any_sync(0xffffffffu, m > calm)) {
+            m = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                double t = fma((double)v[c], C, B);
-                // not below T_LOW: negative numbers order by the high word, read without sign, backwards
-                t = __hiloint2double((int)min((unsigned)__double2hiint(t), (unsigned)0xC0CF4000u), __double2loint(t));
-                double scale, poly;
-                exp16_parts(t, tab, scale, poly);
-                acc[c] = fma(scale, poly, acc[c]);
+            for (int u = 0; u < U; ++u) m = fmaxf(m, fmaxf(fmaxf(b[u].x, b[u].y), fmaxf(b[u].z, b[u].w)));
+            m = warp_max(m);
+            if (m > high) {
+                plain = finite(m) && fabs((double)m * C) <= MOST;
+                if (!plain) return;
+                const double f = ref == -INFINITY ? 0.0 : exp_of((double)ref - (double)m, C, tab);
+#pragma unroll
+                for (int c = 0; c < G; ++c) acc[c] *= f;
+                refer(m);
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                b[u] = make_float4(fmaxf(b[u].x, low), fmaxf(b[u].y, low), fmaxf(b[u].z, low), fmaxf(b[u].w, low));
+        }
+        if (ref == -INFINITY) return;  // nothing finite so far
+#pragma unroll
+        for (int u = 0; u < U; u += G / 4) {
+            double d[G];
+#pragma unroll
+            for (int c = 0; c < G; c += 4)
+                d[c] = (double)b[u + c / 4].x, d[c + 1] = (double)b[u + c / 4].y, d[c + 2] = (double)b[u + c / 4].z,
+                d[c + 3] = (double)b[u + c / 4].w;
+            if (ref != 0.0f) {
+#pragma unroll
+                for (int c = 0; c < G; ++c) d[c] -= (double)ref;
+            }
+            exp_add(d, C, tab, acc);
+        }
+    };
+    Part mine{0.0, ref, 0};
+    float4 b[U];
+    constexpr int TILE = 32 * U;
+    int done = 0, i = 0;  // vectors of the stretch, and which one
+    for (int j = run.j0; j < run.j1 && plain; j += 2 * TILE) {
+        if (j + TILE < run.j1) load_tile(b, row, j + TILE, run.j1, lane);
+        add(a);
+        if (!plain) break;
+        if (j + TILE < run.j1) {
+            if (j + 2 * TILE < run.j1) load_tile(a, row, j + 2 * TILE, run.j1, lane);
+            add(b);
+            if (!plain) break;
+        }
+        if ((done += 2 * TILE) == run.step || j + 2 * TILE >= run.j1) {
+            double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+            if (G == 8) s += (acc[4 % G] + acc[5 % G]) + (acc[6 % G] + acc[7 % G]);
+            s = warp_sum(s);
+            plain = isfinite(s);
+            if (lane == i) mine = Part{s, ref, 0};
+#pragma unroll
+            for (int c = 0; c < G; ++c) acc[c] = 0.0;
+            done = 0, ++i;
         }
     }
-    const double s = warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
-    if (plain && isfinite(s)) return Part{s, ref, 0};
-    return range_sum_any(row, j0, j1, C, tab);
+    if (!plain) mine = run_sum_any(row, run, C, tab);
+    const float m = warp_max(mine.ref);
+    return Part{scaled(mine.sum, mine.ref, m, C, tab), m, 0};
 }
 
 // the first of the greatest finite values (argmax_first's choice)
-__device__ __forceinline__ Part range_max(const Row &row, int j0, int j1) {
+template <int U>
+__device__ __forceinline__ Part run_max(const Row &row, const Run &run, float4 (&a)[U]) {
+    constexpr int TILE = 32 * U;
     const int lane = threadIdx.x & 31;
     float best = -INFINITY;
     int at = INT32_MAX;
-    for (int j = j0; j < j1; j += 32 * U) {
+    for (int j = run.j0; j < run.j1; j += TILE) {
         float4 b[U];
-        load_tile(b, row, j, j1, lane);
+        if (j + TILE < run.j1) load_tile(b, row, j + TILE, run.j1, lane);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float v[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+            const float v[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (v[c] > best && finite(v[c])) best = v[c], at = 4 * (j + 32 * u + lane) + c - row.off;
+            a[u] = b[u];
         }
     }
 #pragma unroll
@@ -221,245 +317,420 @@ __device__ __forceinline__ Part range_max(const Row &row, int j0, int j1) {
     return Part{0.0, best, at};
 }
 
-// r_k of value x before it is divided by its sum; inv[k]: 1 / the sum of r_{k + 1}, or 0 for one without
-// mass (the target's own probabilities then)
-__device__ __forceinline__ double residual(double p, float q, const double *inv, int k) {
-    const double qq = fmax((double)q, 0.0);
-    double r = p;
-    for (int i = 0; i < k; ++i) {
-        const double rest = fmax(r - qq, 0.0);
-        if (i == k - 1) return rest;
-        r = inv[i] > 0.0 ? rest * inv[i] : p;
-    }
-    return r;
+// r_k of a value before it is divided by its sum, from its weight (p = w / Z) and q; inv[k]: 1 / the sum of
+// r_{k + 1}, or 0 for one without mass (the target's own probabilities then)
+__device__ __forceinline__ double residual(double w, double inv_Z, float q, const double *inv, int k) {
+    const double qq = (double)fmaxf(q, 0.0f);
+    double r = k == 0 ? w * inv_Z : fma(w, inv_Z, -qq);
+    for (int i = 1; i < k; ++i) r = inv[i - 1] > 0.0 ? fma(r > 0.0 ? r : 0.0, inv[i - 1], -qq) : fma(w, inv_Z, -qq);
+    return r > 0.0 ? r : 0.0;
 }
 
-// Running sums of the ranges' sums, lanes of one warp with W / 32 ranges each; the whole sum comes back.
-template <int W>
-__device__ __forceinline__ double scan_parts(double (&c)[(W + 31) / 32], double *inc) {
-    constexpr int PER = (W + 31) / 32;
+// The draft's probabilities of a row's vectors.
+struct Draft {
+    const float *q;  // of value 0
+    bool same;       // lies in 16-byte vectors as the row does
+    __device__ __forceinline__ float4 load(const Row &row, int j) const {
+        const int e = 4 * j - row.off;
+        if (same && 4 * j >= row.off && 4 * j + 4 <= row.end) {
+            const int4 r = ldg_stream(q + e);
+            return make_float4(__int_as_float(r.x), __int_as_float(r.y), __int_as_float(r.z), __int_as_float(r.w));
+        }
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = 4 * j + c >= row.off && 4 * j + c < row.end ? __ldg(q + e + c) : 0.0f;
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+};
+
+// weights of values: 0 from 1000 octaves under the reference on, and for what is not finite
+template <int N>
+__device__ __forceinline__ void weights(const float4 (&x)[N / 4], float ref, double C, uint32_t tab, double (&w)[N]) {
+    double d[N];
+    bool none[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        const float v[4] = {x[c / 4].x, x[c / 4].y, x[c / 4].z, x[c / 4].w};
+        d[c] = (double)v[c % 4] - (double)ref;
+        none[c] = !(d[c] * C > -LOW) || !finite(v[c % 4]);
+        if (none[c]) d[c] = 0.0;
+        w[c] = 0.0;
+    }
+    exp_add(d, C, tab, w);
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+        if (none[c]) w[c] = 0.0;
+}
+
+// The sums of r_k over the run's stretches, before r_k is divided by its sum.  CALM: weights as in run_sum,
+// those of what is 1000 octaves below or not finite 2^-1000 in the place of 0, which the sums do not show.
+template <bool CALM>
+__device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const Run &run, float ref, double inv_Z, double C, uint32_t tab,
+                                         const double *inv, int k) {
+    const int lane = threadIdx.x & 31;
+    const float low = (float)((double)ref - LOW / C);
+    constexpr int U = 2;
+    Part mine{0.0, ref, 0};
+    float4 x[U], y[U], nx[U], ny[U];
+    auto load = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = j + 32 * u + lane;
+            nx[u] = at < run.j1 ? row.load(at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            ny[u] = at < run.j1 ? q.load(row, at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    load(run.j0);
+    double acc[8] = {};
+    int done = 0, i = 0;
+    for (int j = run.j0; j < run.j1; j += 32 * U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = nx[u], y[u] = ny[u];
+        if (j + 32 * U < run.j1) load(j + 32 * U);
+        const float f[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+        double w[8] = {};
+        if (CALM) {
+            const float v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+            double d[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) d[c] = (double)(v[c] > low && v[c] < INFINITY ? v[c] : low) - (double)ref;
+            exp_add(d, C, tab, w);
+        } else {
+            weights<8>(x, ref, C, tab, w);
+        }
+        if (k == 1) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const double r = fma(w[c], inv_Z, -(double)fmaxf(f[c], 0.0f));
+                acc[c] += r > 0.0 ? r : 0.0;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] += residual(w[c], inv_Z, f[c], inv, k);
+        }
+        if ((done += 32 * U) == run.step || j + 32 * U >= run.j1) {
+            const double s = warp_sum(((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7])));
+            if (lane == i) mine.sum = s;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] = 0.0;
+            done = 0, ++i;
+        }
+    }
+    return mine;
+}
+
+__device__ __noinline__ Part run_rest_any(Row row, Draft q, Run run, float ref, double inv_Z, double C, uint32_t tab, const double *inv, int k) {
+    return run_rest<false>(row, q, run, ref, inv_Z, C, tab, inv, k);
+}
+
+// running sum over the first N lanes
+template <int N = 32>
+__device__ __forceinline__ double scan(double v) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int k = 1; k < PER; ++k) c[k] += c[k - 1];
-    double run = c[PER - 1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
+    for (int o = 1; o < N; o <<= 1) {
+        const double w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
     }
-    double before = __shfl_up_sync(0xffffffffu, run, 1);
-    if (lane == 0) before = 0.0;
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-        if (lane * PER + k < W) inc[lane * PER + k] = k == PER - 1 ? run : before + c[k];
-    return __shfl_sync(0xffffffffu, run, 31);
+    return v;
 }
 
-// One cluster of CS CTAs per node; every warp takes one run of the row's vectors.  The warps' sums go to
-// every CTA of the cluster, which then all take the same decisions, so that the call needs no workspace
-// and no second launch; the CTA that holds the drawn value's run reads that run once more.
+// The sums of a row's weights by stretch, warp and CTA, and where a drawn value lies.
 template <int CS>
-__global__ void __launch_bounds__(NT) tree_sample_kernel(Sample a, int *err) {
+struct Sums {
+    double stretch[NW][32];  // running sums over a warp's stretches, relative to the CTA's reference
+    double warp[NW];         // running sums over the warps
+    double cta[2][CS];       // sums of the cluster's CTAs (two calls in turn), relative to
+    float cta_ref[2][CS];    // their references
+    float warp_ref[NW];
+    int cta_at[2][CS];       // T = 0: of the maximum (cta_ref)
+};
+
+// A child's token (-1: none that is one), and what it is tried with: its uniform number, its token's
+// probability in the draft, and its logit.
+struct Try {
+    int token;
+    float u, q, l;
+};
+
+// Where a drawn value lies: CTA, warp, stretch, and the running sum up to there.
+struct Place {
+    int cta, warp, stretch;
+    double before, f;  // f: what the CTA's sums are multiplied by
+};
+
+// `mine`: this lane's stretch, relative to the warp's reference.  Then the sums are everywhere, `all` is the
+// whole row's and `ref` what it is relative to; f: what this lane's CTA's are to be multiplied by.
+template <int CS>
+__device__ __forceinline__ void gather(Sums<CS> &s, int turn, int rank, const Part &mine, double C, uint32_t tab, double &all, float &ref,
+                                       double &run, double &f) {
     namespace cg = cooperative_groups;
-    constexpr int W = CS * NW, PER = (W + 31) / 32;
-    __shared__ double s_tab[16], s_inc[W], s_rest[W], s_inv[TREE_MAX_NODES], s_warp[NW];
-    __shared__ Part s_part[2][W];
-    __shared__ double s_total, s_Z;
-    __shared__ float s_ref;
-    __shared__ int s_kid, s_take, s_at, s_found, s_last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) s.warp_ref[warp] = mine.ref;
+    __syncthreads();
+    const float m = warp_max(lane < NW ? s.warp_ref[lane] : -INFINITY);
+    const double up = scan(scaled(mine.sum, mine.ref, m, C, tab));
+    s.stretch[warp][lane] = up;
+    __syncthreads();
+    if (warp == 0) {
+        const double w = scan<NW>(lane < NW ? s.stretch[lane][31] : 0.0);
+        if (lane < NW) s.warp[lane] = w;
+        const double total = __shfl_sync(0xffffffffu, w, NW - 1);
+        if (CS == 1) {
+            if (lane == 0) s.cta[turn][0] = total, s.cta_ref[turn][0] = m;
+        } else if (lane < CS) {
+            cg::cluster_group cl = cg::this_cluster();
+            *cl.map_shared_rank(&s.cta[turn][rank], lane) = total;
+            *cl.map_shared_rank(&s.cta_ref[turn][rank], lane) = m;
+        }
+    }
+    if (CS == 1) __syncthreads();
+    else cg::this_cluster().sync();
+    const float r = lane < CS ? s.cta_ref[turn][lane] : -INFINITY;
+    ref = warp_max(r);
+    f = lane < CS ? scaled(1.0, r, ref, C, tab) : 0.0;
+    run = scan<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0);
+    all = __shfl_sync(0xffffffffu, run, CS - 1);
+    if (lane >= CS) run = all;
+}
+
+// the first place whose running sum is greater than `drawn`, the last with any mass if roundings leave none
+template <int CS>
+__device__ __forceinline__ Place find(const Sums<CS> &s, double run, double f, double drawn, int rank) {
+    const int lane = threadIdx.x & 31;
+    auto first = [&](double up, double drawn) {
+        const unsigned past = __ballot_sync(0xffffffffu, up > drawn);
+        double before = __shfl_up_sync(0xffffffffu, up, 1);
+        if (lane == 0) before = 0.0;
+        const unsigned mass = __ballot_sync(0xffffffffu, up > before);
+        return past ? __ffs(past) - 1 : 31 - __clz(mass | 1u);
+    };
+    Place p;
+    p.cta = first(run, drawn);
+    p.f = __shfl_sync(0xffffffffu, f, p.cta);
+    p.before = p.cta ? __shfl_sync(0xffffffffu, run, max(p.cta - 1, 0)) : 0.0;
+    if (p.cta != rank) return p;
+    const double w = p.before + p.f * s.warp[min(lane, NW - 1)];
+    p.warp = min(first(w, drawn), NW - 1);
+    const double start = __shfl_sync(0xffffffffu, w, max(p.warp - 1, 0));
+    if (p.warp) p.before = start;
+    const double t = p.before + p.f * s.stretch[p.warp][lane];
+    p.stretch = first(t, drawn);
+    const double at = __shfl_sync(0xffffffffu, t, max(p.stretch - 1, 0));
+    if (p.stretch) p.before = at;
+    return p;
+}
+
+// One cluster of CS CTAs per node; every warp takes one run of the row's vectors.  The CTAs' sums go to
+// every CTA of the cluster, which then all take the same decisions, so that the call needs no workspace
+// and no second launch; the CTA that holds the drawn value's stretch reads that stretch once more.
+template <int CS, int U>
+__global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) {
+    namespace cg = cooperative_groups;
+    constexpr int W = CS * NW;
+    __shared__ Table s_table;
+    __shared__ Sums<CS> s_sums;
+    __shared__ double s_inv[TREE_MAX_NODES], s_warp[NW], s_log;
+    __shared__ unsigned short s_kids[TREE_MAX_NODES];
+    __shared__ int s_n_kids, s_last;
+    __shared__ Try s_try[32];  // of the first children
     griddep_launch_dependents();
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row_id = blockIdx.x / CS, rank = blockIdx.x % CS;
     const int s = row_id / a.N, i = row_id - s * a.N;
+    const char *x = a.x + s * a.x_nb2 + i * a.x_nb1;
+    const Row row(x, a.V);
+    const int per = (row.vectors() + W - 1) / W, step = max((per + 32 * 64 * U - 1) / (32 * 64 * U), 1) * 64 * U;
+    auto run_of = [&](int cta, int warp) {
+        const int j0 = min((cta * NW + warp) * per, row.vectors());
+        return Run{j0, min(j0 + per, row.vectors()), step};
+    };
+    const Run run = run_of(rank, warp);
+    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 first[U];
+    load_tile(first, row, run.j0, run.j1, lane);
+    const float4 head = lane < row.vectors() ? row.load(lane) : none;
     const int n = a.n_nodes ? a.n_nodes[s] : a.N;
     const float T = a.temp ? a.temp[s] : 1.0f;
     const float u1 = a.u[s * a.u_ld2 + i * a.u_ld1 + 1];
-    const bool bad = n < 0 || n > a.N || !(T >= 0.0f && T < INFINITY) || (T > 0.0f && i < n && !(u1 >= 0.0f && u1 < 1.0f));
-    if (bad || i >= n) {
-        if (rank == 0 && tid == 0) {
-            if (bad) atomicOr(err, ERR_BAD_INDEX);
-            a.target[s * a.tgt_ld + i] = -1;
-            if (a.logp) a.logp[s * a.logp_ld + i] = 0.0f;
-        }
-        return;
-    }
-    if (CS > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    if (tid < 16) s_tab[tid] = table_entry(tid);
-    __syncthreads();
-    const char *x = a.x + s * a.x_nb2 + i * a.x_nb1;
-    const Row row(x, a.V);
-    const int run = (row.vectors() + W - 1) / W;  // vectors of a warp
-    const int j0 = min((rank * NW + warp) * run, row.vectors()), j1 = min(j0 + run, row.vectors());
-    const double inv_T = T > 0.0f ? 1.0 / (double)T : 0.0, C = LOG2E_16 * inv_T;
-    const Part mine = T > 0.0f ? range_sum(row, j0, j1, C, s_tab) : range_max(row, j0, j1);
-    if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
-
-    // a warp's part to every CTA of the cluster; then all parts are here
-    int parity = 0;
-    auto share = [&](const Part &p) {
-        if (CS == 1) {
-            if (lane == 0) s_part[parity][warp] = p;
-            __syncthreads();
-        } else {
-            cg::cluster_group cl = cg::this_cluster();
-            if (lane < CS) *cl.map_shared_rank(&s_part[parity][rank * NW + warp], lane) = p;
-            cl.sync();
-        }
-    };
+    s_table.fill();
+    if (tid == 0) s_last = -1;
+    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(&s_table.v[0][tid % COPIES]);
     auto put = [&](int token, double logp) {
         a.target[s * a.tgt_ld + i] = token;
         if (a.logp) a.logp[s * a.logp_ld + i] = (float)logp;
     };
-    share(mine);
-    if (T == 0.0f) {
+    const bool bad = n < 0 || n > a.N || !(T >= 0.0f && T < INFINITY) || (T > 0.0f && i < n && !(u1 >= 0.0f && u1 < 1.0f));
+    if (bad || i >= n) {
         if (rank == 0 && tid == 0) {
-            float best = -INFINITY;
-            int at = -1;
-            for (int k = 0; k < W; ++k)
-                if (s_part[0][k].ref > best) best = s_part[0][k].ref, at = s_part[0][k].at;
-            put(at, 0.0);
+            if (bad) atomicOr(err, ERR_BAD_INDEX);
+            put(-1, 0.0);
         }
         return;
     }
-    if (warp == 0) {
-        float m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-            if (lane * PER + k < W) m = fmaxf(m, s_part[0][lane * PER + k].ref);
-        m = warp_max(m);
-        double c[PER];
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const Part p = lane * PER + k < W ? s_part[0][lane * PER + k] : Part{0.0, -INFINITY, 0};
-            c[k] = p.ref > -INFINITY ? p.sum * exp16(((double)p.ref - (double)m) * C, s_tab) : 0.0;
+    if (CS > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const float *logits = reinterpret_cast<const float *>(x);
+    const float *q = reinterpret_cast<const float *>(a.q + s * a.q_nb2 + i * a.q_nb1);
+    auto child = [&](int j) {
+        Try t{a.tokens[s * a.tok_ld + j], a.u[s * a.u_ld2 + j * a.u_ld1], 0.0f, 0.0f};
+        if (t.token < 0 || t.token >= a.V || !(t.u >= 0.0f && t.u < 1.0f)) {
+            if (rank == 0) atomicOr(err, ERR_BAD_INDEX);
+            t.token = -1;
+        } else {
+            t.q = q[t.token], t.l = logits[t.token];
         }
-        const double z = scan_parts<W>(c, s_inc);
-        if (lane == 0) s_Z = z, s_ref = m;
+        return t;
+    };
+    if (a.q && warp == 0 && T > 0.0f) {  // the node's children in order
+        int count = 0;
+        for (int j0 = i + 1; j0 < n; j0 += 32) {
+            const int j = j0 + lane;
+            const bool is = j < n && a.parents[s * a.par_ld + j] == i;
+            const unsigned all = __ballot_sync(0xffffffffu, is);
+            if (is) s_kids[count + __popc(all & ((1u << lane) - 1))] = (unsigned short)j;
+            count += __popc(all);
+        }
+        if (lane == 0) s_n_kids = count;
+        __syncwarp();
+        if (lane < count) s_try[lane] = child(s_kids[lane]);
     }
     __syncthreads();
-    const double Z = s_Z, inv_Z = 1.0 / Z;
-    const float ref = s_ref;
+    if (T == 0.0f) {
+        const Part best = run_max(row, run, first);
+        if (lane == 0) s_sums.warp_ref[warp] = best.ref, s_sums.stretch[warp][0] = best.at;
+        if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
+        __syncthreads();
+        auto most = [&](float v, int at) {  // the first of the greatest over the lanes
+            const float m = warp_max(v);
+            const unsigned is = __ballot_sync(0xffffffffu, v == m && m > -INFINITY);
+            return Part{0.0, m, is ? __shfl_sync(0xffffffffu, at, __ffs(is) - 1) : -1};
+        };
+        if (warp == 0) {
+            const Part p = most(lane < NW ? s_sums.warp_ref[lane] : -INFINITY, lane < NW ? (int)s_sums.stretch[lane][0] : 0);
+            if (lane == 0) {
+                int *at = &s_sums.cta_at[0][rank];
+                float *ref = &s_sums.cta_ref[0][rank];
+                if (CS > 1) at = cg::this_cluster().map_shared_rank(at, 0), ref = cg::this_cluster().map_shared_rank(ref, 0);
+                *at = p.at, *ref = p.ref;
+            }
+        }
+        if (CS == 1) __syncthreads();
+        else cg::this_cluster().sync();
+        if (rank == 0 && warp == 0) {
+            const Part p = most(lane < CS ? s_sums.cta_ref[0][lane] : -INFINITY, lane < CS ? s_sums.cta_at[0][lane] : 0);
+            if (lane == 0) put(p.at, 0.0);
+        }
+        return;
+    }
+    const double inv_T = 1.0 / (double)T, C = STEPS / LN2 * inv_T;
+    float guess = -INFINITY;
+    for (float f : {head.x, head.y, head.z, head.w})
+        if (finite(f)) guess = fmaxf(guess, f);
+    guess = warp_max(guess);
+    // 0, as long as that leaves room on both sides
+    const Part mine = run_sum(row, run, first, fabs((double)guess * C) <= ROOM ? 0.0f : guess, C, tab);
+    if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
+    double Z, upto, f;
+    float ref;
+    gather(s_sums, 0, rank, mine, C, tab, Z, ref, upto, f);
     if (ref == -INFINITY) {  // no finite logit
         if (rank == 0 && tid == 0) put(-1, 0.0);
         return;
     }
-    const float *logits = reinterpret_cast<const float *>(x);
-    auto log_p = [&](int t) { return ((double)logits[t] - (double)ref) * inv_T - log(Z); };
-
-    const float *q = reinterpret_cast<const float *>(a.q + s * a.q_nb2 + i * a.q_nb1);
+    const Draft draft{q, (((uintptr_t)q ^ (uintptr_t)logits) & 15) == 0};
+    const bool calm = fabs((double)ref * C) <= MOST;
     int rounds = 0;
-    double rest = 0.0;  // the last residual's sum
+    bool left = false;  // something is left of p
+    double inv_Z = 0.0, total = Z;
     if (a.q) {
-        for (int prev = i;; ) {
-            if (tid == 0) s_kid = INT32_MAX;
-            __syncthreads();
-            for (int j = prev + 1 + tid; j < n; j += NT)
-                if (a.parents[s * a.par_ld + j] == i) {
-                    atomicMin(&s_kid, j);
-                    break;
-                }
-            __syncthreads();
-            const int kid = s_kid;
-            if (kid == INT32_MAX) break;
-            if (tid == 0) {
-                const int t = a.tokens[s * a.tok_ld + kid];
-                const float u0 = a.u[s * a.u_ld2 + kid * a.u_ld1];
-                s_take = -1;
-                if (t < 0 || t >= a.V || !(u0 >= 0.0f && u0 < 1.0f)) {
-                    atomicOr(err, ERR_BAD_INDEX);
-                } else {
-                    const float qt = q[t];
-                    double r = residual(weight(logits[t], ref, C, s_tab) * inv_Z, qt, s_inv, rounds);
-                    if (rounds) r = s_inv[rounds - 1] > 0.0 ? r * s_inv[rounds - 1] : weight(logits[t], ref, C, s_tab) * inv_Z;
-                    if ((double)u0 * (double)qt < r) s_take = t;
+        inv_Z = 1.0 / Z;
+        auto rest = [&](int k) {
+            return calm ? run_rest<true>(row, draft, run, ref, inv_Z, C, tab, s_inv, k) : run_rest_any(row, draft, run, ref, inv_Z, C, tab, s_inv, k);
+        };
+        const int kids = s_n_kids;
+        while (rounds < kids) {
+            const Try t = rounds < 32 ? s_try[rounds] : child(s_kids[rounds]);
+            if (t.token >= 0) {
+                const double w = weight(t.l, ref, C, tab);
+                double r = residual(w, inv_Z, t.q, s_inv, left ? rounds : 0);
+                if (left) r *= s_inv[rounds - 1];
+                if ((double)t.u * (double)t.q < r) {
+                    if (rank == 0 && tid == 0) put(t.token, ((double)t.l - (double)ref) * inv_T - log(Z));
+                    return;
                 }
             }
-            __syncthreads();
-            if (s_take >= 0) {
-                if (rank == 0 && tid == 0) put(s_take, log_p(s_take));
-                return;
-            }
-            prev = kid;
             ++rounds;
-            double sum = 0.0;
-            for (int j = j0 + lane; j < j1; j += 32) {
-                const float4 v = row.load(j);
-                const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int e = 4 * j + c - row.off;
-                    if (e >= 0 && e < a.V) sum += residual(weight(w[c], ref, C, s_tab) * inv_Z, __ldg(q + e), s_inv, rounds);
-                }
-            }
-            parity ^= 1;
-            share(Part{warp_sum(sum), 0.0f, 0});
-            if (warp == 0) {
-                double c[PER];
-#pragma unroll
-                for (int k = 0; k < PER; ++k) c[k] = lane * PER + k < W ? s_part[parity][lane * PER + k].sum : 0.0;
-                const double all = scan_parts<W>(c, s_rest);
-                if (lane == 0) s_total = all, s_inv[rounds - 1] = all > 0.0 ? 1.0 / all : 0.0;
-            }
+            double sum, up, one;
+            float same;
+            gather(s_sums, rounds & 1, rank, rest(rounds), C, tab, sum, same, up, one);
+            left = sum > 0x1p-900;
+            if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / sum : 0.0;
+            if (left) total = sum, upto = up, f = one;
             __syncthreads();
-            rest = s_total;
+        }
+        if (rounds && !left)  // p once more
+            gather(s_sums, (rounds + 1) & 1, rank, rest(0), C, tab, total, ref, upto, f);
+    }
+    // a number on a border belongs to the value behind it, however the sums up to there were rounded
+    const double drawn = (double)u1 * total + total * 0x1p-44;
+    const Place at = find(s_sums, upto, f, drawn, rank);
+    if (at.cta != rank) return;
+    if (tid == NT - 1) s_log = log(Z);
+    // the value's place in its stretch: `each` vectors of a thread, one after the other
+    const Run found = run_of(rank, at.warp);
+    const int j0 = found.from(at.stretch), j1 = found.from(at.stretch + 1), each = (step + NT - 1) / NT;
+    auto values = [&](int j, const float4 &v, double (&w)[4]) {
+        const float4 one[1] = {v};
+        weights<4>(one, ref, C, tab, w);
+        if (left) {
+            const float4 y = j < j1 ? draft.load(row, j) : zero;
+            const float g[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = residual(w[c], inv_Z, g[c], s_inv, rounds);
+        } else if (rounds) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] *= inv_Z;
+        }
+    };
+    const int b0 = j0 + tid * each, b1 = min(b0 + each, j1);
+    double own = 0.0, w[4];
+    float4 v = none;
+    int last = -1;  // of the values with any mass
+    for (int j = b0; j < b1; ++j) {
+        v = row.load(j);
+        values(j, v, w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            own += w[c];
+            if (w[c] > 0.0) last = 4 * j + c;
         }
     }
-    // the run in which the running sum passes the drawn value, and the value's place in it
-    const bool left = rounds > 0 && rest > 0.0;
-    const double *inc = left ? s_rest : s_inc;
-    const double drawn = (double)u1 * (left ? rest : Z);
-    if (tid == 0) s_at = W - 1;
-    if (tid == 0) s_found = INT32_MAX, s_last = -1;
-    __syncthreads();
-    if (tid < W && inc[tid] > drawn && (tid == 0 || inc[tid - 1] <= drawn)) s_at = tid;
-    __syncthreads();
-    const int at = s_at;
-    if (at / NW != rank) return;
-    const int e0 = max(4 * at * run - row.off, 0), e1 = min(4 * (at + 1) * run - row.off, a.V);
-    const int per = (e1 - e0 + NT - 1) / NT;
-    const int b0 = min(e0 + tid * per, e1), b1 = min(b0 + per, e1);
-    auto value = [&](int e) {
-        const double w = weight(__ldg(logits + e), ref, C, s_tab);
-        return left ? residual(w * inv_Z, __ldg(q + e), s_inv, rounds) : w;
-    };
-    double own = 0.0;
-    int last = -1;  // of the values with any mass
-    for (int e = b0; e < b1; ++e) {
-        const double v = value(e);
-        own += v;
-        if (v > 0.0) last = e;
-    }
-    double scan = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += v;
-    }
-    if (lane == 31) s_warp[warp] = scan;
+    const double up = scan(own);
+    if (lane == 31) s_warp[warp] = up;
     if (last >= 0) atomicMax(&s_last, last);
     __syncthreads();
-    double base = at ? inc[at - 1] : 0.0;
+    double base = at.before;
     for (int k = 0; k < warp; ++k) base += s_warp[k];
-    double before = __shfl_up_sync(0xffffffffu, scan, 1);
+    double before = __shfl_up_sync(0xffffffffu, up, 1);
     before = lane ? base + before : base;
-    if (before <= drawn && base + scan > drawn) {
-        int found = last;  // where roundings let the walk miss it
+    auto report = [&](int e, float l) { put(e - row.off, ((double)l - (double)ref) * inv_T - s_log); };
+    const bool here = before <= drawn && base + up > drawn;
+    if (here) {
+        int e = last;  // where roundings let the walk miss it
         double cum = before;
-        for (int e = b0; e < b1; ++e) {
-            cum += value(e);
-            if (cum > drawn) {
-                found = e;
-                break;
-            }
+        for (int j = b0; j < b1; ++j) {
+            if (each > 1) values(j, row.load(j), w);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (cum <= drawn) {
+                    cum += w[c];
+                    if (cum > drawn) e = 4 * j + c;
+                }
         }
-        atomicMin(&s_found, found);
+        report(e, row.base[e]);
     }
-    __syncthreads();
-    if (tid == 0) {
-        const int t = s_found != INT32_MAX ? s_found : s_last;
-        put(t, t >= 0 ? log_p(t) : 0.0);
-    }
+    if (!__syncthreads_or(here) && tid == 0) report(s_last, row.base[s_last]);
 }
 
 // whether the values of out (4 bytes each) and those of a 4-byte tensor [.., n, n_seq] meet
@@ -477,13 +748,13 @@ bool is_rows3_f32(const oasr_tensor *t, int64_t w, int64_t N, int64_t S) {
            t->ne[3] == 1 && (t->nb[0] == 4 || w <= 1) && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0;
 }
 
-template <int CS>
+template <int CS, int U>
 int launch_sample(oasr_backend *be, const Sample &a, int64_t rows) {
     if (rows * CS > INT32_MAX) return fail_op(be, "tree_sample", "too many nodes");
     if (CS > 8) {
         static OncePerDevice wide;
         const cudaError_t e = (cudaError_t)wide(be->device, [] {
-            return cudaFuncSetAttribute(tree_sample_kernel<CS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            return cudaFuncSetAttribute(tree_sample_kernel<CS, U>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         });
         if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "tree_sample attribute", __LINE__);
     }
@@ -498,7 +769,7 @@ int launch_sample(oasr_backend *be, const Sample &a, int64_t rows) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = be->pdl ? 2 : 1;
-    return launched(be, cudaLaunchKernelEx(&cfg, tree_sample_kernel<CS>, a, be->err_word), "tree_sample");
+    return launched(be, cudaLaunchKernelEx(&cfg, tree_sample_kernel<CS, U>, a, be->err_word), "tree_sample");
 }
 
 }  // namespace
@@ -551,14 +822,19 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
     if (logprob) a.logp = (float *)logprob->data, a.logp_ld = logprob->nb[1] / 4;
     a.N = (int)N, a.V = (int)V;
     const int64_t rows = S * N;
-    // CTAs per node: enough of them for the SMs, of at least 2048 values each
-    int cs = 16;
-    while (cs > 1 && (rows * cs > 4 * be->sm_count || V < 2048 * cs)) cs /= 2;
+    // CTAs per node: enough of them for the SMs, of at least 2048 values each.  Without a draft two per SM (8
+    // nodes of 151936: 10.3 us with 16 CTAs each, 12.4 with 8, 16.5 with 4; 1952 nodes: 272 us with one, 324
+    // with two).  With one, nodes whose children are rejected take three times as long as the others, and
+    // more and smaller CTAs even that out (64 nodes: 39 us with 4 or 8 each, 51 with 16; 124 of 51866: 70, 41,
+    // 38 and 49 us with 2, 4, 8 and 16).
+    const int most = draft_probs ? 8 : 16, per_sm = draft_probs ? 8 : 2;
+    int cs = most;
+    while (cs > 1 && (rows * cs > per_sm * be->sm_count || V < 2048 * cs)) cs /= 2;
     switch (cs) {
-    case 16: return launch_sample<16>(be, a, rows);
-    case 8: return launch_sample<8>(be, a, rows);
-    case 4: return launch_sample<4>(be, a, rows);
-    case 2: return launch_sample<2>(be, a, rows);
-    default: return launch_sample<1>(be, a, rows);
+    case 16: return launch_sample<16, 4>(be, a, rows);
+    case 8: return launch_sample<8, 4>(be, a, rows);
+    case 4: return launch_sample<4, 4>(be, a, rows);
+    case 2: return launch_sample<2, 8>(be, a, rows);
+    default: return launch_sample<1, 8>(be, a, rows);
     }
 }
