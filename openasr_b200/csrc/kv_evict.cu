@@ -9,7 +9,6 @@
 // kv_evict: of a sequence's positions the first n_sink, the last n_recent, and of the others those with the
 // greatest w stay, n_keep in all; their rows move to the front in their order.
 #include <cooperative_groups.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -27,13 +26,15 @@ struct Weights {
     int64_t q_nb1, q_nb2, q_nb3;  // node, head, sequence
     char *w;                      // [page, H_kv, n_pages] f32
     int64_t w_nb1, w_nb2;         // head, page
-    int HKV, G, cs;               // K/V heads, query heads of each, CTAs per cluster
-    int cap;                      // tiles of a warp whose scores stay in shared memory
+    int S, HKV, G, cs;            // sequences, K/V heads, query heads of each, CTAs per cluster
+    int stretch;                  // positions whose scores shared memory holds at a time (a multiple of 16)
+    int stride;                   // scores of a position there
     float scale, decay;
 };
 
 constexpr int WT = 256, WW = WT / 32;  // threads, warps
 constexpr int WTILE = 16;              // positions of a warp's tile
+constexpr int WPAGES = 520;            // pages of a stretch: of 8 positions and more
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -47,6 +48,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ uint4 stream(const void *p) {
+    const int4 v = ldg_stream(p);
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 // (m, l) of two sets of positions to that of both; m = -inf: nothing seen
 __device__ __forceinline__ void join(float &m, float &l, float om, float ol) {
     const float mm = fmaxf(m, om), z = mm == -INFINITY ? 0.0f : mm;
@@ -56,268 +62,315 @@ __device__ __forceinline__ void join(float &m, float &l, float om, float ol) {
 
 // 8 rows of queries per block, in the layout of the product's second operand: lane (g, t) has of row g the
 // values 32 c + 8 t .. + 7 of each run c of 32, the first four for one product of depth 16 and the others
-// for the next; a K row is read the same way, 16 bytes per lane, so that both go from memory to registers
+// for the next; a K row is read the same way, 16 bytes per lane, so that it goes from memory to registers
 // without shared memory.  f32 queries are scaled by a power of two per row and split into two f16 halves.
-template <int D, int NB, bool QF16>
-struct Queries {
+// Up to two blocks stay in registers, more in shared memory.
+template <int D, bool QF16>
+struct Block {
     static constexpr int C = D / 32;
-    uint4 hi[NB][C], lo[QF16 ? 1 : NB][QF16 ? 1 : C];
+    uint4 hi[C], lo[QF16 ? 1 : C];
+    float factor;  // of row g's scores, with log2 e
 };
 
-// One cluster per (sequence, K/V head); its CTAs share out the positions, in tiles of 16 per warp.  The
-// first pass over the tiles takes m and l of every row, which the CTAs then exchange; the second turns the
-// scores, kept in shared memory or computed again, into weights.  Every position belongs to one thread:
-// the sums have one order, and the call needs no workspace.
+template <int D, bool QF16>
+__device__ __forceinline__ Block<D, QF16> load_block(const Weights &a, const FastDiv &group, int r, int rows, int hk, int s) {
+    constexpr int C = D / 32;
+    const int t = threadIdx.x & 3;
+    const int i = group(min(r, rows - 1)), h = hk * a.G + min(r, rows - 1) - i * a.G;
+    const char *row = a.q + i * a.q_nb1 + h * a.q_nb2 + s * a.q_nb3;
+    Block<D, QF16> q;
+    q.factor = a.scale * 1.4426950408889634f;
+    if (QF16) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            q.hi[c] = r < rows ? *reinterpret_cast<const uint4 *>(row + 64 * c + 16 * t) : make_uint4(0, 0, 0, 0);
+        return q;
+    }
+    float v[C][8], most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 x = r < rows ? *reinterpret_cast<const float4 *>(row + 128 * c + 32 * t + 4 * e) : make_float4(0, 0, 0, 0);
+            v[c][e] = x.x, v[c][e + 1] = x.y, v[c][e + 2] = x.z, v[c][e + 3] = x.w;
+#pragma unroll
+            for (int k = e; k < e + 4; ++k) most = fmaxf(most, fabsf(v[c][k]));
+        }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^up brings the greatest value to [2^9, 2^10): two halves of 11 bits have 22 of its bits
+    const int up = most > 0.0f && most < INFINITY ? max(-120, min(100, 9 - ilogbf(most))) : 0;
+    const float m = __int_as_float((127 + up) << 23);
+    q.factor *= __int_as_float((127 - up) << 23);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        __half2 hh[4], ll[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = v[c][2 * e] * m, y = v[c][2 * e + 1] * m;
+            hh[e] = __floats2half2_rn(x, y);
+            ll[e] = __floats2half2_rn(x - __low2float(hh[e]), y - __high2float(hh[e]));
+        }
+        q.hi[c] = *reinterpret_cast<uint4 *>(hh);
+        q.lo[QF16 ? 0 : c] = *reinterpret_cast<uint4 *>(ll);
+    }
+    return q;
+}
+
+// One cluster per (sequence, K/V head); its CTAs share out the positions.  A CTA goes through its own in
+// stretches whose scores its shared memory holds: a warp multiplies 16 positions at a time with the rows and
+// keeps m and l of every row.  The CTAs exchange those; then a thread takes a position and turns its scores
+// into a weight, first of the last stretch, whose scores are still there, then of the others, computed
+// again.  Every position belongs to one thread: the sums have one order, and the call needs no workspace.
+// More rows than 8 NB are taken block by block.  Long caches are bound by HBM while a CTA multiplies (27000 of
+// the 40000 cycles of each of 512 CTAs, two per SM: 16 sequences of 4001 to 8190 positions take 49 us, 4.2
+// TB/s); the rest is the start, the exchange (2800) and the weights (4200).  Short calls are a chain of five
+// round trips: 6.3 us for one token.  K fetched to L2 ahead took 56 us, three CTAs per SM 51, every warp's m
+// and l sent to every CTA 68.
 template <int D, int NB, bool QF16>
-__global__ void __launch_bounds__(WT) attn_weights_kernel(Weights a, KvPages p, KvSeqs sq, FastDiv page, FastDiv group, int *err) {
+__global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages p, KvSeqs sq, FastDiv page, FastDiv group, int *err) {
     namespace cg = cooperative_groups;
     constexpr int C = D / 32, RB = 8 * NB;
-    extern __shared__ float4 s_scores[];  // [tile of the warp][warp][NB][lane]
+    constexpr bool REGS = NB <= 2, AHEAD = NB <= 2 || (NB == 4 && D == 64);  // the next tile of K under way
+    constexpr int PARTS = QF16 ? 1 : 2, HELD = REGS ? 0 : NB * PARTS * C * 32;
+    extern __shared__ uint4 s_dyn4[];  // the blocks [block][half][run][lane], then the scores
+    float *s_scores = reinterpret_cast<float *>(s_dyn4 + HELD);  // [position][stride]
+    __shared__ float s_factor[RB];
     __shared__ float2 s_ml[2][16][RB], s_warp[WW][RB], s_row[RB];
+    __shared__ int s_page[WPAGES];
     griddep_launch_dependents();
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int item = blockIdx.x / a.cs, rank = blockIdx.x % a.cs;
-    const int s = item / a.HKV, hk = item - s * a.HKV;
+    int s = item / a.HKV;
+    const int hk = item - s * a.HKV;
+    if (a.S > 1 && a.S <= 32) {  // the longest sequences first, so that none of them starts when the others end
+        const int own = lane < a.S ? sq.n_past[lane] : INT32_MIN;
+        int before = 0;
+        for (int j = 0; j < a.S; ++j) {
+            const int other = __shfl_sync(0xffffffffu, own, j);
+            before += other > own || (other == own && j < lane);
+        }
+        s = __ffs(__ballot_sync(0xffffffffu, lane < a.S && before == s)) - 1;
+    }
     int past, n;
     if (!seq_lengths(sq, s, p.page, past, n) && rank == 0 && tid == 0) atomicOr(err, ERR_BAD_INDEX);
     if (n == 0) return;
     if (a.cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int T = past + n, tiles = (T + WTILE - 1) / WTILE;
-    const int per = (tiles + a.cs - 1) / a.cs;
-    const int t0 = min(rank * per, tiles), t1 = min(t0 + per, tiles);
+    const int per = (tiles + a.cs - 1) / a.cs * WTILE;  // positions of a CTA
+    const int p0 = (int)min((int64_t)rank * per, (int64_t)T), p1 = min(p0 + per, T);
+    const int stretches = max(1, (p1 - p0 + a.stretch - 1) / a.stretch);
     const int *table = sq.table + s * sq.table_ld;
     const char *kh = p.k + hk * p.k_nb2;
     char *wh = a.w + hk * a.w_nb1;
     const int rows = n * a.G;
 
-    // page and offset of the 8 positions from p8 on (a multiple of 8); -1: none, or not a page
-    auto locate = [&](int p8, int &off) {
-        if (p8 >= T) return -1;
-        const int j = page(p8), pg = table[j];
-        off = p8 - j * p.page;
-        if (pg >= 0 && pg < p.n_pages) return pg;
-        if (lane == 0) atomicOr(err, ERR_BAD_INDEX);
-        return -1;
+    int first_page = 0;
+    auto pages_of = [&](int b0, int b1) {  // the pages of positions [b0, b1), -1 for what is none
+        if (b0 >= b1) return;
+        first_page = page(b0);
+        const int last = page(b1 - 1);
+        for (int j = first_page + tid; j <= last; j += WT) {
+            const int pg = table[j];
+            const bool is = pg >= 0 && pg < p.n_pages;
+            if (!is) atomicOr(err, ERR_BAD_INDEX);
+            s_page[j - first_page] = is ? pg : -1;
+        }
+        __syncthreads();
     };
-    auto load_k = [&](uint4 (&k)[2][C], int tile) {
+    auto load_k = [&](uint4 (&k)[2][C], int at, int end) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            int off;
-            const int p8 = tile * WTILE + 8 * h, pg = locate(p8, off);
-            const bool there = pg >= 0 && p8 + g < T;
-            const char *row = kh + pg * p.k_nb3 + (off + g) * p.k_nb1 + 16 * t;
+            const int p8 = min(at + 8 * h, end - 1), j = page(p8), pg = s_page[j - first_page];
+            const bool there = pg >= 0 && at + 8 * h + g < end;
+            const char *row = kh + pg * p.k_nb3 + (int64_t)(at + 8 * h + g - j * p.page) * p.k_nb1 + 16 * t;
 #pragma unroll
             for (int c = 0; c < C; ++c)
-                k[h][c] = there ? *reinterpret_cast<const uint4 *>(row + 64 * c) : make_uint4(0, 0, 0, 0);
+                k[h][c] = there ? stream(row + 64 * c) : make_uint4(0, 0, 0, 0);
         }
     };
-
     int parity = 0;
     for (int r0 = 0; r0 < rows; r0 += RB, parity ^= 1) {
-        // the block's queries, and what their scores are multiplied by (with log2 e)
-        Queries<D, NB, QF16> q;
-        float factor[NB][2];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int r = r0 + 8 * b + g, i = group(min(r, rows - 1)), h = hk * a.G + min(r, rows - 1) - i * a.G;
-            const char *row = a.q + i * a.q_nb1 + h * a.q_nb2 + s * a.q_nb3;
-            float f = a.scale * 1.4426950408889634f;
-            if (QF16) {
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-                    q.hi[b][c] = r < rows ? *reinterpret_cast<const uint4 *>(row + 64 * c + 16 * t) : make_uint4(0, 0, 0, 0);
-            } else {
-                float v[C][8], most = 0.0f;
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-#pragma unroll
-                    for (int e = 0; e < 8; e += 4) {
-                        const float4 x = r < rows ? *reinterpret_cast<const float4 *>(row + 128 * c + 32 * t + 4 * e) : make_float4(0, 0, 0, 0);
-                        v[c][e] = x.x, v[c][e + 1] = x.y, v[c][e + 2] = x.z, v[c][e + 3] = x.w;
-#pragma unroll
-                        for (int k = e; k < e + 4; ++k) most = fmaxf(most, fabsf(v[c][k]));
-                    }
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                // 2^up brings the greatest value to [2^9, 2^10): two halves of 11 bits have 22 of its bits
-                const int up = most > 0.0f && most < INFINITY ? max(-120, min(100, 9 - ilogbf(most))) : 0;
-                const float m = __int_as_float((127 + up) << 23);
-                f = f * __int_as_float((127 - up) << 23);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    __half2 hh[4], ll[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = v[c][2 * e] * m, y = v[c][2 * e + 1] * m;
-                        hh[e] = __floats2half2_rn(x, y);
-                        ll[e] = __floats2half2_rn(x - __low2float(hh[e]), y - __high2float(hh[e]));
-                    }
-                    q.hi[b][c] = *reinterpret_cast<uint4 *>(hh);
-                    q.lo[b][c] = *reinterpret_cast<uint4 *>(ll);
-                }
-            }
-            // the factors of this lane's columns of the product: rows 2 t, 2 t + 1 of the block
-#pragma unroll
-            for (int e = 0; e < 2; ++e) factor[b][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
-        }
-        auto scores = [&](const uint4 (&k)[2][C], float (&c4)[NB][4]) {
+        const int live = min(RB, rows - r0);
+        Block<D, QF16> q[REGS ? NB : 1];
+        float2 factor[REGS ? NB : 1];  // of this lane's columns of the product: rows 2 t, 2 t + 1 of the block
+        if (REGS) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                c4[b][0] = c4[b][1] = c4[b][2] = c4[b][3] = 0.0f;
+                q[b] = load_block<D, QF16>(a, group, r0 + 8 * b + g, rows, hk, s);
+                factor[b] = make_float2(__shfl_sync(0xffffffffu, q[b].factor, 8 * t), __shfl_sync(0xffffffffu, q[b].factor, 8 * t + 4));
+            }
+        } else {
+            for (int b = warp; b < NB; b += WW) {
+                const Block<D, QF16> x = load_block<D, QF16>(a, group, r0 + 8 * b + g, rows, hk, s);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    if (!QF16) {
-                        mma_f16(c4[b], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q.lo[b][c].x, q.lo[b][c].y);
-                        mma_f16(c4[b], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q.lo[b][c].z, q.lo[b][c].w);
-                    }
-                    mma_f16(c4[b], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, q.hi[b][c].x, q.hi[b][c].y);
-                    mma_f16(c4[b], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, q.hi[b][c].z, q.hi[b][c].w);
+                    s_dyn4[(b * PARTS * C + c) * 32 + lane] = x.hi[c];
+                    if (!QF16) s_dyn4[((b * PARTS + 1) * C + c) * 32 + lane] = x.lo[c];
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c4[b][e] *= factor[b][e & 1];
+                if (t == 0) s_factor[8 * b + g] = x.factor;
             }
-        };
-        // whether the tile has positions that some nodes do not see, and whether value e of block b is such a one
-        auto edge = [&](int tile) { return tile * WTILE + WTILE - 1 > past; };
-        auto hidden = [&](int tile, int b, int e) {
-            return tile * WTILE + g + 8 * (e >> 1) > past + group(min(r0 + 8 * b + 2 * t + (e & 1), rows - 1));
-        };
-
-        // ---- m and l of the block's rows
+            __syncthreads();
+        }
         float m[NB][2], l[NB][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) m[b][e] = -INFINITY, l[b][e] = 0.0f;
-        uint4 next[2][C];
-        if (t0 + warp < t1) load_k(next, t0 + warp);
-        int kept = 0;
-        for (int tile = t0 + warp; tile < t1; tile += WW, ++kept) {
-            uint4 k[2][C];
+        // a stretch: its scores, with what they do to m and l; then, from the last one back, its weights
+        for (int step = 0; step < 2 * stretches - 1; ++step) {
+            const bool stats = step < stretches;
+            const int i = stats ? step : 2 * stretches - 2 - step;
+            const int b0 = p0 + i * a.stretch, b1 = min(b0 + a.stretch, p1);
+            if (stretches > 1 || r0 == 0) pages_of(b0, b1);
+            uint4 next[2][C];
+            if (AHEAD && b0 + warp * WTILE < b1) load_k(next, b0 + warp * WTILE, b1);
+            for (int at = b0 + warp * WTILE; at < b1; at += WW * WTILE) {
+                uint4 k[2][C];
+                if (AHEAD) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int c = 0; c < C; ++c) k[h][c] = next[h][c];
-            if (tile + WW < t1) load_k(next, tile + WW);
-            float c4[NB][4];
-            scores(k, c4);
-            if (edge(tile)) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hidden(tile, b, e)) c4[b][e] = -INFINITY;
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (kept < a.cap) s_scores[((kept * WW + warp) * NB + b) * 32 + lane] = make_float4(c4[b][0], c4[b][1], c4[b][2], c4[b][3]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float mm = fmaxf(m[b][e], fmaxf(c4[b][e], c4[b][e + 2])), z = mm == -INFINITY ? 0.0f : mm;
-                    l[b][e] = l[b][e] * ex2(m[b][e] - z) + ex2(c4[b][e] - z) + ex2(c4[b][e + 2] - z);
-                    m[b][e] = mm;
+                        for (int c = 0; c < C; ++c) k[h][c] = next[h][c];
+                    if (at + WW * WTILE < b1) load_k(next, at + WW * WTILE, b1);
+                } else {
+                    load_k(k, at, b1);
                 }
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1)
-                    join(m[b][e], l[b][e], __shfl_xor_sync(0xffffffffu, m[b][e], o), __shfl_xor_sync(0xffffffffu, l[b][e], o));
-                if (g == 0) s_warp[warp][8 * b + 2 * t + e] = make_float2(m[b][e], l[b][e]);
-            }
-        __syncthreads();
-        if (r0 == 0 && a.cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
-        if (tid < RB) {
-            float2 x = s_warp[0][tid];
-            for (int w = 1; w < WW; ++w) join(x.x, x.y, s_warp[w][tid].x, s_warp[w][tid].y);
-            if (a.cs == 1) {
-                s_ml[parity][0][tid] = x;
-            } else {
-                cg::cluster_group cl = cg::this_cluster();
-                for (int c = 0; c < a.cs; ++c) *cl.map_shared_rank(&s_ml[parity][rank][tid], c) = x;
-            }
-        }
-        if (a.cs == 1) __syncthreads();
-        else cg::this_cluster().sync();
-        if (tid < RB) {
-            float2 x = s_ml[parity][0][tid];
-            for (int c = 1; c < a.cs; ++c) join(x.x, x.y, s_ml[parity][c][tid].x, s_ml[parity][c][tid].y);
-            // 1 / l: 0 for rows of padding, and where all scores are -inf; NaN stays
-            const bool none = r0 + tid >= rows || (x.x == -INFINITY && x.y == x.y);
-            s_row[tid] = make_float2(x.x == -INFINITY ? 0.0f : x.x, none ? 0.0f : 1.0f / x.y);
-        }
-        __syncthreads();
-        float2 ml[NB][2];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) ml[b][e] = s_row[8 * b + 2 * t + e];
-
-        // ---- weights
-        kept = 0;
-        for (int tile = t0 + warp; tile < t1; tile += WW, ++kept) {
-            float c4[NB][4];
-            if (kept < a.cap) {
+                const bool edge = at + WTILE - 1 > past;  // some rows do not see all of it
+                float *to = s_scores + (at - b0 + g) * a.stride + 2 * t;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const float4 x = s_scores[((kept * WW + warp) * NB + b) * 32 + lane];
-                    c4[b][0] = x.x, c4[b][1] = x.y, c4[b][2] = x.z, c4[b][3] = x.w;
-                }
-            } else {
-                uint4 k[2][C];
-                load_k(k, tile);
-                scores(k, c4);
-            }
-            const bool all = !edge(tile);
+                    if (NB == 8 && 8 * b >= live) break;
+                    float c4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float w = 0.0f;
+                    for (int c = 0; c < C; ++c) {
+                        if (!QF16) {
+                            const uint4 lo = REGS ? q[REGS ? b : 0].lo[QF16 ? 0 : c] : s_dyn4[((b * PARTS + 1) * C + c) * 32 + lane];
+                            mma_f16(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, lo.x, lo.y);
+                            mma_f16(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, lo.z, lo.w);
+                        }
+                        const uint4 hi = REGS ? q[REGS ? b : 0].hi[c] : s_dyn4[(b * PARTS * C + c) * 32 + lane];
+                        mma_f16(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, hi.x, hi.y);
+                        mma_f16(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, hi.z, hi.w);
+                    }
+                    const float2 f = REGS ? factor[REGS ? b : 0] : *reinterpret_cast<const float2 *>(s_factor + 8 * b + 2 * t);
+                    c4[0] *= f.x, c4[1] *= f.y, c4[2] *= f.x, c4[3] *= f.y;
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (at + g + 8 * (e >> 1) > past + group(min(r0 + 8 * b + 2 * t + (e & 1), rows - 1))) c4[e] = -INFINITY;
+                    }
+                    if (8 * b + 2 * t < live) {
+                        *reinterpret_cast<float2 *>(to + 8 * b) = make_float2(c4[0], c4[1]);
+                        *reinterpret_cast<float2 *>(to + 8 * b + 8 * a.stride) = make_float2(c4[2], c4[3]);
+                    }
+                    if (stats) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float mm = fmaxf(m[b][e], fmaxf(c4[e], c4[e + 2])), z = mm == -INFINITY ? 0.0f : mm;
+                            l[b][e] = l[b][e] * ex2(m[b][e] - z) + ex2(c4[e] - z) + ex2(c4[e + 2] - z);
+                            m[b][e] = mm;
+                        }
+                    }
+                }
+            }
+            if (step == stretches - 1) {  // the rows' m and l: over the lanes, the warps, the CTAs
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float x = ex2(c4[b][2 * h + e] - ml[b][e].x) * ml[b][e].y;
-                        w += all || !hidden(tile, b, 2 * h + e) ? x : 0.0f;  // also where the row is NaN
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1)
+                            join(m[b][e], l[b][e], __shfl_xor_sync(0xffffffffu, m[b][e], o), __shfl_xor_sync(0xffffffffu, l[b][e], o));
+                        if (g == 0) s_warp[warp][8 * b + 2 * t + e] = make_float2(m[b][e], l[b][e]);
                     }
-                w += __shfl_xor_sync(0xffffffffu, w, 1);
-                w += __shfl_xor_sync(0xffffffffu, w, 2);
-                int off;
-                const int p8 = tile * WTILE + 8 * h, pg = locate(p8, off);
-                if (t == 0 && pg >= 0 && p8 + g < T) {
-                    float *at = reinterpret_cast<float *>(wh + pg * a.w_nb2) + off + g;
-                    if (r0) w += *at;
-                    else if (a.decay != 0.0f && p8 + g < past) w += a.decay * *at;
-                    *at = w;
+                __syncthreads();
+                if (r0 == 0 && a.cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
+                if (tid < RB) {
+                    float2 x = s_warp[0][tid];
+#pragma unroll
+                    for (int w = 1; w < WW; ++w) join(x.x, x.y, s_warp[w][tid].x, s_warp[w][tid].y);
+                    if (a.cs == 1) {
+                        s_ml[parity][0][tid] = x;
+                    } else {
+                        cg::cluster_group cl = cg::this_cluster();
+                        for (int c = 0; c < a.cs; ++c) *cl.map_shared_rank(&s_ml[parity][rank][tid], c) = x;
+                    }
+                }
+                if (a.cs == 1) __syncthreads();
+                else cg::this_cluster().sync();
+                if (tid < RB) {
+                    float2 x = s_ml[parity][0][tid];
+                    for (int c = 1; c < a.cs; ++c) join(x.x, x.y, s_ml[parity][c][tid].x, s_ml[parity][c][tid].y);
+                    // 1 / l: 0 where all scores are -inf; NaN stays
+                    const bool none = x.x == -INFINITY && x.y == x.y;
+                    s_row[tid] = make_float2(x.x == -INFINITY ? 0.0f : x.x, none ? 0.0f : 1.0f / x.y);
                 }
             }
+            __syncthreads();
+            if (step < stretches - 1) continue;
+            constexpr int U = 4;  // positions of a thread with their old weights under way
+            for (int base = b0 + tid; base < b1; base += U * WT) {
+                float *to[U], old[U], sum[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int at = base + u * WT;
+                    const int j = page(min(at, b1 - 1)), pg = s_page[j - first_page];
+                    to[u] = at < b1 && pg >= 0 ? reinterpret_cast<float *>(wh + pg * a.w_nb2) + (at - j * p.page) : nullptr;
+                    old[u] = to[u] && (r0 || (a.decay != 0.0f && at < past)) ? *to[u] : 0.0f;
+                    sum[u] = 0.0f;
+                }
+#pragma unroll 2
+                for (int r = 0; r < live; r += 2) {
+                    const float2 x = s_row[r], y = s_row[r + 1];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int at = min(base + u * WT, b1 - 1);
+                        const float2 v = *reinterpret_cast<const float2 *>(s_scores + (at - b0) * a.stride + r);
+                        // the first row that sees the position: what it does not see a row that is NaN does not reach
+                        const int seen = at > past ? (at - past) * a.G - r0 : 0;
+                        if (r >= seen) sum[u] += ex2(v.x - x.x) * x.y;
+                        if (r + 1 >= seen && r + 1 < live) sum[u] += ex2(v.y - y.x) * y.y;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (to[u]) *to[u] = r0 ? old[u] + sum[u] : a.decay * old[u] + sum[u];
+            }
+            __syncthreads();  // the scores, and at the end s_warp and s_row, are written again
         }
-        __syncthreads();  // s_warp and s_row are written again
     }
 }
 
 template <int D, int NB, bool QF16>
 int launch_weights(oasr_backend *be, Weights a, const KvPages &p, const KvSeqs &sq, int S) {
-    // scores of a warp's tiles in 96 KB: two CTAs per SM
-    constexpr int SMEM = 96 << 10;
-    a.cap = SMEM / (WW * NB * 32 * (int)sizeof(float4));
+    constexpr int HELD = NB <= 2 ? 0 : NB * (QF16 ? 1 : 2) * (D / 32) * 32 * 16;
+    constexpr int SMEM = (NB == 8 ? 84 : NB == 4 ? 92 : 100) << 10;  // two CTAs per SM, with what is static
+    const int rows = (int)std::min<int64_t>((int64_t)sq.N * a.G, 8 * NB);
+    // 8-byte accesses of neighbouring positions fall on different banks if half the stride is odd
+    a.stride = (rows + 1) / 2 * 2;
+    if (a.stride % 4 == 0) a.stride += 2;
+    a.stretch = std::min((SMEM - HELD) / (4 * a.stride) / WTILE * WTILE, (WPAGES - 2) * 8 / WTILE * WTILE);
     static OncePerDevice once;
     cudaError_t e = (cudaError_t)once(be->device, [] {
         const cudaError_t x = cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         return x != cudaSuccess ? x : cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "attn_weights attribute", __LINE__);
-    const int64_t items = (int64_t)S * a.HKV, tiles = ((int64_t)sq.MP * p.page + WTILE - 1) / WTILE;
-    a.cs = 16;
-    while (a.cs > 1 && (items * a.cs > 2 * be->sm_count || tiles < a.cs)) a.cs /= 2;
+    const int64_t items = (int64_t)S * a.HKV, most = (int64_t)sq.MP * p.page;
+    // two CTAs per SM, of 128 positions (a tile per warp) at least; more where shared memory would not hold a
+    // CTA's scores, since those of all stretches but the last are computed twice (128 heads of 4001 to 8190
+    // positions: 120, 78, 50, 56 us with 1, 2, 4, 8 CTAs each)
+    const int64_t even = std::min(2 * be->sm_count / items, (most + 127) / 128), whole = (most + a.stretch - 1) / a.stretch;
+    a.cs = (int)std::max<int64_t>(1, std::min<int64_t>(16, std::max(even, whole)));
+    if (a.cs > 8 && a.cs < 16) a.cs = 8;
     if (items * a.cs > INT32_MAX) return fail_op(be, "attn_weights", "too many sequences");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * a.cs));
     cfg.blockDim = dim3(WT);
-    cfg.dynamicSmemBytes = SMEM;
+    const int64_t held = std::min<int64_t>(a.stretch, ((most + a.cs - 1) / a.cs + WTILE) / WTILE * WTILE);
+    cfg.dynamicSmemBytes = HELD + (size_t)held * a.stride * 4;
     cfg.stream = be->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -683,13 +736,14 @@ int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_te
     a.q = (const char *)q->data;
     a.q_nb1 = q->nb[1], a.q_nb2 = q->nb[2], a.q_nb3 = q->nb[3];
     a.w = (char *)weights->data, a.w_nb1 = weights->nb[1], a.w_nb2 = weights->nb[2];
-    a.HKV = (int)HKV, a.G = (int)(H / HKV);
+    a.S = (int)S, a.HKV = (int)HKV, a.G = (int)(H / HKV);
     a.scale = scale, a.decay = decay;
-    const bool two = N * a.G > 8;
-#define AW(DD, NB, Q) \
-    if (D == DD && two == (NB == 2) && f16 == Q) return launch_weights<DD, NB, Q>(be, a, p, sq, (int)S)
-    AW(64, 1, false); AW(64, 1, true); AW(64, 2, false); AW(64, 2, true);
-    AW(128, 1, false); AW(128, 1, true); AW(128, 2, false); AW(128, 2, true);
+    const int64_t rows = N * a.G;
+    const int nb = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8;
+#define AW(DD, NB) \
+    if (D == DD && nb == NB) return f16 ? launch_weights<DD, NB, true>(be, a, p, sq, (int)S) : launch_weights<DD, NB, false>(be, a, p, sq, (int)S)
+    AW(64, 1); AW(64, 2); AW(64, 4); AW(64, 8);
+    AW(128, 1); AW(128, 2); AW(128, 4); AW(128, 8);
 #undef AW
     return fail_op(be, op, "head_dim must be 64 or 128");
 }
