@@ -710,9 +710,9 @@ extern "C" {
 
 int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages, const oasr_tensor *page_table,
                            const oasr_tensor *n_past, const oasr_tensor *n_nodes, float scale, float decay, oasr_tensor *weights) {
-    int st = oasr_internal_precheck(be);
-    if (st) return st;
     const char *op = "attn_weights";
+    if (!be) return oasr_internal_precheck(be);
+    int st;
     if (!q) return fail_op(be, op, "null argument");
     KvPages p;
     KvSeqs sq;
@@ -726,12 +726,14 @@ int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_te
     if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages] with contiguous rows");
     if (!(scale == scale)) return fail_op(be, op, "scale must be a number");
     if (!(decay >= 0.0f && decay < INFINITY)) return fail_op(be, op, "decay must not be negative, and finite");
-    if (N == 0 || S == 0) return OASR_STATUS_SUCCESS;
+    if (N == 0 || S == 0) return oasr_internal_precheck(be);
     st = seqs_check(be, op, page_table, n_past, n_nodes, S, N, &sq);
     if (st) return st;
     if (N * (H / HKV) > INT32_MAX / 2) return fail_op(be, op, "too many rows");
     if (!q->data) return fail_op(be, op, "null argument");
     if (!rows16(q)) return fail_op(be, op, "rows must be 16-byte aligned");
+    st = oasr_internal_precheck(be);  // the arguments need no device
+    if (st) return st;
     Weights a = {};
     a.q = (const char *)q->data;
     a.q_nb1 = q->nb[1], a.q_nb2 = q->nb[2], a.q_nb3 = q->nb[3];
@@ -751,9 +753,9 @@ int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_te
 int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const oasr_tensor *page_table, const oasr_tensor *n_past,
                        const oasr_tensor *n_keep, int32_t n_sink, int32_t n_recent, oasr_tensor *k_pages, oasr_tensor *v_pages,
                        int32_t n_layers, oasr_tensor *n_past_out) {
-    int st = oasr_internal_precheck(be);
-    if (st) return st;
     const char *op = "kv_evict";
+    if (!be) return oasr_internal_precheck(be);
+    int st;
     if (!n_past) return fail_op(be, op, "null argument");
     KvPages p;
     KvSeqs sq;
@@ -762,13 +764,15 @@ int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const oasr_tensor
     const int64_t S = n_past->ne[0], HKV = k_pages->ne[2];
     if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages] with contiguous rows");
     if (n_sink < 0 || n_recent < 0) return fail_op(be, op, "n_sink and n_recent must not be negative");
-    if (S == 0) return OASR_STATUS_SUCCESS;
+    if (S == 0) return oasr_internal_precheck(be);
     st = seqs_check(be, op, page_table, n_past, nullptr, S, 0, &sq);
     if (st) return st;
     if (!is_vec_i32(n_keep, S) || !is_vec_i32(n_past_out, S)) return fail_op(be, op, "n_keep and n_past_out must be I32 [n_seq]");
     for (const oasr_tensor *t : {n_past, n_keep, page_table})
         if (share_values(int_rows(n_past_out), int_rows(t)))
             return fail_op(be, op, "n_past_out must not overlap an input (it is still read while it is written)");
+    st = oasr_internal_precheck(be);  // the arguments need no device
+    if (st) return st;
     Evict a = {};
     a.w = (char *)weights->data, a.w_nb1 = weights->nb[1], a.w_nb2 = weights->nb[2];
     a.n_keep = (const int *)n_keep->data, a.n_past_out = (int *)n_past_out->data;

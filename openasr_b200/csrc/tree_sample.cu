@@ -320,7 +320,7 @@ __device__ __forceinline__ Part run_max(const Row &row, const Run &run, float4 (
 // r_k of a value before it is divided by its sum, from its weight (p = w / Z) and q; inv[k]: 1 / the sum of
 // r_{k + 1}, or 0 for one without mass (the target's own probabilities then)
 __device__ __forceinline__ double residual(double w, double inv_Z, float q, const double *inv, int k) {
-    const double qq = (double)fmaxf(q, 0.0f);
+    const double qq = (double)q;
     double r = k == 0 ? w * inv_Z : fma(w, inv_Z, -qq);
     for (int i = 1; i < k; ++i) r = inv[i - 1] > 0.0 ? fma(r > 0.0 ? r : 0.0, inv[i - 1], -qq) : fma(w, inv_Z, -qq);
     return r > 0.0 ? r : 0.0;
@@ -362,16 +362,16 @@ __device__ __forceinline__ void weights(const float4 (&x)[N / 4], float ref, dou
         if (none[c]) w[c] = 0.0;
 }
 
-// The sums of r_k over the run's stretches, before r_k is divided by its sum.  CALM: weights as in run_sum,
-// those of what is 1000 octaves below or not finite 2^-1000 in the place of 0, which the sums do not show.
+// The sums of r_k over the run's stretches, before r_k is divided by its sum.  CALM: p is exp((l - at) / T) with
+// at = ref + T ln Z, and what is 1000 octaves below or not finite counts as 2^-1000, which the sums do not show.
 template <bool CALM>
-__device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const Run &run, float ref, double inv_Z, double C, uint32_t tab,
-                                         const double *inv, int k) {
+__device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const Run &run, float ref, double at, double inv_Z, double C,
+                                         uint32_t tab, const double *inv, int k) {
     const int lane = threadIdx.x & 31;
-    const float low = (float)((double)ref - LOW / C);
+    const float low = (float)((double)ref - LOW / C), calm = fminf(-low, 3.402823466e38f);
     constexpr int U = 2;
     Part mine{0.0, ref, 0};
-    float4 x[U], y[U], nx[U], ny[U];
+    float4 nx[U], ny[U];
     auto load = [&](int j) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -384,30 +384,43 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
     double acc[8] = {};
     int done = 0, i = 0;
     for (int j = run.j0; j < run.j1; j += 32 * U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = nx[u], y[u] = ny[u];
+        float4 x[U] = {nx[0], nx[1]};
+        const float f[8] = {ny[0].x, ny[0].y, ny[0].z, ny[0].w, ny[1].x, ny[1].y, ny[1].z, ny[1].w};
         if (j + 32 * U < run.j1) load(j + 32 * U);
-        const float f[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
-        double w[8] = {};
+        double r[8];  // p - q
         if (CALM) {
+            float m = abs_max3(abs_max3(x[0].x, x[0].y, x[0].z), abs_max3(x[0].w, x[1].x, x[1].y), fmaxf(fabsf(x[1].z), fabsf(x[1].w)));
+            if (__any_sync(0xffffffffu, !(m <= calm && x[0].x + x[0].y + x[0].z + x[0].w + x[1].x + x[1].y + x[1].z + x[1].w < INFINITY))) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    for (float *v : {&x[u].x, &x[u].y, &x[u].z, &x[u].w}) *v = *v > low && *v < INFINITY ? *v : low;
+            }
             const float v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
             double d[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) d[c] = (double)(v[c] > low && v[c] < INFINITY ? v[c] : low) - (double)ref;
-            exp_add(d, C, tab, w);
+            for (int c = 0; c < 8; ++c) d[c] = (double)v[c] - at, r[c] = k ? -(double)f[c] : 0.0;
+            exp_add(d, C, tab, r);
         } else {
+            double w[8];
             weights<8>(x, ref, C, tab, w);
-        }
-        if (k == 1) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const double r = fma(w[c], inv_Z, -(double)fmaxf(f[c], 0.0f));
-                acc[c] += r > 0.0 ? r : 0.0;
+            for (int c = 0; c < 8; ++c) r[c] = k ? fma(w[c], inv_Z, -(double)f[c]) : w[c] * inv_Z;
+        }
+        if (k > 1) {
+            double s[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) s[c] = r[c];
+            for (int n = 1; n < k; ++n) {
+                const double g = inv[n - 1];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s[c] = g > 0.0 ? fma(s[c] > 0.0 ? s[c] : 0.0, g, -(double)f[c]) : r[c];
             }
-        } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) acc[c] += residual(w[c], inv_Z, f[c], inv, k);
+            for (int c = 0; c < 8; ++c) r[c] = s[c];
         }
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            if (__double2hiint(r[c]) >= 0) acc[c] += r[c];
         if ((done += 32 * U) == run.step || j + 32 * U >= run.j1) {
             const double s = warp_sum(((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7])));
             if (lane == i) mine.sum = s;
@@ -420,7 +433,7 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
 }
 
 __device__ __noinline__ Part run_rest_any(Row row, Draft q, Run run, float ref, double inv_Z, double C, uint32_t tab, const double *inv, int k) {
-    return run_rest<false>(row, q, run, ref, inv_Z, C, tab, inv, k);
+    return run_rest<false>(row, q, run, ref, 0.0, inv_Z, C, tab, inv, k);
 }
 
 // running sum over the first N lanes
@@ -524,14 +537,14 @@ __device__ __forceinline__ Place find(const Sums<CS> &s, double run, double f, d
 // One cluster of CS CTAs per node; every warp takes one run of the row's vectors.  The CTAs' sums go to
 // every CTA of the cluster, which then all take the same decisions, so that the call needs no workspace
 // and no second launch; the CTA that holds the drawn value's stretch reads that stretch once more.
-template <int CS, int U>
+template <int CS, int U, bool DRAFT>
 __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) {
     namespace cg = cooperative_groups;
     constexpr int W = CS * NW;
     __shared__ Table s_table;
     __shared__ Sums<CS> s_sums;
-    __shared__ double s_inv[TREE_MAX_NODES], s_warp[NW], s_log;
-    __shared__ unsigned short s_kids[TREE_MAX_NODES];
+    __shared__ double s_inv[DRAFT ? TREE_MAX_NODES : 1], s_warp[NW], s_log;
+    __shared__ unsigned short s_kids[DRAFT ? TREE_MAX_NODES : 1];
     __shared__ int s_n_kids, s_last;
     __shared__ Try s_try[32];  // of the first children
     griddep_launch_dependents();
@@ -582,7 +595,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
         }
         return t;
     };
-    if (a.q && warp == 0 && T > 0.0f) {  // the node's children in order
+    if (DRAFT && warp == 0 && T > 0.0f) {  // the node's children in order
         int count = 0;
         for (int j0 = i + 1; j0 < n; j0 += 32) {
             const int j = j0 + lane;
@@ -643,10 +656,13 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     int rounds = 0;
     bool left = false;  // something is left of p
     double inv_Z = 0.0, total = Z;
-    if (a.q) {
+    if (DRAFT) {
         inv_Z = 1.0 / Z;
+        double at_Z = 0.0;
         auto rest = [&](int k) {
-            return calm ? run_rest<true>(row, draft, run, ref, inv_Z, C, tab, s_inv, k) : run_rest_any(row, draft, run, ref, inv_Z, C, tab, s_inv, k);
+            if (k == 1) at_Z = (double)ref + (double)T * log(Z);
+            return calm ? run_rest<true>(row, draft, run, ref, at_Z, inv_Z, C, tab, s_inv, k)
+                        : run_rest_any(row, draft, run, ref, inv_Z, C, tab, s_inv, k);
         };
         const int kids = s_n_kids;
         while (rounds < kids) {
@@ -683,12 +699,12 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     auto values = [&](int j, const float4 &v, double (&w)[4]) {
         const float4 one[1] = {v};
         weights<4>(one, ref, C, tab, w);
-        if (left) {
+        if (DRAFT && left) {
             const float4 y = j < j1 ? draft.load(row, j) : zero;
             const float g[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int c = 0; c < 4; ++c) w[c] = residual(w[c], inv_Z, g[c], s_inv, rounds);
-        } else if (rounds) {
+        } else if (DRAFT && rounds) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) w[c] *= inv_Z;
         }
@@ -748,13 +764,13 @@ bool is_rows3_f32(const oasr_tensor *t, int64_t w, int64_t N, int64_t S) {
            t->ne[3] == 1 && (t->nb[0] == 4 || w <= 1) && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0;
 }
 
-template <int CS, int U>
+template <int CS, int U, bool DRAFT>
 int launch_sample(oasr_backend *be, const Sample &a, int64_t rows) {
     if (rows * CS > INT32_MAX) return fail_op(be, "tree_sample", "too many nodes");
     if (CS > 8) {
         static OncePerDevice wide;
         const cudaError_t e = (cudaError_t)wide(be->device, [] {
-            return cudaFuncSetAttribute(tree_sample_kernel<CS, U>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            return cudaFuncSetAttribute(tree_sample_kernel<CS, U, DRAFT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         });
         if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "tree_sample attribute", __LINE__);
     }
@@ -769,7 +785,7 @@ int launch_sample(oasr_backend *be, const Sample &a, int64_t rows) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = be->pdl ? 2 : 1;
-    return launched(be, cudaLaunchKernelEx(&cfg, tree_sample_kernel<CS, U>, a, be->err_word), "tree_sample");
+    return launched(be, cudaLaunchKernelEx(&cfg, tree_sample_kernel<CS, U, DRAFT>, a, be->err_word), "tree_sample");
 }
 
 }  // namespace
@@ -778,15 +794,14 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
                                      const oasr_tensor *uniforms, const oasr_tensor *tokens, const oasr_tensor *parents,
                                      const oasr_tensor *draft_probs, const oasr_tensor *n_nodes, oasr_tensor *target,
                                      oasr_tensor *logprob) {
-    int st = oasr_internal_precheck(be);
-    if (st) return st;
     const char *op = "tree_sample";
+    if (!be) return oasr_internal_precheck(be);
     if (!logits || !uniforms || !target) return fail_op(be, op, "null argument");
     if (!draft_probs != !tokens || !draft_probs != !parents)
         return fail_op(be, op, "tokens, parents and draft_probs come together");
     const int64_t V = logits->ne[0], N = logits->ne[1], S = logits->ne[2];
     if (S < 0 || N < 0 || S > (1 << 20) || N > (1 << 24) || S * N > INT32_MAX / 16) return fail_op(be, op, "too many nodes");
-    if (S == 0 || N == 0) return OASR_STATUS_SUCCESS;
+    if (S == 0 || N == 0) return oasr_internal_precheck(be);
     if (V < 1 || V > (1 << 30)) return fail_op(be, op, "1 to 2^30 tokens");
     if (!is_rows3_f32(logits, V, N, S)) return fail_op(be, op, "logits must be F32 [n_vocab, n, n_seq] with contiguous rows");
     if (!is_rows3_f32(uniforms, 2, N, S)) return fail_op(be, op, "uniforms must be F32 [2, n, n_seq]");
@@ -808,6 +823,8 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
             if (meets(int_rows(o), t)) return fail_op(be, op, "target and logprob must not overlap an input");
     }
     if (logprob && share_values(int_rows(target), int_rows(logprob))) return fail_op(be, op, "target and logprob must not overlap");
+    const int st = oasr_internal_precheck(be);  // the arguments need no device
+    if (st) return st;
     Sample a = {};
     a.x = (const char *)logits->data, a.x_nb1 = logits->nb[1], a.x_nb2 = logits->nb[2];
     if (draft_probs) {
@@ -831,10 +848,10 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
     int cs = most;
     while (cs > 1 && (rows * cs > per_sm * be->sm_count || V < 2048 * cs)) cs /= 2;
     switch (cs) {
-    case 16: return launch_sample<16, 4>(be, a, rows);
-    case 8: return launch_sample<8, 4>(be, a, rows);
-    case 4: return launch_sample<4, 4>(be, a, rows);
-    case 2: return launch_sample<2, 8>(be, a, rows);
-    default: return launch_sample<1, 8>(be, a, rows);
+    case 16: return launch_sample<16, 4, false>(be, a, rows);
+    case 8: return draft_probs ? launch_sample<8, 4, true>(be, a, rows) : launch_sample<8, 4, false>(be, a, rows);
+    case 4: return draft_probs ? launch_sample<4, 4, true>(be, a, rows) : launch_sample<4, 4, false>(be, a, rows);
+    case 2: return draft_probs ? launch_sample<2, 8, true>(be, a, rows) : launch_sample<2, 8, false>(be, a, rows);
+    default: return draft_probs ? launch_sample<1, 8, true>(be, a, rows) : launch_sample<1, 8, false>(be, a, rows);
     }
 }
