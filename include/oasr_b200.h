@@ -371,14 +371,15 @@ int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits, const oas
 int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor *v_pages, int32_t n_layers,
                             const oasr_tensor *pairs);
 /* A bounded cache: how much attention each cached position gets, and eviction by it.  weights F32
- * [page, H_kv, n_pages] lies beside the pages (rows contiguous, other strides free): entry (j, h,
- * page id) belongs to that page's row of K/V head h.
+ * [page, H_kv, n_pages] lies beside the pages (rows contiguous, other strides free, no two entries in
+ * one place): entry (j, h, page id) belongs to that page's row of K/V head h.
  *
  * oasr_b200_attn_weights: q F32 or F16 [D, n, H, n_seq] as in oasr_b200_flash_attn_tree, the nodes
  * being a chain (node i sees the positions up to n_past + i).  To a position's entry it adds the
  * softmax weights that the position gets from all live nodes and all query heads of its K/V head,
  * after the old value was multiplied by decay; with decay 0, and for the positions from n_past on,
  * which are new, the old value is not read.  Entries of positions past the last node stay as they are.
+ * n_past + n_nodes is at most 2^30 here.
  * One call per layer and step, with the queries and the lengths of that layer's flash_attn_tree; or
  * one after the prompt with its last rows and decay 0, which scores all of it.  A row with something
  * that is not finite (a query, a K row that it sees) makes the entries of what it sees NaN; a position

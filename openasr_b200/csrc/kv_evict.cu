@@ -34,6 +34,7 @@ struct Weights {
 
 constexpr int WT = 256, WW = WT / 32;  // threads, warps
 constexpr int WTILE = 16;              // positions of a warp's tile
+constexpr int WEIGHTS_MOST = 1 << 30;  // positions of a sequence, so that steps past them stay in 32 bits
 constexpr int WPAGES = 520;            // pages of a stretch: of 8 positions and more
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -154,8 +155,9 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages 
         s = __ffs(__ballot_sync(0xffffffffu, lane < a.S && before == s)) - 1;
     }
     int past, n;
-    if (!seq_lengths(sq, s, p.page, past, n) && rank == 0 && tid == 0) atomicOr(err, ERR_BAD_INDEX);
-    if (n == 0) return;
+    const bool fits = seq_lengths(sq, s, p.page, past, n) && past <= WEIGHTS_MOST - n;
+    if (!fits && rank == 0 && tid == 0) atomicOr(err, ERR_BAD_INDEX);
+    if (n == 0 || !fits) return;
     if (a.cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int T = past + n, tiles = (T + WTILE - 1) / WTILE;
     const int per = (tiles + a.cs - 1) / a.cs * WTILE;  // positions of a CTA
@@ -699,9 +701,18 @@ int launch_evict(oasr_backend *be, Evict a, const KvPages &p, const KvSeqs &sq, 
 
 // F32 [page, H_kv, n_pages] beside the pages
 bool is_weights(const oasr_tensor *w, const oasr_tensor *k) {
-    return w && w->type == OASR_TYPE_F32 && w->data && aligned4(w) && w->ne[0] == k->ne[1] && w->ne[1] == k->ne[2] &&
-           w->ne[2] == k->ne[3] && w->ne[3] == 1 && w->nb[0] == 4 && w->nb[1] % 4 == 0 && w->nb[2] % 4 == 0 && w->nb[1] >= 0 &&
-           w->nb[2] >= 0;
+    if (!w || w->type != OASR_TYPE_F32 || !w->data || !aligned4(w) || w->ne[0] != k->ne[1] || w->ne[1] != k->ne[2] ||
+        w->ne[2] != k->ne[3] || w->ne[3] != 1 || w->nb[0] != 4 || w->nb[1] % 4 || w->nb[2] % 4)
+        return false;
+    // entries are read and written: no two of them in one place
+    int64_t extent = 4 * w->ne[0];
+    const bool pages_inside = w->nb[2] < w->nb[1];
+    for (int i : {pages_inside ? 2 : 1, pages_inside ? 1 : 2}) {
+        if (w->ne[i] == 1) continue;
+        if (w->nb[i] < extent) return false;
+        extent += (w->ne[i] - 1) * w->nb[i];
+    }
+    return true;
 }
 
 }  // namespace
@@ -723,7 +734,7 @@ int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_te
         return fail_op(be, op, "q must be F32 or F16 [D, n, H, n_seq] with H a multiple of H_kv");
     const bool f16 = q->type == OASR_TYPE_F16;
     if (q->nb[0] != (f16 ? 2 : 4)) return fail_op(be, op, "rows must be contiguous");
-    if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages] with contiguous rows");
+    if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages], rows contiguous and apart");
     if (!(scale == scale)) return fail_op(be, op, "scale must be a number");
     if (!(decay >= 0.0f && decay < INFINITY)) return fail_op(be, op, "decay must not be negative, and finite");
     if (N == 0 || S == 0) return oasr_internal_precheck(be);
@@ -762,7 +773,7 @@ int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const oasr_tensor
     st = pages_check(be, op, k_pages, v_pages, n_layers, &p);
     if (st) return st;
     const int64_t S = n_past->ne[0], HKV = k_pages->ne[2];
-    if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages] with contiguous rows");
+    if (!is_weights(weights, k_pages)) return fail_op(be, op, "weights must be F32 [page, H_kv, n_pages], rows contiguous and apart");
     if (n_sink < 0 || n_recent < 0) return fail_op(be, op, "n_sink and n_recent must not be negative");
     if (S == 0) return oasr_internal_precheck(be);
     st = seqs_check(be, op, page_table, n_past, nullptr, S, 0, &sq);

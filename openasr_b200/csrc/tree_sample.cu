@@ -381,13 +381,12 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
         }
     };
     load(run.j0);
-    double acc[8] = {};
+    double acc[4] = {};
     int done = 0, i = 0;
     for (int j = run.j0; j < run.j1; j += 32 * U) {
         float4 x[U] = {nx[0], nx[1]};
-        const float f[8] = {ny[0].x, ny[0].y, ny[0].z, ny[0].w, ny[1].x, ny[1].y, ny[1].z, ny[1].w};
+        const float4 y[U] = {ny[0], ny[1]};
         if (j + 32 * U < run.j1) load(j + 32 * U);
-        double r[8];  // p - q
         if (CALM) {
             float m = abs_max3(abs_max3(x[0].x, x[0].y, x[0].z), abs_max3(x[0].w, x[1].x, x[1].y), fmaxf(fabsf(x[1].z), fabsf(x[1].w)));
             if (__any_sync(0xffffffffu, !(m <= calm && x[0].x + x[0].y + x[0].z + x[0].w + x[1].x + x[1].y + x[1].z + x[1].w < INFINITY))) {
@@ -395,37 +394,44 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
                 for (int u = 0; u < U; ++u)
                     for (float *v : {&x[u].x, &x[u].y, &x[u].z, &x[u].w}) *v = *v > low && *v < INFINITY ? *v : low;
             }
-            const float v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-            double d[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) d[c] = (double)v[c] - at, r[c] = k ? -(double)f[c] : 0.0;
-            exp_add(d, C, tab, r);
-        } else {
-            double w[8];
-            weights<8>(x, ref, C, tab, w);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) r[c] = k ? fma(w[c], inv_Z, -(double)f[c]) : w[c] * inv_Z;
         }
-        if (k > 1) {
-            double s[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) s[c] = r[c];
-            for (int n = 1; n < k; ++n) {
-                const double g = inv[n - 1];
+        for (int u = 0; u < U; ++u) {
+            const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, f[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+            double r[4];  // p - q
+            if (CALM) {
+                double d[4];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) s[c] = g > 0.0 ? fma(s[c] > 0.0 ? s[c] : 0.0, g, -(double)f[c]) : r[c];
+                for (int c = 0; c < 4; ++c) d[c] = (double)v[c] - at, r[c] = k ? -(double)f[c] : 0.0;
+                exp_add(d, C, tab, r);
+            } else {
+                double w[4];
+                const float4 one[1] = {x[u]};
+                weights<4>(one, ref, C, tab, w);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) r[c] = k ? fma(w[c], inv_Z, -(double)f[c]) : w[c] * inv_Z;
+            }
+            if (k > 1) {
+                double s[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[c] = r[c];
+                for (int n = 1; n < k; ++n) {
+                    const double g = inv[n - 1];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[c] = g > 0.0 ? fma(s[c] > 0.0 ? s[c] : 0.0, g, -(double)f[c]) : r[c];
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) r[c] = s[c];
             }
 #pragma unroll
-            for (int c = 0; c < 8; ++c) r[c] = s[c];
+            for (int c = 0; c < 4; ++c)
+                if (__double2hiint(r[c]) >= 0) acc[c] += r[c];
         }
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-            if (__double2hiint(r[c]) >= 0) acc[c] += r[c];
         if ((done += 32 * U) == run.step || j + 32 * U >= run.j1) {
-            const double s = warp_sum(((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7])));
+            const double s = warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
             if (lane == i) mine.sum = s;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) acc[c] = 0.0;
+            for (int c = 0; c < 4; ++c) acc[c] = 0.0;
             done = 0, ++i;
         }
     }

@@ -523,3 +523,48 @@ def test_supports_op(be):
         assert be.supports_op(op, ob.describe(yes), k)
         assert not be.supports_op(op, ob.describe(no), k)
         assert not be.supports_op(op, ob.describe(yes))
+
+
+def test_lengths_past_the_limits_are_reported(be):
+    """2^30 positions for attn_weights, 2^18 for kv_evict: a table of one page over and over, which stays as it was"""
+    import torch
+
+    import openasr_b200 as ob
+
+    page, MP = 1 << 20, 1 << 11
+    k = torch.zeros(1, 1, page, 64, dtype=torch.float16, device="cuda")
+    v, w = torch.zeros_like(k), torch.full((1, 1, page), 5.0, device="cuda")
+    table = torch.zeros(1, MP, dtype=torch.int32, device="cuda")
+    out = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for past, n in (((1 << 30), 1), ((1 << 30) - 1, 2), ((1 << 31) - 130, 1)):
+        be.attn_weights(torch.zeros(1, 1, n, 64, device="cuda"), k, table, cuda(np.array([past], np.int32)), None, 0.1, 0.0, w)
+        with pytest.raises(ob.GgmlBackendError, match="out-of-range"):
+            be.synchronize()
+    for past in ((1 << 18) + 1, (1 << 31) - 129):
+        be.kv_evict(w, table, cuda(np.array([past], np.int32)), cuda(np.array([7], np.int32)), 0, 0, k, v, 1, out)
+        with pytest.raises(ob.GgmlBackendError, match="out-of-range"):
+            be.synchronize()
+        assert int(out[0]) == past
+    assert (w == 5).all()
+
+
+def test_the_longest_sequence_that_may_be_evicted(be):
+    rng = np.random.default_rng(31)
+    c = Cache(rng, 1, 0, 1, 64, 4096, [1 << 18], fill=None, spare=0)
+    w = rng.integers(0, 1 << 16, (c.P, 1, 4096)).astype(np.float32)
+    same_after(be, c, w, [100001], 3, 1000)
+
+
+@pytest.mark.parametrize("S", [32, 33, 70])
+def test_many_sequences_of_all_lengths(be, S):
+    """their order by length is worked out by one warp up to 32 of them"""
+    rng = np.random.default_rng(S)
+    c = Cache(rng, S, 2, 2, 64, 16, rng.integers(0, 300, S))
+    c.past[3] = c.past[4]
+    q = rng.standard_normal((S, 4, 2, 64)).astype(np.float32)
+    old = entries(rng, c)
+    for s in range(S):
+        for p in range(c.past[s], c.past[s] + 2):
+            c.k[c.table[s, p // 16], :, p % 16] = rng.standard_normal((2, 64)).astype(np.float16)
+    want, tol = added64(c, q, [2] * S, 0.125, 1.0, old)
+    check(run_weights(be, c, q, None, 0.125, 1.0, old), want, tol)

@@ -110,6 +110,7 @@ NAN, INF = float("nan"), float("inf")
     (sample, dict(x=lambda a: at(a["x"], nb1=4 * 53, nb2=4 * 400))),
     (sample, dict(t=lambda a: at(a["t"], data=a["u"].data + 4096))),
     (weights, {}), (weights, dict(live=None, decay=0.0)), (weights, dict(q=lambda a: h(2, 4, 3, 64))),
+    (weights, dict(w=lambda a: at(a["w"], nb1=384, nb2=64))), (weights, dict(w=lambda a: at(a["w"], nb1=68, nb2=132))),
     (evict, {}), (evict, dict(L=3)), (evict, dict(sink=5, recent=7)),
 ])
 def test_calls_in_order_reach_the_device(be, call, change):
@@ -146,7 +147,9 @@ def test_calls_in_order_reach_the_device(be, call, change):
     (weights, dict(k=lambda a: h(6, 2, 16, 96), q=lambda a: f(2, 4, 3, 96)), "64 or 128"),
     (weights, dict(w=lambda a: f(6, 2, 17)), "weights must be"), (weights, dict(w=lambda a: f(7, 2, 16)), "weights must be"),
     (weights, dict(w=lambda a: h(6, 2, 16)), "weights must be"), (weights, dict(w=lambda a: at(a["w"], nb0=8)), "weights must be"),
-    (weights, dict(w=lambda a: at(a["w"], nb1=-64)), "weights must be"), (weights, dict(w=lambda a: at(a["w"], data=a["w"].data + 2)), "weights must be"),
+    (weights, dict(w=lambda a: at(a["w"], nb1=-64)), "weights must be"), (weights, dict(w=lambda a: at(a["w"], nb1=0)), "weights must be"),
+    (weights, dict(w=lambda a: at(a["w"], nb2=64)), "weights must be"), (weights, dict(w=lambda a: at(a["w"], nb1=60, nb2=600)), "weights must be"),
+    (weights, dict(w=lambda a: at(a["w"], nb1=380, nb2=64)), "weights must be"), (weights, dict(w=lambda a: at(a["w"], data=a["w"].data + 2)), "weights must be"),
     (weights, dict(scale=NAN), "scale"), (weights, dict(decay=-1.0), "decay"), (weights, dict(decay=NAN), "decay"), (weights, dict(decay=INF), "decay"),
     (weights, dict(table=lambda a: i(3, 3)), "page_table"), (weights, dict(past=lambda a: i(3)), "n_past"), (weights, dict(live=lambda a: f(2)), "n_nodes"),
     (evict, dict(past=None), "null argument"), (evict, dict(w=None), "weights must be"), (evict, dict(keep=None), "n_keep"),
