@@ -54,8 +54,8 @@ constexpr int STEPS = 256, COPIES = 16;
 constexpr double LN2 = 0.69314718055994530942;
 constexpr double LOW = 1000 * STEPS;   // steps below the reference: a weight under 2^-1000, left out
 constexpr double HIGH = 800 * STEPS;   // steps above it: a new reference is taken
-constexpr double ROOM = 300 * STEPS;
-constexpr double MOST = 1e6 * STEPS;   // reference / T in steps up to which numbers of 32 bits are fine enough to hold the reference less 1000 T
+constexpr double ROOM = 300 * STEPS;   // a maximum in steps up to which weights are taken relative to exp(0)
+constexpr double MOST = 1e6 * STEPS;   // a reference in steps up to which 32 bits resolve what lies LOW below it
 
 struct Table {
     double v[STEPS][COPIES];
@@ -202,14 +202,19 @@ __device__ __forceinline__ float abs_max3(float a, float b, float c) {
     return m;
 }
 
-// The run in one pass, relative to exp(ref / T); ref is 0 as long as the row's values are of the common
-// size (ROOM), so that no maximum has to be known first, the runs' sums need no scaling to one another,
-// and the subtraction is left out.  A value far above it makes the tile's maximum the reference.  Values
+// The run in one pass, relative to exp(ref / T); ref is 0 as long as the values are of the common size
+// (ROOM), so that no maximum has to be known first, the runs' sums need no scaling to one another, and
+// the subtraction is left out.  A value far above it makes the tile's maximum the reference.  Values
 // 1000 octaves below it and -inf count as 2^-1000; +inf, NaN and a reference too large (a temperature of
 // some 1e-5 and less) are left to run_sum_any.  The next tile is on its way while one is summed.
 template <int U>
-__device__ __forceinline__ Part run_sum(const Row &row, const Run &run, float4 (&a)[U], float ref, double C, uint32_t tab) {
+__device__ __forceinline__ Part run_sum(const Row &row, const Run &run, float4 (&a)[U], double C, uint32_t tab) {
     const int lane = threadIdx.x & 31;
+    float ref = -INFINITY;  // the first tile's maximum, or 0 where that leaves room on both sides
+#pragma unroll
+    for (int u = 0; u < U; ++u) ref = fmaxf(ref, fmaxf(fmaxf(a[u].x, a[u].y), fmaxf(a[u].z, a[u].w)));
+    ref = warp_max(ref);
+    if (fabs((double)ref * C) <= ROOM) ref = 0.0f;
     constexpr int G = 4;    // values at a time
     float low, high, calm;  // between -calm and calm lies nothing under low or over high
     double acc[G] = {};
@@ -543,6 +548,12 @@ __device__ __forceinline__ Place find(const Sums<CS> &s, double run, double f, d
 // One cluster of CS CTAs per node; every warp takes one run of the row's vectors.  The CTAs' sums go to
 // every CTA of the cluster, which then all take the same decisions, so that the call needs no workspace
 // and no second launch; the CTA that holds the drawn value's stretch reads that stretch once more.
+// Many nodes are bound by issue: a 64-bit instruction takes the slots of two, which leaves 4.5 values per
+// clock and SM (1952 nodes of 151936: 266 us, 4.1 TB/s; a loop of nothing but loads, weights and sum takes
+// 215).  CTAs that take one node after another with the next one's first tile ahead were slower (300 to
+// 324: the nodes are then dealt out evenly, not as CTAs end), and so were three CTAs per SM (272).  A few
+// nodes are a chain of latencies: 2700 cycles to the first values, 2500 for a warp's tile, 2400 to gather
+// the sums over a cluster, 2000 for the drawn value (one token of 51866: 8.3 us).
 template <int CS, int U, bool DRAFT>
 __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) {
     namespace cg = cooperative_groups;
@@ -569,7 +580,6 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float4 first[U];
     load_tile(first, row, run.j0, run.j1, lane);
-    const float4 head = lane < row.vectors() ? row.load(lane) : none;
     const int n = a.n_nodes ? a.n_nodes[s] : a.N;
     const float T = a.temp ? a.temp[s] : 1.0f;
     const float u1 = a.u[s * a.u_ld2 + i * a.u_ld1 + 1];
@@ -643,12 +653,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
         return;
     }
     const double inv_T = 1.0 / (double)T, C = STEPS / LN2 * inv_T;
-    float guess = -INFINITY;
-    for (float f : {head.x, head.y, head.z, head.w})
-        if (finite(f)) guess = fmaxf(guess, f);
-    guess = warp_max(guess);
-    // 0, as long as that leaves room on both sides
-    const Part mine = run_sum(row, run, first, fabs((double)guess * C) <= ROOM ? 0.0f : guess, C, tab);
+    const Part mine = run_sum(row, run, first, C, tab);
     if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
     double Z, upto, f;
     float ref;
@@ -846,10 +851,10 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
     a.N = (int)N, a.V = (int)V;
     const int64_t rows = S * N;
     // CTAs per node: enough of them for the SMs, of at least 2048 values each.  Without a draft two per SM (8
-    // nodes of 151936: 10.3 us with 16 CTAs each, 12.4 with 8, 16.5 with 4; 1952 nodes: 272 us with one, 324
+    // nodes of 151936: 10.3 us with 16 CTAs each, 12.4 with 8, 16.5 with 4; 1952 nodes: 266 us with one, 324
     // with two).  With one, nodes whose children are rejected take three times as long as the others, and
-    // more and smaller CTAs even that out (64 nodes: 39 us with 4 or 8 each, 51 with 16; 124 of 51866: 70, 41,
-    // 38 and 49 us with 2, 4, 8 and 16).
+    // more and smaller CTAs even that out (64 nodes: 39 us with 4, 38 with 8, 51 with 16; 124 of 51866: 48, 33
+    // and 31 us with 2, 4 and 8).
     const int most = draft_probs ? 8 : 16, per_sm = draft_probs ? 8 : 2;
     int cs = most;
     while (cs > 1 && (rows * cs > per_sm * be->sm_count || V < 2048 * cs)) cs /= 2;
