@@ -354,11 +354,15 @@ int launch_weights(oasr_backend *be, Weights a, const KvPages &p, const KvSeqs &
     a.stride = (rows + 1) / 2 * 2;
     if (a.stride % 4 == 0) a.stride += 2;
     a.stretch = std::min((SMEM - HELD) / (4 * a.stride) / WTILE * WTILE, (WPAGES - 2) * 8 / WTILE * WTILE);
-    static OncePerDevice once;
-    cudaError_t e = (cudaError_t)once(be->device, [] {
-        const cudaError_t x = cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-        return x != cudaSuccess ? x : cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static OncePerDevice smem;
+    cudaError_t e = (cudaError_t)smem(be->device, [] {
+        return cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     });
+    static OncePerDevice wide;
+    if (e == cudaSuccess)
+        e = (cudaError_t)wide(be->device, [] {
+            return cudaFuncSetAttribute(attn_weights_kernel<D, NB, QF16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        });
     if (e != cudaSuccess) return oasr_internal_cuda_fail(be, e, "attn_weights attribute", __LINE__);
     const int64_t items = (int64_t)S * a.HKV, most = (int64_t)sq.MP * p.page;
     // two CTAs per SM, of 128 positions (a tile per warp) at least; more where shared memory would not hold a

@@ -215,12 +215,12 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return status([&] { return s_kv_evict(at.be, x[0].p, x[1].p, x[2].p, x[3].p, sink, recent, y[0].p, y[1].p, layers, z[0].p); });
 }
 
-// bind(unsupported, addresses of the C functions in the order below)
+// bind(unsupported, addresses of the C functions in the order below: the first four, or all)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-    constexpr int N = 7;
-    if (!count(n, 1 + N)) return nullptr;
-    void *f[N];
-    for (int i = 0; i < N; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
+    constexpr int FEW = 4, ALL = 7;
+    if (n != 1 + FEW && !count(n, 1 + ALL)) return nullptr;
+    void *f[ALL];
+    for (int i = 0; i < n - 1; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(a[0]);
     Py_XSETREF(s_unsupported, a[0]);
@@ -228,9 +228,11 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     s_flash_attn_tree = reinterpret_cast<decltype(s_flash_attn_tree)>(f[1]);
     s_tree_commit = reinterpret_cast<decltype(s_tree_commit)>(f[2]);
     s_kv_pages_copy = reinterpret_cast<decltype(s_kv_pages_copy)>(f[3]);
-    s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
-    s_attn_weights = reinterpret_cast<decltype(s_attn_weights)>(f[5]);
-    s_kv_evict = reinterpret_cast<decltype(s_kv_evict)>(f[6]);
+    if (n == 1 + ALL) {
+        s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
+        s_attn_weights = reinterpret_cast<decltype(s_attn_weights)>(f[5]);
+        s_kv_evict = reinterpret_cast<decltype(s_kv_evict)>(f[6]);
+    }
     Py_RETURN_NONE;
 }
 

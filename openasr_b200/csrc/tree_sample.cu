@@ -78,7 +78,7 @@ __device__ __forceinline__ void exp_add(const double (&d)[N], double C, uint32_t
     for (int i = 0; i < N; ++i) z[i] = fma(d[i], C, MAGIC);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-        asm("ld.shared.f64 %0, [%1];" : "=d"(v[i]) : "r"((__double2loint(z[i]) & (STEPS - 1)) * (COPIES * 8) + tab));
+        asm volatile("ld.shared.f64 %0, [%1];" : "=d"(v[i]) : "r"((__double2loint(z[i]) & (STEPS - 1)) * (COPIES * 8) + tab));
 #pragma unroll
     for (int i = 0; i < N; ++i) r[i] = MAGIC - z[i];
 #pragma unroll
