@@ -59,4 +59,20 @@ inline bool share_values(const IntRows &a, const IntRows &b) {
     return false;
 }
 
+// F32 [page, H_kv, n_pages] beside the pages
+inline bool is_weights(const oasr_tensor *w, const oasr_tensor *k) {
+    if (!w || w->type != OASR_TYPE_F32 || !w->data || !aligned4(w) || w->ne[0] != k->ne[1] || w->ne[1] != k->ne[2] ||
+        w->ne[2] != k->ne[3] || w->ne[3] != 1 || w->nb[0] != 4 || w->nb[1] % 4 || w->nb[2] % 4)
+        return false;
+    // entries are read and written: no two of them in one place
+    int64_t extent = 4 * w->ne[0];
+    const bool pages_inside = w->nb[2] < w->nb[1];
+    for (int i : {pages_inside ? 2 : 1, pages_inside ? 1 : 2}) {
+        if (w->ne[i] == 1) continue;
+        if (w->nb[i] < extent) return false;
+        extent += (w->ne[i] - 1) * w->nb[i];
+    }
+    return true;
+}
+
 }  // namespace oasr
