@@ -568,3 +568,97 @@ def test_many_sequences_of_all_lengths(be, S):
             c.k[c.table[s, p // 16], :, p % 16] = rng.standard_normal((2, 64)).astype(np.float16)
     want, tol = added64(c, q, [2] * S, 0.125, 1.0, old)
     check(run_weights(be, c, q, None, 0.125, 1.0, old), want, tol)
+
+
+# ---- more rows than fit into registers: groups of rows, scores kept or not ------------------------
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("S,N,H,HKV,D,page,past", [
+    (1, 17, 2, 2, 128, 8, [3]),                 # one row more than the registers hold
+    (2, 12, 6, 3, 64, 24, [200, 0]),            # 24 and fewer of 64 values
+    (2, 25, 4, 4, 64, 16, [100, 300]),          # 25
+    (1, 11, 8, 4, 128, 16, [611]),              # 22
+    (3, 13, 16, 2, 128, 16, [901, 17, 333]),    # 104: two groups of 52
+    (2, 61, 8, 1, 64, 16, [1700, 400]),         # 488: eight groups over the CTAs of a cluster
+    (50, 10, 32, 4, 128, 64, [7 * s for s in range(50)]),  # 80, a CTA per head
+    (7, 33, 15, 5, 128, 40, [257] * 7),         # 99
+])
+def test_many_rows(be, S, N, H, HKV, D, page, past, f16):
+    rng = np.random.default_rng(S * 100 + N)
+    c = Cache(rng, S, N, HKV, D, page, past)
+    q = rng.standard_normal((S, H, N, D)).astype(np.float16 if f16 else np.float32)
+    live = np.array([N if s % 3 == 0 else rng.integers(0, N + 1) for s in range(S)], np.int32)
+    for s in range(S):
+        for p in range(c.past[s] + live[s], c.past[s] + N):
+            c.k[c.table[s, p // page], :, p % page] = np.nan
+    old = entries(rng, c)
+    want, tol = added64(c, q, live, 0.1, 0.75, old)
+    got = run_weights(be, c, q, live, 0.1, 0.75, old, f16=f16)
+    check(got, want, tol)
+    np.testing.assert_array_equal(got, run_weights(be, c, q, live, 0.1, 0.75, old, f16=f16))
+
+
+@pytest.mark.parametrize("N,H,D,past,decay", [(20, 4, 128, 30011, 1.0), (20, 4, 128, 83009, 0.5), (7, 4, 64, 83009, 0.0)])
+def test_many_rows_of_a_long_cache(be, N, H, D, past, decay):
+    """scores of a part of the positions kept; sums too many to keep"""
+    rng = np.random.default_rng(past)
+    c = Cache(rng, 1, N, 1, D, 128, [past], spare=0)
+    q = rng.standard_normal((1, H, N, D)).astype(np.float32)
+    old = entries(rng, c)
+    want, tol = added64(c, q, [N], 0.1, decay, old)
+    check(run_weights(be, c, q, None, 0.1, decay, old), want, tol)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("D,N,HKV", [(128, 20, 1), (64, 45, 1), (128, 36, 2)])
+def test_what_is_not_finite_stays_with_its_row_of_many(be, bad, f16, D, N, HKV):
+    rng = np.random.default_rng(D + N)
+    c = Cache(rng, 2, N, HKV, D, 16, [300, 20])
+    q = rng.standard_normal((2, 2, N, D)).astype(np.float16 if f16 else np.float32)
+    row = N - 3
+    q[0, 0, row, 7] = bad                                        # sees positions 0 .. 300 + row
+    c.k[c.table[1, 5 // 16], :, 5 % 16, 3] = bad                 # with finite queries a score of +-inf, or NaN
+    got = run_weights(be, c, q, None, 0.125, 0.0, entries(rng, c), f16=f16)
+    at = lambda s, h, n: got[c.table[s, np.arange(n) // 16], h, np.arange(n) % 16]  # noqa: E731
+    assert np.isnan(at(0, 0, 300 + N)[: 301 + row]).all() and np.isfinite(at(0, 0, 300 + N)[301 + row:]).all()
+    if HKV == 2:
+        assert np.isfinite(at(0, 1, 300 + N)).all()
+    if math.isnan(bad):
+        assert np.isnan(at(1, 0, 20 + N)).all()
+
+
+def test_a_key_of_minus_inf_gets_nothing_from_many_rows(be):
+    """nor do rows of padding, whose products with it are NaN, spoil it"""
+    rng = np.random.default_rng(21)
+    N, at = 18, 77
+    c = Cache(rng, 1, N, 1, 128, 16, [500])
+    q = rng.standard_normal((1, 1, N, 128)).astype(np.float16)
+    q[..., 9] = np.abs(q[..., 9]) + 1
+    key = c.k[c.table[0, at // 16], 0, at % 16]
+    key[:] = 0
+    old = entries(rng, c)
+    _, tol = added64(c, q, [N], 0.1, 0.0, old)  # of the others, which gain less than 1 part in 2 without it
+    key[9] = -65504                             # times 1 or more: e^-6550 of the row
+    want, _ = added64(c, q, [N], 0.1, 0.0, old)
+    key[9] = -np.inf
+    got = run_weights(be, c, q, None, 0.1, 0.0, old, f16=True)
+    assert got[c.table[0, at // 16], 0, at % 16] == 0
+    p = np.delete(np.arange(500 + N), at)
+    pg, off = c.table[0, p // 16], p % 16
+    assert (np.abs(got[pg, 0, off] - want[pg, 0, off]) <= 2 * tol[pg, 0, off]).all()
+
+
+def test_pages_out_of_range_are_reported_with_many_rows(be):
+    import openasr_b200 as ob
+
+    rng = np.random.default_rng(22)
+    c = Cache(rng, 2, 20, 2, 128, 16, [140, 20])
+    q, old = rng.standard_normal((2, 4, 20, 128)).astype(np.float32), entries(rng, c)
+    want = run_weights(be, c, q, None, 0.1, 1.0, old)
+    other = c.table[1, :2].copy()
+    c.table[0, 3], c.table[0, 8] = c.P, -1
+    with pytest.raises(ob.GgmlBackendError, match="out-of-range"):
+        w = cuda(old)
+        be.attn_weights(cuda(q), c.device()[0], cuda(c.table), cuda(c.past), None, 0.1, 1.0, w)
+        be.synchronize()
+    np.testing.assert_array_equal(w.cpu().numpy()[other].astype(np.float64), want[other])
