@@ -134,7 +134,7 @@ __device__ __forceinline__ int sequence_of(const Weights &a, const KvSeqs &sq, i
 // For up to 16 rows, whose queries stay in registers (24 of 64 values; the kernel below takes 18.5 us where
 // this one takes 24.6 with 20 rows of 128 values at 0 to 1490 positions, and 24.2 to 18.5 with 12 rows of 64
 // at 3454 to 6908).  Long caches are bound by HBM while a CTA multiplies (27000 of the 40000 cycles of each of
-// 512 CTAs, two per SM: 16 sequences of 4001 to 8190 positions take 49 us, 4.2 TB/s); the rest is the start,
+// 512 CTAs, two per SM: 16 sequences of 4001 to 8190 positions take 47 to 49 us, 4.3 TB/s); the rest is the start,
 // the exchange (2800) and the weights (4200).  Short calls are a chain of five round trips: 6.3 us for one
 // token.  K fetched to L2 ahead took 56 us, three CTAs per SM 51, every warp's m and l sent to every CTA 68.
 template <int D, int NB, bool QF16>
@@ -626,7 +626,7 @@ int launch_weights(oasr_backend *be, Weights a, const KvPages &p, const KvSeqs &
     // positions: 120, 78, 50, 56 us with 1, 2, 4, 8 CTAs each)
     const int64_t even = std::min(2 * be->sm_count / items, (most + 127) / 128), whole = (most + a.stretch - 1) / a.stretch;
     a.cs = (int)std::max<int64_t>(1, std::min<int64_t>(16, std::max(even, whole)));
-    if (a.cs > 8 && a.cs < 16) a.cs = 8;
+    if (a.cs > 8 && a.cs < 16) a.cs = 8;  // 24 heads of 0 to 4661 positions: 16.5 us with 12, 12.4 with 8 (32 of 9755 to 19511: 35 with 9, 39)
     const int64_t held = std::min<int64_t>(a.stretch, ((most + a.cs - 1) / a.cs + WTILE) / WTILE * WTILE);
     return launch_cluster(be, attn_weights_kernel<D, NB, QF16>, items, (size_t)held * a.stride * 4, a, p, sq);
 }
