@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
         return;
     }
     const Draft draft{q, (((uintptr_t)q ^ (uintptr_t)logits) & 15) == 0};
-    const bool calm = fabs((double)ref * C) <= MOST;
+    const bool calm = fabs((double)ref * C) <= MOST && LOW / C < 3e38;  // low (run_rest) has to be a number
     int rounds = 0;
     bool left = false;  // something is left of p
     double inv_Z = 0.0, total = Z;

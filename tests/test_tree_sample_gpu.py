@@ -219,6 +219,22 @@ def test_a_residual_without_mass_leaves_the_targets_probabilities(be):
     same(run(be, x, temp, u, None, tok, par, q), want64(x, temp, u, [N] * S, tok, par, q))
 
 
+@pytest.mark.parametrize("T", [1e-30, 1e-4, 1e30, 3e35, 1e37, 3e38])
+def test_rejection_at_any_temperature(be, T):
+    """and with logits that are not finite, a row's end inside a tile"""
+    rng = np.random.default_rng(5)
+    S, N, V = 6, 7, 3001
+    x, q, tok, par = chains_and_trees(rng, S, N, V, "tree")
+    x[0, :, ::3] = -np.inf
+    x[1, :, 1::5] = np.nan
+    x[2, :, ::7] = np.inf
+    x[3] *= 1e30
+    q = softmax(rng.standard_normal(x.shape).astype(np.float32))
+    u = rng.random((S, N, 2), np.float32)
+    temp = np.full(S, T, np.float32)
+    same(run(be, x, temp, u, None, tok, par, q), want64(x, temp, u, [N] * S, tok, par, q))
+
+
 def test_accepted_tokens_are_distributed_as_the_targets(be):
     """65536 sequences with one drafted child: the token after the root is distributed as p, whatever the
     draft's q (five standard deviations of a count at fixed seeds)"""
