@@ -373,6 +373,10 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
 /* A bounded cache: how much attention each cached position gets, and eviction by it.  weights F32
  * [page, H_kv, n_pages] lies beside the pages (rows contiguous, other strides free, no two entries in
  * one place): entry (j, h, page id) belongs to that page's row of K/V head h.
+ * Both operators write what belongs to a sequence's own positions: no page may be in the rows of two
+ * sequences of an attn_weights call (its entries would be those of one or the other), and none that
+ * another sequence holds in the rows of one that kv_evict shortens (instead of a fork, a sequence that is
+ * opened and extended, its pages filled by oasr_b200_kv_pages_copy; entries are not copied).
  *
  * oasr_b200_attn_weights: q F32 or F16 [D, n, H, n_seq] as in oasr_b200_flash_attn_tree, the nodes
  * being a chain (node i sees the positions up to n_past + i).  To a position's entry it adds the

@@ -747,7 +747,8 @@ class Backend:
 
     def attn_weights(self, q, k_pages, page_table, n_past, n_nodes, scale: float, decay: float, weights) -> None:
         """Add the attention that each position gets from the nodes q f32|f16 [S, H, n, D] (a chain) to its
-        entry of weights f32 [P, H_kv, page], old entries times decay (0: not read)."""
+        entry of weights f32 [P, H_kv, page], old entries times decay (0: not read).  No two sequences of
+        a call share a page."""
         self._check((_OPS or _ops()).attn_weights((self.handle.value or 0, self.ordinal), q, k_pages, page_table, n_past,
                                                   n_nodes, scale, decay, weights))
 
@@ -755,7 +756,8 @@ class Backend:
                  n_past_out) -> None:
         """Keep n_keep i32 [S] positions of each longer sequence -- the first n_sink, the last n_recent and
         the greatest weights f32 [n_layers * P, H_kv, page] between -- and move their rows to the front of
-        pages f16 [n_layers * P, H_kv, page, D], every layer and head for itself; n_past_out i32 [S]."""
+        pages f16 [n_layers * P, H_kv, page, D], every layer and head for itself; n_past_out i32 [S].  The
+        pages of a sequence that is shortened are held by no other."""
         self._check((_OPS or _ops()).kv_evict((self.handle.value or 0, self.ordinal), weights, page_table, n_past, n_keep, n_sink,
                                               n_recent, k_pages, v_pages, n_layers, n_past_out))
 
