@@ -353,8 +353,9 @@ int oasr_b200_tree_commit(oasr_backend *be, const oasr_tensor *tokens, const oas
  * that the children of node c were drawn from, one after the other and each on its own.  They
  * are then accepted by rejection: with r = p, child j in ascending order becomes the target
  * if uniforms[0] of j times draft_probs[tokens[j]] is less than r(tokens[j]); otherwise r becomes
- * max(r - draft_probs, 0) over its sum (p, if that sum is 0).  When all children are rejected the
- * target is drawn from r as from p above, and is none of their tokens.  So the tokens that
+ * max(r - draft_probs, 0) over its sum (p, if that sum is 0).  A difference within the roundings of r,
+ * 2^-40 of it, counts as 0.  When all children are rejected the target is drawn from r as from p above,
+ * and, unless that is p once more, is none of their tokens.  So the tokens that
  * tree_commit then accepts are distributed as if each had been sampled from the model alone.
  * (A draft without probabilities needs none of this: a child is accepted if it is the token
  * drawn.)  Sums are of 64 bits.  What cannot be drawn from -- a temperature or a uniform number

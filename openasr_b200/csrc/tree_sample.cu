@@ -322,13 +322,34 @@ __device__ __forceinline__ Part run_max(const Row &row, const Run &run, float4 (
     return Part{0.0, best, at};
 }
 
-// r_k of a value before it is divided by its sum, from its weight (p = w / Z) and q; inv[k]: 1 / the sum of
-// r_{k + 1}, or 0 for one without mass (the target's own probabilities then)
-__device__ __forceinline__ double residual(double w, double inv_Z, float q, const double *inv, int k) {
-    const double qq = (double)q;
-    double r = k == 0 ? w * inv_Z : fma(w, inv_Z, -qq);
-    for (int i = 1; i < k; ++i) r = inv[i - 1] > 0.0 ? fma(r > 0.0 ? r : 0.0, inv[i - 1], -qq) : fma(w, inv_Z, -qq);
-    return r > 0.0 ? r : 0.0;
+// A weight is good to 2^-42.  What a difference leaves of m, if it is more than that error: above 2^-40 of m.
+__device__ __forceinline__ double left_of(double m, double difference) {
+    return __double2hiint(difference) > max(__double2hiint(m) - (40 << 20), 0) ? difference : 0.0;
+}
+
+// r_k of values, k >= 1, from their weights w and q, before it is divided by its sum: r_1 = w - q Z, in units of
+// Z, so that nothing is left where p = q = 1; r_{n + 1} = r_n inv[n - 1] - q, inv[n - 1] being 1 / the sum of r_n,
+// or 0 for one without mass (then once more from p).  The sums and the draw both have their values from
+// here: what has a sum has a value that it came from.
+template <int N>
+__device__ __forceinline__ void residual(double (&w)[N], double Z, const float (&q)[N], const double *inv, int k) {
+    double r[N], m[N];  // m: w in the units of r
+#pragma unroll
+    for (int c = 0; c < N; ++c) r[c] = left_of(w[c], fma(-(double)q[c], Z, w[c]));
+    if (k > 1) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) m[c] = w[c];
+        for (int n = 1; n < k; ++n) {
+            const double g = inv[n - 1];
+#pragma unroll
+            for (int c = 0; c < N; ++c) {
+                m[c] = g > 0.0 ? m[c] * g : w[c];
+                r[c] = left_of(m[c], g > 0.0 ? fma(r[c], g, -(double)q[c]) : fma(-(double)q[c], Z, w[c]));
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) w[c] = r[c];
 }
 
 // The draft's probabilities of a row's vectors.
@@ -348,32 +369,32 @@ struct Draft {
     }
 };
 
-// weights of values: 0 from 1000 octaves under the reference on, and for what is not finite
-template <int N>
-__device__ __forceinline__ void weights(const float4 (&x)[N / 4], float ref, double C, uint32_t tab, double (&w)[N]) {
-    double d[N];
-    bool none[N];
+// Weights of four values: 0 from 1000 octaves under the reference on, and for what is not finite; `plain`: there
+// is nothing of the kind.
+__device__ __forceinline__ void weights(const float4 &x, float ref, double C, uint32_t tab, double (&w)[4], bool plain = false) {
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    double d[4];
+    unsigned none = 0;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-        const float v[4] = {x[c / 4].x, x[c / 4].y, x[c / 4].z, x[c / 4].w};
-        d[c] = (double)v[c % 4] - (double)ref;
-        none[c] = !(d[c] * C > -LOW) || !finite(v[c % 4]);
-        if (none[c]) d[c] = 0.0;
-        w[c] = 0.0;
+    for (int c = 0; c < 4; ++c) d[c] = (double)v[c] - (double)ref, w[c] = 0.0;
+    if (!plain) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (!(d[c] * C > -LOW) || !finite(v[c])) d[c] = 0.0, none |= 1u << c;
     }
     exp_add(d, C, tab, w);
+    if (!plain) {
 #pragma unroll
-    for (int c = 0; c < N; ++c)
-        if (none[c]) w[c] = 0.0;
+        for (int c = 0; c < 4; ++c)
+            if (none >> c & 1) w[c] = 0.0;
+    }
 }
 
-// The sums of r_k over the run's stretches, before r_k is divided by its sum.  CALM: p is exp((l - at) / T) with
-// at = ref + T ln Z, and what is 1000 octaves below or not finite counts as 2^-1000, which the sums do not show.
-template <bool CALM>
-__device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const Run &run, float ref, double at, double inv_Z, double C,
+// The sums over the run's stretches of r_k (residual), or of the weights for k = 0.  Where all of a tile lies
+// between -calm and calm it is finite and less than 1000 octaves below the reference.
+__device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const Run &run, float ref, float calm, double Z, double C,
                                          uint32_t tab, const double *inv, int k) {
     const int lane = threadIdx.x & 31;
-    const float low = (float)((double)ref - LOW / C), calm = fminf(-low, 3.402823466e38f);
     constexpr int U = 2;
     Part mine{0.0, ref, 0};
     float4 nx[U], ny[U];
@@ -389,48 +410,19 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
     double acc[4] = {};
     int done = 0, i = 0;
     for (int j = run.j0; j < run.j1; j += 32 * U) {
-        float4 x[U] = {nx[0], nx[1]};
-        const float4 y[U] = {ny[0], ny[1]};
+        const float4 x[U] = {nx[0], nx[1]}, y[U] = {ny[0], ny[1]};
         if (j + 32 * U < run.j1) load(j + 32 * U);
-        if (CALM) {
-            float m = abs_max3(abs_max3(x[0].x, x[0].y, x[0].z), abs_max3(x[0].w, x[1].x, x[1].y), fmaxf(fabsf(x[1].z), fabsf(x[1].w)));
-            if (__any_sync(0xffffffffu, !(m <= calm && x[0].x + x[0].y + x[0].z + x[0].w + x[1].x + x[1].y + x[1].z + x[1].w < INFINITY))) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    for (float *v : {&x[u].x, &x[u].y, &x[u].z, &x[u].w}) *v = *v > low && *v < INFINITY ? *v : low;
-            }
-        }
+        const float m = abs_max3(abs_max3(x[0].x, x[0].y, x[0].z), abs_max3(x[0].w, x[1].x, x[1].y), fmaxf(fabsf(x[1].z), fabsf(x[1].w)));
+        // the maximum leaves NaN out, the sum does not
+        const bool all = __all_sync(0xffffffffu, m <= calm && x[0].x + x[0].y + x[0].z + x[0].w + x[1].x + x[1].y + x[1].z + x[1].w < INFINITY);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, f[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-            double r[4];  // p - q
-            if (CALM) {
-                double d[4];
+            const float f[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+            double w[4];
+            weights(x[u], ref, C, tab, w, all);
+            if (k) residual(w, Z, f, inv, k);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) d[c] = (double)v[c] - at, r[c] = k ? -(double)f[c] : 0.0;
-                exp_add(d, C, tab, r);
-            } else {
-                double w[4];
-                const float4 one[1] = {x[u]};
-                weights<4>(one, ref, C, tab, w);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) r[c] = k ? fma(w[c], inv_Z, -(double)f[c]) : w[c] * inv_Z;
-            }
-            if (k > 1) {
-                double s[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[c] = r[c];
-                for (int n = 1; n < k; ++n) {
-                    const double g = inv[n - 1];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) s[c] = g > 0.0 ? fma(s[c] > 0.0 ? s[c] : 0.0, g, -(double)f[c]) : r[c];
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) r[c] = s[c];
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (__double2hiint(r[c]) >= 0) acc[c] += r[c];
+            for (int c = 0; c < 4; ++c) acc[c] += w[c];
         }
         if ((done += 32 * U) == run.step || j + 32 * U >= run.j1) {
             const double s = warp_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
@@ -441,10 +433,6 @@ __device__ __forceinline__ Part run_rest(const Row &row, const Draft &q, const R
         }
     }
     return mine;
-}
-
-__device__ __noinline__ Part run_rest_any(Row row, Draft q, Run run, float ref, double inv_Z, double C, uint32_t tab, const double *inv, int k) {
-    return run_rest<false>(row, q, run, ref, 0.0, inv_Z, C, tab, inv, k);
 }
 
 // running sum over the first N lanes
@@ -584,7 +572,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     const float T = a.temp ? a.temp[s] : 1.0f;
     const float u1 = a.u[s * a.u_ld2 + i * a.u_ld1 + 1];
     s_table.fill();
-    if (tid == 0) s_last = -1;
+    if (tid == 0) s_last = row.off;  // a value of the row whatever happens
     const uint32_t tab = (uint32_t)__cvta_generic_to_shared(&s_table.v[0][tid % COPIES]);
     auto put = [&](int token, double logp) {
         a.target[s * a.tgt_ld + i] = token;
@@ -663,26 +651,22 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
         return;
     }
     const Draft draft{q, (((uintptr_t)q ^ (uintptr_t)logits) & 15) == 0};
-    const bool calm = fabs((double)ref * C) <= MOST && LOW / C < 3e38;  // low (run_rest) has to be a number
     int rounds = 0;
     bool left = false;  // something is left of p
-    double inv_Z = 0.0, total = Z;
+    double total = Z;
     if (DRAFT) {
-        inv_Z = 1.0 / Z;
-        double at_Z = 0.0;
-        auto rest = [&](int k) {
-            if (k == 1) at_Z = (double)ref + (double)T * log(Z);
-            return calm ? run_rest<true>(row, draft, run, ref, at_Z, inv_Z, C, tab, s_inv, k)
-                        : run_rest_any(row, draft, run, ref, inv_Z, C, tab, s_inv, k);
-        };
+        const double inv_Z = 1.0 / Z;
+        // 64 steps of the 1000 octaves are left for its rounding to 32 bits
+        const float low = (float)((double)ref - (LOW - 64) / C), calm = fabs((double)ref * C) <= MOST ? fminf(-low, 3.402823466e38f) : -1.0f;
+        auto rest = [&](int k) { return run_rest(row, draft, run, ref, calm, Z, C, tab, s_inv, k); };
         const int kids = s_n_kids;
         while (rounds < kids) {
             const Try t = rounds < 32 ? s_try[rounds] : child(s_kids[rounds]);
             if (t.token >= 0) {
-                const double w = weight(t.l, ref, C, tab);
-                double r = residual(w, inv_Z, t.q, s_inv, left ? rounds : 0);
-                if (left) r *= s_inv[rounds - 1];
-                if ((double)t.u * (double)t.q < r) {
+                double w[1] = {weight(t.l, ref, C, tab)};
+                const float f[1] = {t.q};
+                if (left) residual(w, Z, f, s_inv, rounds);
+                if ((double)t.u * (double)t.q < w[0] * (left ? s_inv[rounds - 1] : inv_Z)) {
                     if (rank == 0 && tid == 0) put(t.token, ((double)t.l - (double)ref) * inv_T - log(Z));
                     return;
                 }
@@ -691,7 +675,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
             double sum, up, one;
             float same;
             gather(s_sums, rounds & 1, rank, rest(rounds), C, tab, sum, same, up, one);
-            left = sum > 0x1p-900;
+            left = sum > 0x1p-1000;
             if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / sum : 0.0;
             if (left) total = sum, upto = up, f = one;
             __syncthreads();
@@ -708,16 +692,11 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     const Run found = run_of(rank, at.warp);
     const int j0 = found.from(at.stretch), j1 = found.from(at.stretch + 1), each = (step + NT - 1) / NT;
     auto values = [&](int j, const float4 &v, double (&w)[4]) {
-        const float4 one[1] = {v};
-        weights<4>(one, ref, C, tab, w);
+        weights(v, ref, C, tab, w);
         if (DRAFT && left) {
             const float4 y = j < j1 ? draft.load(row, j) : zero;
             const float g[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = residual(w[c], inv_Z, g[c], s_inv, rounds);
-        } else if (DRAFT && rounds) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] *= inv_Z;
+            residual(w, Z, g, s_inv, rounds);
         }
     };
     const int b0 = j0 + tid * each, b1 = min(b0 + each, j1);
@@ -744,7 +723,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     auto report = [&](int e, float l) { put(e - row.off, ((double)l - (double)ref) * inv_T - s_log); };
     const bool here = before <= drawn && base + up > drawn;
     if (here) {
-        int e = last;  // where roundings let the walk miss it
+        int e = max(last, row.off);  // where roundings let the walk miss it
         double cum = before;
         for (int j = b0; j < b1; ++j) {
             if (each > 1) values(j, row.load(j), w);
