@@ -450,8 +450,8 @@ __device__ __forceinline__ double scan(double v) {
 // The sums of a row's weights by stretch, warp and CTA, and where a drawn value lies.
 template <int CS>
 struct Sums {
-    double stretch[NW][32];  // running sums over a warp's stretches, relative to the CTA's reference
-    double warp[NW];         // running sums over the warps
+    double stretch[NW][32];  // of a warp's stretches, relative to the CTA's reference
+    double warp[NW];         // of the warps
     double cta[2][CS];       // sums of the cluster's CTAs (two calls in turn), relative to
     float cta_ref[2][CS];    // their references
     float warp_ref[NW];
@@ -468,26 +468,29 @@ struct Try {
 // Where a drawn value lies: CTA, warp, stretch, and the running sum up to there.
 struct Place {
     int cta, warp, stretch;
-    double before, f;  // f: what the CTA's sums are multiplied by
+    double before;
 };
 
 // `mine`: this lane's stretch, relative to the warp's reference.  Then the sums are everywhere, `all` is the
 // whole row's and `ref` what it is relative to; f: what this lane's CTA's are to be multiplied by.
 template <int CS>
 __device__ __forceinline__ void gather(Sums<CS> &s, int turn, int rank, const Part &mine, double C, uint32_t tab, double &all, float &ref,
-                                       double &run, double &f) {
+                                       double &f) {
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane == 0) s.warp_ref[warp] = mine.ref;
     __syncthreads();
     const float m = warp_max(lane < NW ? s.warp_ref[lane] : -INFINITY);
-    const double up = scan(scaled(mine.sum, mine.ref, m, C, tab));
-    s.stretch[warp][lane] = up;
+    const double own = scaled(mine.sum, mine.ref, m, C, tab);
+    s.stretch[warp][lane] = own;
+    const double sum = warp_sum(own);
+    if (lane == 0) s.warp[warp] = sum;
     __syncthreads();
     if (warp == 0) {
-        const double w = scan<NW>(lane < NW ? s.stretch[lane][31] : 0.0);
-        if (lane < NW) s.warp[lane] = w;
-        const double total = __shfl_sync(0xffffffffu, w, NW - 1);
+        double total = lane < NW ? s.warp[lane] : 0.0;
+#pragma unroll
+        for (int o = NW / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o, NW);
+        total = __shfl_sync(0xffffffffu, total, 0);
         if (CS == 1) {
             if (lane == 0) s.cta[turn][0] = total, s.cta_ref[turn][0] = m;
         } else if (lane < CS) {
@@ -501,35 +504,39 @@ __device__ __forceinline__ void gather(Sums<CS> &s, int turn, int rank, const Pa
     const float r = lane < CS ? s.cta_ref[turn][lane] : -INFINITY;
     ref = warp_max(r);
     f = lane < CS ? scaled(1.0, r, ref, C, tab) : 0.0;
-    run = scan<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0);
-    all = __shfl_sync(0xffffffffu, run, CS - 1);
-    if (lane >= CS) run = all;
+    all = lane < CS ? s.cta[turn][lane] * f : 0.0;
+#pragma unroll
+    for (int o = CS / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o, CS);
+    all = __shfl_sync(0xffffffffu, all, 0);
 }
 
-// the first place whose running sum is greater than `drawn`, the last with any mass if roundings leave none
-template <int CS>
-__device__ __forceinline__ Place find(const Sums<CS> &s, double run, double f, double drawn, int rank) {
+// The first of N lanes with mass whose running sum from `before` on is greater than `drawn`, the last with
+// mass if roundings leave none; `before` then is the running sum up to it.  Running sums of lanes next to one another are
+// rounded differently, so that one may rise past `drawn` at a lane that adds nothing: mass is more than `least`.
+template <int N>
+__device__ __forceinline__ int first_past(double own, double least, double drawn, double &before) {
     const int lane = threadIdx.x & 31;
-    auto first = [&](double up, double drawn) {
-        const unsigned past = __ballot_sync(0xffffffffu, up > drawn);
-        double before = __shfl_up_sync(0xffffffffu, up, 1);
-        if (lane == 0) before = 0.0;
-        const unsigned mass = __ballot_sync(0xffffffffu, up > before);
-        return past ? __ffs(past) - 1 : 31 - __clz(mass | 1u);
-    };
+    const double up = before + scan<N>(own);
+    const unsigned mass = __ballot_sync(0xffffffffu, lane < N && own > least), past = __ballot_sync(0xffffffffu, up > drawn) & mass;
+    const int at = past ? __ffs(past) - 1 : 31 - __clz(mass | 1u);
+    const double to = __shfl_sync(0xffffffffu, up, max(at - 1, 0));
+    if (at) before = to;
+    return at;
+}
+
+// The place whose running sum is the first to pass `drawn`.  Its sum is more than 2^-210 of the whole (there is
+// such a stretch in such a warp of such a CTA: the greatest of 16, 8 and 32 parts), far above what values
+// without weight may have been counted as.
+template <int CS>
+__device__ __forceinline__ Place find(const Sums<CS> &s, int turn, double all, double f, double drawn, int rank) {
+    const int lane = threadIdx.x & 31;
     Place p;
-    p.cta = first(run, drawn);
-    p.f = __shfl_sync(0xffffffffu, f, p.cta);
-    p.before = p.cta ? __shfl_sync(0xffffffffu, run, max(p.cta - 1, 0)) : 0.0;
+    p.before = 0.0;
+    p.cta = first_past<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0, all * 0x1p-200, drawn, p.before);
     if (p.cta != rank) return p;
-    const double w = p.before + p.f * s.warp[min(lane, NW - 1)];
-    p.warp = min(first(w, drawn), NW - 1);
-    const double start = __shfl_sync(0xffffffffu, w, max(p.warp - 1, 0));
-    if (p.warp) p.before = start;
-    const double t = p.before + p.f * s.stretch[p.warp][lane];
-    p.stretch = first(t, drawn);
-    const double at = __shfl_sync(0xffffffffu, t, max(p.stretch - 1, 0));
-    if (p.stretch) p.before = at;
+    f = __shfl_sync(0xffffffffu, f, p.cta);
+    p.warp = first_past<NW>(lane < NW ? f * s.warp[lane] : 0.0, all * 0x1p-204, drawn, p.before);
+    p.stretch = first_past<32>(f * s.stretch[p.warp][lane], all * 0x1p-210, drawn, p.before);
     return p;
 }
 
@@ -550,7 +557,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     __shared__ Sums<CS> s_sums;
     __shared__ double s_inv[DRAFT ? TREE_MAX_NODES : 1], s_warp[NW], s_log;
     __shared__ unsigned short s_kids[DRAFT ? TREE_MAX_NODES : 1];
-    __shared__ int s_n_kids, s_last;
+    __shared__ int s_n_kids, s_last, s_first;
     __shared__ Try s_try[32];  // of the first children
     griddep_launch_dependents();
     griddep_wait();
@@ -565,14 +572,14 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
         return Run{j0, min(j0 + per, row.vectors()), step};
     };
     const Run run = run_of(rank, warp);
-    const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float4 first[U];
     load_tile(first, row, run.j0, run.j1, lane);
     const int n = a.n_nodes ? a.n_nodes[s] : a.N;
     const float T = a.temp ? a.temp[s] : 1.0f;
     const float u1 = a.u[s * a.u_ld2 + i * a.u_ld1 + 1];
     s_table.fill();
-    if (tid == 0) s_last = row.off;  // a value of the row whatever happens
+    if (tid == 0) s_last = -1, s_first = NT;
     const uint32_t tab = (uint32_t)__cvta_generic_to_shared(&s_table.v[0][tid % COPIES]);
     auto put = [&](int token, double logp) {
         a.target[s * a.tgt_ld + i] = token;
@@ -643,9 +650,10 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     const double inv_T = 1.0 / (double)T, C = STEPS / LN2 * inv_T;
     const Part mine = run_sum(row, run, first, C, tab);
     if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
-    double Z, upto, f;
+    double Z, f;
     float ref;
-    gather(s_sums, 0, rank, mine, C, tab, Z, ref, upto, f);
+    int turn = 0;  // of the sums that the token is drawn from
+    gather(s_sums, 0, rank, mine, C, tab, Z, ref, f);
     if (ref == -INFINITY) {  // no finite logit
         if (rank == 0 && tid == 0) put(-1, 0.0);
         return;
@@ -672,20 +680,21 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
                 }
             }
             ++rounds;
-            double sum, up, one;
             float same;
-            gather(s_sums, rounds & 1, rank, rest(rounds), C, tab, sum, same, up, one);
-            left = sum > 0x1p-1000;
-            if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / sum : 0.0;
-            if (left) total = sum, upto = up, f = one;
+            turn ^= 1;
+            gather(s_sums, turn, rank, rest(rounds), C, tab, total, same, f);
+            left = total > 0x1p-1000;
+            if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / total : 0.0;
             __syncthreads();
         }
-        if (rounds && !left)  // p once more
-            gather(s_sums, (rounds + 1) & 1, rank, rest(0), C, tab, total, ref, upto, f);
+        if (rounds && !left) {  // p once more
+            turn ^= 1;
+            gather(s_sums, turn, rank, rest(0), C, tab, total, ref, f);
+        }
     }
     // a number on a border belongs to the value behind it, however the sums up to there were rounded
     const double drawn = (double)u1 * total + total * 0x1p-44;
-    const Place at = find(s_sums, upto, f, drawn, rank);
+    const Place at = find(s_sums, turn, total, f, drawn, rank);
     if (at.cta != rank) return;
     if (tid == NT - 1) s_log = log(Z);
     // the value's place in its stretch: `each` vectors of a thread, one after the other
@@ -701,11 +710,9 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     };
     const int b0 = j0 + tid * each, b1 = min(b0 + each, j1);
     double own = 0.0, w[4];
-    float4 v = none;
     int last = -1;  // of the values with any mass
     for (int j = b0; j < b1; ++j) {
-        v = row.load(j);
-        values(j, v, w);
+        values(j, row.load(j), w);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             own += w[c];
@@ -720,23 +727,25 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     for (int k = 0; k < warp; ++k) base += s_warp[k];
     double before = __shfl_up_sync(0xffffffffu, up, 1);
     before = lane ? base + before : base;
-    auto report = [&](int e, float l) { put(e - row.off, ((double)l - (double)ref) * inv_T - s_log); };
-    const bool here = before <= drawn && base + up > drawn;
-    if (here) {
-        int e = max(last, row.off);  // where roundings let the walk miss it
+    // the first thread with mass whose running sum passes `drawn`; where roundings leave none, the last value with mass
+    const unsigned past = __ballot_sync(0xffffffffu, last >= 0 && base + up > drawn);
+    if (past && lane == __ffs(past) - 1) atomicMin(&s_first, tid);
+    __syncthreads();
+    auto report = [&](int e) { put(e - row.off, ((double)row.base[e] - (double)ref) * inv_T - s_log); };
+    if (tid == s_first) {
+        int e = -1;
         double cum = before;
         for (int j = b0; j < b1; ++j) {
             if (each > 1) values(j, row.load(j), w);
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (cum <= drawn) {
-                    cum += w[c];
-                    if (cum > drawn) e = 4 * j + c;
-                }
+            for (int c = 0; c < 4; ++c) {
+                cum += w[c];
+                if (e < 0 && w[c] > 0.0 && cum > drawn) e = 4 * j + c;
+            }
         }
-        report(e, row.base[e]);
+        report(e < 0 ? last : e);
     }
-    if (!__syncthreads_or(here) && tid == 0) report(s_last, row.base[s_last]);
+    if (s_first == NT && tid == 0) report(s_last);
 }
 
 // whether the values of out (4 bytes each) and those of a 4-byte tensor [.., n, n_seq] meet
