@@ -394,7 +394,8 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * K/V head of every layer keeps the first n_sink, the last n_recent and, of those between, the ones
  * with the greatest weights (of equal ones the first; NaN after all others) to n_keep in all.  Their K
  * and V rows and weights move to positions 0, 1, ... in their order; n_past_out I32 [n_seq] is n_keep
- * for those sequences and n_past for the others, which stay as they are.  What pages hold from n_keep
+ * for those sequences and n_past for the others, which stay as they are (also one that is out of range:
+ * a length, its n_keep, a page of it).  What pages hold from n_keep
  * on stays as it was; oasr_b200_kv_pool_truncate gives those pages back.  Keys keep the rotation of the
  * positions that they had: later nodes pass pos to oasr_b200_qk_norm_rope, counting on from there.
  * weights has the pages of all layers along ne[2], as k_pages along ne[3].  n_keep of a longer sequence

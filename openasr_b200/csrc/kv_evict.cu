@@ -98,18 +98,21 @@ __global__ void __launch_bounds__(ET) kv_evict_kernel(Evict a, KvPages p, KvSeqs
     const int keep = a.n_keep[s];
     const bool ok = fits && (past <= keep || (keep >= a.sink && keep - a.sink >= a.recent));
     const bool full = ok && past > keep;
-    if (layer == 0 && h == 0 && rank == 0 && tid == 0) {
+    const bool reports = layer == 0 && h == 0 && rank == 0 && tid == 0;
+    if (!full) {
+        if (!reports) return;
         if (!ok) atomicOr(err, ERR_BAD_INDEX);
-        a.n_past_out[s] = full ? keep : sq.n_past[s];
+        a.n_past_out[s] = sq.n_past[s];
+        return;
     }
-    if (!full) return;
     const int *table = sq.table + s * sq.table_ld;
     if (tid == 0) s_bad = 0;
     __syncthreads();
     for (int j = tid; j <= page(past - 1); j += ET)
         if (table[j] < 0 || table[j] >= p.n_pages) s_bad = 1;
     __syncthreads();
-    if (s_bad) {  // in every CTA of the cluster
+    if (reports) a.n_past_out[s] = s_bad ? past : keep;
+    if (s_bad) {  // in every CTA of all its clusters: nothing moves
         if (tid == 0) atomicOr(err, ERR_BAD_INDEX);
         return;
     }

@@ -662,3 +662,34 @@ def test_pages_out_of_range_are_reported_with_many_rows(be):
         be.attn_weights(cuda(q), c.device()[0], cuda(c.table), cuda(c.past), None, 0.1, 1.0, w)
         be.synchronize()
     np.testing.assert_array_equal(w.cpu().numpy()[other].astype(np.float64), want[other])
+
+
+@pytest.mark.parametrize("spoil", ["page", "low", "past", "more", "keep", "negative"])
+def test_a_sequence_that_is_not_shortened_keeps_its_length(be, spoil):
+    """n_past_out goes into the next captured call: a sequence whose rows stay has the length that it had"""
+    import torch
+
+    import openasr_b200 as ob
+
+    rng = np.random.default_rng(25)
+    c = Cache(rng, 3, 0, 2, 64, 16, [60, 33, 47], fill=None)
+    w = rng.random((c.P, 2, 16)).astype(np.float32)
+    table, past, keep = c.table.copy(), c.past.copy(), np.array([40, 20, 47], np.int32)
+    if spoil == "page":
+        table[0, 3] = c.P
+    elif spoil == "low":
+        table[0, 0] = -1
+    elif spoil == "past":
+        past[0] = -1
+    elif spoil == "more":
+        past[0] = 16 * c.MP + 1
+    else:
+        keep[0] = 11 if spoil == "keep" else -1
+    k, v, wd = (*c.device(), cuda(w))
+    out = torch.full((3,), -5, dtype=torch.int32, device="cuda")
+    be.kv_evict(wd, cuda(table), cuda(past), cuda(keep), 4, 8, k, v, 1, out)
+    with pytest.raises(ob.GgmlBackendError, match="out-of-range"):
+        be.synchronize()
+    assert out.tolist() == [int(past[0]), 20, 47]
+    np.testing.assert_array_equal(k.cpu().numpy()[c.table[0]], c.k[c.table[0]])
+    np.testing.assert_array_equal(wd.cpu().numpy()[c.table[0]], w[c.table[0]])
