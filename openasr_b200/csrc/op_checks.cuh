@@ -2,6 +2,9 @@
 // verification share (host side).
 #pragma once
 
+#include <stdlib.h>
+
+#include <algorithm>
 #include <string>
 
 #include "common.cuh"
@@ -57,6 +60,63 @@ inline bool share_values(const IntRows &a, const IntRows &b) {
         else return true;
     }
     return false;
+}
+
+// The bytes that a tensor covers: runs of `run` bytes from `at` on, `n` of them in each dimension at a stride,
+// the greatest stride first; dimensions that continue a run are part of it.
+struct Runs {
+    const char *at;
+    int64_t run, extent, n[4], stride[4], inner[4];  // inner: extent of what repeats in that dimension
+    int dims = 0;
+
+    explicit Runs(const oasr_tensor *t) : at((const char *)t->data), run(t->type == OASR_TYPE_F16 ? 2 : t->type == OASR_TYPE_I64 ? 8 : 4) {
+        int order[4], k = 0;
+        for (int i = 0; i < 4; ++i) {
+            if (t->ne[i] <= 1 || t->nb[i] == 0) continue;
+            if (t->nb[i] < 0) at += (t->ne[i] - 1) * t->nb[i];
+            int j = k++;
+            for (; j > 0 && llabs(t->nb[order[j - 1]]) > llabs(t->nb[i]); --j) order[j] = order[j - 1];
+            order[j] = i;
+        }
+        int from = 0;
+        for (; from < k && llabs(t->nb[order[from]]) <= run; ++from) run += (t->ne[order[from]] - 1) * llabs(t->nb[order[from]]);
+        extent = run;
+        dims = k - from;
+        for (int j = 0; j < dims; ++j) {
+            const int i = order[from + j], d = dims - 1 - j;
+            n[d] = t->ne[i], stride[d] = llabs(t->nb[i]), inner[d] = extent;
+            extent += (n[d] - 1) * stride[d];
+        }
+    }
+    int64_t extent_of(int d) const { return d ? inner[d - 1] : extent; }  // of dimensions d, d + 1, ...
+};
+
+// Whether a's dimensions from da on meet b's from db on, `off` bytes further.  Equal strides go together, one step
+// for the few places where the insides meet (views of one buffer); of others the greater is taken apart.
+inline bool runs_meet(const Runs &a, int da, const Runs &b, int db, int64_t off) {
+    if (off >= a.extent_of(da) || -off >= b.extent_of(db)) return false;
+    auto up = [](int64_t x, int64_t y) { return x >= 0 ? (x + y - 1) / y : -(-x / y); };  // x / y rounded up
+    const int64_t sa = da < a.dims ? a.stride[da] : 0, sb = db < b.dims ? b.stride[db] : 0;
+    if (!sa && !sb) return true;
+    if (sa == sb) {  // index of a minus index of b
+        const int64_t lo = std::max(1 - b.n[db], up(off - a.inner[da] + 1, sa)), hi = std::min(a.n[da] - 1, -up(-off - b.inner[db] + 1, sa));
+        for (int64_t c = lo; c <= hi; ++c)
+            if (runs_meet(a, da + 1, b, db + 1, off - c * sa)) return true;
+        return false;
+    }
+    if (sa < sb) return runs_meet(b, db, a, da, -off);
+    const int64_t lo = std::max<int64_t>(0, up(off - a.inner[da] + 1, sa)), hi = std::min(a.n[da] - 1, -up(-off - b.extent_of(db) + 1, sa));
+    for (int64_t c = lo; c <= hi; ++c)
+        if (runs_meet(a, da + 1, b, db, off - c * sa)) return true;
+    return false;
+}
+
+// Whether two tensors have a byte in common; either may be null or empty.
+inline bool share_bytes(const oasr_tensor *x, const oasr_tensor *y) {
+    for (const oasr_tensor *t : {x, y})
+        if (!t || !t->data || !t->ne[0] || !t->ne[1] || !t->ne[2] || !t->ne[3]) return false;
+    const Runs a(x), b(y);
+    return runs_meet(a, 0, b, 0, b.at - a.at);
 }
 
 // F32 [page, H_kv, n_pages] beside the pages

@@ -748,16 +748,6 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     if (s_first == NT && tid == 0) report(s_last);
 }
 
-// whether the values of out (4 bytes each) and those of a 4-byte tensor [.., n, n_seq] meet
-bool meets(const IntRows &out, const oasr_tensor *t) {
-    if (!t) return false;
-    for (int64_t s = 0; s < t->ne[2]; ++s)
-        if (share_values(out, IntRows{(const int *)((const char *)t->data + s * t->nb[2]), t->ne[1], t->ne[0],
-                                      t->ne[1] > 1 ? t->nb[1] / 4 : 0}))
-            return true;
-    return false;
-}
-
 bool is_rows3_f32(const oasr_tensor *t, int64_t w, int64_t N, int64_t S) {
     return t && t->type == OASR_TYPE_F32 && t->data && aligned4(t) && t->ne[0] == w && t->ne[1] == N && t->ne[2] == S &&
            t->ne[3] == 1 && (t->nb[0] == 4 || w <= 1) && t->nb[1] % 4 == 0 && t->nb[2] % 4 == 0;
@@ -819,9 +809,9 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
         if (!o) continue;
         if (S > 1 && llabs(o->nb[1] / 4) < N) return fail_op(be, op, "rows of target and logprob must not overlap");
         for (const oasr_tensor *t : ins)
-            if (meets(int_rows(o), t)) return fail_op(be, op, "target and logprob must not overlap an input");
+            if (share_bytes(o, t)) return fail_op(be, op, "target and logprob must not overlap an input");
     }
-    if (logprob && share_values(int_rows(target), int_rows(logprob))) return fail_op(be, op, "target and logprob must not overlap");
+    if (share_bytes(target, logprob)) return fail_op(be, op, "target and logprob must not overlap");
     const int st = oasr_internal_precheck(be);  // the arguments need no device
     if (st) return st;
     Sample a = {};

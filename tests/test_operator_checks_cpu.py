@@ -199,3 +199,19 @@ def test_the_python_calls(ops):
     for call in calls(b, torch.zeros(2, 2, dtype=torch.bfloat16)):
         with pytest.raises(bk.UnsupportedInputs, match="dtype"):
             call()
+
+
+def test_results_beside_many_rows_are_checked_at_once(be):
+    """a column of results in the buffer of the logits: nothing is shared, and that does not take a step per pair of rows"""
+    import time
+
+    S, V = 1 << 17, 2
+    x, t = f(S, 1, V), i(S, 1)
+    at_once = dict(x=at(x, nb1=12, nb2=12), t=at(t, data=x.data + 8, nb1=12), u=f(S, 1, 2), temp=f(S), live=i(S), tok=None, par=None, q=None,
+                   lp=f(S, 1))
+    start = time.perf_counter()
+    with pytest.raises(ob.GgmlBackendError) as e:
+        sample(be, **at_once)
+    assert e.value.status == bk.STATUS_DEVICE_LOST and time.perf_counter() - start < 1.0
+    with pytest.raises(bk.UnsupportedInputs, match="overlap an input"):
+        sample(be, **{**at_once, "t": at(t, data=x.data + 4, nb1=12)})
