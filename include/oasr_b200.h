@@ -384,7 +384,7 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * softmax weights that the position gets from all live nodes and all query heads of its K/V head,
  * after the old value was multiplied by decay; with decay 0, and for the positions from n_past on,
  * which are new, the old value is not read.  Entries of positions past the last node stay as they are.
- * n_past + n_nodes is at most 2^30 here.
+ * n_past + n_nodes is at most 2^30 here.  weights may not overlap another argument.
  * One call per layer and step, with the queries and the lengths of that layer's flash_attn_tree; or
  * one after the prompt with its last rows and decay 0, which scores all of it.  A row with something
  * that is not finite (a query, a K row that it sees) makes the entries of what it sees NaN; a position

@@ -690,6 +690,8 @@ extern "C" int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, co
     if (N * (H / HKV) > INT32_MAX / 2) return fail_op(be, op, "too many rows");
     if (!q->data) return fail_op(be, op, "null argument");
     if (!rows16(q)) return fail_op(be, op, "rows must be 16-byte aligned");
+    for (const oasr_tensor *t : {q, k_pages, page_table, n_past, n_nodes})
+        if (share_bytes(weights, t)) return fail_op(be, op, "weights must not overlap an input (it is still read while they are written)");
     st = oasr_internal_precheck(be);  // the arguments need no device
     if (st) return st;
     Weights a = {};

@@ -215,3 +215,24 @@ def test_results_beside_many_rows_are_checked_at_once(be):
     assert e.value.status == bk.STATUS_DEVICE_LOST and time.perf_counter() - start < 1.0
     with pytest.raises(bk.UnsupportedInputs, match="overlap an input"):
         sample(be, **{**at_once, "t": at(t, data=x.data + 4, nb1=12)})
+
+
+@pytest.mark.parametrize("change", [
+    dict(w=lambda a: at(a["w"], data=a["q"].data + 4 * 1535)), dict(q=lambda a: at(a["q"], data=a["w"].data + 4 * 176)),
+    dict(w=lambda a: at(a["w"], data=a["k"].data + 2 * 6 * 2 * 16 * 64 - 4)), dict(w=lambda a: at(a["w"], data=a["table"].data)),
+    dict(w=lambda a: at(a["w"], data=a["past"].data + 4)), dict(live=lambda a: at(a["live"], data=a["w"].data + 764)),
+    dict(k=lambda a: at(a["k"], nb3=4096 + 128), w=lambda a: at(a["w"], data=a["k"].data + 4092, nb1=64, nb2=4096 + 128)),
+])
+def test_weights_in_an_input_are_refused(be, change):
+    with pytest.raises(bk.UnsupportedInputs, match="weights must not overlap an input"):
+        weights(be, **change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(w=lambda a: at(a["w"], data=a["q"].data + 4 * 1536)), dict(w=lambda a: at(a["w"], data=a["past"].data + 8)),
+    dict(k=lambda a: at(a["k"], nb3=4096 + 128), w=lambda a: at(a["w"], data=a["k"].data + 4096, nb1=64, nb2=4096 + 128)),  # behind each page
+])
+def test_weights_beside_an_input_are_not(be, change):
+    with pytest.raises(ob.GgmlBackendError) as e:
+        weights(be, **change)
+    assert e.value.status == bk.STATUS_DEVICE_LOST
