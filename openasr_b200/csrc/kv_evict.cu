@@ -349,9 +349,19 @@ extern "C" int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const 
     st = seqs_check(be, op, page_table, n_past, nullptr, S, 0, &sq);
     if (st) return st;
     if (!is_vec_i32(n_keep, S) || !is_vec_i32(n_past_out, S)) return fail_op(be, op, "n_keep and n_past_out must be I32 [n_seq]");
-    for (const oasr_tensor *t : {n_past, n_keep, page_table})
-        if (share_values(int_rows(n_past_out), int_rows(t)))
-            return fail_op(be, op, "n_past_out must not overlap an input (it is still read while it is written)");
+    // all of them are read while others are written
+    const oasr_tensor *moved[] = {weights, k_pages, v_pages}, *read[] = {n_past, n_keep, page_table};
+    for (const oasr_tensor *pages : {k_pages, v_pages})
+        if (!apart(pages)) return fail_op(be, op, "rows of the pages must not overlap");
+    if (share_bytes(weights, k_pages) || share_bytes(weights, v_pages) || share_bytes(k_pages, v_pages))
+        return fail_op(be, op, "weights, k_pages and v_pages must not overlap");
+    for (const oasr_tensor *t : read) {
+        if (share_bytes(n_past_out, t)) return fail_op(be, op, "n_past_out must not overlap an input (it is still read while it is written)");
+        for (const oasr_tensor *m : moved)
+            if (share_bytes(m, t)) return fail_op(be, op, "weights and pages must not overlap lengths or page table");
+    }
+    for (const oasr_tensor *m : moved)
+        if (share_bytes(n_past_out, m)) return fail_op(be, op, "n_past_out must not overlap an input (it is still read while it is written)");
     st = oasr_internal_precheck(be);  // the arguments need no device
     if (st) return st;
     Evict a = {};

@@ -119,6 +119,17 @@ inline bool share_bytes(const oasr_tensor *x, const oasr_tensor *y) {
     return runs_meet(a, 0, b, 0, b.at - a.at);
 }
 
+// Whether no two elements of a tensor lie in one place, its dimensions inside one another.
+inline bool apart(const oasr_tensor *t) {
+    const Runs r(t);
+    int64_t count = r.run / (t->type == OASR_TYPE_F16 ? 2 : t->type == OASR_TYPE_I64 ? 8 : 4);
+    for (int d = 0; d < r.dims; ++d) {
+        if (r.stride[d] < r.inner[d]) return false;
+        count *= r.n[d];
+    }
+    return count == t->ne[0] * t->ne[1] * t->ne[2] * t->ne[3];
+}
+
 // F32 [page, H_kv, n_pages] beside the pages
 inline bool is_weights(const oasr_tensor *w, const oasr_tensor *k) {
     if (!w || w->type != OASR_TYPE_F32 || !w->data || !aligned4(w) || w->ne[0] != k->ne[1] || w->ne[1] != k->ne[2] ||

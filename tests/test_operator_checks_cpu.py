@@ -236,3 +236,37 @@ def test_weights_beside_an_input_are_not(be, change):
     with pytest.raises(ob.GgmlBackendError) as e:
         weights(be, **change)
     assert e.value.status == bk.STATUS_DEVICE_LOST
+
+
+EVICT_PAGES = 6 * 2 * 16 * 128 * 2  # bytes
+
+
+@pytest.mark.parametrize("change,says", [
+    (dict(out=lambda a: at(a["out"], data=a["w"].data + 764)), "n_past_out must not overlap an input"),
+    (dict(out=lambda a: at(a["out"], data=a["k"].data + EVICT_PAGES - 4)), "n_past_out must not overlap an input"),
+    (dict(out=lambda a: at(a["out"], data=a["v"].data)), "n_past_out must not overlap an input"),
+    (dict(v=lambda a: a["k"]), "weights, k_pages and v_pages must not overlap"),
+    (dict(v=lambda a: at(a["k"], data=a["k"].data + EVICT_PAGES - 16)), "weights, k_pages and v_pages must not overlap"),
+    (dict(w=lambda a: at(a["w"], data=a["v"].data + 4096)), "weights, k_pages and v_pages must not overlap"),
+    (dict(w=lambda a: at(a["w"], data=a["table"].data + 8)), "lengths or page table"),
+    (dict(past=lambda a: at(a["past"], data=a["k"].data + 512)), "lengths or page table"),
+    (dict(keep=lambda a: at(a["keep"], data=a["v"].data + EVICT_PAGES - 8)), "lengths or page table"),
+    (dict(k=lambda a: at(a["k"], nb2=0)), "rows of the pages must not overlap"), (dict(v=lambda a: at(a["v"], nb3=0)), "rows of the pages must not overlap"),
+    (dict(k=lambda a: at(a["k"], nb1=240)), "rows of the pages must not overlap"),
+])
+def test_evictions_over_what_is_still_read_are_refused(be, change, says):
+    with pytest.raises(bk.UnsupportedInputs, match=says):
+        evict(be, **change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(v=lambda a: at(a["k"], data=a["k"].data + EVICT_PAGES)), dict(out=lambda a: at(a["out"], data=a["past"].data + 8)),
+    # K and V rows in turn; K, V and weights of a page one after the other
+    dict(k=lambda a: at(a["k"], nb1=512, nb2=8192, nb3=16384), v=lambda a: at(a["v"], data=a["k"].data + 256, nb1=512, nb2=8192, nb3=16384)),
+    dict(k=lambda a: at(a["k"], nb3=16512), v=lambda a: at(a["v"], data=a["k"].data + 8192, nb3=16512),
+         w=lambda a: at(a["w"], data=a["k"].data + 16384, nb2=16512)),
+])
+def test_evictions_in_one_buffer_are_not(be, change):
+    with pytest.raises(ob.GgmlBackendError) as e:
+        evict(be, **change)
+    assert e.value.status == bk.STATUS_DEVICE_LOST

@@ -17,6 +17,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr
 SOURCE = r"""
 #include "op_checks.cuh"
 extern "C" int shared(const oasr_tensor *a, const oasr_tensor *b) { return oasr::share_bytes(a, b); }
+extern "C" int alone(const oasr_tensor *a) { return oasr::apart(a); }
 """
 
 
@@ -28,11 +29,15 @@ def build(d, source):
 
 
 @pytest.fixture(scope="module")
-def shared(tmp_path_factory):
+def checks(tmp_path_factory):
     if not NVCC:
         pytest.skip("no nvcc")
-    fn = build(tmp_path_factory.mktemp("share"), SOURCE).shared
-    return lambda a, b: bool(fn(ctypes.byref(a) if a else None, ctypes.byref(b) if b else None))
+    return build(tmp_path_factory.mktemp("share"), SOURCE)
+
+
+@pytest.fixture(scope="module")
+def shared(checks):
+    return lambda a, b: bool(checks.shared(ctypes.byref(a) if a else None, ctypes.byref(b) if b else None))
 
 
 SIZE = {bk.F32: 4, bk.F16: 2, bk.I32: 4, bk.I64: 8}
@@ -112,3 +117,21 @@ def test_views_of_one_buffer_of_pages(shared, layout):
     assert not shared(k, v)
     v.data -= 2
     assert shared(k, v)
+
+
+def test_elements_in_one_place(checks):
+    """what is said to be apart is; what is one dimension inside the other is found to be"""
+    r = random.Random(2)
+    seen = [0, 0]
+    for _ in range(6000):
+        t = some(r)
+        n = t.ne[0] * t.ne[1] * t.ne[2] * t.ne[3]
+        said = bool(checks.alone(ctypes.byref(t)))
+        seen[said] += 1
+        if said:
+            assert len(covered(t)) == n * SIZE[t.type], (t.type, list(t.ne), list(t.nb))
+        nested, size = True, SIZE[t.type]
+        for b, m in sorted((abs(b), m) for b, m in zip(t.nb, t.ne) if m > 1):
+            nested, size = nested and b >= size, size + (m - 1) * b
+        assert said == nested, (t.type, list(t.ne), list(t.nb))
+    assert min(seen) > 100
