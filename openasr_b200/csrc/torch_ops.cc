@@ -119,11 +119,16 @@ bool take(Arg (&t)[N], PyObject *const *args, const Where &at) {
     return true;
 }
 
-template <class F>
-PyObject *status(F &&call) {
+// The status of call(f).
+template <class Fn, class F>
+PyObject *status(Fn *f, F &&call) {
+    if (!f) {
+        PyErr_SetString(PyExc_RuntimeError, "this function has not been bound");
+        return nullptr;
+    }
     int rc;
     Py_BEGIN_ALLOW_THREADS;
-    rc = call();
+    rc = call(f);
     Py_END_ALLOW_THREADS;
     return PyLong_FromLong(rc);
 }
@@ -135,8 +140,8 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!take(x, a + 1, at) || !take(y, a + 5, at)) return nullptr;
     const float eps = (float)PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) return nullptr;
-    return status([&] {
-        return s_qk_norm_rope(at.be, x[0].p, x[1].p, x[2].p, eps, y[0].p, y[1].p, y[2].p, y[3].p, y[4].p, y[5].p, y[6].p, y[7].p);
+    return status(s_qk_norm_rope, [&](auto f) {
+        return f(at.be, x[0].p, x[1].p, x[2].p, eps, y[0].p, y[1].p, y[2].p, y[3].p, y[4].p, y[5].p, y[6].p, y[7].p);
     });
 }
 
@@ -147,8 +152,8 @@ PyObject *flash_attn_tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!take(x, a + 1, at) || !take(y, a + 9, at)) return nullptr;
     const float scale = (float)PyFloat_AsDouble(a[8]);
     if (PyErr_Occurred()) return nullptr;
-    return status([&] {
-        return s_flash_attn_tree(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, scale, y[0].p);
+    return status(s_flash_attn_tree, [&](auto f) {
+        return f(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, scale, y[0].p);
     });
 }
 
@@ -169,9 +174,8 @@ PyObject *tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!count(n, 14)) return nullptr;
     const Where at(a[0]);
     if (!take(x, a + 1, at) || !int32(a[9], &layers) || !take(y, a + 10, at)) return nullptr;
-    return status([&] {
-        return s_tree_commit(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, layers, y[0].p, y[1].p, y[2].p,
-                             y[3].p);
+    return status(s_tree_commit, [&](auto f) {
+        return f(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, layers, y[0].p, y[1].p, y[2].p, y[3].p);
     });
 }
 
@@ -181,7 +185,7 @@ PyObject *kv_pages_copy(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!count(n, 5)) return nullptr;
     const Where at(a[0]);
     if (!take(x, a + 1, at) || !int32(a[3], &layers) || !take(y, a + 4, at)) return nullptr;
-    return status([&] { return s_kv_pages_copy(at.be, x[0].p, x[1].p, layers, y[0].p); });
+    return status(s_kv_pages_copy, [&](auto f) { return f(at.be, x[0].p, x[1].p, layers, y[0].p); });
 }
 
 PyObject *tree_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -189,8 +193,8 @@ PyObject *tree_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!count(n, 10)) return nullptr;
     const Where at(a[0]);
     if (!take(x, a + 1, at)) return nullptr;
-    return status([&] {
-        return s_tree_sample(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, x[8].p);
+    return status(s_tree_sample, [&](auto f) {
+        return f(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, x[5].p, x[6].p, x[7].p, x[8].p);
     });
 }
 
@@ -201,7 +205,7 @@ PyObject *attn_weights(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!take(x, a + 1, at) || !take(y, a + 8, at)) return nullptr;
     const float scale = (float)PyFloat_AsDouble(a[6]), decay = (float)PyFloat_AsDouble(a[7]);
     if (PyErr_Occurred()) return nullptr;
-    return status([&] { return s_attn_weights(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, scale, decay, y[0].p); });
+    return status(s_attn_weights, [&](auto f) { return f(at.be, x[0].p, x[1].p, x[2].p, x[3].p, x[4].p, scale, decay, y[0].p); });
 }
 
 PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -212,14 +216,14 @@ PyObject *kv_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!take(x, a + 1, at) || !int32(a[5], &sink) || !int32(a[6], &recent) || !take(y, a + 7, at) || !int32(a[9], &layers) ||
         !take(z, a + 10, at))
         return nullptr;
-    return status([&] { return s_kv_evict(at.be, x[0].p, x[1].p, x[2].p, x[3].p, sink, recent, y[0].p, y[1].p, layers, z[0].p); });
+    return status(s_kv_evict, [&](auto f) { return f(at.be, x[0].p, x[1].p, x[2].p, x[3].p, sink, recent, y[0].p, y[1].p, layers, z[0].p); });
 }
 
-// bind(unsupported, addresses of the C functions in the order below: the first four, or all)
+// bind(unsupported, addresses of the C functions in the order below: the first four, or all); what has no address raises
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     constexpr int FEW = 4, ALL = 7;
     if (n != 1 + FEW && !count(n, 1 + ALL)) return nullptr;
-    void *f[ALL];
+    void *f[ALL] = {};
     for (int i = 0; i < n - 1; ++i) f[i] = PyLong_AsVoidPtr(a[1 + i]);
     if (PyErr_Occurred()) return nullptr;
     Py_INCREF(a[0]);
@@ -228,11 +232,9 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     s_flash_attn_tree = reinterpret_cast<decltype(s_flash_attn_tree)>(f[1]);
     s_tree_commit = reinterpret_cast<decltype(s_tree_commit)>(f[2]);
     s_kv_pages_copy = reinterpret_cast<decltype(s_kv_pages_copy)>(f[3]);
-    if (n == 1 + ALL) {
-        s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
-        s_attn_weights = reinterpret_cast<decltype(s_attn_weights)>(f[5]);
-        s_kv_evict = reinterpret_cast<decltype(s_kv_evict)>(f[6]);
-    }
+    s_tree_sample = reinterpret_cast<decltype(s_tree_sample)>(f[4]);
+    s_attn_weights = reinterpret_cast<decltype(s_attn_weights)>(f[5]);
+    s_kv_evict = reinterpret_cast<decltype(s_kv_evict)>(f[6]);
     Py_RETURN_NONE;
 }
 

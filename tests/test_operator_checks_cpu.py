@@ -270,3 +270,50 @@ def test_evictions_in_one_buffer_are_not(be, change):
     with pytest.raises(ob.GgmlBackendError) as e:
         evict(be, **change)
     assert e.value.status == bk.STATUS_DEVICE_LOST
+
+
+UNBOUND = """
+import ctypes
+
+import torch
+
+from openasr_b200 import _torch_ops as ext, backend as bk
+
+t = bk.describe(torch.zeros(2, 2))
+calls = [lambda: ext.tree_sample(5, *[t] * 9), lambda: ext.attn_weights(5, *[t] * 5, 0.5, 1.0, t),
+         lambda: ext.kv_evict(5, t, t, t, t, 0, 0, t, t, 1, t)]
+first = [lambda: ext.kv_pages_copy(5, t, t, 1, t), lambda: ext.flash_attn_tree(5, *[t] * 7, 0.5, t),
+         lambda: ext.qk_norm_rope(5, t, t, t, 0.5, *[t] * 8), lambda: ext.tree_commit(5, *[t] * 8, 1, *[t] * 4)]
+
+
+def unbound(some):
+    for call in some:
+        try:
+            call()
+        except RuntimeError as e:
+            assert "has not been bound" in str(e)
+        else:
+            raise SystemExit("no error")
+
+
+unbound(calls + first)
+copy = ctypes.CFUNCTYPE(ctypes.c_int, *[ctypes.c_void_p] * 3, ctypes.c_int32, ctypes.c_void_p)(lambda *a: 7)
+addr = ctypes.cast(copy, ctypes.c_void_p).value
+ext.bind(bk._unsupported, *[addr] * 4)
+unbound(calls)
+assert ext.kv_pages_copy(5, t, t, 1, t) == 7
+ext.bind(bk._unsupported, *[addr] * 7)
+ext.bind(bk._unsupported, *[addr] * 4)
+unbound(calls)
+print("done")
+"""
+
+
+def test_a_function_without_an_address_raises():
+    """in a process of its own: bound to the first four functions, or to none, the others are not called"""
+    if isinstance(bk._ops(), bk._CtypesOps):
+        pytest.skip("built without torch's headers")
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", UNBOUND], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "done", (r.returncode, r.stdout, r.stderr)
