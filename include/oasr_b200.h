@@ -385,8 +385,12 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * after the old value was multiplied by decay; with decay 0, and for the positions from n_past on,
  * which are new, the old value is not read.  Entries of positions past the last node stay as they are.
  * n_past + n_nodes is at most 2^30 here.  weights may not overlap another argument.
- * One call per layer and step, with the queries and the lengths of that layer's flash_attn_tree; or
- * one after the prompt with its last rows and decay 0, which scores all of it.  A row with something
+ * One call per layer and step: with the queries and the lengths of that layer's flash_attn_tree where all
+ * nodes are a chain and stay in the cache (a plain step, a prompt's chunk); or one after the prompt
+ * with its last rows and decay 0, which scores all of it.  What a node pays is added for good, so a draft is
+ * scored after oasr_b200_tree_commit, by what was accepted: n_past as it was before, n_nodes = n_accept, and
+ * as q the rows of the nodes in path, in their order (for a chain the rows as they are, for a tree
+ * gathered); their K rows lie there already.  A row with something
  * that is not finite (a query, a K row that it sees) makes the entries of what it sees NaN; a position
  * whose score is -inf gets nothing.
  *

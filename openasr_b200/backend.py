@@ -747,8 +747,9 @@ class Backend:
 
     def attn_weights(self, q, k_pages, page_table, n_past, n_nodes, scale: float, decay: float, weights) -> None:
         """Add the attention that each position gets from the nodes q f32|f16 [S, H, n, D] (a chain) to its
-        entry of weights f32 [P, H_kv, page], old entries times decay (0: not read).  No two sequences of
-        a call share a page."""
+        entry of weights f32 [P, H_kv, page], old entries times decay (0: not read).  After a draft: the
+        accepted nodes alone, once tree_commit has moved their rows, with the old n_past, n_nodes =
+        n_accept and q gathered by path.  No two sequences of a call share a page."""
         self._check((_OPS or _ops()).attn_weights((self.handle.value or 0, self.ordinal), q, k_pages, page_table, n_past,
                                                   n_nodes, scale, decay, weights))
 
