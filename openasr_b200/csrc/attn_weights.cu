@@ -8,6 +8,7 @@
 
 #include <algorithm>
 
+#include "mma_frag.cuh"
 #include "once_per_device.h"
 #include "op_checks.cuh"
 #include "pages.cuh"
@@ -34,18 +35,6 @@ constexpr int WTILE = 16;              // positions of a warp's tile
 constexpr int WEIGHTS_MOST = 1 << 30;  // positions of a sequence, so that steps past them stay in 32 bits
 constexpr int WPAGES = 520;            // pages of a stretch: of 8 positions and more
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ uint4 stream(const void *p) {
     const int4 v = ldg_stream(p);
     return make_uint4(v.x, v.y, v.z, v.w);
@@ -54,7 +43,7 @@ __device__ __forceinline__ uint4 stream(const void *p) {
 // (m, l) of two sets of positions to that of both; m = -inf: nothing seen
 __device__ __forceinline__ void join(float &m, float &l, float om, float ol) {
     const float mm = fmaxf(m, om), z = mm == -INFINITY ? 0.0f : mm;
-    l = l * ex2(m - z) + ol * ex2(om - z);
+    l = l * tree_exp2(m - z) + ol * tree_exp2(om - z);
     m = mm;
 }
 
@@ -222,12 +211,12 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages 
                 for (int c = 0; c < C; ++c) {
                     if (!QF16) {
                         const uint4 lo = q[b].lo[QF16 ? 0 : c];
-                        mma_f16(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, lo.x, lo.y);
-                        mma_f16(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, lo.z, lo.w);
+                        mma_f16_16816_add(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, lo.x, lo.y);
+                        mma_f16_16816_add(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, lo.z, lo.w);
                     }
                     const uint4 hi = q[b].hi[c];
-                    mma_f16(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, hi.x, hi.y);
-                    mma_f16(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, hi.z, hi.w);
+                    mma_f16_16816_add(c4, k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, hi.x, hi.y);
+                    mma_f16_16816_add(c4, k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, hi.z, hi.w);
                 }
                 const float2 f = factor[b];
                 c4[0] *= f.x, c4[1] *= f.y, c4[2] *= f.x, c4[3] *= f.y;
@@ -244,7 +233,7 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages 
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float mm = fmaxf(m[b][e], fmaxf(c4[e], c4[e + 2])), z = mm == -INFINITY ? 0.0f : mm;
-                        l[b][e] = l[b][e] * ex2(m[b][e] - z) + ex2(c4[e] - z) + ex2(c4[e + 2] - z);
+                        l[b][e] = l[b][e] * tree_exp2(m[b][e] - z) + tree_exp2(c4[e] - z) + tree_exp2(c4[e + 2] - z);
                         m[b][e] = mm;
                     }
                 }
@@ -305,8 +294,8 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages 
                     const float2 v = *reinterpret_cast<const float2 *>(s_scores + (at - b0) * a.stride + r);
                     // the first row that sees the position: what it does not see a row that is NaN does not reach
                     const int seen = at > past ? (at - past) * a.G : 0;
-                    if (r >= seen) sum[u] += ex2(v.x - x.x) * x.y;
-                    if (r + 1 >= seen && r + 1 < rows) sum[u] += ex2(v.y - y.x) * y.y;
+                    if (r >= seen) sum[u] += tree_exp2(v.x - x.x) * x.y;
+                    if (r + 1 >= seen && r + 1 < rows) sum[u] += tree_exp2(v.y - y.x) * y.y;
                 }
             }
 #pragma unroll
@@ -396,12 +385,12 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_wide_kernel(Weights a, KvP
 #pragma unroll
             for (int i = 0; i < 2 && b + i < NB; ++i) {
                 const uint4 hi = s_q[((b + i) * PARTS * C + c) * 32 + lane];
-                mma_f16(x[i], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, hi.x, hi.y);
-                mma_f16(x[i], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, hi.z, hi.w);
+                mma_f16_16816_add(x[i], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, hi.x, hi.y);
+                mma_f16_16816_add(x[i], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, hi.z, hi.w);
                 if (!QF16) {
                     const uint4 rest = s_q[(((b + i) * PARTS + PARTS - 1) * C + c) * 32 + lane];
-                    mma_f16(lo[i], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, rest.x, rest.y);
-                    mma_f16(lo[i], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, rest.z, rest.w);
+                    mma_f16_16816_add(lo[i], k[0][c].x, k[1][c].x, k[0][c].y, k[1][c].y, rest.x, rest.y);
+                    mma_f16_16816_add(lo[i], k[0][c].z, k[1][c].z, k[0][c].w, k[1][c].w, rest.z, rest.w);
                 }
             }
         const bool edge = hides(at, b);
@@ -477,7 +466,7 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_wide_kernel(Weights a, KvP
                         for (int e = 0; e < 2; ++e) {
                             float &mm = m[b + i][e], &ll = l[b + i][e];
                             const float up = fmaxf(mm, fmaxf(x[i][e], x[i][e + 2])), z = up == -INFINITY ? 0.0f : up;
-                            ll = ll * ex2(mm - z) + ex2(x[i][e] - z) + ex2(x[i][e + 2] - z);
+                            ll = ll * tree_exp2(mm - z) + tree_exp2(x[i][e] - z) + tree_exp2(x[i][e + 2] - z);
                             mm = up;
                         }
                 }
@@ -534,7 +523,7 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_wide_kernel(Weights a, KvP
                     const float4 y = s_row[4 * (b + i) + t];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float u = ex2(x[i][2 * h] - y.x) * y.y, v = ex2(x[i][2 * h + 1] - y.z) * y.w;
+                        const float u = tree_exp2(x[i][2 * h] - y.x) * y.y, v = tree_exp2(x[i][2 * h + 1] - y.z) * y.w;
                         // what it does not see a row that is NaN does not reach
                         w[h] += edge && at + g + 8 * h > last.x ? 0.0f : u;
                         w[h] += edge && at + g + 8 * h > last.y ? 0.0f : v;

@@ -211,12 +211,6 @@ static __device__ __noinline__ float4 tree_nonfinite4(const TreeAttn &a, const K
     return o;
 }
 
-static __device__ __forceinline__ float tree_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Two f32 in one register pair: one instruction for both.
 typedef unsigned long long f32x2;
 static __device__ __forceinline__ f32x2 pack2(float x, float y) {

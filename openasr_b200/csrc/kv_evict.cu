@@ -77,8 +77,8 @@ __device__ __forceinline__ int nth_bit(uint32_t word, int n) {
 // counts going to every CTA; then every CTA gets the whole choice, one bit per position, and how many bits
 // are set up to each word.  The rows are moved by columns, each CTA its own 16 LPR bytes of every K row or
 // every V row, so that from here on no CTA waits for another: row g of the kept ones comes from the
-// position of bit g, never before position g, in rounds of 256 rows that are all loaded before any of them
-// is stored.  What is stored lies before all later rounds' rows.
+// position of bit g, never before position g, in rounds of BATCH rows (256; 128 in columns of 256 bytes) that
+// are all loaded before any of them is stored.  What is stored lies before all later rounds' rows.
 template <int CS, int LPR>
 __global__ void __launch_bounds__(ET) kv_evict_kernel(Evict a, KvPages p, KvSeqs sq, FastDiv page, int *err) {
     namespace cg = cooperative_groups;
@@ -371,7 +371,7 @@ extern "C" int oasr_b200_kv_evict(oasr_backend *be, oasr_tensor *weights, const 
     const int64_t items = S * HKV * n_layers;
     // a K row and a V row for a CTA each; half a row where that leaves SMs without work (96 heads of 128 and
     // 32000 positions: 171 us in halves, 343 in rows; 224 of 512: 38 and 22, 1792 of 390 to 1990: 279 and 205)
-    const bool halves = items * 4 <= 4 * be->sm_count;
+    const bool halves = items <= be->sm_count;
     if (k_pages->ne[0] == 128) return halves ? launch_evict<4, 8>(be, a, p, sq, items) : launch_evict<2, 16>(be, a, p, sq, items);
     return halves ? launch_evict<4, 4>(be, a, p, sq, items) : launch_evict<2, 8>(be, a, p, sq, items);
 }

@@ -1,5 +1,6 @@
 // mma_frag.cuh -- decode-tile layout constants and mma.sync fragment helpers shared by
-// the decode GEMV (mmv_tc.cu) and the fused decoder GEMV (dgemv.cu).
+// the decode GEMV (mmv_tc.cu) and the fused decoder GEMV (dgemv.cu); the attention's weights
+// (attn_weights.cu) use one that adds up.
 #pragma once
 
 #include "kernels.cuh"
@@ -23,6 +24,14 @@ static __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0,
         "{%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// d += a b
+static __device__ __forceinline__ void mma_f16_16816_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                         uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 static __device__ __forceinline__ int ldg_nc_b32(const void *p) {

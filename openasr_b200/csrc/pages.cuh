@@ -63,6 +63,13 @@ struct FastDiv {
     }
 };
 
+// 2^x of the softmax weights over the pages: an error of 2^-22, results below 2^-126 are 0.
+static __device__ __forceinline__ float tree_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // attention of N nodes per sequence over the pages (fattn_tree.cu)
 struct TreeAttn {
     const char *q;

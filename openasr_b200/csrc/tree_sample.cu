@@ -20,7 +20,6 @@ using namespace oasr;
 
 namespace {
 
-
 constexpr int NT = 256, NW = NT / 32;
 
 struct Sample {
@@ -252,12 +251,8 @@ __device__ __forceinline__ Part run_sum(const Row &row, const Run &run, float4 (
         }
         if (ref == -INFINITY) return;  // nothing finite so far
 #pragma unroll
-        for (int u = 0; u < U; u += G / 4) {
-            double d[G];
-#pragma unroll
-            for (int c = 0; c < G; c += 4)
-                d[c] = (double)b[u + c / 4].x, d[c + 1] = (double)b[u + c / 4].y, d[c + 2] = (double)b[u + c / 4].z,
-                d[c + 3] = (double)b[u + c / 4].w;
+        for (int u = 0; u < U; ++u) {
+            double d[G] = {(double)b[u].x, (double)b[u].y, (double)b[u].z, (double)b[u].w};
             if (ref != 0.0f) {
 #pragma unroll
                 for (int c = 0; c < G; ++c) d[c] -= (double)ref;
@@ -280,7 +275,6 @@ __device__ __forceinline__ Part run_sum(const Row &row, const Run &run, float4 (
         }
         if ((done += 2 * TILE) == run.step || j + 2 * TILE >= run.j1) {
             double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-            if (G == 8) s += (acc[4 % G] + acc[5 % G]) + (acc[6 % G] + acc[7 % G]);
             s = warp_sum(s);
             plain = isfinite(s);
             if (lane == i) mine = Part{s, ref, 0};
