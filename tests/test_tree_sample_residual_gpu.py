@@ -117,3 +117,25 @@ def test_differences_above_the_roundings_are_kept(be):
     u[..., 0] = 0.999
     temp = np.ones(S, np.float32)
     same(run(be, x, temp, u, None, tok, par, q), want64(x, temp, u, [2] * S, tok, par, q))
+
+
+@pytest.mark.parametrize("kids", [2, 3, 5])
+def test_tokens_after_several_children_are_distributed_as_the_targets(be, kids):
+    """65536 roots with children drawn from q one after the other: the token after the root is distributed as p (five
+    standard deviations of a count at fixed seeds), and each further child is taken now and then"""
+    rng = np.random.default_rng(kids)
+    S, V, N = 65536, 7, 1 + kids
+    x1 = np.array([0.3, -1.0, 2.0, 0.0, 1.0, -3.0, 0.5], np.float32)
+    q1 = np.exp(np.array([1.0, 1.0, -1.0, 0.0, 2.0, 0.0, -2.0]))
+    q1 = (q1 / q1.sum()).astype(np.float32)
+    p = np.exp(x1.astype(np.float64))
+    p /= p.sum()
+    x, q = np.broadcast_to(x1, (S, N, V)), np.broadcast_to(q1, (S, N, V))
+    tok = rng.choice(V, (S, N), p=q1.astype(np.float64) / q1.astype(np.float64).sum()).astype(np.int32)
+    par = np.zeros((S, N), np.int32)
+    par[:, 0] = -1
+    t, _ = run(be, x, None, rng.random((S, N, 2), np.float32), None, tok, par, q)
+    count = np.bincount(t[:, 0], minlength=V)
+    assert (np.abs(count - S * p) <= 5 * np.sqrt(S * p * (1 - p))).all()
+    first = [(t[:, 0] == tok[:, j]) & (t[:, :1] != tok[:, 1:j]).all(-1) for j in range(1, N)]
+    assert all(f.mean() > 0.01 for f in first), [f.mean() for f in first]
