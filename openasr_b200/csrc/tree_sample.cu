@@ -316,7 +316,7 @@ __device__ __forceinline__ Part run_max(const Row &row, const Run &run, float4 (
     return Part{0.0, best, at};
 }
 
-// A weight is good to 2^-42.  What a difference leaves of m, if it is more than that error: above 2^-40 of m.
+// A weight is good to 2^-42: m - b, if that is more than such an error, above 2^-40 of m.
 __device__ __forceinline__ double left_of(double m, double difference) {
     return __double2hiint(difference) > max(__double2hiint(m) - (40 << 20), 0) ? difference : 0.0;
 }
@@ -327,20 +327,14 @@ __device__ __forceinline__ double left_of(double m, double difference) {
 // here: what has a sum has a value that it came from.
 template <int N>
 __device__ __forceinline__ void residual(double (&w)[N], double Z, const float (&q)[N], const double *inv, int k) {
-    double r[N], m[N];  // m: w in the units of r
+    double r[N];
 #pragma unroll
     for (int c = 0; c < N; ++c) r[c] = left_of(w[c], fma(-(double)q[c], Z, w[c]));
-    if (k > 1) {
+    for (int n = 1; n < k; ++n) {
+        const double g = inv[n - 1];
 #pragma unroll
-        for (int c = 0; c < N; ++c) m[c] = w[c];
-        for (int n = 1; n < k; ++n) {
-            const double g = inv[n - 1];
-#pragma unroll
-            for (int c = 0; c < N; ++c) {
-                m[c] = g > 0.0 ? m[c] * g : w[c];
-                r[c] = left_of(m[c], g > 0.0 ? fma(r[c], g, -(double)q[c]) : fma(-(double)q[c], Z, w[c]));
-            }
-        }
+        for (int c = 0; c < N; ++c)
+            r[c] = g > 0.0 ? left_of(r[c] * g, fma(r[c], g, -(double)q[c])) : left_of(w[c], fma(-(double)q[c], Z, w[c]));
     }
 #pragma unroll
     for (int c = 0; c < N; ++c) w[c] = r[c];

@@ -139,3 +139,27 @@ def test_tokens_after_several_children_are_distributed_as_the_targets(be, kids):
     assert (np.abs(count - S * p) <= 5 * np.sqrt(S * p * (1 - p))).all()
     first = [(t[:, 0] == tok[:, j]) & (t[:, :1] != tok[:, 1:j]).all(-1) for j in range(1, N)]
     assert all(f.mean() > 0.01 for f in first), [f.mean() for f in first]
+
+
+@pytest.mark.parametrize("q0", [0.5, 0.9, 0.99])
+@pytest.mark.parametrize("N", [14, 64, 1024])
+def test_one_token_is_left_after_any_number_of_children(be, N, q0):
+    """what is left of p is one token's from the first rejected child on, and is 1 again after each: the next ones take
+    q0 of it and no more, although together they have taken all but (1 - q0)^N"""
+    rng = np.random.default_rng(N)
+    S, V = 3, 37
+    p = np.full((S, N, V), 0.004 / (V - 1))
+    p[..., 5] = 0.996
+    q = np.full((S, N, V), (1 - q0) / (V - 1), np.float32)
+    q[..., 5] = q0
+    x = np.log(p).astype(np.float32)
+    tok = rng.integers(6, V, (S, N)).astype(np.int32)
+    par = np.zeros((S, N), np.int32)
+    par[:, 0] = -1
+    u = rng.random((S, N, 2), np.float32)
+    u[..., 0] = 0.999
+    u[:, 0, 1] = 0.9999  # another one of p's
+    temp = np.ones(S, np.float32)
+    got = run(be, x, temp, u, None, tok, par, q)
+    same(got, want64(x, temp, u, [N] * S, tok, par, q))
+    assert (got[0][:, 0] == 5).all()
