@@ -438,8 +438,8 @@ __device__ __forceinline__ double scan(double v) {
 // The sums of a row's weights by stretch, warp and CTA, and where a drawn value lies.
 template <int CS>
 struct Sums {
-    double stretch[NW][32];  // of a warp's stretches, relative to the CTA's reference
-    double warp[NW];         // of the warps
+    double stretch[NW][32], stretch_to[NW][32];  // of a warp's stretches, and up to them, relative to the CTA's reference
+    double warp[NW], warp_to[NW];                // of the warps
     double cta[2][CS];       // sums of the cluster's CTAs (two calls in turn), relative to
     float cta_ref[2][CS];    // their references
     float warp_ref[NW];
@@ -460,25 +460,23 @@ struct Place {
 };
 
 // `mine`: this lane's stretch, relative to the warp's reference.  Then the sums are everywhere, `all` is the
-// whole row's and `ref` what it is relative to; f: what this lane's CTA's are to be multiplied by.
+// whole row's and `ref` what it is relative to; f: what this lane's CTA's are to be multiplied by, `to` the
+// running sum up to it.
 template <int CS>
 __device__ __forceinline__ void gather(Sums<CS> &s, int turn, int rank, const Part &mine, double C, uint32_t tab, double &all, float &ref,
-                                       double &f) {
+                                       double &to, double &f) {
     namespace cg = cooperative_groups;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane == 0) s.warp_ref[warp] = mine.ref;
     __syncthreads();
     const float m = warp_max(lane < NW ? s.warp_ref[lane] : -INFINITY);
-    const double own = scaled(mine.sum, mine.ref, m, C, tab);
-    s.stretch[warp][lane] = own;
-    const double sum = warp_sum(own);
-    if (lane == 0) s.warp[warp] = sum;
+    const double own = scaled(mine.sum, mine.ref, m, C, tab), up = scan(own);
+    s.stretch[warp][lane] = own, s.stretch_to[warp][lane] = up;
     __syncthreads();
     if (warp == 0) {
-        double total = lane < NW ? s.warp[lane] : 0.0;
-#pragma unroll
-        for (int o = NW / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o, NW);
-        total = __shfl_sync(0xffffffffu, total, 0);
+        const double of_warp = lane < NW ? s.stretch_to[lane][31] : 0.0, w = scan<NW>(of_warp);
+        if (lane < NW) s.warp[lane] = of_warp, s.warp_to[lane] = w;
+        const double total = __shfl_sync(0xffffffffu, w, NW - 1);
         if (CS == 1) {
             if (lane == 0) s.cta[turn][0] = total, s.cta_ref[turn][0] = m;
         } else if (lane < CS) {
@@ -492,23 +490,20 @@ __device__ __forceinline__ void gather(Sums<CS> &s, int turn, int rank, const Pa
     const float r = lane < CS ? s.cta_ref[turn][lane] : -INFINITY;
     ref = warp_max(r);
     f = lane < CS ? scaled(1.0, r, ref, C, tab) : 0.0;
-    all = lane < CS ? s.cta[turn][lane] * f : 0.0;
-#pragma unroll
-    for (int o = CS / 2; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o, CS);
-    all = __shfl_sync(0xffffffffu, all, 0);
+    to = scan<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0);
+    all = __shfl_sync(0xffffffffu, to, CS - 1);
 }
 
-// The first of N lanes with mass whose running sum from `before` on is greater than `drawn`, the last with
-// mass if roundings leave none; `before` then is the running sum up to it.  Running sums of lanes next to one another are
+// The first of N lanes with mass whose running sum `to` is greater than `drawn`, the last with mass if roundings
+// leave none; `before` then is the running sum up to it.  Running sums of lanes next to one another are
 // rounded differently, so that one may rise past `drawn` at a lane that adds nothing: mass is more than `least`.
 template <int N>
-__device__ __forceinline__ int first_past(double own, double least, double drawn, double &before) {
+__device__ __forceinline__ int first_past(double own, double to, double least, double drawn, double &before) {
     const int lane = threadIdx.x & 31;
-    const double up = before + scan<N>(own);
-    const unsigned mass = __ballot_sync(0xffffffffu, lane < N && own > least), past = __ballot_sync(0xffffffffu, up > drawn) & mass;
+    const unsigned mass = __ballot_sync(0xffffffffu, lane < N && own > least), past = __ballot_sync(0xffffffffu, to > drawn) & mass;
     const int at = past ? __ffs(past) - 1 : 31 - __clz(mass | 1u);
-    const double to = __shfl_sync(0xffffffffu, up, max(at - 1, 0));
-    if (at) before = to;
+    const double up = __shfl_sync(0xffffffffu, to, max(at - 1, 0));
+    if (at) before = up;
     return at;
 }
 
@@ -516,15 +511,16 @@ __device__ __forceinline__ int first_past(double own, double least, double drawn
 // such a stretch in such a warp of such a CTA: the greatest of 16, 8 and 32 parts), far above what values
 // without weight may have been counted as.
 template <int CS>
-__device__ __forceinline__ Place find(const Sums<CS> &s, int turn, double all, double f, double drawn, int rank) {
+__device__ __forceinline__ Place find(const Sums<CS> &s, int turn, double all, double to, double f, double drawn, int rank) {
     const int lane = threadIdx.x & 31;
     Place p;
     p.before = 0.0;
-    p.cta = first_past<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0, all * 0x1p-200, drawn, p.before);
+    p.cta = first_past<CS>(lane < CS ? s.cta[turn][lane] * f : 0.0, to, all * 0x1p-200, drawn, p.before);
     if (p.cta != rank) return p;
     f = __shfl_sync(0xffffffffu, f, p.cta);
-    p.warp = first_past<NW>(lane < NW ? f * s.warp[lane] : 0.0, all * 0x1p-204, drawn, p.before);
-    p.stretch = first_past<32>(f * s.stretch[p.warp][lane], all * 0x1p-210, drawn, p.before);
+    const int w = min(lane, NW - 1);
+    p.warp = first_past<NW>(f * s.warp[w], p.before + f * s.warp_to[w], all * 0x1p-204, drawn, p.before);
+    p.stretch = first_past<32>(f * s.stretch[p.warp][lane], p.before + f * s.stretch_to[p.warp][lane], all * 0x1p-210, drawn, p.before);
     return p;
 }
 
@@ -638,10 +634,10 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
     const double inv_T = 1.0 / (double)T, C = STEPS / LN2 * inv_T;
     const Part mine = run_sum(row, run, first, C, tab);
     if (CS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all CTAs have started
-    double Z, f;
+    double Z, to, f;
     float ref;
     int turn = 0;  // of the sums that the token is drawn from
-    gather(s_sums, 0, rank, mine, C, tab, Z, ref, f);
+    gather(s_sums, 0, rank, mine, C, tab, Z, ref, to, f);
     if (ref == -INFINITY) {  // no finite logit
         if (rank == 0 && tid == 0) put(-1, 0.0);
         return;
@@ -670,19 +666,19 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
             ++rounds;
             float same;
             turn ^= 1;
-            gather(s_sums, turn, rank, rest(rounds), C, tab, total, same, f);
+            gather(s_sums, turn, rank, rest(rounds), C, tab, total, same, to, f);
             left = total > 0x1p-1000;
             if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / total : 0.0;
             __syncthreads();
         }
         if (rounds && !left) {  // p once more
             turn ^= 1;
-            gather(s_sums, turn, rank, rest(0), C, tab, total, ref, f);
+            gather(s_sums, turn, rank, rest(0), C, tab, total, ref, to, f);
         }
     }
     // a number on a border belongs to the value behind it, however the sums up to there were rounded
     const double drawn = (double)u1 * total + total * 0x1p-44;
-    const Place at = find(s_sums, turn, total, f, drawn, rank);
+    const Place at = find(s_sums, turn, total, to, f, drawn, rank);
     if (at.cta != rank) return;
     if (tid == NT - 1) s_log = log(Z);
     // the value's place in its stretch: `each` vectors of a thread, one after the other
