@@ -50,7 +50,8 @@ __device__ __forceinline__ void join(float &m, float &l, float om, float ol) {
 // 8 rows of queries per block, in the layout of the product's second operand: lane (g, t) has of row g the
 // values 32 c + 8 t .. + 7 of each run c of 32, the first four for one product of depth 16 and the others
 // for the next; a K row is read the same way, 16 bytes per lane, so that it goes from memory to registers
-// without shared memory.  f32 queries are scaled by a power of two per row and split into two f16 halves.
+// without shared memory.  f32 queries are scaled by a power of two per row and split into two f16 halves: 22 of
+// the 24 bits of a row's greatest value, fewer of its small ones, in two products instead of three.
 template <int D, bool QF16>
 struct Block {
     static constexpr int C = D / 32;
@@ -317,6 +318,10 @@ __global__ void __launch_bounds__(WT, 2) attn_weights_kernel(Weights a, KvPages 
 // units below 20%; 210 CTAs for 14 heads of 272 rows at 368 to 737 positions, f32: 27 us).  With
 // the positions alone shared out it took 61 us there; without kept scores 32 rows of 64 values at 700 to 1468
 // positions took 20.5 instead of 16.4.  The page of a tile read two tiles ahead changed nothing.
+// On mma.sync, since a group has 64 rows at most and K goes to registers; hundreds of rows of long caches would
+// want tiles of 128 rows on tcgen05 (four chunks of 512 rows behind 3500 positions, 16 / 8 heads of 128: f16 432 us, f32
+// 653; the tree attention takes 133 for 4000).  The last 32 rows of eight such prompts, which score
+// all of them, take 53 us.
 template <int D, int NB, bool QF16>
 __global__ void __launch_bounds__(WT, 2) attn_weights_wide_kernel(Weights a, KvPages p, KvSeqs sq, FastDiv page, FastDiv group, int *err) {
     namespace cg = cooperative_groups;

@@ -316,7 +316,7 @@ __device__ __forceinline__ Part run_max(const Row &row, const Run &run, float4 (
     return Part{0.0, best, at};
 }
 
-// A weight is good to 2^-42: m - b, if that is more than such an error, above 2^-40 of m.
+// A weight is good to 2^-42: a difference from m, if it is more than such errors, above 2^-40 of m; else nothing.
 __device__ __forceinline__ double left_of(double m, double difference) {
     return __double2hiint(difference) > max(__double2hiint(m) - (40 << 20), 0) ? difference : 0.0;
 }
@@ -527,12 +527,14 @@ __device__ __forceinline__ Place find(const Sums<CS> &s, int turn, double all, d
 // One cluster of CS CTAs per node; every warp takes one run of the row's vectors.  The CTAs' sums go to
 // every CTA of the cluster, which then all take the same decisions, so that the call needs no workspace
 // and no second launch; the CTA that holds the drawn value's stretch reads that stretch once more.
-// Many nodes are bound by issue: a 64-bit instruction takes the slots of two, which leaves 4.5 values per
-// clock and SM (1952 nodes of 151936: 266 us, 4.1 TB/s; a loop of nothing but loads, weights and sum takes
-// 215).  CTAs that take one node after another with the next one's first tile ahead were slower (300 to
-// 324: the nodes are then dealt out evenly, not as CTAs end), and so were three CTAs per SM (272).  A few
-// nodes are a chain of latencies: 2700 cycles to the first values, 2500 for a warp's tile, 2400 to gather
-// the sums over a cluster, 2000 for the drawn value (one token of 51866: 8.3 us).
+// Many nodes (1952 of 151936: 266 us, 4.1 TB/s) take 18.8 instructions a value, 7.7 of them of 64 bits, which keep
+// the issue slot for a second cycle: with those, slots are taken 72% of the time a CTA runs.  A loop of nothing but
+// loads, weights and sum takes 215 us; the other 50 are starts, gathers and draws, which one other CTA per SM
+// (126 registers) hides in part, and in the loop a warp waits 2.2 of the 6.4 cycles between two of its instructions
+// for its own results, 1.2 for memory.  CTAs that take one node after another with the next one's first tile
+// ahead were slower (300 to 324: the nodes are then dealt out evenly, not as CTAs end), and so were three CTAs
+// per SM (272).  A few nodes are a chain of latencies: 2500 cycles to the first values, 2600 for a warp's tile,
+// 2400 to gather the sums over a cluster, 2400 for the drawn value (one token of 51866: 8.3 us).
 template <int CS, int U, bool DRAFT>
 __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) {
     namespace cg = cooperative_groups;
@@ -813,10 +815,10 @@ extern "C" int oasr_b200_tree_sample(oasr_backend *be, const oasr_tensor *logits
     a.N = (int)N, a.V = (int)V;
     const int64_t rows = S * N;
     // CTAs per node: enough of them for the SMs, of at least 2048 values each.  Without a draft two per SM (8
-    // nodes of 151936: 10.3 us with 16 CTAs each, 12.4 with 8, 16.5 with 4; 1952 nodes: 266 us with one, 324
-    // with two).  With one, nodes whose children are rejected take three times as long as the others, and
-    // more and smaller CTAs even that out (64 nodes: 39 us with 4, 38 with 8, 51 with 16; 124 of 51866: 48, 33
-    // and 31 us with 2, 4 and 8).
+    // nodes of 151936: 10.3 us with 16 CTAs each, 12.4 with 8, 15.1 with 4; 1952 nodes: 266 us with one, 315
+    // with two).  With one, nodes whose children are rejected take two to four times as long as the others, and
+    // more and smaller CTAs even that out (64 nodes: 38.7 us with 4, 37.5 with 8, 49.5 with 16; 124 of 51866: 43,
+    // 31.4, 30.8 and 47 us with 2, 4, 8 and 16).
     const int most = draft_probs ? 8 : 16, per_sm = draft_probs ? 8 : 2;
     int cs = most;
     while (cs > 1 && (rows * cs > per_sm * be->sm_count || V < 2048 * cs)) cs /= 2;
