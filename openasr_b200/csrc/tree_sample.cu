@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(NT, 2) tree_sample_kernel(Sample a, int *err) 
             float same;
             turn ^= 1;
             gather(s_sums, turn, rank, rest(rounds), C, tab, total, same, to, f);
-            left = total > 0x1p-1000;
+            left = total > 0x1p-1000 && total < INFINITY;  // (a draft's -inf or NaN leaves p, not a sum without a place)
             if (tid == 0) s_inv[rounds - 1] = left ? 1.0 / total : 0.0;
             __syncthreads();
         }

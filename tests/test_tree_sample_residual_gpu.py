@@ -163,3 +163,21 @@ def test_one_token_is_left_after_any_number_of_children(be, N, q0):
     got = run(be, x, temp, u, None, tok, par, q)
     same(got, want64(x, temp, u, [N] * S, tok, par, q))
     assert (got[0][:, 0] == 5).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, -3e38, 3e38, -1.0])
+@pytest.mark.parametrize("V", [9, 5003, 60001])
+def test_a_draft_that_is_no_probability_still_gives_a_token(be, bad, V):
+    """the outputs are then undefined, but tokens of the vocabulary, and the other sequences' their own"""
+    rng = np.random.default_rng(V)
+    S, N = 12, 4
+    x, top, tok, par, u = certain(rng, S, N, V, 3.0)
+    q = np.exp(x.astype(np.float64) + rng.standard_normal(x.shape))
+    q = (q / q.sum(-1, keepdims=True)).astype(np.float32)
+    want = want64(x, np.ones(S), u, [N] * S, tok, par, q)
+    spoiled = q.copy()
+    spoiled[::2, :, rng.integers(0, V, 3)] = bad
+    spoiled[::4] = bad
+    t, lp = run(be, inside(x, 2), None, u, None, tok, par, spoiled)
+    assert ((0 <= t) & (t < V)).all() and np.isfinite(lp).all()
+    same((t[1::2], lp[1::2]), (want[0][1::2], want[1][1::2]))
