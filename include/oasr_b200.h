@@ -404,7 +404,7 @@ int oasr_b200_kv_pages_copy(oasr_backend *be, oasr_tensor *k_pages, oasr_tensor 
  * positions that they had: later nodes pass pos to oasr_b200_qk_norm_rope, counting on from there.
  * weights has the pages of all layers along ne[2], as k_pages along ne[3].  n_keep of a longer sequence
  * must be n_sink + n_recent or more, and n_past at most 2^18 (both checked on the device like the lengths).
- * No argument may overlap another, and no two rows of the pages may lie in one place. */
+ * weights, pages and n_past_out may not overlap another argument, nor rows of the pages one another. */
 int oasr_b200_attn_weights(oasr_backend *be, const oasr_tensor *q, const oasr_tensor *k_pages,
                            const oasr_tensor *page_table, const oasr_tensor *n_past, const oasr_tensor *n_nodes,
                            float scale, float decay, oasr_tensor *weights);
